@@ -248,6 +248,7 @@ def prepare(case, seed):
         state["new"], state["lengths"] = new, lengths
         state["k"] = torch.randn(pages, size, case["kv_heads"], case["head_dim"], generator=g, device=device, dtype=dtype)
         state["v"] = torch.randn(pages, size, case["kv_heads"], case["head_dim"], generator=g, device=device, dtype=dtype)
+        _with_caches(state, [(state["k"], state["v"])])
         state["page_table"] = _place(lengths, size, pages, max(counts) + 3, seed).to(device)
         state["key_lengths"] = torch.tensor(lengths, dtype=torch.int32, device=device)
         starts = [0]
@@ -277,7 +278,15 @@ def prepare(case, seed):
         shape = (pages, size, case["kv_heads"], case["head_dim"])
         state["caches"] = [(torch.randn(shape, generator=g, device=device, dtype=_DTYPES[case["dtype"]]),
                             torch.randn(shape, generator=g, device=device, dtype=_DTYPES[case["dtype"]])) for _ in range(case["layers"])]
+        _with_caches(state, state["caches"])
     return state
+
+
+def _with_caches(state, pairs):
+    """The caches' handles, which a program keeps as long as the caches."""
+    if own:
+        from vibe_compiler_b200.paged_cache import PagedCache
+        state["handles"] = [PagedCache(k, v) for k, v in pairs]
 
 
 def _with_table(state, rotary_dim, scaling):
@@ -300,8 +309,8 @@ def _run_own(state):
     if op == "rope":
         return backend.rope(state["x"], state["positions"], state["rotary"], interleaved=case["interleaved"], backward=case["backward"])
     if op in ("append", "attention"):
-        from vibe_compiler_b200.paged_cache import PagedBatch, PagedCache
-        cache = PagedCache(state["k"], state["v"])
+        from vibe_compiler_b200.paged_cache import PagedBatch
+        cache = state["handles"][0]
         batch = PagedBatch(state["page_table"], state["key_lengths"], state["query_starts"], max_query=max(state["new"]))
         if op == "append":
             q = backend.rope_append(state["qkv"], cache, batch, state["rotary"], q_heads=case["q_heads"], interleaved=case["interleaved"])
@@ -312,8 +321,7 @@ def _run_own(state):
     size = case["page_size"]
     if op == "reserve":
         return backend.pages_reserve(state["table"], state["held"], state["refs"], state["wanted"], size)
-    from vibe_compiler_b200.paged_cache import PagedCache
-    caches = [PagedCache(k, v) for k, v in state["caches"]]
+    caches = state["handles"]
     if op == "fork":
         table, held, refs = backend.pages_free(state["table"], state["held"], state["refs"], state["freed"], size)
         table, held, refs, sources, destinations, result = backend.pages_fork(table, held, refs, state["parents"], state["children"], size)
