@@ -462,6 +462,138 @@ wb200_status wb200_decoder_layer(wb200_backend *backend, const wb200_decoder_lay
  * layer's last kernel is done. *count = 4 parts + 1 (0 if there was no such call); ms may be null to ask for the count. */
 wb200_status wb200_decoder_layer_timeline(wb200_backend *backend, float *ms, uint32_t capacity, uint32_t *count);
 
+/* ------------------------------------------------------------------ serving from a paged KV cache
+ * A cache of K and V rows cut into pages of `page_size` tokens, a page table that says which pages a sequence's rows lie
+ * in, and the operators that write, read and keep it. The reference has no counterpart: it decodes from one compact cache
+ * per invocation. All buffers are device buffers of the backend's device; every call enqueues its kernels on `stream`,
+ * allocates nothing and returns without synchronising, so calls can be captured into CUDA graphs. What the kernels find
+ * wrong in device data (a page outside the cache, lengths outside the table, an index twice) they leave out, never reading
+ * or writing outside the given buffers, and the next wb200_backend_poll() returns WB200_ERR_INVALID_ARGUMENT. */
+
+/* Rotary positions: for a token at position p and pair i < rotary_dim / 2 of a head,
+ *   (y_a, y_b) = magnitude * (x_a cos t - x_b sin t, x_b cos t + x_a sin t),   t = 2 pi p turns_i
+ * with (a, b) = (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; elements from rotary_dim on are copied.
+ * `turns[i]` is the part of a full turn per position in units of 2^-64 turns. The product with the position wraps at whole
+ * turns in 64-bit integers, so the angle is right to 2^-65 turns per position at any position. Arithmetic in f32, one
+ * rounding to the storage format. */
+typedef struct wb200_rope_table {
+  uint32_t rotary_dim;      /* even, at most 512 and the head dimension; 0 rotates nothing */
+  float magnitude;          /* scale of the rotated elements */
+  const uint64_t *turns;    /* host array of rotary_dim / 2, read during the call */
+} wb200_rope_table;
+typedef struct wb200_rope_params {
+  uint32_t tokens, heads, head_dim;
+  uint8_t format;           /* WB200_BF16, WB200_F16 or WB200_F32 */
+  uint8_t interleaved;
+  uint8_t backward;         /* the transposed map: x is the gradient of y and out the gradient of x */
+  uint8_t position_bytes;   /* 4 or 8: positions are int32 or int64 */
+  wb200_rope_table table;
+  const void *positions;    /* [tokens] */
+  const void *x;            /* element (token, head, d) at token * x_token_stride + head * x_head_stride + d */
+  void *out;                /* likewise; may be x with the same strides, else must not overlap it */
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  void *stream;
+} wb200_rope_params;
+wb200_status wb200_rope(wb200_backend *backend, const wb200_rope_params *params);
+
+/* K row (page, r, head) begins at page * k_page_stride + r * k_row_stride + head * k_head_stride (in elements), V likewise:
+ * any order of rows and heads inside a page, K and V apart or side by side. No two rows may overlap. */
+typedef struct wb200_paged_cache {
+  uint32_t pages, page_size, kv_heads, head_dim;
+  uint32_t format;          /* WB200_BF16 or WB200_F16 (wb200_pages_copy: WB200_F32 too) */
+  uint32_t reserved;
+  void *k, *v;
+  int64_t k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride;
+} wb200_paged_cache;
+/* The new tokens of all sequences lie one behind the other: sequence s has tokens query_starts[s] .. query_starts[s + 1] - 1.
+ * key_lengths[s] counts its keys, the new tokens' among them, so that its new token i stands at position
+ * key_lengths[s] - (query_starts[s + 1] - query_starts[s]) + i. Key j lies in row j % page_size of page
+ * page_table[s * table_stride + j / page_size]. Tokens from query_starts[sequences] on belong to no sequence: nothing is
+ * read or written for them. */
+typedef struct wb200_paged_batch {
+  uint32_t sequences, table_width, tokens;
+  uint32_t max_query;       /* most new tokens of one sequence, as far as the caller knows (0: unknown). It chooses between
+                               kernels; results do not depend on it being right */
+  const int32_t *page_table, *key_lengths, *query_starts;
+  int64_t table_stride;
+} wb200_paged_batch;
+
+/* Rows [q heads | k heads | v heads] of the fused projection: Q is rotated and stored token-major, K is rotated and V
+ * copied into the cache rows of their tokens. `positions` replaces the cache positions in the rotation (null: those). The
+ * cache has to hold the rows' pages already (wb200_pages_reserve). */
+typedef struct wb200_rope_append_params {
+  uint32_t q_heads;
+  uint8_t interleaved, position_bytes, reserved[2];
+  wb200_rope_table table;
+  const void *positions;    /* [tokens] or null */
+  const void *qkv;          /* row of token t at t * qkv_token_stride elements */
+  void *q;                  /* [tokens, q_heads, head_dim] at q_token_stride, q_head_stride; cache's format */
+  int64_t qkv_token_stride, q_token_stride, q_head_stride;
+  void *stream;
+} wb200_rope_append_params;
+wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
+                               const wb200_rope_append_params *params);
+
+/* Attention of every sequence's new tokens over its paged keys, grouped queries (q_heads % kv_heads == 0):
+ *   s_j = scale q.k_j,   out = sum_j exp(s_j - lse) v_j,   lse = ln sum_j exp(s_j)
+ * over the keys j < key_lengths[s], with `causal` those up to the token's own position. Statistics and sums are kept in
+ * f32; probabilities may be rounded to the storage format in front of the product with V. A row without keys is NaN (0 with
+ * zero_fully_masked) and its lse -inf. Cache rows behind key_lengths[s] may hold anything; a NaN or infinite V element of a
+ * key inside the length reaches the rows that do not see the key too, as 0 * v does.
+ * head_dim is a multiple of 8 up to 256. `workspace` needs wb200_attention_paged_workspace_bytes() bytes, 256-byte
+ * aligned, of any content; calls that may run at the same time need one each. */
+typedef struct wb200_attention_paged_params {
+  uint32_t q_heads;
+  uint8_t causal, zero_fully_masked, reserved[2];
+  float scale;              /* > 0 */
+  uint32_t reserved2;
+  const void *q;            /* [tokens, q_heads, head_dim] at q_token_stride, q_head_stride; cache's format */
+  void *out;                /* likewise */
+  float *lse;               /* [tokens, q_heads] or null */
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  void *workspace;
+  uint64_t workspace_bytes;
+  void *stream;
+} wb200_attention_paged_params;
+uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, const wb200_paged_cache *cache,
+                                               const wb200_paged_batch *batch, const wb200_attention_paged_params *params);
+wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
+                                   const wb200_attention_paged_params *params);
+
+/* The pages of a cache are kept in three arrays: page table, tokens held by each sequence, and how many sequences hold each
+ * page (0: free). The four calls below take them and write them to the *_out arrays, each of which may be the input itself;
+ * table entries behind a sequence's pages keep their value unless said otherwise. Every result is one the order of threads
+ * has no part in: pages are taken lowest index first, sequence by sequence. The keys themselves are moved by
+ * wb200_pages_copy with the page numbers that fork and compact return, once per layer or for many layers in one call. */
+typedef struct wb200_page_tables {
+  uint32_t sequences, table_width, pages, page_size;   /* at most 32768 sequences */
+  const int32_t *table, *lengths, *refs;               /* [sequences, table_width] at table_stride, [sequences], [pages] */
+  int32_t *table_out, *lengths_out, *refs_out;         /* table_out at table_out_stride */
+  int64_t table_stride, table_out_stride;
+  void *stream;
+} wb200_page_tables;
+/* Room for wanted[s] tokens in sequence s (nothing to do where it holds as many). *result: 0 done; n > 0: n pages too few;
+ * -1: a sequence would outgrow the table, or its length says it has. Unless 0, the arrays come out as they went in. */
+wb200_status wb200_pages_reserve(wb200_backend *backend, const wb200_page_tables *tables, const int32_t *wanted, int32_t *result);
+/* Sequence children[i], which holds nothing, becomes a copy of parents[i]: full pages are shared, a last page that is not
+ * full gets a page of its own, to which the caller copies its rows: sources[i] -> destinations[i] (-1, -1 where there is
+ * none); the child's table entries behind its pages become -1. *result: 0 done; n > 0: n pages too few; -1: an index or
+ * length out of range, a child that holds tokens, is named twice or is a parent too. Unless 0, the arrays come out as they went in, the lists -1. */
+wb200_status wb200_pages_fork(wb200_backend *backend, const wb200_page_tables *tables, uint32_t count, const int32_t *parents,
+                              const int32_t *children, int32_t *sources, int32_t *destinations, int32_t *result);
+/* The listed sequences give their pages back and hold nothing: length 0, the table entries of those that held something -1.
+ * A page is free once no sequence holds it. Negative indices are passed over, a sequence named twice is freed once. */
+wb200_status wb200_pages_free(wb200_backend *backend, const wb200_page_tables *tables, uint32_t count, const int32_t *sequences);
+/* Moves the pages in use to the front of the cache: the i-th used page behind the first n (n: pages in use) to the i-th free
+ * one among them. sources and destinations, pages / 2 entries each, list the moves, -1 behind the last. lengths_out may be
+ * null: lengths do not change. */
+wb200_status wb200_pages_compact(wb200_backend *backend, const wb200_page_tables *tables, int32_t *sources, int32_t *destinations);
+/* Whole pages of K and V, sources[i] -> destinations[i], in each of `caches` (same extents, strides and format). Entries with
+ * a negative number are passed over. No page may be a destination twice, or a source and a destination: its content would be
+ * undefined. */
+wb200_status wb200_pages_copy(wb200_backend *backend, const wb200_paged_cache *caches, uint32_t cache_count, uint32_t count,
+                              const int32_t *sources, const int32_t *destinations, void *stream);
+
 /* Sum over the shards of a tensor-parallel region (the `allreduce` of wb200_decoder_layer, or any buffer) as one kernel
  * per GPU that lets the NVSwitch add and broadcast: the reference's Tile collectives realise such a sum as reduce-scatter
  * followed by all-gather over the dies (lib/Wafer/Transforms/Tile/DistributedCollectiveMovement.cpp:675-735); here rank
@@ -497,7 +629,8 @@ uint64_t wb200_switch_sum_signal_bytes(uint32_t world);
 wb200_status wb200_switch_sum(wb200_backend *backend, const wb200_switch_sum_params *params);
 
 /* Reads and clears the device status word of asynchronous (WB200_MEM_DEVICE) calls after
- * synchronising `stream`. Returns WB200_ERR_DEVICE_TIMEOUT if a kernel gave up a bounded wait. */
+ * synchronising `stream`. Returns WB200_ERR_DEVICE_TIMEOUT if a kernel gave up a bounded wait, WB200_ERR_INVALID_ARGUMENT if
+ * one of the paged-cache kernels found device data it had to leave out. */
 wb200_status wb200_backend_poll(wb200_backend *backend, void *stream);
 
 /* Self-test of the bounded device-side waits: launches a kernel that waits, for at most `cycle_limit` SM clocks, on a

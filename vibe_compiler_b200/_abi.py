@@ -138,6 +138,50 @@ class FdExchange(C.Structure):
     _fields_ = [("rank", C.c_uint32), ("world", C.c_uint32), ("peer_buffers", C.c_void_p * 16), ("epoch", C.c_void_p)]
 
 
+class RopeTable(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint32), ("magnitude", C.c_float), ("turns", C.c_void_p)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("format", C.c_uint8), ("interleaved", C.c_uint8), ("backward", C.c_uint8), ("position_bytes", C.c_uint8),
+                ("table", RopeTable), ("positions", C.c_void_p), ("x", C.c_void_p), ("out", C.c_void_p),
+                ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("stream", C.c_void_p)]
+
+
+class PagedCacheDesc(C.Structure):
+    _fields_ = [("pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("format", C.c_uint32), ("reserved", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_page_stride", C.c_int64), ("k_row_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64)]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [("sequences", C.c_uint32), ("table_width", C.c_uint32), ("tokens", C.c_uint32), ("max_query", C.c_uint32),
+                ("page_table", C.c_void_p), ("key_lengths", C.c_void_p), ("query_starts", C.c_void_p), ("table_stride", C.c_int64)]
+
+
+class RopeAppendParams(C.Structure):
+    _fields_ = [("q_heads", C.c_uint32), ("interleaved", C.c_uint8), ("position_bytes", C.c_uint8), ("reserved", C.c_uint8 * 2),
+                ("table", RopeTable), ("positions", C.c_void_p), ("qkv", C.c_void_p), ("q", C.c_void_p),
+                ("qkv_token_stride", C.c_int64), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("stream", C.c_void_p)]
+
+
+class AttentionPagedParams(C.Structure):
+    _fields_ = [("q_heads", C.c_uint32), ("causal", C.c_uint8), ("zero_fully_masked", C.c_uint8), ("reserved", C.c_uint8 * 2),
+                ("scale", C.c_float), ("reserved2", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("stream", C.c_void_p)]
+
+
+class PageTablesDesc(C.Structure):
+    _fields_ = [("sequences", C.c_uint32), ("table_width", C.c_uint32), ("pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("table", C.c_void_p), ("lengths", C.c_void_p), ("refs", C.c_void_p),
+                ("table_out", C.c_void_p), ("lengths_out", C.c_void_p), ("refs_out", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_out_stride", C.c_int64), ("stream", C.c_void_p)]
+
+
 class ProgramStats(C.Structure):
     _fields_ = [("instructions", C.c_uint64), ("commands", C.c_uint64), ("gemm_commands", C.c_uint64), ("movement_commands", C.c_uint64),
                 ("fill_commands", C.c_uint64), ("transfer_commands", C.c_uint64), ("sync_commands", C.c_uint64),
@@ -199,6 +243,15 @@ SIGNATURES = {
     "wb200_decoder_layer_workspace_bytes": (C.c_uint64, [C.POINTER(DecoderLayerParams)]),
     "wb200_decoder_layer": (C.c_int, [C.c_void_p, C.POINTER(DecoderLayerParams)]),
     "wb200_decoder_layer_timeline": (C.c_int, [C.c_void_p, C.POINTER(C.c_float), C.c_uint32, C.POINTER(C.c_uint32)]),
+    "wb200_rope": (C.c_int, [C.c_void_p, C.POINTER(RopeParams)]),
+    "wb200_rope_append": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(RopeAppendParams)]),
+    "wb200_attention_paged_workspace_bytes": (C.c_uint64, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
+    "wb200_attention_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
+    "wb200_pages_reserve": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_void_p, C.c_void_p]),
+    "wb200_pages_fork": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_uint32] + [C.c_void_p] * 5),
+    "wb200_pages_free": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_uint32, C.c_void_p]),
+    "wb200_pages_compact": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_void_p, C.c_void_p]),
+    "wb200_pages_copy": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "wb200_target_call_rdma": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _U32x3, _U32x3]),
     "wb200_target_call_wdma": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _U32x3, _U32x3]),
     "wb200_target_call_gather_scatter": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _U32x3, _U32x3, _U32x3, _U32x3]),

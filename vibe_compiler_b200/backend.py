@@ -37,7 +37,13 @@ FORMAT_BYTES = {abi.F16: 2, abi.BF16: 2, abi.F32: 4}
 # time on the device than one assignment per ctypes field takes here (attention_fd 13 us of Python per call, now 3).
 _ATTENTION_PACK = struct.Struct("=6I4Bf3q8Q2I").pack
 _GEMM_PACK = struct.Struct("=3I6B6x5Q").pack
+_ROPE_PACK = struct.Struct("=3I4BIfQ3Q4qQ").pack
+_APPEND_PACK = struct.Struct("=IBBxxIfQ3Q3qQ").pack
+_PAGED_PACK = struct.Struct("=IBBxxfI3Q4q3Q").pack
+_TABLES_PACK = struct.Struct("=4I6Q2qQ").pack
 assert len(_ATTENTION_PACK(*[0] * 24)) == C.sizeof(abi.AttentionParams) and len(_GEMM_PACK(*[0] * 14)) == C.sizeof(abi.GemmEpilogueParams)
+assert len(_ROPE_PACK(*[0] * 18)) == C.sizeof(abi.RopeParams) and len(_APPEND_PACK(*[0] * 13)) == C.sizeof(abi.RopeAppendParams)
+assert len(_PAGED_PACK(*[0] * 15)) == C.sizeof(abi.AttentionPagedParams) and len(_TABLES_PACK(*[0] * 13)) == C.sizeof(abi.PageTablesDesc)
 
 
 def _current_stream() -> int:
@@ -534,6 +540,203 @@ class B200TargetModelBackend:
         self._check(self._lib.wb200_residual_add(self._handle, _TORCH_FORMATS[a.dtype], a.data_ptr(), b.data_ptr(), out.data_ptr(),
                                                  a.numel(), stream))
         return out
+
+    # ------------------------------------------------------------------ serving from a paged KV cache (CUDA tensors)
+    def _stream_of(self, stream: Optional[int]) -> int:
+        """The stream a paged call runs on: the given one, or the current one of the backend's device."""
+        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else stream
+
+    def _empty(self, shape, dtype, stream: int):
+        """Memory of the backend's device that belongs to `stream`: what the call writes there is ordered behind what the
+        memory's last holder did, also when `stream` is not the current one."""
+        device = torch.device("cuda", self.device)
+        if stream == torch._C._cuda_getCurrentRawStream(self.device):
+            return torch.empty(shape, dtype=dtype, device=device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)):
+            return torch.empty(shape, dtype=dtype, device=device)
+
+    def _rows(self, name: str, t, heads: Optional[int] = None, head_dim: Optional[int] = None, tokens: Optional[int] = None, dtype=None):
+        """Checks a [tokens, heads, head_dim] tensor of this device."""
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous rows")
+        if (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim) or \
+                (tokens is not None and t.shape[0] != tokens) or (dtype is not None and t.dtype != dtype):
+            raise ValueError(f"{name} does not match the shape or type of the other tensors")
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{name} must be on the backend's device")
+
+    def _positions(self, positions, tokens: int):
+        if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int32 or int64 tensor with one entry per token")
+        if positions.device.type != "cuda" or positions.device.index != self.device:
+            raise ValueError("positions must be on the backend's device")
+
+    def rope(self, x, positions, table, *, interleaved: bool = False, backward: bool = False, out=None, stream: Optional[int] = None):
+        """Rotary positions on rows x [tokens, heads, head_dim] (bf16 / f16 / f32, any token and head strides), token t at
+        positions[t]: pairs (i, i + R/2) of the first R = table.rotary_dim elements, or (2i, 2i + 1) when `interleaved`, the
+        rest copied. `table`: a paged_cache.RotaryTable. `backward` applies the transposed map: x is the gradient of the
+        rotated rows, the result the gradient of the rows. `out` may be x."""
+        self._rows("x", x)
+        if x.dtype not in _TORCH_FORMATS:
+            raise ValueError("x must be bfloat16, float16 or float32")
+        tokens, heads, head_dim = x.shape
+        self._positions(positions, tokens)
+        stream = self._stream_of(stream)
+        if out is None:
+            out = self._empty((tokens, heads, head_dim), x.dtype, stream)
+        else:
+            self._rows("out", out, heads, head_dim, tokens, x.dtype)
+        p = abi.RopeParams.from_buffer_copy(_ROPE_PACK(
+            tokens, heads, head_dim, _TORCH_FORMATS[x.dtype], bool(interleaved), bool(backward), positions.element_size(),
+            table.rotary_dim, table.magnitude, table._address, positions.data_ptr(), x.data_ptr(), out.data_ptr(),
+            x.stride(0), x.stride(1), out.stride(0), out.stride(1), stream))
+        self._check(self._lib.wb200_rope(self._handle, C.byref(p)))
+        return out
+
+    def _paged(self, cache, batch):
+        if cache.device_index != self.device or batch.device_index != self.device:
+            raise ValueError("the cache and the batch must be on the backend's device")
+
+    def rope_append(self, qkv, cache, batch, table, *, q_heads: int, interleaved: bool = False, positions=None, out=None,
+                    stream: Optional[int] = None):
+        """Rows [q heads | k heads | v heads] of the fused projection, qkv [tokens, (q_heads + 2 kv_heads) head_dim]: returns
+        the rotated queries [tokens, q_heads, head_dim] and stores the rotated K and the V rows to their sequences' pages of
+        `cache` (a paged_cache.PagedCache). `batch`: a paged_cache.PagedBatch whose pages are reserved. `table` None rotates
+        nothing. `positions` replace the cache positions in the rotation. Rows of tokens that belong to no sequence are not
+        written."""
+        self._paged(cache, batch)
+        kv_heads, head_dim, dtype = cache.k.shape[2], cache.k.shape[3], cache.k.dtype
+        if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.dtype != dtype or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+            raise ValueError("qkv must be [tokens, (q_heads + 2 kv_heads) head_dim] of the cache's type with contiguous rows")
+        if qkv.device.type != "cuda" or qkv.device.index != self.device:
+            raise ValueError("qkv must be on the backend's device")
+        tokens = qkv.shape[0]
+        if positions is not None:
+            self._positions(positions, tokens)
+        stream = self._stream_of(stream)
+        if out is None:
+            out = self._empty((tokens, q_heads, head_dim), dtype, stream)
+        else:
+            self._rows("out", out, q_heads, head_dim, tokens, dtype)
+        p = abi.RopeAppendParams.from_buffer_copy(_APPEND_PACK(
+            q_heads, bool(interleaved), positions.element_size() if positions is not None else 4,
+            table.rotary_dim if table is not None else 0, table.magnitude if table is not None else 1.0,
+            table._address if table is not None else 0, positions.data_ptr() if positions is not None else 0, qkv.data_ptr(), out.data_ptr(),
+            qkv.stride(0), out.stride(0), out.stride(1), stream))
+        self._check(self._lib.wb200_rope_append(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
+        return out
+
+    def attention_paged(self, q, cache, batch, scale: float, *, causal: bool = True, zero_fully_masked: bool = False, out=None,
+                        lse=None, stream: Optional[int] = None):
+        """Attention of every sequence's new tokens, q [tokens, q_heads, head_dim], over its keys in the pages of `cache`
+        (grouped queries; with `causal` up to the token's own position). `lse` [tokens, q_heads] f32 receives the
+        log-sum-exp. Rows of tokens that belong to no sequence are not written. Scratch memory comes from torch's allocator,
+        per call and stream, so calls may overlap and be captured into CUDA graphs."""
+        self._paged(cache, batch)
+        self._rows("q", q, head_dim=cache.k.shape[3], dtype=cache.k.dtype)
+        tokens, q_heads, head_dim = q.shape
+        stream = self._stream_of(stream)
+        if out is None:
+            out = self._empty((tokens, q_heads, head_dim), q.dtype, stream)
+        else:
+            self._rows("out", out, q_heads, head_dim, tokens, q.dtype)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous() or lse.device != q.device):
+            raise ValueError("lse must be a contiguous float32 [tokens, q_heads] tensor on the same device")
+        desc = batch._desc(tokens)
+        fields = (q_heads, bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
+                  lse.data_ptr() if lse is not None else 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1))
+        p = abi.AttentionPagedParams.from_buffer_copy(_PAGED_PACK(*fields, 0, 0, stream))
+        needed = self._lib.wb200_attention_paged_workspace_bytes(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p))
+        workspace = self._empty(needed, torch.uint8, stream)
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), needed
+        self._check(self._lib.wb200_attention_paged(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
+        return out
+
+    def _tables(self, table, lengths, refs, page_size, out, stream, with_lengths=True):
+        """Checks the page arrays and makes the outputs; returns the C form and the outputs."""
+        for name, t, dims in (("table", table, 2), ("lengths", lengths, 1), ("refs", refs, 1)):
+            if t.dtype != torch.int32 or t.dim() != dims or t.device.type != "cuda" or t.device.index != self.device:
+                raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s) on the backend's device")
+            if t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"rows of {name} must be contiguous")
+        if lengths.shape[0] != table.shape[0]:
+            raise ValueError("table and lengths must describe the same sequences")
+        inputs = (table, lengths, refs) if with_lengths else (table, refs)
+        if out is None:
+            out = tuple(self._empty(t.shape, torch.int32, stream) for t in inputs)
+        else:
+            out = tuple(out)
+            if len(out) != len(inputs) or any(o.shape != t.shape or o.dtype != torch.int32 or o.device != t.device or
+                                              (o.shape[-1] > 1 and o.stride(-1) != 1) for o, t in zip(out, inputs)):
+                raise ValueError("out must be tensors like the page arrays")
+        desc = abi.PageTablesDesc.from_buffer_copy(_TABLES_PACK(
+            table.shape[0], table.shape[1], refs.shape[0], page_size, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+            out[0].data_ptr(), out[1].data_ptr() if with_lengths else 0, out[-1].data_ptr(), table.stride(0), out[0].stride(0), stream))
+        return desc, out
+
+    def _indices(self, name, t, count=None):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.device or \
+                (count is not None and t.shape[0] != count):
+            raise ValueError(f"{name} must be a contiguous int32 vector of matching length on the backend's device")
+
+    def pages_reserve(self, table, lengths, refs, wanted, page_size: int, *, out=None, stream: Optional[int] = None):
+        """Room for wanted[s] tokens in every sequence: (table, lengths, refs, result). `table` [sequences, width] lists the
+        sequences' pages, `lengths` their tokens, `refs` [pages] how many sequences hold a page; all int32. New pages are the
+        free ones of lowest index, sequence by sequence. result[0]: 0 done, n > 0 pages too few, -1 a sequence outgrows the
+        table; unless 0, the arrays come out as they went in. `out`: (table, lengths, refs) to write, may be the inputs."""
+        stream = self._stream_of(stream)
+        self._indices("wanted", wanted, table.shape[0])
+        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
+        result = self._empty(1, torch.int32, stream)
+        self._check(self._lib.wb200_pages_reserve(self._handle, C.byref(desc), wanted.data_ptr(), result.data_ptr()))
+        return (*out, result)
+
+    def pages_fork(self, table, lengths, refs, parents, children, page_size: int, *, out=None, stream: Optional[int] = None):
+        """children[i], empty so far, becomes a copy of parents[i]: (table, lengths, refs, sources, destinations, result). Full
+        pages are shared; a last page that is not full gets a page of its own, whose rows `pages_copy(caches, sources,
+        destinations)` copies (-1 where there is none). result[0]: 0 done, n > 0 pages too few, -1 indices that cannot be
+        forked; unless 0, the arrays come out as they went in."""
+        stream = self._stream_of(stream)
+        self._indices("parents", parents)
+        self._indices("children", children, parents.shape[0])
+        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
+        count = parents.shape[0]
+        lists = self._empty(2 * count + 1, torch.int32, stream)
+        sources, destinations, result = lists[:count], lists[count:2 * count], lists[2 * count:]
+        self._check(self._lib.wb200_pages_fork(self._handle, C.byref(desc), count, parents.data_ptr(), children.data_ptr(), sources.data_ptr(),
+                                               destinations.data_ptr(), result.data_ptr()))
+        return (*out, sources, destinations, result)
+
+    def pages_free(self, table, lengths, refs, sequences, page_size: int, *, out=None, stream: Optional[int] = None):
+        """The listed sequences give their pages back: (table, lengths, refs). Negative entries are passed over."""
+        stream = self._stream_of(stream)
+        self._indices("sequences", sequences)
+        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
+        self._check(self._lib.wb200_pages_free(self._handle, C.byref(desc), sequences.shape[0], sequences.data_ptr()))
+        return out
+
+    def pages_compact(self, table, lengths, refs, page_size: int, *, out=None, stream: Optional[int] = None):
+        """The pages in use to the front of the cache: (table, refs, sources, destinations), the moves for `pages_copy` with
+        -1 behind the last. `out`: (table, refs)."""
+        stream = self._stream_of(stream)
+        desc, out = self._tables(table, lengths, refs, page_size, out, stream, with_lengths=False)
+        moves = self._empty((2, refs.shape[0] // 2), torch.int32, stream)
+        sources, destinations = moves[0], moves[1]
+        self._check(self._lib.wb200_pages_compact(self._handle, C.byref(desc), sources.data_ptr(), destinations.data_ptr()))
+        return (*out, sources, destinations)
+
+    def pages_copy(self, caches, sources, destinations, *, stream: Optional[int] = None) -> None:
+        """Whole pages of every cache (a PagedCache or a sequence of them with one shape, strides and type): K and V of page
+        sources[i] to page destinations[i]; negative entries are passed over. No page may be a destination twice, or both a
+        source and a destination."""
+        caches = (caches,) if hasattr(caches, "_desc") else caches
+        stream = self._stream_of(stream)
+        self._indices("sources", sources)
+        self._indices("destinations", destinations, sources.shape[0])
+        if any(c.device_index != self.device for c in caches):
+            raise ValueError("the caches must be on the backend's device")
+        descs = (abi.PagedCacheDesc * len(caches))(*[c._desc for c in caches])
+        self._check(self._lib.wb200_pages_copy(self._handle, descs, len(caches), sources.shape[0], sources.data_ptr(), destinations.data_ptr(), stream))
 
     def decoder_layer(self, x, *, norm1, wqkv, wo, norm2, wgu, wdown, q_heads: int, kv_heads: int, head_dim: int, eps: float,
                       rope_theta: float, position_offset: int = 0, allreduce=None, workspace=None, out=None,

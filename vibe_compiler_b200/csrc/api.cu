@@ -30,9 +30,9 @@ wb200_status wb200_backend_create(int device, wb200_backend **out) {
   backend->sm_count = prop.multiProcessorCount;
   snprintf(backend->digest, sizeof(backend->digest), "b200:%s:sm_%d%d:abi%d", prop.name, prop.major, prop.minor, WB200_ABI_VERSION);
   cudaError_t err = cudaStreamCreateWithFlags(&backend->stream, cudaStreamNonBlocking);
-  if (err == cudaSuccess) err = cudaHostAlloc(reinterpret_cast<void **>(&backend->h_status), 2 * sizeof(int), cudaHostAllocMapped);
+  if (err == cudaSuccess) err = cudaHostAlloc(reinterpret_cast<void **>(&backend->h_status), 3 * sizeof(int), cudaHostAllocMapped);
   if (err == cudaSuccess) err = cudaHostGetDevicePointer(reinterpret_cast<void **>(&backend->d_status), backend->h_status, 0);
-  if (err == cudaSuccess) backend->h_status[0] = backend->h_status[1] = 0;
+  if (err == cudaSuccess) backend->h_status[0] = backend->h_status[1] = backend->h_status[2] = 0;
   if (err != cudaSuccess) {
     delete backend;
     return fail(WB200_ERR_CUDA, std::string("backend setup: ") + cudaGetErrorString(err));
@@ -73,7 +73,11 @@ uint64_t wb200_backend_launch_count(const wb200_backend *backend) { return backe
 wb200_status wb200_backend_poll(wb200_backend *backend, void *stream) {
   if (!backend) return fail(WB200_ERR_INVALID_ARGUMENT, "backend is null");
   DeviceGuard guard(backend->device);
-  return read_device_status(backend, static_cast<cudaStream_t>(stream), nullptr);
+  const wb200_status st = read_device_status(backend, static_cast<cudaStream_t>(stream), nullptr);
+  volatile int *refused = backend->h_status + 2;
+  const int code = *refused;
+  if (code != 0) *refused = 0;
+  return st != WB200_OK || code == 0 ? st : fail(WB200_ERR_INVALID_ARGUMENT, refused_data_message(code));
 }
 
 wb200_status wb200_physical_geometry(const wb200_tensor_desc *desc, wb200_geometry *out) {

@@ -1,0 +1,30 @@
+// What the paged attention kernels share: a sequence of the batch as the device arrays describe it, and where its keys lie.
+#pragma once
+
+#include "kernels.h"
+#include "ptx_sm100.cuh"
+
+namespace wb200 {
+
+// Sequence s of a batch: its new tokens [begin, begin + count) and its keys. What does not fit the buffers leaves it empty and
+// is reported (by one thread: `report`).
+struct PagedSequence {
+  int begin, count, keys;
+};
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatchArgs &b, const PagedCacheArgs &c, int s, int *refused, bool report) {
+  const int begin = b.query_starts[s], end = b.query_starts[s + 1], keys = b.key_lengths[s];
+  if (end <= begin) return {begin, 0, 0};
+  if (begin < 0 || end > b.tokens || keys < 0 || keys > static_cast<long long>(b.table_width) * c.page_size) {
+    if (report) raise_status(refused, kRefusedLength);
+    return {0, 0, 0};
+  }
+  return {begin, end - begin, keys};
+}
+// Keys that new token `index` of a sequence sees: key j with j <= keys - count + index under the causal mask.
+__device__ __forceinline__ int paged_visible(const PagedSequence &s, int index, int causal) {
+  if (!causal) return s.keys;
+  const int last = s.keys - s.count + index + 1;
+  return last < 0 ? 0 : last;
+}
+
+}  // namespace wb200

@@ -17,7 +17,7 @@ struct wb200_backend {
   int device = 0;
   int sm_count = 0;
   cudaStream_t stream = nullptr;  // used by WB200_MEM_HOST calls
-  // [0] bounded-wait status, [1] NaN flag: pinned host memory the kernels store to when something is wrong, so that reading
+  // [0] bounded-wait status, [1] NaN flag, [2] RefusedData of the paged-cache kernels: pinned host memory the kernels store to when something is wrong, so that reading
   // it takes no copy (d_status: its device address).
   int *h_status = nullptr, *d_status = nullptr;
   // Pinned, device-mapped staging area of the command calls (command_io.h), grown on demand up to kMaxStageBytes. Behind its

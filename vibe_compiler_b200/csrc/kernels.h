@@ -279,6 +279,76 @@ wb200_status launch_rope_split(int format, const void *qkv, void *q, void *k, vo
                                int kv_heads, int head_dim, float theta, int position_offset, cudaStream_t stream, bool beside = false);
 wb200_status launch_residual_add(int format, const void *a, const void *b, void *out, size_t elements, cudaStream_t stream, bool beside = false);
 
+// ---- paged KV cache (rotary.cu, attention_paged*.cu, cache_pages.cu); device pointers
+// What a kernel found wrong in device data and left out; stored to the backend's third status word.
+enum RefusedData : int {
+  kRefusedPage = 1,       // a page number outside the cache
+  kRefusedLength = 2,     // a length, token range or position outside the table or the buffers
+  kRefusedSequence = 3,   // a sequence index outside the table
+  kRefusedReference = 4,  // a page freed more often than it is held
+};
+const char *refused_data_message(int code);
+
+constexpr int kMaxRotaryPairs = 256;
+struct RotaryConstants {
+  int pairs;                            // rotated pairs per head
+  float magnitude;
+  unsigned long long turns[kMaxRotaryPairs];   // units of 2^-64 turns per position
+};
+struct PagedCacheArgs {
+  int pages, page_size, kv_heads, head_dim, format;
+  void *k, *v;
+  int64_t k_page, k_row, k_head, v_page, v_row, v_head;   // strides in elements
+};
+struct PagedBatchArgs {
+  int sequences, table_width, tokens, max_query;
+  const int *page_table, *key_lengths, *query_starts;
+  int64_t table_stride;
+};
+struct RopeArgs {
+  int tokens, heads, head_dim, format;
+  int interleaved, backward, position_bytes;
+  const void *positions, *x;
+  void *out;
+  int64_t x_token, x_head, out_token, out_head;
+};
+wb200_status launch_rope(const RopeArgs &args, const RotaryConstants &constants, cudaStream_t stream);
+// args: x the fused rows (heads = q_heads + 2 kv_heads, x_head = head_dim), out the rotated q heads.
+wb200_status launch_rope_append(const RopeArgs &args, const RotaryConstants &constants, const PagedCacheArgs &cache, const PagedBatchArgs &batch,
+                                int *refused, cudaStream_t stream);
+
+struct AttentionPagedArgs {
+  PagedCacheArgs cache;
+  PagedBatchArgs batch;
+  int q_heads, causal, zero_fully_masked;
+  float scale;
+  const void *q;
+  void *out;
+  float *lse;
+  int64_t q_token, q_head, out_token, out_head;
+  void *workspace;
+  int *refused;       // RefusedData
+  int *status;        // bounded waits
+};
+wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cudaStream_t stream);
+
+struct PageTablesArgs {
+  int sequences, table_width, pages, page_size;
+  const int *table, *lengths, *refs;
+  int *table_out, *lengths_out, *refs_out;
+  int64_t table_stride, table_out_stride;
+  int *refused;
+};
+constexpr int kMaxPagedSequences = 32768;
+wb200_status launch_pages_reserve(const PageTablesArgs &args, const int *wanted, int *result, cudaStream_t stream);
+wb200_status launch_pages_fork(const PageTablesArgs &args, int count, const int *parents, const int *children, int *sources, int *destinations,
+                               int *result, cudaStream_t stream);
+wb200_status launch_pages_free(const PageTablesArgs &args, int count, const int *sequences, cudaStream_t stream);
+wb200_status launch_pages_compact(const PageTablesArgs &args, int *sources, int *destinations, cudaStream_t stream);
+constexpr int kMaxCachesPerCopy = 64;
+wb200_status launch_pages_copy(const PagedCacheArgs *caches, int cache_count, int count, const int *sources, const int *destinations, int *refused,
+                               cudaStream_t stream);
+
 // ---- movement commands on device-resident memory images (tile_movement.cu)
 struct StridedLayout {
   uint32_t inner_bytes;

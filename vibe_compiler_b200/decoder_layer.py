@@ -119,6 +119,24 @@ class ShardedDecoderLayer:
         return self.backend.residual_add(x1, partial2).reshape(batch, seq, d)
 
 
+    def forward_paged(self, x: torch.Tensor, cache, batch, rotary=None) -> torch.Tensor:
+        """One serving step of this layer: x [tokens, d_model] holds the new tokens of the sequences of `batch`
+        (paged_cache.PagedBatch), whose earlier keys lie in `cache` (paged_cache.PagedCache of this rank's KV heads). The
+        step's K and V rows are written to their pages, which have to be reserved. `rotary` (paged_cache.RotaryTable):
+        default the configuration's theta over the whole head. Rows of tokens that belong to no sequence are undefined."""
+        be, cfg = self.backend, self.cfg
+        if rotary is None:
+            if not hasattr(self, "_rotary"):
+                from .paged_cache import RotaryTable
+                self._rotary = RotaryTable(cfg.head_dim, theta=cfg.rope_theta)
+            rotary = self._rotary
+        qkv = be.gemm_epilogue(be.rmsnorm(x, self.norm1, cfg.eps), self.wqkv)
+        q = be.rope_append(qkv, cache, batch, rotary, q_heads=self.hq)
+        attn = be.attention_paged(q, cache, batch, cfg.head_dim ** -0.5)
+        partial = self._all_reduce(be.gemm_epilogue(attn.view(x.shape[0], self.hq * cfg.head_dim), self.wo))   # sum over head shards
+        x1 = be.residual_add(x, partial)
+        return be.residual_add(x1, self._all_reduce(self.ffn_partial(x1)))                                    # sum over FFN shards
+
     def default_micro_batches(self, batch: int) -> int:
         """Parts the batch is cut into so that the sums of one part travel while the next computes. More parts hide more of
         the communication but shrink the per-part GEMMs, which costs more the narrower the shard (measured on 8 GPUs: the
