@@ -248,6 +248,7 @@ def test_a_serving_run(backend):
     outputs[1] = finished
     for s, parts in outputs.items():
         got = torch.cat(parts)
-        whole = layer.forward(texts[s][None, :got.shape[0]])[0]
+        text = torch.nn.functional.pad(texts[s][:len(got)], (0, 0, 0, -len(got) % 8))       # the layer takes rows by eights
+        whole = layer.forward(text[None])[0, :len(got)]
         # both round every stage to bf16 on the way; the suite's bound for the layer
         assert (got.double() - whole.double()).abs().max().item() <= 1e-2 * whole.double().abs().max().item()

@@ -130,12 +130,15 @@ class ShardedDecoderLayer:
                 from .paged_cache import RotaryTable
                 self._rotary = RotaryTable(cfg.head_dim, theta=cfg.rope_theta)
             rotary = self._rotary
+        tokens = x.shape[0]
+        if tokens % 8:                         # the GEMMs take rows by eights; the rows behind belong to no sequence
+            x = torch.nn.functional.pad(x, (0, 0, 0, 8 - tokens % 8))
         qkv = be.gemm_epilogue(be.rmsnorm(x, self.norm1, cfg.eps), self.wqkv)
         q = be.rope_append(qkv, cache, batch, rotary, q_heads=self.hq)
         attn = be.attention_paged(q, cache, batch, cfg.head_dim ** -0.5)
         partial = self._all_reduce(be.gemm_epilogue(attn.view(x.shape[0], self.hq * cfg.head_dim), self.wo))   # sum over head shards
         x1 = be.residual_add(x, partial)
-        return be.residual_add(x1, self._all_reduce(self.ffn_partial(x1)))                                    # sum over FFN shards
+        return be.residual_add(x1, self._all_reduce(self.ffn_partial(x1)))[:tokens]                           # sum over FFN shards
 
     def default_micro_batches(self, batch: int) -> int:
         """Parts the batch is cut into so that the sums of one part travel while the next computes. More parts hide more of
