@@ -93,6 +93,7 @@ wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cach
   if (p->q_heads == 0 || p->q_heads > 0xffffu || p->q_heads % cache->kv_heads != 0)
     return fail(WB200_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
   if (cache->head_dim % 8 != 0 || cache->head_dim > 256) return fail(WB200_ERR_UNSUPPORTED, "paged attention takes head dimensions that are multiples of 8, up to 256");
+  if (static_cast<uint64_t>(batch->tokens) * p->q_heads > 0x7fffffffull) return fail(WB200_ERR_LIMIT, "more than 2^31 - 1 rows in one paged attention");
   if (!(p->scale > 0.f) || p->scale > 3.402823466e38f) return fail(WB200_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
   a->q_heads = static_cast<int>(p->q_heads);
   a->causal = p->causal ? 1 : 0;
@@ -191,7 +192,9 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
 uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
                                                const wb200_attention_paged_params *p) {
   if (!backend || !cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
-  return 256;
+  AttentionPagedArgs a{};
+  if (make_attention_paged(nullptr, cache, batch, p, &a) != WB200_OK) return 0;
+  return attention_paged_rows_supports(a) ? attention_paged_rows_workspace(backend->sm_count) : 256;
 }
 
 wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
@@ -204,9 +207,13 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   if (!a.q || !a.out) return fail(WB200_ERR_INVALID_ARGUMENT, "q and out must not be null");
   if (!output_rows_apart(a.cache.head_dim, a.out_token, a.out_head, a.batch.tokens, a.q_heads))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
+  const bool rows = attention_paged_rows_supports(a);
+  if (rows && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < attention_paged_rows_workspace(backend->sm_count)))
+    return fail(WB200_ERR_INVALID_ARGUMENT, "the workspace must be 256-byte aligned and hold wb200_attention_paged_workspace_bytes() bytes");
   DeviceGuard guard(backend->device);
-  st = launch_attention_paged_general(a, static_cast<cudaStream_t>(p->stream));
-  if (st == WB200_OK) backend->launches += 1;
+  if (rows) st = launch_attention_paged_rows(a, backend->sm_count, static_cast<cudaStream_t>(p->stream));
+  else st = launch_attention_paged_general(a, static_cast<cudaStream_t>(p->stream));
+  if (st == WB200_OK) backend->launches += rows ? 2 : 1;
   return st;
 }
 

@@ -1,0 +1,564 @@
+// Attention of few new tokens over a paged KV cache: decoding and drafted tokens (bf16 / f16, head_dim 64 and 128).
+//
+// The rows that share a KV head, (token, query head of its group), are packed into tiles of 16 (or 8) MMA rows: row r of a
+// tile is token r / group, head r % group, so a step of one token per sequence reads every key once whatever the group. A
+// unit of work is one tile of rows of one KV head of one sequence; its keys are cut into steps of 64. All units lie one
+// behind the other on one axis of steps, which is cut into as many equal shares as there are CTAs: every CTA streams the
+// same number of keys however ragged the lengths are, and the lengths are only read on the device (each CTA sums up the
+// sequences' steps for itself, one load per thread for up to 128 sequences). A share that ends inside a unit leaves an
+// un-finalized record (m, l, acc) in the workspace, which the second kernel folds with the unit's other records; the shares
+// and the order of the fold depend on the lengths alone, so results repeat bit for bit.
+//
+// A CTA is four warps. Each streams every fourth 16-key tile of the share through a ring of its own (cp.async, 16-byte
+// copies, rows XOR-swizzled), S = Q K^T and acc += P V by mma.sync m16n8k16 (matrix work is far from the bound: decoding
+// reads 4 bytes of cache per 2 flop and query head), the running maximum and sum in f32. With 8 rows the PV product runs
+// transposed, rows on the 8-wide side: half the products.
+// Bound: HBM, the K and V bytes of the visible keys.
+#include "attention_paged.cuh"
+
+namespace wb200 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kTileKeys = 16;
+constexpr int kStepKeys = kWarps * kTileKeys;
+
+template <int kD>
+struct RowsShape {
+  static constexpr int kRowBytes = kD * 2;
+  static constexpr int kTileBytes = kTileKeys * kRowBytes;
+  static constexpr int kStages = kD == 128 ? 3 : 6;          // 24 KiB of copies in flight per warp either way
+  static constexpr int kRingBytes = kStages * 2 * kTileBytes;
+  static constexpr int kSmemBytes = kWarps * kRingBytes;
+  static constexpr int kRecord = kD + 4;                     // floats: acc[D], m, l and padding to 16 bytes
+  static_assert(kWarps * 16 * kRecord * 4 <= kSmemBytes, "the warps' records must fit the rings");
+};
+
+// What the fold has to know about the unit that a CTA's share ends inside of; `records` 0: no such unit.
+struct RowsSplit {
+  int records, begin, count, tile, kv_head, reserved[3];
+};
+
+struct RowsParams {
+  AttentionPagedArgs a;
+  int group;                        // query heads per KV head
+  int least_steps;                  // no share is made smaller than this many steps
+  float scale_log2;
+  float *records;                   // [grid][2][rows per tile][kRecord]: a share's end of a unit (0), its start of one (1)
+  RowsSplit *splits;                // [grid]
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBf16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+  }
+}
+// Byte offset of 16-byte chunk c of row r in a tile of rows of kRowBytes.
+template <int kRowBytes>
+__device__ __forceinline__ uint32_t tile_offset(int r, int c) { return static_cast<uint32_t>(r * kRowBytes + ((c ^ (r & 7)) << 4)); }
+
+// A lane's elements of a row of kD floats.
+template <int kD>
+struct Slice {
+  static constexpr int kPer = kD / 32;
+  float v[kPer];
+  __device__ __forceinline__ void load(const float *row, int lane) {
+    if constexpr (kPer == 4) {
+      const float4 w = *reinterpret_cast<const float4 *>(row + 4 * lane);
+      v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+      const float2 w = *reinterpret_cast<const float2 *>(row + 2 * lane);
+      v[0] = w.x; v[1] = w.y;
+    }
+  }
+  __device__ __forceinline__ void store(float *row, int lane) const {
+    if constexpr (kPer == 4) *reinterpret_cast<float4 *>(row + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<float2 *>(row + 2 * lane) = make_float2(v[0], v[1]);
+  }
+};
+
+// Writes a finished row (statistics in the log2 domain): out = acc / l, one rounding.
+template <bool kBf16, int kD>
+__device__ __forceinline__ void write_row(const AttentionPagedArgs &a, int token, int head, int lane, float m, float l, const Slice<kD> &acc) {
+  constexpr uint32_t kNan = kBf16 ? 0x7fc07fc0u : 0x7e007e00u;
+  const bool empty = l == 0.f;
+  const float coefficient = empty ? 0.f : 1.0f / l;
+  uint32_t bits[Slice<kD>::kPer / 2];
+#pragma unroll
+  for (int i = 0; i < Slice<kD>::kPer / 2; ++i) {
+    bits[i] = pack2<kBf16>(acc.v[2 * i] * coefficient, acc.v[2 * i + 1] * coefficient);
+    if (empty) bits[i] = a.zero_fully_masked ? 0u : kNan;
+  }
+  uint16_t *out = static_cast<uint16_t *>(a.out) + token * a.out_token + head * a.out_head + Slice<kD>::kPer * lane;
+  if constexpr (kD == 128) *reinterpret_cast<uint2 *>(out) = make_uint2(bits[0], bits[1]);
+  else *reinterpret_cast<uint32_t *>(out) = bits[0];
+  if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * a.q_heads + head] = empty ? -INFINITY : m * 0.69314718055994530942f + logf(l);
+}
+
+// Steps of a sequence: tiles of rows x KV heads x steps of keys (at least one, so that rows without keys are written).
+struct RowsUnits {
+  int steps;
+  long long weight;
+};
+template <int kRows>
+__device__ __forceinline__ RowsUnits rows_units(const RowsParams &p, const PagedSequence &s) {
+  const int steps = s.keys == 0 ? 1 : (s.keys - 1) / kStepKeys + 1;
+  const long long tiles = (static_cast<long long>(s.count) * p.group + kRows - 1) / kRows;
+  return {steps, tiles * p.a.cache.kv_heads * steps};
+}
+
+template <bool kBf16, int kD, bool kNarrow, bool kAligned>
+__global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(const __grid_constant__ RowsParams p) {
+  using S = RowsShape<kD>;
+  constexpr int kRows = kNarrow ? 8 : 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long warp_totals[kWarps], start_prefix;
+  __shared__ int start_sequence;
+  __shared__ int seen_keys[kWarps][S::kStages];       // bit i: key i of the tile in that slot takes part
+  const AttentionPagedArgs &a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const bool reports = blockIdx.x == 0;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // This CTA's share of all steps. A thread sums up a run of consecutive sequences.
+  const int per_thread = (a.batch.sequences + kWarps * 32 - 1) / (kWarps * 32);
+  const int first_mine = min(a.batch.sequences, static_cast<int>(threadIdx.x) * per_thread), end_mine = min(a.batch.sequences, first_mine + per_thread);
+  long long mine = 0;
+  for (int s = first_mine; s < end_mine; ++s) {
+    const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, reports);
+    if (sequence.count > 0) mine += rows_units<kRows>(p, sequence).weight;
+  }
+  long long before = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long other = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += other;
+  }
+  if (lane == 31) warp_totals[warp] = before;
+  if (threadIdx.x == 0) start_sequence = -1;
+  __syncthreads();
+  long long total = 0;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_totals[w];
+    total += warp_totals[w];
+  }
+  long long shares = total / p.least_steps;
+  shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
+  const long long index = blockIdx.x;
+  auto boundary = [&](long long c) { return total * c / shares; };
+  long long at = index < shares ? boundary(index) : total;
+  const long long share_end = index < shares ? boundary(index + 1) : total;
+  if (at < share_end && before <= at && at < before + mine) {
+    long long prefix = before;
+    for (int s = first_mine; s < end_mine; ++s) {
+      const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
+      const long long weight = sequence.count > 0 ? rows_units<kRows>(p, sequence).weight : 0;
+      if (at < prefix + weight) {
+        start_sequence = s;
+        start_prefix = prefix;
+        break;
+      }
+      prefix += weight;
+    }
+  }
+  __syncthreads();
+  int s = start_sequence;
+  long long prefix = s >= 0 ? start_prefix : 0;
+  RowsSplit split = {};
+
+  uint8_t *ring = smem + warp * S::kRingBytes;
+  const uint32_t ring_addr = smem_u32(ring);
+  float *records = reinterpret_cast<float *>(smem);   // [warp][kRows][kRecord], over the rings once they are read
+
+  while (s >= 0 && at < share_end) {
+    const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
+    const RowsUnits units = sequence.count > 0 ? rows_units<kRows>(p, sequence) : RowsUnits{1, 0};
+    if (at >= prefix + units.weight) {                 // on to the next sequence that has rows
+      prefix += units.weight;
+      if (++s >= a.batch.sequences) break;
+      continue;
+    }
+    const long long unit = (at - prefix) / units.steps;
+    const int step0 = static_cast<int>(at - prefix - unit * units.steps);
+    const int step1 = static_cast<int>(min(static_cast<long long>(units.steps), step0 + (share_end - at)));
+    const int kv_head = static_cast<int>(unit % a.cache.kv_heads), row_tile = static_cast<int>(unit / a.cache.kv_heads);
+    const int row0 = row_tile * kRows;                 // first packed row
+    const int rows_here = static_cast<int>(min(static_cast<long long>(sequence.count) * p.group - row0, static_cast<long long>(kRows)));
+    // keys that the tile's last token sees bound what is read
+    const int tile_keys = min(sequence.keys, paged_visible(sequence, (row0 + rows_here - 1) / p.group, a.causal));
+    const int key_begin = step0 * kStepKeys, key_end = min(tile_keys, step1 * kStepKeys);
+    const int first_key = key_begin + warp * kTileKeys;
+    const int tiles = key_end > first_key ? (key_end - first_key + kStepKeys - 1) / kStepKeys : 0;
+
+    const uint16_t *k_base = static_cast<const uint16_t *>(a.cache.k) + kv_head * a.cache.k_head;
+    const uint16_t *v_base = static_cast<const uint16_t *>(a.cache.v) + kv_head * a.cache.v_head;
+    const int *pages = a.batch.page_table + s * a.batch.table_stride;
+    // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
+    auto look_up = [&](int tile) {
+      const int key = first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
+      return tile < tiles && key < key_end ? __ldg(pages + key / a.cache.page_size) : -1;
+    };
+    auto issue_tile = [&](int tile, int slot, int page) {
+      if (tile < tiles) {
+        const int key0 = first_key + tile * kStepKeys;
+        const uint32_t k_dst = ring_addr + slot * (2 * S::kTileBytes), v_dst = k_dst + S::kTileBytes;
+        const int own_key = key0 + (lane & 15);
+        const bool inside = page >= 0 && page < a.cache.pages;
+        if (!inside && own_key < key_end) raise_status(a.refused, kRefusedPage);
+        const unsigned int seen = __ballot_sync(0xffffffffu, inside && own_key < key_end) & 0xffffu;
+        if (lane == 0) seen_keys[warp][slot] = static_cast<int>(seen);
+        const int in_page = (kAligned ? key0 : own_key) % a.cache.page_size;
+        const int64_t k_row = (inside ? page : 0) * a.cache.k_page + in_page * a.cache.k_row;
+        const int64_t v_row = (inside ? page : 0) * a.cache.v_page + in_page * a.cache.v_row;
+        constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
+#pragma unroll
+        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+          const int r = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
+          int64_t k_at, v_at;
+          if constexpr (kAligned) {
+            k_at = k_row + r * a.cache.k_row;
+            v_at = v_row + r * a.cache.v_row;
+          } else {
+            k_at = __shfl_sync(0xffffffffu, k_row, r);
+            v_at = __shfl_sync(0xffffffffu, v_row, r);
+          }
+          const bool reads = (seen >> r) & 1u;         // other rows are zeros
+          cp_async16(k_dst + tile_offset<S::kRowBytes>(r, c), k_base + (reads ? k_at + c * 8 : 0), reads ? 16u : 0u);
+          cp_async16(v_dst + tile_offset<S::kRowBytes>(r, c), v_base + (reads ? v_at + c * 8 : 0), reads ? 16u : 0u);
+        }
+      }
+      cp_async_commit();
+    };
+
+    constexpr int kHalves = kNarrow ? 1 : 2;           // softmax rows per lane: g (and g + 8)
+    constexpr int kAccs = kNarrow ? kD / 16 : kD / 8;  // fragments: 16 elements x 8 rows, or 16 rows x 8 elements
+    float m_run[kHalves], l_run[kHalves], acc[kAccs][4];
+    int last_key[kHalves];                             // last key the lane's row sees
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      m_run[h] = -INFINITY;
+      l_run[h] = 0.f;
+      last_key[h] = paged_visible(sequence, (row0 + g + 8 * h) / p.group, a.causal) - 1;
+    }
+#pragma unroll
+    for (int j = 0; j < kAccs; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+
+    int page = look_up(0);
+#pragma unroll 1
+    for (int i = 0; i < S::kStages; ++i) {
+      const int next = look_up(i + 1);
+      issue_tile(i, i, page);
+      page = next;
+    }
+    // The tile's rows as A fragments (rows behind the last are zero).
+    uint32_t q_frag[kD / 16][4];
+    {
+      const uint32_t *rows[2] = {nullptr, nullptr};
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const int packed = row0 + g + 8 * h, token = packed / p.group;
+        if (g + 8 * h < rows_here)
+          rows[h] = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + static_cast<int64_t>(sequence.begin + token) * a.q_token +
+                                                       (kv_head * p.group + packed - token * p.group) * a.q_head) + t;
+      }
+#pragma unroll
+      for (int ks = 0; ks < kD / 16; ++ks) {
+        q_frag[ks][0] = rows[0] ? rows[0][ks * 8] : 0u;
+        q_frag[ks][1] = rows[1] ? rows[1][ks * 8] : 0u;
+        q_frag[ks][2] = rows[0] ? rows[0][ks * 8 + 4] : 0u;
+        q_frag[ks][3] = rows[1] ? rows[1][ks * 8 + 4] : 0u;
+      }
+    }
+
+    int slot = 0;
+#pragma unroll 1
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int next = look_up(tile + S::kStages + 1);
+      cp_async_wait<S::kStages - 1>();
+      __syncwarp();
+      const uint32_t k_src = ring_addr + slot * (2 * S::kTileBytes), v_src = k_src + S::kTileBytes;
+      const int key0 = first_key + tile * kStepKeys + 2 * t;
+      const unsigned int seen = static_cast<unsigned int>(seen_keys[warp][slot]) >> (2 * t);
+      float part[2][2][4] = {};                        // even and odd k-steps apart: four short chains
+#pragma unroll
+      for (int ks = 0; ks < kD / 16; ++ks) {
+        const int mi = lane >> 3;
+        uint32_t bfrag[4];
+        ldmatrix_x4(k_src + tile_offset<S::kRowBytes>((mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), bfrag);
+        mma_16816<kBf16>(part[ks & 1][0], q_frag[ks], bfrag[0], bfrag[1]);
+        mma_16816<kBf16>(part[ks & 1][1], q_frag[ks], bfrag[2], bfrag[3]);
+      }
+      float alpha[kHalves], pr[kHalves][4];            // keys 2t, 2t + 1, 8 + 2t, 9 + 2t
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int offset = (i >> 1) * 8 + (i & 1);
+          sc[i] = (part[0][i >> 1][2 * h + (i & 1)] + part[1][i >> 1][2 * h + (i & 1)]) * p.scale_log2;
+          if (!((seen >> offset) & 1u) || key0 + offset > last_key[h]) sc[i] = -INFINITY;
+        }
+        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(top, m_run[h]), m_exp = m_new == -INFINITY ? 0.f : m_new;
+        alpha[h] = exp2_fast(m_run[h] - m_exp);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pr[h][i] = exp2_fast(sc[i] - m_exp);
+          sum += pr[h][i];
+        }
+        l_run[h] = l_run[h] * alpha[h] + sum;
+        m_run[h] = m_new;
+      }
+      // Probabilities are rounded to the storage type for the product with V; the sum keeps them in f32.
+      if constexpr (kNarrow) {
+        const uint32_t p_lo = pack2<kBf16>(pr[0][0], pr[0][1]), p_hi = pack2<kBf16>(pr[0][2], pr[0][3]);
+        const float alpha0 = __shfl_sync(0xffffffffu, alpha[0], 8 * t), alpha1 = __shfl_sync(0xffffffffu, alpha[0], 8 * t + 4);   // rows 2t, 2t + 1
+#pragma unroll
+        for (int j = 0; j < kAccs; ++j) {
+          const int mi = lane >> 3;
+          uint32_t vfrag[4];
+          ldmatrix_x4_trans(v_src + tile_offset<S::kRowBytes>((mi >> 1) * 8 + (lane & 7), 2 * j + (mi & 1)), vfrag);
+          acc[j][0] *= alpha0; acc[j][1] *= alpha1; acc[j][2] *= alpha0; acc[j][3] *= alpha1;
+          mma_16816<kBf16>(acc[j], vfrag, p_lo, p_hi);
+        }
+      } else {
+        const uint32_t p_frag[4] = {pack2<kBf16>(pr[0][0], pr[0][1]), pack2<kBf16>(pr[kHalves - 1][0], pr[kHalves - 1][1]),
+                                    pack2<kBf16>(pr[0][2], pr[0][3]), pack2<kBf16>(pr[kHalves - 1][2], pr[kHalves - 1][3])};
+#pragma unroll
+        for (int j = 0; j < kAccs; ++j) {
+          acc[j][0] *= alpha[0]; acc[j][1] *= alpha[0];
+          acc[j][2] *= alpha[kHalves - 1]; acc[j][3] *= alpha[kHalves - 1];
+        }
+#pragma unroll
+        for (int j = 0; j < kAccs; j += 2) {
+          const int mi = lane >> 3;
+          uint32_t vfrag[4];
+          ldmatrix_x4_trans(v_src + tile_offset<S::kRowBytes>((mi & 1) * 8 + (lane & 7), j + (mi >> 1)), vfrag);
+          mma_16816<kBf16>(acc[j], p_frag, vfrag[0], vfrag[1]);
+          mma_16816<kBf16>(acc[j + 1], p_frag, vfrag[2], vfrag[3]);
+        }
+      }
+      __syncwarp();   // every lane has read the slot
+      issue_tile(tile + S::kStages, slot, page);
+      page = next;
+      if (++slot == S::kStages) slot = 0;
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+      l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+    }
+    __syncthreads();   // the rings are free
+    {
+      float *mine_records = records + warp * (kRows * S::kRecord);
+      if constexpr (kNarrow) {
+#pragma unroll
+        for (int j = 0; j < kAccs; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mine_records[(2 * t + (i & 1)) * S::kRecord + j * 16 + g + 8 * (i >> 1)] = acc[j][i];
+      }
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        float *row = mine_records + (g + 8 * h) * S::kRecord;
+        if constexpr (!kNarrow) {
+#pragma unroll
+          for (int j = 0; j < kAccs; ++j) *reinterpret_cast<float2 *>(row + j * 8 + 2 * t) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+        }
+        if (t == 0) *reinterpret_cast<float2 *>(row + kD) = make_float2(m_run[h], l_run[h]);
+      }
+    }
+    __syncthreads();
+    // Fold over the warps, a warp per row, with the row's maximum as the common exponent reference.
+    const bool whole = step0 == 0 && step1 == units.steps;
+    for (int r = warp; r < rows_here; r += kWarps) {
+      float2 ml[kWarps];
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        ml[w] = *reinterpret_cast<const float2 *>(records + (w * kRows + r) * S::kRecord + kD);
+        top = fmaxf(top, ml[w].x);
+      }
+      const float m_exp = top == -INFINITY ? 0.f : top;
+      float l = 0.f;
+      Slice<kD> sum = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float weight = exp2_fast(ml[w].x - m_exp);
+        Slice<kD> part;
+        part.load(records + (w * kRows + r) * S::kRecord, lane);
+        l = fmaf(ml[w].y, weight, l);
+#pragma unroll
+        for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(part.v[e], weight, sum.v[e]);
+      }
+      if (whole) {
+        const int packed = row0 + r, token = packed / p.group;
+        write_row<kBf16, kD>(a, sequence.begin + token, kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+      } else {
+        float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (step0 == 0 ? 1 : 0)) * kRows + r) * S::kRecord;
+        sum.store(record, lane);
+        if (lane == 0) *reinterpret_cast<float2 *>(record + kD) = make_float2(top, l);
+      }
+    }
+    at += step1 - step0;
+    if (step0 == 0 && step1 < units.steps) {           // the unit starts here and goes on in the CTAs behind this one
+      const long long unit_end = at + (units.steps - step1);
+      const long long last = (unit_end * shares - 1) / total;   // the last share that begins in front of the unit's end
+      split = {1 + static_cast<int>(last - index), sequence.begin, sequence.count, row_tile, kv_head, {}};
+    }
+    __syncthreads();   // the records have been read before the rings are written again
+  }
+  if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
+}
+
+// Folds the records of the unit that starts in share blockIdx.x and goes on in the shares behind it, a warp per row.
+template <bool kBf16, int kD, bool kNarrow>
+__global__ void __launch_bounds__(kWarps * 32) attention_paged_fold_kernel(const __grid_constant__ RowsParams p) {
+  using S = RowsShape<kD>;
+  constexpr int kRows = kNarrow ? 8 : 16;
+  pdl_wait();
+  pdl_launch_dependents();
+  const RowsSplit split = p.splits[blockIdx.x];
+  if (split.records == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = split.tile * kRows;
+  for (int r = warp; r < kRows; r += kWarps) {
+    const int packed = row0 + r, token = packed / p.group;
+    if (token >= split.count) break;
+    // record i: the start (slot 1) of the first share, the ends (slot 0) of the others
+    auto record = [&](int i) { return p.records + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + r) * S::kRecord; };
+    float top = -INFINITY;
+    for (int i = lane; i < split.records; i += 32) top = fmaxf(top, record(i)[kD]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float m_exp = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    Slice<kD> sum = {};
+    for (int base = 0; base < split.records; base += 32) {
+      float weight = 0.f;
+      if (base + lane < split.records) {
+        const float2 ml = *reinterpret_cast<const float2 *>(record(base + lane) + kD);
+        weight = exp2_fast(ml.x - m_exp);
+        l = fmaf(ml.y, weight, l);
+      }
+      const int count = min(32, split.records - base);
+#pragma unroll 4
+      for (int i = 0; i < count; ++i) {
+        Slice<kD> part;
+        part.load(record(base + i), lane);
+        const float w = __shfl_sync(0xffffffffu, weight, i);
+#pragma unroll
+        for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(part.v[e], w, sum.v[e]);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    write_row<kBf16, kD>(p.a, split.begin + token, split.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+  }
+}
+
+using RowsKernel = void (*)(const RowsParams);
+template <bool kBf16, int kD, bool kNarrow>
+constexpr RowsKernel rows_kernel(bool aligned) {
+  return aligned ? attention_paged_rows_kernel<kBf16, kD, kNarrow, true> : attention_paged_rows_kernel<kBf16, kD, kNarrow, false>;
+}
+#define WB200_ROWS_KERNELS(D, NARROW)                                                                               \
+  {{rows_kernel<false, D, NARROW>(false), rows_kernel<false, D, NARROW>(true)},                                     \
+   {rows_kernel<true, D, NARROW>(false), rows_kernel<true, D, NARROW>(true)}}
+const RowsKernel kRowsKernels[2][2][2][2] = {   // [head_dim 128][narrow][bf16][aligned]
+    {WB200_ROWS_KERNELS(64, false), WB200_ROWS_KERNELS(64, true)}, {WB200_ROWS_KERNELS(128, false), WB200_ROWS_KERNELS(128, true)}};
+const RowsKernel kFoldKernels[2][2][2] = {      // [head_dim 128][narrow][bf16]
+    {{attention_paged_fold_kernel<false, 64, false>, attention_paged_fold_kernel<true, 64, false>},
+     {attention_paged_fold_kernel<false, 64, true>, attention_paged_fold_kernel<true, 64, true>}},
+    {{attention_paged_fold_kernel<false, 128, false>, attention_paged_fold_kernel<true, 128, false>},
+     {attention_paged_fold_kernel<false, 128, true>, attention_paged_fold_kernel<true, 128, true>}}};
+
+constexpr int kCtasPerSm = 2;
+size_t rows_record_bytes(int sm_count) { return static_cast<size_t>(sm_count) * kCtasPerSm * 2 * 16 * (128 + 4) * sizeof(float); }
+
+}  // namespace
+
+bool attention_paged_rows_supports(const AttentionPagedArgs &a) {
+  if (a.cache.head_dim != 64 && a.cache.head_dim != 128) return false;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a.cache.k) | reinterpret_cast<uintptr_t>(a.cache.v) | reinterpret_cast<uintptr_t>(a.q) |
+                        reinterpret_cast<uintptr_t>(a.out) |
+                        static_cast<uint64_t>((a.cache.k_page | a.cache.k_row | a.cache.k_head | a.cache.v_page | a.cache.v_row | a.cache.v_head |
+                                               a.q_token | a.q_head | a.out_token | a.out_head) * 2);
+  return (bits & 15u) == 0;     // rows begin on 16 bytes
+}
+
+size_t attention_paged_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kCtasPerSm * sizeof(RowsSplit); }
+
+wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_count, cudaStream_t stream) {
+  RowsParams p{};
+  p.a = a;
+  p.group = a.q_heads / a.cache.kv_heads;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.least_steps = 2;
+  p.records = static_cast<float *>(a.workspace);
+  p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
+  // Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
+  const bool narrow = static_cast<int64_t>(p.group) * (a.batch.max_query > 0 ? a.batch.max_query : 1) <= 8;
+  const int wide = a.cache.head_dim == 128 ? 1 : 0, bf16 = a.cache.format == WB200_BF16 ? 1 : 0;
+  static PerDeviceOnce attributes;
+  const wb200_status st = attributes.run([]() -> wb200_status {
+    for (int d = 0; d < 2; ++d)
+      for (int n = 0; n < 2; ++n)
+        for (int b = 0; b < 2; ++b)
+          for (int al = 0; al < 2; ++al)
+            WB200_CUDA_CHECK(cudaFuncSetAttribute(kRowsKernels[d][n][b][al], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  d ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes));
+    return WB200_OK;
+  });
+  if (st != WB200_OK) return st;
+  const unsigned grid = static_cast<unsigned>(sm_count * kCtasPerSm);
+  WB200_CUDA_CHECK(launch_dependent(kRowsKernels[wide][narrow][bf16][a.cache.page_size % kTileKeys == 0], grid, kWarps * 32,
+                                    wide ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], grid, kWarps * 32, 0, stream, p));
+  return WB200_OK;
+}
+
+}  // namespace wb200

@@ -331,6 +331,10 @@ struct AttentionPagedArgs {
   int *status;        // bounded waits
 };
 wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cudaStream_t stream);
+// Few rows per KV head (attention_paged_rows.cu): two launches.
+bool attention_paged_rows_supports(const AttentionPagedArgs &args);
+size_t attention_paged_rows_workspace(int sm_count);
+wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int sm_count, cudaStream_t stream);
 
 struct PageTablesArgs {
   int sequences, table_width, pages, page_size;
