@@ -1,0 +1,891 @@
+// Attention of chunks of new tokens over a paged KV cache on tcgen05 tensor cores (bf16 / f16, head_dim 64 and 128).
+//
+// The arithmetic of a tile is that of the prefill kernel (attention_fa.cu): S = Q K^T in TMEM, a thread per row for the
+// softmax with a lagging exponent reference, the rounded P back into TMEM as the A operand of P V. What differs is what the
+// rows and the tiles are:
+//   rows     The rows that share a KV head, (token, query head of its group), are packed: row r of a tile is token r / group,
+//            head r % group, 128 / group tokens to a tile. A chunk of 64 tokens of a group of 4 fills the two tiles of an item,
+//            which then reads its keys once instead of four times; Q comes in by one TMA box per tile and half.
+//   keys     A 128-key tile is one TMA box per page part of 2^n rows that divides both (whole tiles of 128-row pages, sixteen
+//            boxes at 8). The loader's lanes look up and issue a box each; page numbers are looked up one tile ahead.
+//   tails    Rows behind a sequence's last key are not masked by TMA's fill, as the page goes on, and 0 * v is not 0 for what a
+//            stale row may hold. A warp of its own zeroes those rows of V in shared memory before the products see them.
+//   shares   An item is two row tiles of one KV head of one sequence, its steps are its 128-key tiles under the causal limit.
+//            All items lie one behind the other on one axis of steps, cut into equal shares for the CTAs, so ragged batches and
+//            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A share's ends inside
+//            items leave f32 records, folded by a second kernel.
+// Results depend on the lengths and the number of SMs only: repeats give the same bits.
+// Bound: the chain S -> softmax -> P V of a step (see attention_fa.cu), 4 * head_dim flop per visible (row, key) pair.
+#include <type_traits>
+
+#include "attention_paged.cuh"
+
+namespace wb200 {
+namespace {
+
+constexpr int kTileM = 128;                     // packed rows per Q tile (TMEM lanes)
+constexpr int kTileN = 128;                     // keys per tile
+constexpr int kBlockBytes = 128 * 128;          // [128 rows][128 B], swizzled
+constexpr int kOutStageBytes = 32 * 128;        // a softmax warp's 32 rows x 64 columns of output
+constexpr int kThreads = 384;                   // warps: loader, MMA, cleaner, idle, 2 x 4 softmax
+constexpr int kPParts = 2;
+constexpr int kFirstChunks = 3;                 // 32-key chunks of the first part of P, of 4
+constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
+constexpr int kMaxSequences = 4096;             // staged in shared memory
+constexpr int kLeastSteps = 2;                  // no share is made smaller
+
+template <int kHd>
+struct Shape {
+  static constexpr int kHalves = kHd / 64;                   // 64-element column blocks
+  static constexpr int kTileBytes = kHalves * kBlockBytes;
+  static constexpr int kSlots = 8 / kHalves;                 // 128 KiB of K and V tiles
+  static constexpr int kQOff = 0;
+  static constexpr int kRingOff = 2 * kTileBytes;
+  static constexpr int kOutOff = kRingOff + kSlots * kTileBytes;
+  static constexpr int kBarOff = kOutOff + 8 * kOutStageBytes;
+  static constexpr int kWalkOff = kBarOff + 512;             // where the softmax warps keep their place in the share
+  static constexpr size_t kBytes = kWalkOff + 8 * 96 + 1024;
+  static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
+  static constexpr int kRecordFloats = kTileM * kHd + 2 * kTileM;   // acc as [kHd / 4][128 rows][4], then (m, l) per row
+  static_assert(kMaxSequences * 16 <= kSlots * kTileBytes, "the staged lengths must fit the ring");
+};
+
+// What the fold has to know about the item that a CTA's share ends inside of; `records` 0: none.
+struct ChunkSplit {
+  int records, begin, count, pair, kv_head, reserved[3];
+};
+
+struct ChunkParams {
+  AttentionPagedArgs a;
+  int group, tile_tokens;          // query heads per KV head; tokens per Q tile
+  int box_rows;                    // keys per TMA box
+  int rows_inside;                 // the cache's tensor maps have rows inside heads
+  int rows_limit;                  // sequences with at most this many packed rows are another kernel's
+  float scale_log2;
+  float *records;                  // [grid][2][2 tiles][kRecordFloats]: a share's end of an item (0), its start of one (1)
+  ChunkSplit *splits;              // [grid]
+};
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <int kRegs>
+__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+__device__ __forceinline__ unsigned long long pack_f32x2(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(unsigned long long v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma_f32x2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBf16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+  }
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "setp.ne.b32 P, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, P;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
+
+// 128-key tiles that Q tile (or pair) whose last token is `last` visits.
+__device__ __forceinline__ int tiles_to(int keys, int count, int causal, int last) {
+  int visible = keys;
+  if (causal) visible = keys - count + min(last, count - 1) + 1;
+  return visible <= 0 ? 0 : (visible + kTileN - 1) / kTileN;
+}
+
+// One CTA's part of an item: key tiles [t0, t1) of the `steps` of two row tiles of a KV head of a sequence.
+struct Segment {
+  int begin, count, keys;          // the sequence
+  int sequence, kv_head, pair;
+  int n0, n1;                      // key tiles that Q tile 0 / 1 visits in all
+  int steps, t0, t1;
+  __device__ __forceinline__ int of(int t) const {            // tiles of this segment for Q tile t
+    const int n = min(t ? n1 : n0, t1) - t0;
+    return n < 0 ? 0 : n;
+  }
+};
+// Walks a CTA's share: the same sequence of segments in every warp.
+struct ShareWalk {
+  long long left;                  // steps of the share not yet walked
+  int sequence, kv_head, pair, t0;
+  int begin, count, keys, pairs;   // of the current sequence; count 0: to be looked up
+
+  __device__ __forceinline__ void look_up(const ChunkParams &p) {
+    const PagedSequence s = paged_sequence(p.a.batch, p.a.cache, sequence, p.a.refused, false);
+    const bool mine = static_cast<long long>(s.count) * p.group > p.rows_limit;
+    begin = s.begin; count = mine ? s.count : 0; keys = s.keys;
+    pairs = (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+  }
+  __device__ __forceinline__ bool next(const ChunkParams &p, Segment &out) {
+    if (left <= 0) return false;
+    while (count == 0 || kv_head == p.a.cache.kv_heads) {
+      kv_head = pair = t0 = 0;
+      if (++sequence >= p.a.batch.sequences) return false;
+      look_up(p);
+    }
+    out.begin = begin; out.count = count; out.keys = keys; out.sequence = sequence; out.kv_head = kv_head; out.pair = pair;
+    const int first = pair * 2 * p.tile_tokens;
+    out.n0 = tiles_to(keys, count, p.a.causal, first + p.tile_tokens - 1);
+    out.n1 = first + p.tile_tokens < count ? tiles_to(keys, count, p.a.causal, first + 2 * p.tile_tokens - 1) : 0;
+    const int tiles = max(out.n0, out.n1);
+    out.steps = max(tiles, 1);
+    out.t0 = t0;
+    out.t1 = static_cast<int>(min(static_cast<long long>(out.steps), t0 + left));
+    left -= out.t1 - out.t0;
+    t0 = 0;
+    if (++pair == pairs) { pair = 0; ++kv_head; }
+    return true;
+  }
+  // The next segment with keys to visit.
+  __device__ __forceinline__ bool next_working(const ChunkParams &p, Segment &out) {
+    while (next(p, out))
+      if (out.of(0) > 0 || out.of(1) > 0) return true;
+    return false;
+  }
+};
+
+// A softmax warp's place in its share, in shared memory: its threads need their registers for the scores.
+struct WarpPlace {
+  ShareWalk walk;
+  Segment segment;
+};
+static_assert(sizeof(WarpPlace) <= 96, "the places' area");
+
+template <bool kBf16, int kHd>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                             const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkParams p) {
+  using L = Shape<kHd>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t *smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  const uint32_t smem_base = smem_u32(smem);
+
+  const uint32_t bar_base = smem_base + L::kBarOff;
+  auto kv_full = [&](int s) { return bar_base + 8u * s; };
+  auto kv_empty = [&](int s) { return bar_base + 8u * (L::kSlots + s); };
+  auto tail_full = [&](int s) { return bar_base + 8u * (2 * L::kSlots + s); };   // a V tile whose tail is still to be zeroed
+  constexpr int kFixed = 3 * L::kSlots;
+  const uint32_t q_full = bar_base + 8u * kFixed;
+  auto s_full = [&](int t) { return bar_base + 8u * (kFixed + 1 + t); };
+  auto p_part = [&](int t, int part) { return bar_base + 8u * (kFixed + 3 + kPParts * t + part); };
+  auto o_done = [&](int t) { return bar_base + 8u * (kFixed + 3 + 2 * kPParts + t); };
+  const uint32_t q_empty = bar_base + 8u * (kFixed + 5 + 2 * kPParts);
+  uint8_t *bar_ptr = smem + L::kBarOff;
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 6 + 2 * kPParts));
+  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 7 + 2 * kPParts));
+  static_assert(8 * (kFixed + 8 + 2 * kPParts) <= 512, "the barriers must fit their area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kSlots; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+      mbar_init(tail_full(s), 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      for (int part = 0; part < kPParts; ++part) mbar_init(p_part(t, part), kTileM / 32);
+      mbar_init(o_done(t), 1);
+    }
+    *abort_word = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- this CTA's share of all steps; the lengths are staged in the ring's memory
+  ShareWalk walk;
+  long long total, shares;
+  {
+    int2 *staged = reinterpret_cast<int2 *>(smem + L::kRingOff);                                       // (count, keys)
+    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int2));
+    const int sequences = p.a.batch.sequences;
+    for (int s = threadIdx.x; s < sequences; s += kThreads) {
+      const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, s, p.a.refused, blockIdx.x == 0);
+      staged[s] = make_int2(static_cast<long long>(q.count) * p.group > p.rows_limit ? q.count : 0, q.keys);
+    }
+    __syncthreads();
+    auto pair_steps = [&](int2 s, int pair) {
+      return max(1, tiles_to(s.y, s.x, p.a.causal, (pair + 1) * 2 * p.tile_tokens - 1));
+    };
+    for (int s = warp; s < sequences; s += kThreads / 32) {
+      const int2 q = staged[s];
+      const int pairs = (q.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+      long long steps = 0;
+      for (int pair = lane; pair < pairs; pair += 32) steps += pair_steps(q, pair);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, off);
+      if (lane == 0) prefix[s] = steps * p.a.cache.kv_heads;
+    }
+    __syncthreads();
+    // Inclusive sums, by every warp for itself from here on where reads suffice.
+    if (warp == 0) {
+      long long base = 0;
+      for (int start = 0; start < sequences; start += 32) {
+        long long value = start + lane < sequences ? prefix[start + lane] : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const long long other = __shfl_up_sync(0xffffffffu, value, off);
+          if (lane >= off) value += other;
+        }
+        if (start + lane < sequences) prefix[start + lane] = base + value;
+        base += __shfl_sync(0xffffffffu, value, 31);
+      }
+    }
+    __syncthreads();
+    total = sequences > 0 ? prefix[sequences - 1] : 0;
+    shares = total / kLeastSteps;
+    shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
+    long long at = total;
+    walk.left = 0;
+    if (static_cast<long long>(blockIdx.x) < shares) {
+      at = total * blockIdx.x / shares;
+      walk.left = total * (blockIdx.x + 1) / shares - at;
+    }
+    walk.sequence = walk.kv_head = walk.pair = walk.t0 = walk.begin = walk.count = walk.keys = walk.pairs = 0;
+    if (walk.left > 0) {
+      int low = 0, high = sequences - 1;             // first sequence whose inclusive sum is beyond `at`
+      while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (prefix[mid] > at) high = mid;
+        else low = mid + 1;
+      }
+      const long long before = low > 0 ? prefix[low - 1] : 0, per_head = (prefix[low] - before) / p.a.cache.kv_heads;
+      const int2 q = staged[low];
+      walk.sequence = low;
+      walk.kv_head = static_cast<int>((at - before) / per_head);
+      long long rest = at - before - walk.kv_head * per_head;
+      for (int start = 0;; start += 32) {            // the pair that step `rest` of the head lies in
+        const int pair = start + lane, pairs = (q.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+        long long sum = pair < pairs ? pair_steps(q, pair) : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const long long other = __shfl_up_sync(0xffffffffu, sum, off);
+          if (lane >= off) sum += other;
+        }
+        const unsigned int beyond = __ballot_sync(0xffffffffu, sum > rest);
+        if (beyond || start + 32 >= pairs) {
+          const int found = beyond ? __ffs(beyond) - 1 : 31;
+          const long long in_front = found > 0 ? __shfl_sync(0xffffffffu, sum, found - 1) : 0;
+          walk.pair = start + found;
+          walk.t0 = static_cast<int>(rest - in_front);
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+      walk.look_up(p);
+    }
+  }
+  fence_proxy_async_smem();      // the staged lengths give way to tiles
+  __syncthreads();
+
+  // setmaxnreg.inc waits until the CTA's own register pool can supply the request: the totals must fit the launch's.
+  static_assert(128 * 104 + 256 * 200 <= kThreads * 168, "setmaxnreg totals exceed the launch allocation");
+  if (warp < 4) {
+  setmaxnreg_dec<104>();
+  if (warp == 0) {
+    // ------------------------------------------------------------ loader: one box per lane
+    int slot = 0;
+    uint32_t phase = 0, q_loads = 0;
+    bool ok = true;
+    Segment seg;
+    const int boxes = kTileN / p.box_rows;           // of 64 columns, per tile and half
+    const int box = lane / L::kHalves, half = lane % L::kHalves;
+    const bool has_box = box < boxes;
+    const int q_bytes = p.tile_tokens * p.group * 128 * L::kHalves;
+    ChunkSplit split = {};
+    while (ok && walk.next_working(p, seg)) {
+      if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (q_loads - 1) & 1u, abort_word, 101))) break;
+      ++q_loads;
+      if (seg.t0 == 0 && seg.t1 < seg.steps) {
+        // The item goes on in the shares behind this one, up to the last that begins in front of its end.
+        const long long item_end = total * (blockIdx.x + 1) / shares + (seg.steps - seg.t1);
+        const long long last = (item_end * shares - 1) / total;
+        split = {static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1, seg.begin, seg.count, seg.pair, seg.kv_head, {}};
+      }
+      const int tiles = max(seg.of(0), seg.of(1));
+      const int last_token = seg.begin + seg.count - 1;
+      const int token0 = seg.begin + seg.pair * 2 * p.tile_tokens, token1 = token0 + p.tile_tokens;
+      const bool second = token1 <= last_token;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, second ? 2 * q_bytes : q_bytes);
+        for (int c = 0; c < L::kHalves; ++c) {
+          tma_load_3d(smem_base + L::kQOff + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token0);
+          if (second) tma_load_3d(smem_base + L::kQOff + L::kTileBytes + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token1);
+        }
+      }
+      const int *pages = p.a.batch.page_table + seg.sequence * p.a.batch.table_stride;
+      auto key_of = [&](int j) { return (seg.t0 + j) * kTileN + box * p.box_rows; };
+      auto look_up = [&](int j) { return has_box && j < tiles && key_of(j) < seg.keys ? __ldg(pages + key_of(j) / p.a.cache.page_size) : -1; };
+      int page = look_up(0);
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int next_page = look_up(j + 1);
+        const int key = key_of(j);
+        const bool loads = has_box && key < seg.keys;
+        if (loads && (page < 0 || page >= p.a.cache.pages)) raise_status(p.a.refused, kRefusedPage);   // the box is filled with zeros
+        const int in_page = loads ? key % p.a.cache.page_size : 0;
+        const int y = p.rows_inside ? in_page : seg.kv_head, z = p.rows_inside ? seg.kv_head : in_page;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, loads)) * p.box_rows * 128;
+        const bool tail = (seg.t0 + j + 1) * kTileN > seg.keys;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {    // K_j, then V_j
+          if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), phase ^ 1u, abort_word, 102))) { ok = false; break; }
+          const uint32_t bar = which && tail ? tail_full(slot) : kv_full(slot);
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
+          if (loads)
+            tma_load_4d(smem_base + L::kRingOff + slot * L::kTileBytes + half * kBlockBytes + box * p.box_rows * 128, which ? &tmap_v : &tmap_k, bar,
+                        half * 64, y, z, page);
+          if (++slot == L::kSlots) { slot = 0; phase ^= 1u; }
+        }
+        page = next_page;
+      }
+    }
+    if (lane == 0) p.splits[blockIdx.x] = split;
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (the whole warp walks, one elected lane issues)
+    {
+      constexpr uint32_t idesc_s = umma_idesc_f16(kTileM, kTileN, kBf16, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_f16(kTileM, kHd, kBf16, false, true);
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      auto advance = [&]() { if (++slot == L::kSlots) { slot = 0; phase ^= 1u; } };
+      const uint64_t q_desc0 = umma_desc_kmajor(smem_base + L::kQOff);
+      const uint64_t q_desc1 = umma_desc_kmajor(smem_base + L::kQOff + L::kTileBytes);
+      const uint64_t ring_k_desc = umma_desc_kmajor(smem_base + L::kRingOff);
+      const uint64_t ring_v_desc = umma_desc_mnmajor(smem_base + L::kRingOff, kBlockBytes);
+      constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
+      auto issue_s = [&](auto tile_tag, int k_slot) {
+        constexpr int t = decltype(tile_tag)::value;
+        const uint64_t k_desc = ring_k_desc + static_cast<uint32_t>(k_slot) * kSlotStep;
+        const uint64_t q_desc = t ? q_desc1 : q_desc0;
+        const uint32_t d_tmem = tmem_base + kColS0 + t * 128;
+        if (elect_one_sync()) {
+#pragma unroll
+          for (int ks = 0; ks < kHd / 16; ++ks) {
+            constexpr uint32_t kBlockStep = kBlockBytes >> 4;
+            const uint32_t off = (ks >> 2) * kBlockStep + (ks & 3) * 2;
+            umma_f16_ss(d_tmem, q_desc + off, k_desc + off, idesc_s, ks != 0 ? 1u : 0u);
+          }
+          umma_commit(s_full(t));
+        }
+        __syncwarp();
+      };
+      auto issue_pv_part = [&](auto tile_tag, auto part_tag, int v_slot, bool accumulate, bool last) {
+        constexpr int t = decltype(tile_tag)::value;
+        constexpr int part = decltype(part_tag)::value;
+        const uint64_t v_desc = ring_v_desc + static_cast<uint32_t>(v_slot) * kSlotStep;
+        const uint32_t d_tmem = tmem_base + kColO0 + t * 128;
+        if (elect_one_sync()) {
+#pragma unroll
+          for (int ks = part ? 2 * kFirstChunks : 0; ks < (part ? 8 : 2 * kFirstChunks); ++ks) {
+            const uint64_t bdesc = v_desc + static_cast<uint32_t>((ks * 2048) >> 4);
+            const uint32_t acc = (accumulate || ks != 0) ? 1u : 0u;
+            umma_f16_ts(d_tmem, tmem_base + kColS0 + t * 128 + ks * 8, bdesc, idesc_o, acc);
+          }
+          if (part == kPParts - 1 && last) umma_commit(o_done(t));
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint32_t bar) {
+        if (elect_one_sync()) umma_commit(bar);
+        __syncwarp();
+      };
+
+      uint32_t base0 = 0, base1 = 0;
+      uint32_t q_count = 0;
+      Segment seg;
+      while (ok && walk.next_working(p, seg)) {
+        const int n0 = seg.of(0), n1 = seg.of(1);
+        const int n_max = max(n0, n1);
+        ok = mbar_wait(q_full, q_count & 1u, abort_word);
+        ++q_count;
+        if (ok) ok = mbar_wait(kv_full(slot), phase, abort_word);
+        if (ok) {
+          tc_fence_after();
+          if (n0 > 0) issue_s(std::integral_constant<int, 0>{}, slot);
+          if (n1 > 0) issue_s(std::integral_constant<int, 1>{}, slot);
+          commit(kv_empty(slot));
+          if (n_max == 1) commit(q_empty);
+          advance();
+        }
+        for (int j = 0; ok && j < n_max; ++j) {
+          const int v_slot = slot;
+          const uint32_t v_phase = phase;
+          advance();
+          const int k_slot = slot;
+          const uint32_t k_phase = phase;
+          const bool has_next = j + 1 < n_max;
+          if (has_next) advance();
+          if (!mbar_wait(kv_full(v_slot), v_phase, abort_word)) { ok = false; break; }
+          bool k_ready = false;
+          auto tile_step = [&](auto tile_tag, int n_tiles, uint32_t tile_base) {
+            constexpr int t = decltype(tile_tag)::value;
+            if (j < n_tiles) {
+              if (!mbar_wait_spin(p_part(t, 0), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
+              tc_fence_after();
+              issue_pv_part(tile_tag, std::integral_constant<int, 0>{}, v_slot, j > 0, false);
+              if (!mbar_wait_spin(p_part(t, 1), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
+              tc_fence_after();
+              issue_pv_part(tile_tag, std::integral_constant<int, 1>{}, v_slot, j > 0, j + 1 == n_tiles);
+            }
+            if (j + 1 < n_tiles) {
+              if (!k_ready) {
+                if (!mbar_wait(kv_full(k_slot), k_phase, abort_word)) { ok = false; return; }
+                tc_fence_after();
+                k_ready = true;
+              }
+              issue_s(tile_tag, k_slot);
+            }
+          };
+          tile_step(std::integral_constant<int, 0>{}, n0, base0);
+          if (ok) tile_step(std::integral_constant<int, 1>{}, n1, base1);
+          if (!ok) break;
+          commit(kv_empty(v_slot));
+          if (has_next) commit(kv_empty(k_slot));
+          if (j + 2 == n_max) commit(q_empty);
+        }
+        base0 += n0;
+        base1 += n1;
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ cleaner: zeroes V rows behind a sequence's last key
+    int slot = 0;
+    uint32_t phases = 0;                             // bit s: parity of the next tail in slot s
+    bool ok = true;
+    Segment seg;
+    while (ok && walk.next_working(p, seg)) {
+      const int tiles = max(seg.of(0), seg.of(1));
+      const int end = seg.t0 + tiles;
+      const int v_slot = (slot + 2 * tiles - 1) % L::kSlots;    // the last tile's V
+      if (end * kTileN > seg.keys) {
+        if (!__all_sync(0xffffffffu, mbar_wait(tail_full(v_slot), (phases >> v_slot) & 1u, abort_word, 105))) { ok = false; break; }
+        phases ^= 1u << v_slot;
+        const int valid = seg.keys - (end - 1) * kTileN;
+        const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+        const int chunks = (kTileN - valid) * 8;     // of 16 bytes, per half
+#pragma unroll
+        for (int h = 0; h < L::kHalves; ++h)
+          for (int i = lane; i < chunks; i += 32)
+            st_shared_v4(smem_base + L::kRingOff + v_slot * L::kTileBytes + h * kBlockBytes + valid * 128 + i * 16, zero);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kv_full(v_slot));
+      }
+      slot = (slot + 2 * tiles) % L::kSlots;
+    }
+  }
+  } else {
+    setmaxnreg_inc<200>();
+    // ------------------------------------------------------------ softmax / rescale / epilogue
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row_in_tile = quarter * 32 + lane;
+    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_sel + kColS0 + t * 128;
+    const uint32_t o_addr = tmem_base + lane_sel + kColO0 + t * 128;
+    uint32_t tiles_done = 0, items_done = 0;
+    bool ok = true;
+    const uint32_t out_stage = smem_base + L::kOutOff + (warp - 4) * kOutStageBytes;
+    WarpPlace *place = reinterpret_cast<WarpPlace *>(smem + L::kWalkOff + (warp - 4) * 96);
+    if (lane == 0) place->walk = walk;
+    __syncwarp();
+    while (ok) {
+      int my_tiles, row_limit, masked_from, key_base;     // keys from masked_from on are hidden from some row of the tile
+      {
+        ShareWalk at = place->walk;
+        Segment seg;
+        const bool more = at.next(p, seg);
+        __syncwarp();
+        if (lane == 0) { place->walk = at; place->segment = seg; }
+        __syncwarp();
+        if (!more) break;
+        my_tiles = seg.of(t);
+        key_base = seg.t0 * kTileN;
+        row_limit = seg.keys - 1;
+        masked_from = seg.keys;
+        if (p.a.causal) {                                   // token i sees keys up to keys - count + i
+          const int first = seg.keys - seg.count + (2 * seg.pair + t) * p.tile_tokens;
+          row_limit = min(row_limit, first + row_in_tile / p.group);
+          masked_from = min(masked_from, first + 1);
+        }
+      }
+      constexpr float kRescaleThreshold = 8.0f;
+      float m_ref = -INFINITY, m_true = -INFINITY, l_run = 0.f;
+
+      for (int j = 0; ok && j < my_tiles; ++j, ++tiles_done) {
+        if (!mbar_wait(s_full(t), tiles_done & 1u, abort_word, 110 + t)) { ok = false; break; }
+        tc_fence_after();
+        const int key0 = key_base + j * kTileN;
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+        tmem_wait_ld();
+        if (key0 + kTileN > masked_from) {
+          const int visible_in_tile = row_limit - key0;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i > visible_in_tile) r[i] = 0xff800000u;   // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) mx[a] = fmax3(__uint_as_float(r[32 * a]), __uint_as_float(r[32 * a + 1]), __uint_as_float(r[32 * a + 2]));
+#pragma unroll
+        for (int i = 3; i + 1 < 32; i += 2) {
+#pragma unroll
+          for (int a = 0; a < 4; ++a) mx[a] = fmax3(mx[a], __uint_as_float(r[32 * a + i]), __uint_as_float(r[32 * a + i + 1]));
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], __uint_as_float(r[32 * a + 31]));
+        const float raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        m_true = fmaxf(m_true, raw_max * p.scale_log2);
+        float alpha = 1.0f;
+        const bool moves = m_true - m_ref > kRescaleThreshold, any_moves = __any_sync(0xffffffffu, moves);
+        if (moves) {
+          alpha = exp2f(m_ref - m_true);
+          m_ref = m_true;
+        }
+        const float m_exp = (m_ref == -INFINITY) ? 0.f : m_ref;
+        const unsigned long long scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg_m2 = pack_f32x2(-m_exp, -m_exp);
+        unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const unsigned long long x2 = fma_f32x2(pack_f32x2(__uint_as_float(r[32 * c + i]), __uint_as_float(r[32 * c + i + 1])), scale2, neg_m2);
+            float x0, x1;
+            unpack_f32x2(x2, x0, x1);
+            const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+            sum2[(i >> 1) & 3] = add_f32x2(sum2[(i >> 1) & 3], pack_f32x2(e0, e1));
+            packed[i >> 1] = pack2<kBf16>(e0, e1);   // P is rounded to the storage type for the product with V; the sum is not
+          }
+          tmem_st_32x16(s_addr + c * 16, packed);    // P lies over the first 64 columns of S
+          if (c == kFirstChunks - 1 && j > 0 && any_moves) {
+#pragma unroll 1
+            for (int oc = 0; oc < kHd / 32; ++oc) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_addr + oc * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32(o_addr + oc * 32, o);
+            }
+          }
+          if (c == kFirstChunks - 1 || c == 3) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_part(t, c == 3 ? 1 : 0));
+          }
+        }
+        float s0, s1, s2, s3, s4, s5, s6, s7;
+        unpack_f32x2(sum2[0], s0, s1); unpack_f32x2(sum2[1], s2, s3); unpack_f32x2(sum2[2], s4, s5); unpack_f32x2(sum2[3], s6, s7);
+        l_run = l_run * alpha + (((s0 + s1) + (s2 + s3)) + ((s4 + s5) + (s6 + s7)));
+      }
+
+      if (ok && my_tiles > 0) ok = mbar_wait(o_done(t), items_done++ & 1u, abort_word, 114 + t);
+      const Segment seg = place->segment;
+      const int first_token = (2 * seg.pair + t) * p.tile_tokens;       // of the tile, within the sequence
+      const bool tile_used = first_token < seg.count;
+      const bool whole = seg.t0 == 0 && seg.t1 == seg.steps;
+      if (ok && tile_used && whole) {
+        tc_fence_after();
+        const bool empty = l_run == 0.f;
+        const float coefficient = empty ? 0.f : 1.0f / l_run;
+        const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
+        // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes.
+#pragma unroll 1
+        for (int half = 0; half < L::kHalves; ++half) {
+          uint32_t r[64];
+          if (my_tiles > 0) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_ld_32x32(o_addr + half * 64 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) r[i] = 0u;
+          }
+          __syncwarp();                              // the stage's previous contents have been read
+#pragma unroll
+          for (int i = 0; i < 64; i += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]) * coefficient, __uint_as_float(r[i + 2 * k + 1]) * coefficient);
+              if (empty) w[k] = filled;
+            }
+            st_shared_v4(out_stage + lane * 128 + (((i >> 3) ^ (lane & 7)) << 4), w);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r_out = i * 4 + (lane >> 3), chunk = lane & 7;
+            const int packed = quarter * 32 + r_out, at = packed / p.group, token_out = first_token + at;
+            if (at < p.tile_tokens && token_out < seg.count) {
+              uint32_t w[4];
+              ld_shared_v4(out_stage + r_out * 128 + ((chunk ^ (r_out & 7)) << 4), w);
+              uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(seg.begin + token_out) * p.a.out_token +
+                              (seg.kv_head * p.group + packed - at * p.group) * p.a.out_head + half * 64 + chunk * 8;
+              *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        const int at = row_in_tile / p.group, token = first_token + at;
+        if (p.a.lse && at < p.tile_tokens && token < seg.count)
+          p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + seg.kv_head * p.group + row_in_tile - at * p.group] =
+              empty ? -INFINITY : m_ref * 0.69314718055994530942f + logf(l_run);
+      } else if (ok && tile_used) {
+        // A part of an item: the state as it is, four columns of 32 rows to a store.
+        tc_fence_after();
+        float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (seg.t0 == 0 ? 1 : 0)) * 2 + t) * L::kRecordFloats;
+#pragma unroll 1
+        for (int part = 0; part < kHd / 32; ++part) {
+          uint32_t r[32];
+          if (my_tiles > 0) {
+            tmem_ld_32x32(o_addr + part * 32, r);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4 *>(record + ((part * 8 + (i >> 2)) * kTileM + row_in_tile) * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        }
+        *reinterpret_cast<float2 *>(record + kTileM * kHd + 2 * row_in_tile) = make_float2(m_ref, l_run);
+      }
+      // The accumulator has been read before this warp lets the next segment's first product over it, by its next arrival.
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_word != 0) {
+    for (int i = 0; i < 64; ++i) __nanosleep(10000);
+    if (threadIdx.x == 0) raise_status(p.a.status, *abort_word);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is the Q tile, blockIdx.z 32 columns, a thread a row.
+template <bool kBf16, int kHd>
+__global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
+  using L = Shape<kHd>;
+  pdl_wait();
+  pdl_launch_dependents();
+  const ChunkSplit split = p.splits[blockIdx.x];
+  const int t = blockIdx.y, row = threadIdx.x;
+  const int at = row / p.group, token = (2 * split.pair + t) * p.tile_tokens + at;
+  if (split.records == 0 || at >= p.tile_tokens || token >= split.count) return;
+  auto record = [&](int i) { return p.records + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * 2 + t) * L::kRecordFloats; };
+  float top = -INFINITY;
+  for (int i = 0; i < split.records; ++i) {
+    const float2 ml = *reinterpret_cast<const float2 *>(record(i) + kTileM * kHd + 2 * row);
+    if (ml.y > 0.f) top = fmaxf(top, ml.x);
+  }
+  const float m_exp = top == -INFINITY ? 0.f : top;
+  float l = 0.f, acc[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+  for (int i = 0; i < split.records; ++i) {
+    const float *r = record(i);
+    const float2 ml = *reinterpret_cast<const float2 *>(r + kTileM * kHd + 2 * row);
+    const float weight = ml.y > 0.f ? ex2_approx(ml.x - m_exp) : 0.f;
+    l = fmaf(ml.y, weight, l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float4 v = *reinterpret_cast<const float4 *>(r + ((blockIdx.z * 8 + e) * kTileM + row) * 4);
+      acc[4 * e] = fmaf(v.x, weight, acc[4 * e]);
+      acc[4 * e + 1] = fmaf(v.y, weight, acc[4 * e + 1]);
+      acc[4 * e + 2] = fmaf(v.z, weight, acc[4 * e + 2]);
+      acc[4 * e + 3] = fmaf(v.w, weight, acc[4 * e + 3]);
+    }
+  }
+  const bool empty = l == 0.f;
+  const float coefficient = empty ? 0.f : 1.0f / l;
+  const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
+  const int head = split.kv_head * p.group + row - at * p.group;
+  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.z * 32;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = pack2<kBf16>(acc[8 * e + 2 * k] * coefficient, acc[8 * e + 2 * k + 1] * coefficient);
+      if (empty) w[k] = filled;
+    }
+    *reinterpret_cast<uint4 *>(dst + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (p.a.lse && blockIdx.z == 0)
+    p.a.lse[static_cast<int64_t>(split.begin + token) * p.a.q_heads + head] = empty ? -INFINITY : top * 0.69314718055994530942f + logf(l);
+}
+
+// The largest power of two that divides the page size, at most a tile.
+int box_rows_of(int page_size) {
+  int rows = 1;
+  while (rows < kTileN && page_size % (2 * rows) == 0) rows *= 2;
+  return rows;
+}
+
+// Extents and strides (in bytes) of the cache's tensor maps, innermost first: rows inside heads or heads inside rows, pages
+// outside both, K and V alike; false for other orders. Strides of extents of one are free, but the map wants them to span
+// what lies inside.
+struct CacheMap {
+  int rows_inside;
+  uint64_t extents[4], strides[2][3];
+};
+bool make_cache_map(const PagedCacheArgs &c, CacheMap *m) {
+  const int64_t strides[2][3] = {{c.k_row, c.k_head, c.k_page}, {c.v_row, c.v_head, c.v_page}};
+  m->rows_inside = c.kv_heads > 1 && (c.page_size == 1 || c.k_row < c.k_head) ? 1 : 0;
+  const int order[3] = {m->rows_inside ? 0 : 1, m->rows_inside ? 1 : 0, 2};
+  const uint64_t extents[3] = {static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.kv_heads), static_cast<uint64_t>(c.pages)};
+  m->extents[0] = static_cast<uint64_t>(c.head_dim);
+  for (int i = 0; i < 3; ++i) m->extents[i + 1] = extents[order[i]];
+  for (int kind = 0; kind < 2; ++kind) {
+    uint64_t span = m->extents[0] * 2;
+    for (int i = 0; i < 3; ++i) {
+      uint64_t stride = static_cast<uint64_t>(strides[kind][order[i]]) * 2;
+      if (m->extents[i + 1] == 1) stride = span;
+      if (stride < span) return false;
+      m->strides[kind][i] = stride;
+      span = stride * m->extents[i + 1];
+    }
+  }
+  return true;
+}
+
+size_t chunk_record_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 4 * Shape<128>::kRecordFloats * sizeof(float); }
+
+}  // namespace
+
+bool attention_paged_chunk_supports(const AttentionPagedArgs &a) {
+  const int group = a.q_heads / a.cache.kv_heads;
+  if (!attention_paged_rows_supports(a) || group > kTileM || a.batch.sequences > kMaxSequences) return false;
+  if (box_rows_of(a.cache.page_size) < 8) return false;      // a box covers whole 8-row groups of the swizzle
+  CacheMap map;
+  return make_cache_map(a.cache, &map) &&
+         (a.q_heads == 1 || a.batch.tokens == 1 || a.q_token >= static_cast<int64_t>(a.q_heads - 1) * a.q_head + a.cache.head_dim);   // tokens outside heads
+}
+
+size_t attention_paged_chunk_workspace(int sm_count) { return chunk_record_bytes(sm_count) + static_cast<size_t>(sm_count) * sizeof(ChunkSplit); }
+
+wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int rows_limit, int sm_count, cudaStream_t stream) {
+  ChunkParams p{};
+  p.a = a;
+  p.group = a.q_heads / a.cache.kv_heads;
+  p.tile_tokens = kTileM / p.group;
+  p.box_rows = box_rows_of(a.cache.page_size);
+  p.rows_limit = rows_limit;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.records = static_cast<float *>(a.workspace);
+  p.splits = reinterpret_cast<ChunkSplit *>(static_cast<uint8_t *>(a.workspace) + chunk_record_bytes(sm_count));
+  CUtensorMap tq, tk, tv;
+  // Strides of extents of one are free, but the map wants them to span what lies inside.
+  const uint64_t d = static_cast<uint64_t>(a.cache.head_dim);
+  const uint64_t q_head = a.q_heads == 1 ? d * 2 : static_cast<uint64_t>(a.q_head) * 2;
+  const uint64_t q_token = a.batch.tokens == 1 ? q_head * a.q_heads : static_cast<uint64_t>(a.q_token) * 2;
+  wb200_status st = encode_tmap_strided(&tq, a.q, a.cache.format, 3, {d, static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.batch.tokens), 1},
+                                        {q_head, q_token, 0}, {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.tile_tokens), 1});
+  if (st != WB200_OK) return st;
+  CacheMap map;
+  if (!make_cache_map(a.cache, &map)) return fail(WB200_ERR_UNSUPPORTED, "paged cache outside the chunk kernel's domain");
+  p.rows_inside = map.rows_inside;
+  const uint32_t box = static_cast<uint32_t>(p.box_rows);
+  for (int kind = 0; kind < 2; ++kind) {
+    st = encode_tmap_strided(kind ? &tv : &tk, kind ? a.cache.v : a.cache.k, a.cache.format, 4, map.extents, map.strides[kind],
+                             {64, map.rows_inside ? box : 1u, map.rows_inside ? 1u : box, 1});
+    if (st != WB200_OK) return st;
+  }
+  const bool bf16 = a.cache.format == WB200_BF16, wide = a.cache.head_dim == 128;
+  const auto kernel = wide ? (bf16 ? attention_paged_chunk_kernel<true, 128> : attention_paged_chunk_kernel<false, 128>)
+                           : (bf16 ? attention_paged_chunk_kernel<true, 64> : attention_paged_chunk_kernel<false, 64>);
+  const auto fold = wide ? (bf16 ? attention_paged_chunk_fold_kernel<true, 128> : attention_paged_chunk_fold_kernel<false, 128>)
+                         : (bf16 ? attention_paged_chunk_fold_kernel<true, 64> : attention_paged_chunk_fold_kernel<false, 64>);
+  static PerDeviceOnce attributes;
+  st = attributes.run([]() -> wb200_status {
+    WB200_CUDA_CHECK(cudaFuncSetAttribute(attention_paged_chunk_kernel<true, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<128>::kBytes)));
+    WB200_CUDA_CHECK(cudaFuncSetAttribute(attention_paged_chunk_kernel<false, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<128>::kBytes)));
+    WB200_CUDA_CHECK(cudaFuncSetAttribute(attention_paged_chunk_kernel<true, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<64>::kBytes)));
+    WB200_CUDA_CHECK(cudaFuncSetAttribute(attention_paged_chunk_kernel<false, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<64>::kBytes)));
+    return WB200_OK;
+  });
+  if (st != WB200_OK) return st;
+  WB200_CUDA_CHECK(launch_dependent(kernel, sm_count, kThreads, wide ? Shape<128>::kBytes : Shape<64>::kBytes, stream, tq, tk, tv, p));
+  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, 2, a.cache.head_dim / 32), kTileM, 0, stream, p));
+  return WB200_OK;
+}
+
+}  // namespace wb200

@@ -83,6 +83,10 @@ wb200_status encode_tmap_3d(CUtensorMap *map, const void *base, int format, uint
 // Four dimensions without gaps, innermost first, and the box in the same order.
 wb200_status encode_tmap_4d_dense(CUtensorMap *map, const void *base, int format, const uint64_t (&extents)[4], const uint32_t (&box_extents)[4]);
 
+// Up to four dimensions with the pitches (bytes) of all but the innermost; entries from `rank` on are not read.
+wb200_status encode_tmap_strided(CUtensorMap *map, const void *base, int format, uint32_t rank, const uint64_t (&extents)[4],
+                                 const uint64_t (&pitches)[3], const uint32_t (&box_extents)[4]);
+
 // All of [host, host + bytes) lies in one page-locked allocation or registration, which the device addresses alike.
 bool page_locked_range(const void *host, size_t bytes);
 
@@ -334,7 +338,13 @@ wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cuda
 // Few rows per KV head (attention_paged_rows.cu): two launches.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
 size_t attention_paged_rows_workspace(int sm_count);
-wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int sm_count, cudaStream_t stream);
+wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int rows_limit, int sm_count, cudaStream_t stream);
+// Chunks of tokens on tcgen05 tensor cores (attention_paged_chunk.cu): two launches. `rows_limit` cuts a batch between the two:
+// sequences of at most that many (token, query head of a group) rows are the rows kernel's (0 there: all are), the others the
+// chunk kernel's (0 there: all are).
+bool attention_paged_chunk_supports(const AttentionPagedArgs &args);
+size_t attention_paged_chunk_workspace(int sm_count);
+wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &args, int rows_limit, int sm_count, cudaStream_t stream);
 
 struct PageTablesArgs {
   int sequences, table_width, pages, page_size;

@@ -81,6 +81,18 @@ wb200_status encode_tmap_4d_dense(CUtensorMap *map, const void *base, int format
   return encode(map, base, format, 4, dims, strides, box);
 }
 
+wb200_status encode_tmap_strided(CUtensorMap *map, const void *base, int format, uint32_t rank, const uint64_t (&extents)[4],
+                                 const uint64_t (&pitches)[3], const uint32_t (&box_extents)[4]) {
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4];
+  for (int i = 0; i < 4; ++i) {
+    dims[i] = extents[i];
+    box[i] = box_extents[i];
+    if (i < 3) strides[i] = pitches[i];
+  }
+  return encode(map, base, format, rank, dims, strides, box);
+}
+
 bool page_locked_range(const void *host, size_t bytes) {
   static const PointerAttributesFn fn = reinterpret_cast<PointerAttributesFn>(driver_function("cuPointerGetAttributes"));
   if (!fn) return false;
