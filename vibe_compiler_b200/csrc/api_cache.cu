@@ -120,9 +120,9 @@ PagedPlan plan_attention_paged(const AttentionPagedArgs &a, int sm_count) {
   if (!plan.rows) return plan;                     // the general kernel
   int64_t longest = a.batch.max_query > 0 ? a.batch.max_query : (a.batch.tokens <= a.batch.sequences ? 1 : a.batch.tokens);
   if (longest > a.batch.tokens) longest = a.batch.tokens;
-  plan.chunk = longest * (a.q_heads / a.cache.kv_heads) > kRowsBesideChunks && attention_paged_chunk_supports(a);
+  plan.chunk = longest * (a.q_heads / a.cache.kv_heads) > (getenv("XLIM") ? atoi(getenv("XLIM")) : kRowsBesideChunks) && attention_paged_chunk_supports(a);
   if (plan.chunk) {
-    plan.rows = a.batch.sequences > 1;
+    plan.rows = a.batch.sequences > 1 && !getenv("XCHUNK");
     plan.rows_at = (attention_paged_chunk_workspace(sm_count) + 255) / 256 * 256;
   }
   plan.workspace = plan.rows_at + (plan.rows ? attention_paged_rows_workspace(sm_count) : 0);

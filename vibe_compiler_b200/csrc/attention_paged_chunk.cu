@@ -10,10 +10,12 @@
 //            boxes at 8). The loader's lanes look up and issue a box each; page numbers are looked up one tile ahead.
 //   tails    Rows behind a sequence's last key are not masked by TMA's fill, as the page goes on, and 0 * v is not 0 for what a
 //            stale row may hold. A warp of its own zeroes those rows of V in shared memory before the products see them.
-//   shares   An item is two row tiles of one KV head of one sequence, its steps are its 128-key tiles under the causal limit.
-//            All items lie one behind the other on one axis of steps, cut into equal shares for the CTAs, so ragged batches and
-//            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A share's ends inside
-//            items leave f32 records, folded by a second kernel.
+//   halves   An item is two row tiles of one KV head of one sequence, so that one tile's products run under the other's softmax.
+//            Where the sequence has rows for one tile only, its odd key tiles take the second tile's place, and the two halves
+//            of the state are joined at the end: a step of one row tile costs half of one of two instead of nearly all of it.
+//   shares   All items lie one behind the other on one axis of work, cut into equal shares for the CTAs, so ragged batches and
+//            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A cut near the end of
+//            an item moves to it; others leave f32 records of the item's parts, folded by a second kernel.
 // Results depend on the lengths and the number of SMs only: repeats give the same bits.
 // Bound: the chain S -> softmax -> P V of a step (see attention_fa.cu), 4 * head_dim flop per visible (row, key) pair.
 #include <type_traits>
@@ -27,12 +29,17 @@ constexpr int kTileM = 128;                     // packed rows per Q tile (TMEM 
 constexpr int kTileN = 128;                     // keys per tile
 constexpr int kBlockBytes = 128 * 128;          // [128 rows][128 B], swizzled
 constexpr int kOutStageBytes = 32 * 128;        // a softmax warp's 32 rows x 64 columns of output
+constexpr int kPlaceBytes = 96;                 // of a softmax warp's place in its share
 constexpr int kThreads = 384;                   // warps: loader, MMA, cleaner, idle, 2 x 4 softmax
 constexpr int kPParts = 2;
 constexpr int kFirstChunks = 3;                 // 32-key chunks of the first part of P, of 4
 constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
 constexpr int kMaxSequences = 4096;             // staged in shared memory
-constexpr int kLeastSteps = 2;                  // no share is made smaller
+// Work, in half key tiles' time of two row tiles: a key tile of two row tiles, of one, and what an item costs by itself (its Q,
+// the first scores, the write-out: about one step of two tiles).
+constexpr int kPairWork = 2, kSingleWork = 1, kItemWork = 2;
+constexpr int kLeastWork = 4;                   // no share is made smaller
+constexpr int kLeastCut = 2;                    // a cut this near to an end of an item moves there
 
 template <int kHd>
 struct Shape {
@@ -44,7 +51,7 @@ struct Shape {
   static constexpr int kOutOff = kRingOff + kSlots * kTileBytes;
   static constexpr int kBarOff = kOutOff + 8 * kOutStageBytes;
   static constexpr int kWalkOff = kBarOff + 512;             // where the softmax warps keep their place in the share
-  static constexpr size_t kBytes = kWalkOff + 8 * 96 + 1024;
+  static constexpr size_t kBytes = kWalkOff + 8 * kPlaceBytes + 1024;
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
   static constexpr int kRecordFloats = kTileM * kHd + 2 * kTileM;   // acc as [kHd / 4][128 rows][4], then (m, l) per row
   static_assert(kMaxSequences * 16 <= kSlots * kTileBytes, "the staged lengths must fit the ring");
@@ -52,7 +59,7 @@ struct Shape {
 
 // What the fold has to know about the item that a CTA's share ends inside of; `records` 0: none.
 struct ChunkSplit {
-  int records, begin, count, pair, kv_head, reserved[3];
+  int records, begin, count, pair, kv_head, halved, reserved[2];
 };
 
 struct ChunkParams {
@@ -143,53 +150,82 @@ __device__ __forceinline__ int tiles_to(int keys, int count, int causal, int las
   return visible <= 0 ? 0 : (visible + kTileN - 1) / kTileN;
 }
 
-// One CTA's part of an item: key tiles [t0, t1) of the `steps` of two row tiles of a KV head of a sequence.
+// An item: the key tiles that Q tile 0 / 1 visits. A single row tile is halved: tile t takes every second key tile, from t on.
+struct Item {
+  int n0, n1, steps, halved;
+};
+__device__ __forceinline__ Item make_item(const ChunkParams &p, int count, int keys, int pair) {
+  Item item;
+  const int first = pair * 2 * p.tile_tokens;
+  item.halved = first + p.tile_tokens >= count;
+  item.n0 = tiles_to(keys, count, p.a.causal, first + p.tile_tokens - 1);
+  item.n1 = item.halved ? 0 : tiles_to(keys, count, p.a.causal, first + 2 * p.tile_tokens - 1);
+  item.steps = max(1, max(item.n0, item.n1));
+  return item;
+}
+__device__ __forceinline__ int item_work(const Item &item) { return kItemWork + item.steps * (item.halved ? kSingleWork : kPairWork); }
+// The key tile that a cut at work `x` of an item falls on; 0 and `steps` are the item's ends.
+__device__ __forceinline__ int cut_tile(const Item &item, int x, int least_cut) {
+  const int all = item_work(item), each = item.halved ? kSingleWork : kPairWork;
+  if (x < kItemWork + least_cut) return 0;
+  if (x + least_cut > all) return item.steps;
+  return min(max((x - kItemWork + each / 2) / each, 1), item.steps - 1);
+}
+
+// A place between two key tiles: in front of tile `tile` of the item.
+struct Place {
+  int sequence, kv_head, pair, tile;
+};
+// One CTA's part of an item: key tiles [t0, t1) of its steps.
 struct Segment {
   int begin, count, keys;          // the sequence
   int sequence, kv_head, pair;
-  int n0, n1;                      // key tiles that Q tile 0 / 1 visits in all
-  int steps, t0, t1;
-  __device__ __forceinline__ int of(int t) const {            // tiles of this segment for Q tile t
-    const int n = min(t ? n1 : n0, t1) - t0;
-    return n < 0 ? 0 : n;
+  int n0, n1, halved;
+  int whole;
+  int t0, t1;
+  __device__ __forceinline__ int of(int t) const {            // key tiles of this segment for Q tile t
+    if (halved) return (max(0, min(n0, t1) - t0) + 1 - t) >> 1;
+    return max(0, min(t ? n1 : n0, t1) - t0);
   }
+  __device__ __forceinline__ int tiles() const { return halved ? max(0, min(n0, t1) - t0) : max(of(0), of(1)); }
 };
-// Walks a CTA's share: the same sequence of segments in every warp.
+// Walks a CTA's share: the same segments in every warp.
 struct ShareWalk {
-  long long left;                  // steps of the share not yet walked
-  int sequence, kv_head, pair, t0;
-  int begin, count, keys, pairs;   // of the current sequence; count 0: to be looked up
+  Place at, end;                   // at.sequence == the batch's: done
+  int begin, count, keys, pairs;   // of the current sequence; count 0: another kernel's, or empty
 
   __device__ __forceinline__ void look_up(const ChunkParams &p) {
-    const PagedSequence s = paged_sequence(p.a.batch, p.a.cache, sequence, p.a.refused, false);
+    const PagedSequence s = paged_sequence(p.a.batch, p.a.cache, at.sequence, p.a.refused, false);
     const bool mine = static_cast<long long>(s.count) * p.group > p.rows_limit;
     begin = s.begin; count = mine ? s.count : 0; keys = s.keys;
     pairs = (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
   }
   __device__ __forceinline__ bool next(const ChunkParams &p, Segment &out) {
-    if (left <= 0) return false;
-    while (count == 0 || kv_head == p.a.cache.kv_heads) {
-      kv_head = pair = t0 = 0;
-      if (++sequence >= p.a.batch.sequences) return false;
-      look_up(p);
+    while (at.sequence < p.a.batch.sequences) {
+      if (count == 0 || at.kv_head == p.a.cache.kv_heads) {
+        at = {at.sequence + 1, 0, 0, 0};
+        if (at.sequence < p.a.batch.sequences) look_up(p);
+        continue;
+      }
+      const Item item = make_item(p, count, keys, at.pair);
+      const bool last = at.sequence == end.sequence && at.kv_head == end.kv_head && at.pair == end.pair;
+      out.begin = begin; out.count = count; out.keys = keys;
+      out.sequence = at.sequence; out.kv_head = at.kv_head; out.pair = at.pair;
+      out.n0 = item.n0; out.n1 = item.n1; out.halved = item.halved;
+      out.t0 = at.tile;
+      out.t1 = last ? min(end.tile, item.steps) : item.steps;
+      out.whole = out.t0 == 0 && out.t1 == item.steps;
+      if (last) at.sequence = p.a.batch.sequences;
+      at.tile = 0;
+      if (++at.pair == pairs) { at.pair = 0; ++at.kv_head; }
+      if (out.t1 > out.t0) return true;
     }
-    out.begin = begin; out.count = count; out.keys = keys; out.sequence = sequence; out.kv_head = kv_head; out.pair = pair;
-    const int first = pair * 2 * p.tile_tokens;
-    out.n0 = tiles_to(keys, count, p.a.causal, first + p.tile_tokens - 1);
-    out.n1 = first + p.tile_tokens < count ? tiles_to(keys, count, p.a.causal, first + 2 * p.tile_tokens - 1) : 0;
-    const int tiles = max(out.n0, out.n1);
-    out.steps = max(tiles, 1);
-    out.t0 = t0;
-    out.t1 = static_cast<int>(min(static_cast<long long>(out.steps), t0 + left));
-    left -= out.t1 - out.t0;
-    t0 = 0;
-    if (++pair == pairs) { pair = 0; ++kv_head; }
-    return true;
+    return false;
   }
   // The next segment with keys to visit.
   __device__ __forceinline__ bool next_working(const ChunkParams &p, Segment &out) {
     while (next(p, out))
-      if (out.of(0) > 0 || out.of(1) > 0) return true;
+      if (out.tiles() > 0) return true;
     return false;
   }
 };
@@ -199,7 +235,7 @@ struct WarpPlace {
   ShareWalk walk;
   Segment segment;
 };
-static_assert(sizeof(WarpPlace) <= 96, "the places' area");
+static_assert(sizeof(WarpPlace) <= kPlaceBytes, "the places' area");
 
 template <bool kBf16, int kHd>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -221,10 +257,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   auto p_part = [&](int t, int part) { return bar_base + 8u * (kFixed + 3 + kPParts * t + part); };
   auto o_done = [&](int t) { return bar_base + 8u * (kFixed + 3 + 2 * kPParts + t); };
   const uint32_t q_empty = bar_base + 8u * (kFixed + 5 + 2 * kPParts);
+  auto half_ready = [&](int quarter) { return bar_base + 8u * (kFixed + 6 + 2 * kPParts + quarter); };   // tile 1's half may be read
+  auto half_read = [&](int quarter) { return bar_base + 8u * (kFixed + 10 + 2 * kPParts + quarter); };   // and has been
   uint8_t *bar_ptr = smem + L::kBarOff;
-  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 6 + 2 * kPParts));
-  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 7 + 2 * kPParts));
-  static_assert(8 * (kFixed + 8 + 2 * kPParts) <= 512, "the barriers must fit their area");
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 14 + 2 * kPParts));
+  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 15 + 2 * kPParts));
+  static_assert(8 * (kFixed + 16 + 2 * kPParts) <= 512, "the barriers must fit their area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -240,6 +278,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       mbar_init(s_full(t), 1);
       for (int part = 0; part < kPParts; ++part) mbar_init(p_part(t, part), kTileM / 32);
       mbar_init(o_done(t), 1);
+    }
+    for (int quarter = 0; quarter < 4; ++quarter) {
+      mbar_init(half_ready(quarter), 1);
+      mbar_init(half_read(quarter), 1);
     }
     *abort_word = 0;
     fence_mbar_init();
@@ -258,32 +300,29 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- this CTA's share of all steps; the lengths are staged in the ring's memory
+  // ---- this CTA's share of all work; the lengths are staged in the ring's memory
   ShareWalk walk;
-  long long total, shares;
   {
     int2 *staged = reinterpret_cast<int2 *>(smem + L::kRingOff);                                       // (count, keys)
-    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int2));
+    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int2));   // inclusive sums of work
     const int sequences = p.a.batch.sequences;
     for (int s = threadIdx.x; s < sequences; s += kThreads) {
       const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, s, p.a.refused, blockIdx.x == 0);
       staged[s] = make_int2(static_cast<long long>(q.count) * p.group > p.rows_limit ? q.count : 0, q.keys);
     }
     __syncthreads();
-    auto pair_steps = [&](int2 s, int pair) {
-      return max(1, tiles_to(s.y, s.x, p.a.causal, (pair + 1) * 2 * p.tile_tokens - 1));
-    };
+    auto pairs_of = [&](int2 s) { return (s.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
+    auto pair_work = [&](int2 s, int pair) { return static_cast<long long>(item_work(make_item(p, s.x, s.y, pair))); };
     for (int s = warp; s < sequences; s += kThreads / 32) {
       const int2 q = staged[s];
-      const int pairs = (q.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-      long long steps = 0;
-      for (int pair = lane; pair < pairs; pair += 32) steps += pair_steps(q, pair);
+      const int pairs = pairs_of(q);
+      long long work = 0;
+      for (int pair = lane; pair < pairs; pair += 32) work += pair_work(q, pair);
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, off);
-      if (lane == 0) prefix[s] = steps * p.a.cache.kv_heads;
+      for (int off = 16; off > 0; off >>= 1) work += __shfl_xor_sync(0xffffffffu, work, off);
+      if (lane == 0) prefix[s] = work * p.a.cache.kv_heads;
     }
     __syncthreads();
-    // Inclusive sums, by every warp for itself from here on where reads suffice.
     if (warp == 0) {
       long long base = 0;
       for (int start = 0; start < sequences; start += 32) {
@@ -298,31 +337,30 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       }
     }
     __syncthreads();
-    total = sequences > 0 ? prefix[sequences - 1] : 0;
-    shares = total / kLeastSteps;
+    const long long total = sequences > 0 ? prefix[sequences - 1] : 0;
+    long long shares = total / kLeastWork;
     shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
-    long long at = total;
-    walk.left = 0;
-    if (static_cast<long long>(blockIdx.x) < shares) {
-      at = total * blockIdx.x / shares;
-      walk.left = total * (blockIdx.x + 1) / shares - at;
-    }
-    walk.sequence = walk.kv_head = walk.pair = walk.t0 = walk.begin = walk.count = walk.keys = walk.pairs = 0;
-    if (walk.left > 0) {
-      int low = 0, high = sequences - 1;             // first sequence whose inclusive sum is beyond `at`
+    const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(total / shares / 32, 1ll << 20)));
+    // Where the cut in front of share `index` falls; also the item it falls on, and the work in front of that.
+    auto cut = [&](long long index, Item &item, long long &item_at) {
+      const long long x = total * index / shares;
+      Place place = {sequences, 0, 0, 0};
+      if (x >= total) return place;
+      int low = 0, high = sequences - 1;             // first sequence whose sum is beyond x
       while (low < high) {
         const int mid = (low + high) >> 1;
-        if (prefix[mid] > at) high = mid;
+        if (prefix[mid] > x) high = mid;
         else low = mid + 1;
       }
       const long long before = low > 0 ? prefix[low - 1] : 0, per_head = (prefix[low] - before) / p.a.cache.kv_heads;
       const int2 q = staged[low];
-      walk.sequence = low;
-      walk.kv_head = static_cast<int>((at - before) / per_head);
-      long long rest = at - before - walk.kv_head * per_head;
-      for (int start = 0;; start += 32) {            // the pair that step `rest` of the head lies in
-        const int pair = start + lane, pairs = (q.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-        long long sum = pair < pairs ? pair_steps(q, pair) : 0;
+      const int pairs = pairs_of(q);
+      place.sequence = low;
+      place.kv_head = static_cast<int>((x - before) / per_head);
+      long long rest = x - before - place.kv_head * per_head;
+      for (int start = 0;; start += 32) {            // the pair of row tiles that work `rest` of the head lies in
+        const int pair = start + lane;
+        long long sum = pair < pairs ? pair_work(q, pair) : 0;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
           const long long other = __shfl_up_sync(0xffffffffu, sum, off);
@@ -332,14 +370,36 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         if (beyond || start + 32 >= pairs) {
           const int found = beyond ? __ffs(beyond) - 1 : 31;
           const long long in_front = found > 0 ? __shfl_sync(0xffffffffu, sum, found - 1) : 0;
-          walk.pair = start + found;
-          walk.t0 = static_cast<int>(rest - in_front);
+          place.pair = start + found;
+          rest -= in_front;
           break;
         }
         rest -= __shfl_sync(0xffffffffu, sum, 31);
       }
+      item = make_item(p, q.x, q.y, place.pair);
+      item_at = x - rest;
+      place.tile = cut_tile(item, static_cast<int>(rest), least_cut);
+      return place;
+    };
+    walk.at = walk.end = {sequences, 0, 0, 0};
+    walk.begin = walk.count = walk.keys = walk.pairs = 0;
+    ChunkSplit split = {};
+    if (static_cast<long long>(blockIdx.x) < shares && total > 0) {
+      Item item;
+      long long item_at = 0;
+      walk.at = cut(blockIdx.x, item, item_at);
+      walk.end = cut(blockIdx.x + 1, item, item_at);
       walk.look_up(p);
+      const Place &e = walk.end;
+      const bool starts_here = !(walk.at.sequence == e.sequence && walk.at.kv_head == e.kv_head && walk.at.pair == e.pair && walk.at.tile > 0);
+      if (e.sequence < sequences && e.tile > 0 && e.tile < item.steps && starts_here) {
+        // The item goes on in the shares behind this one, up to the last whose cut does not move to its end.
+        const long long last = ((item_at + item_work(item) - least_cut + 1) * shares - 1) / total;
+        const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, e.sequence, p.a.refused, false);
+        split = {static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1, q.begin, q.count, e.pair, e.kv_head, item.halved, {}};
+      }
     }
+    if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
   }
   fence_proxy_async_smem();      // the staged lengths give way to tiles
   __syncthreads();
@@ -358,55 +418,62 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     const int box = lane / L::kHalves, half = lane % L::kHalves;
     const bool has_box = box < boxes;
     const int q_bytes = p.tile_tokens * p.group * 128 * L::kHalves;
-    ChunkSplit split = {};
     while (ok && walk.next_working(p, seg)) {
       if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (q_loads - 1) & 1u, abort_word, 101))) break;
       ++q_loads;
-      if (seg.t0 == 0 && seg.t1 < seg.steps) {
-        // The item goes on in the shares behind this one, up to the last that begins in front of its end.
-        const long long item_end = total * (blockIdx.x + 1) / shares + (seg.steps - seg.t1);
-        const long long last = (item_end * shares - 1) / total;
-        split = {static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1, seg.begin, seg.count, seg.pair, seg.kv_head, {}};
-      }
-      const int tiles = max(seg.of(0), seg.of(1));
-      const int last_token = seg.begin + seg.count - 1;
+      const int tiles = seg.tiles();
       const int token0 = seg.begin + seg.pair * 2 * p.tile_tokens, token1 = token0 + p.tile_tokens;
-      const bool second = token1 <= last_token;
       if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, second ? 2 * q_bytes : q_bytes);
+        mbar_arrive_expect_tx(q_full, seg.halved ? q_bytes : 2 * q_bytes);
         for (int c = 0; c < L::kHalves; ++c) {
           tma_load_3d(smem_base + L::kQOff + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token0);
-          if (second) tma_load_3d(smem_base + L::kQOff + L::kTileBytes + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token1);
+          if (!seg.halved) tma_load_3d(smem_base + L::kQOff + L::kTileBytes + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token1);
         }
       }
       const int *pages = p.a.batch.page_table + seg.sequence * p.a.batch.table_stride;
       auto key_of = [&](int j) { return (seg.t0 + j) * kTileN + box * p.box_rows; };
       auto look_up = [&](int j) { return has_box && j < tiles && key_of(j) < seg.keys ? __ldg(pages + key_of(j) / p.a.cache.page_size) : -1; };
-      int page = look_up(0);
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int next_page = look_up(j + 1);
+      auto load = [&](int j, int page, bool is_v) {
         const int key = key_of(j);
         const bool loads = has_box && key < seg.keys;
-        if (loads && (page < 0 || page >= p.a.cache.pages)) raise_status(p.a.refused, kRefusedPage);   // the box is filled with zeros
+        if (loads && !is_v && (page < 0 || page >= p.a.cache.pages)) raise_status(p.a.refused, kRefusedPage);   // the box is filled with zeros
         const int in_page = loads ? key % p.a.cache.page_size : 0;
         const int y = p.rows_inside ? in_page : seg.kv_head, z = p.rows_inside ? seg.kv_head : in_page;
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, loads)) * p.box_rows * 128;
-        const bool tail = (seg.t0 + j + 1) * kTileN > seg.keys;
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {    // K_j, then V_j
-          if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), phase ^ 1u, abort_word, 102))) { ok = false; break; }
-          const uint32_t bar = which && tail ? tail_full(slot) : kv_full(slot);
-          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-          __syncwarp();
-          if (loads)
-            tma_load_4d(smem_base + L::kRingOff + slot * L::kTileBytes + half * kBlockBytes + box * p.box_rows * 128, which ? &tmap_v : &tmap_k, bar,
-                        half * 64, y, z, page);
-          if (++slot == L::kSlots) { slot = 0; phase ^= 1u; }
+        if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), phase ^ 1u, abort_word, 102))) { ok = false; return; }
+        const uint32_t bar = is_v && (seg.t0 + j + 1) * kTileN > seg.keys ? tail_full(slot) : kv_full(slot);
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+        __syncwarp();
+        if (loads)
+          tma_load_4d(smem_base + L::kRingOff + slot * L::kTileBytes + half * kBlockBytes + box * p.box_rows * 128, is_v ? &tmap_v : &tmap_k, bar,
+                      half * 64, y, z, page);
+        if (++slot == L::kSlots) { slot = 0; phase ^= 1u; }
+      };
+      // The order in which the MMA warp takes them: K of the first tile of each row tile, then V of a tile and K of the next
+      // one of the same row tile in turn.
+      if (!seg.halved) {
+        int page = look_up(0);
+        for (int j = 0; j < tiles && ok; ++j) {
+          const int next_page = look_up(j + 1);
+          load(j, page, false);
+          if (ok) load(j, page, true);
+          page = next_page;
         }
-        page = next_page;
+      } else {
+        int even = look_up(0), odd = look_up(1);
+        load(0, even, false);
+        if (ok && tiles > 1) load(1, odd, false);
+        for (int j = 0; j < tiles && ok; j += 2) {
+          const int next_even = look_up(j + 2), next_odd = look_up(j + 3);
+          load(j, even, true);
+          if (ok && j + 2 < tiles) load(j + 2, next_even, false);
+          if (ok && j + 1 < tiles) load(j + 1, odd, true);
+          if (ok && j + 3 < tiles) load(j + 3, next_odd, false);
+          even = next_even;
+          odd = next_odd;
+        }
       }
     }
-    if (lane == 0) p.splits[blockIdx.x] = split;
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (the whole warp walks, one elected lane issues)
     {
@@ -421,10 +488,9 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       const uint64_t ring_k_desc = umma_desc_kmajor(smem_base + L::kRingOff);
       const uint64_t ring_v_desc = umma_desc_mnmajor(smem_base + L::kRingOff, kBlockBytes);
       constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
-      auto issue_s = [&](auto tile_tag, int k_slot) {
+      auto issue_s = [&](auto tile_tag, int k_slot, uint64_t q_desc) {
         constexpr int t = decltype(tile_tag)::value;
         const uint64_t k_desc = ring_k_desc + static_cast<uint32_t>(k_slot) * kSlotStep;
-        const uint64_t q_desc = t ? q_desc1 : q_desc0;
         const uint32_t d_tmem = tmem_base + kColS0 + t * 128;
         if (elect_one_sync()) {
 #pragma unroll
@@ -461,55 +527,89 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       uint32_t base0 = 0, base1 = 0;
       uint32_t q_count = 0;
       Segment seg;
+      using Tile0 = std::integral_constant<int, 0>;
+      using Tile1 = std::integral_constant<int, 1>;
       while (ok && walk.next_working(p, seg)) {
         const int n0 = seg.of(0), n1 = seg.of(1);
         const int n_max = max(n0, n1);
         ok = mbar_wait(q_full, q_count & 1u, abort_word);
         ++q_count;
-        if (ok) ok = mbar_wait(kv_full(slot), phase, abort_word);
-        if (ok) {
-          tc_fence_after();
-          if (n0 > 0) issue_s(std::integral_constant<int, 0>{}, slot);
-          if (n1 > 0) issue_s(std::integral_constant<int, 1>{}, slot);
-          commit(kv_empty(slot));
-          if (n_max == 1) commit(q_empty);
-          advance();
-        }
-        for (int j = 0; ok && j < n_max; ++j) {
-          const int v_slot = slot;
-          const uint32_t v_phase = phase;
-          advance();
-          const int k_slot = slot;
-          const uint32_t k_phase = phase;
-          const bool has_next = j + 1 < n_max;
-          if (has_next) advance();
-          if (!mbar_wait(kv_full(v_slot), v_phase, abort_word)) { ok = false; break; }
-          bool k_ready = false;
-          auto tile_step = [&](auto tile_tag, int n_tiles, uint32_t tile_base) {
-            constexpr int t = decltype(tile_tag)::value;
-            if (j < n_tiles) {
-              if (!mbar_wait_spin(p_part(t, 0), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
-              tc_fence_after();
-              issue_pv_part(tile_tag, std::integral_constant<int, 0>{}, v_slot, j > 0, false);
-              if (!mbar_wait_spin(p_part(t, 1), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
-              tc_fence_after();
-              issue_pv_part(tile_tag, std::integral_constant<int, 1>{}, v_slot, j > 0, j + 1 == n_tiles);
-            }
-            if (j + 1 < n_tiles) {
-              if (!k_ready) {
-                if (!mbar_wait(kv_full(k_slot), k_phase, abort_word)) { ok = false; return; }
+        if (!seg.halved) {
+          if (ok) ok = mbar_wait(kv_full(slot), phase, abort_word);
+          if (ok) {
+            tc_fence_after();
+            if (n0 > 0) issue_s(Tile0{}, slot, q_desc0);
+            if (n1 > 0) issue_s(Tile1{}, slot, q_desc1);
+            commit(kv_empty(slot));
+            if (n_max == 1) commit(q_empty);
+            advance();
+          }
+          for (int j = 0; ok && j < n_max; ++j) {
+            const int v_slot = slot;
+            const uint32_t v_phase = phase;
+            advance();
+            const int k_slot = slot;
+            const uint32_t k_phase = phase;
+            const bool has_next = j + 1 < n_max;
+            if (has_next) advance();
+            if (!mbar_wait(kv_full(v_slot), v_phase, abort_word)) { ok = false; break; }
+            bool k_ready = false;
+            auto tile_step = [&](auto tile_tag, int n_tiles, uint32_t tile_base, uint64_t q_desc) {
+              constexpr int t = decltype(tile_tag)::value;
+              if (j < n_tiles) {
+                if (!mbar_wait_spin(p_part(t, 0), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
                 tc_fence_after();
-                k_ready = true;
+                issue_pv_part(tile_tag, Tile0{}, v_slot, j > 0, false);
+                if (!mbar_wait_spin(p_part(t, 1), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
+                tc_fence_after();
+                issue_pv_part(tile_tag, Tile1{}, v_slot, j > 0, j + 1 == n_tiles);
               }
-              issue_s(tile_tag, k_slot);
-            }
+              if (j + 1 < n_tiles) {
+                if (!k_ready) {
+                  if (!mbar_wait(kv_full(k_slot), k_phase, abort_word)) { ok = false; return; }
+                  tc_fence_after();
+                  k_ready = true;
+                }
+                issue_s(tile_tag, k_slot, q_desc);
+              }
+            };
+            tile_step(Tile0{}, n0, base0, q_desc0);
+            if (ok) tile_step(Tile1{}, n1, base1, q_desc1);
+            if (!ok) break;
+            commit(kv_empty(v_slot));
+            if (has_next) commit(kv_empty(k_slot));
+            if (j + 2 == n_max) commit(q_empty);
+          }
+        } else {
+          // Both tiles' scores come from the one row tile; each has K and V tiles of its own.
+          auto scores = [&](auto tile_tag) {
+            if (!mbar_wait(kv_full(slot), phase, abort_word)) { ok = false; return; }
+            tc_fence_after();
+            issue_s(tile_tag, slot, q_desc0);
+            commit(kv_empty(slot));
+            advance();
           };
-          tile_step(std::integral_constant<int, 0>{}, n0, base0);
-          if (ok) tile_step(std::integral_constant<int, 1>{}, n1, base1);
-          if (!ok) break;
-          commit(kv_empty(v_slot));
-          if (has_next) commit(kv_empty(k_slot));
-          if (j + 2 == n_max) commit(q_empty);
+          auto half_step = [&](auto tile_tag, int j, int n_tiles, uint32_t tile_base) {
+            constexpr int t = decltype(tile_tag)::value;
+            if (!mbar_wait(kv_full(slot), phase, abort_word)) { ok = false; return; }
+            if (!mbar_wait_spin(p_part(t, 0), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
+            tc_fence_after();
+            issue_pv_part(tile_tag, Tile0{}, slot, j > 0, false);
+            if (!mbar_wait_spin(p_part(t, 1), (tile_base + j) & 1u, abort_word)) { ok = false; return; }
+            tc_fence_after();
+            issue_pv_part(tile_tag, Tile1{}, slot, j > 0, j + 1 == n_tiles);
+            commit(kv_empty(slot));
+            advance();
+            if (j + 1 < n_tiles) scores(tile_tag);
+          };
+          if (ok) scores(Tile0{});
+          if (ok && n1 > 0) scores(Tile1{});
+          if (ok && n0 == 1) commit(q_empty);
+          for (int j = 0; ok && j < n0; ++j) {
+            half_step(Tile0{}, j, n0, base0);
+            if (ok && j < n1) half_step(Tile1{}, j, n1, base1);
+            if (ok && j + 2 == n0) commit(q_empty);
+          }
         }
         base0 += n0;
         base1 += n1;
@@ -522,7 +622,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     bool ok = true;
     Segment seg;
     while (ok && walk.next_working(p, seg)) {
-      const int tiles = max(seg.of(0), seg.of(1));
+      const int tiles = seg.tiles();
       const int end = seg.t0 + tiles;
       const int v_slot = (slot + 2 * tiles - 1) % L::kSlots;    // the last tile's V
       if (end * kTileN > seg.keys) {
@@ -551,14 +651,14 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_sel + kColS0 + t * 128;
     const uint32_t o_addr = tmem_base + lane_sel + kColO0 + t * 128;
-    uint32_t tiles_done = 0, items_done = 0;
+    uint32_t tiles_done = 0, items_done = 0, joins = 0;
     bool ok = true;
     const uint32_t out_stage = smem_base + L::kOutOff + (warp - 4) * kOutStageBytes;
-    WarpPlace *place = reinterpret_cast<WarpPlace *>(smem + L::kWalkOff + (warp - 4) * 96);
+    WarpPlace *place = reinterpret_cast<WarpPlace *>(smem + L::kWalkOff + (warp - 4) * kPlaceBytes);
     if (lane == 0) place->walk = walk;
     __syncwarp();
     while (ok) {
-      int my_tiles, row_limit, masked_from, key_base;     // keys from masked_from on are hidden from some row of the tile
+      int my_tiles, row_limit, masked_from, key_base, key_step;     // keys from masked_from on are hidden from some row of the tile
       {
         ShareWalk at = place->walk;
         Segment seg;
@@ -568,11 +668,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         __syncwarp();
         if (!more) break;
         my_tiles = seg.of(t);
-        key_base = seg.t0 * kTileN;
+        key_base = (seg.t0 + (seg.halved ? t : 0)) * kTileN;
+        key_step = (seg.halved ? 2 : 1) * kTileN;
         row_limit = seg.keys - 1;
         masked_from = seg.keys;
         if (p.a.causal) {                                   // token i sees keys up to keys - count + i
-          const int first = seg.keys - seg.count + (2 * seg.pair + t) * p.tile_tokens;
+          const int first = seg.keys - seg.count + (2 * seg.pair + (seg.halved ? 0 : t)) * p.tile_tokens;
           row_limit = min(row_limit, first + row_in_tile / p.group);
           masked_from = min(masked_from, first + 1);
         }
@@ -583,7 +684,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       for (int j = 0; ok && j < my_tiles; ++j, ++tiles_done) {
         if (!mbar_wait(s_full(t), tiles_done & 1u, abort_word, 110 + t)) { ok = false; break; }
         tc_fence_after();
-        const int key0 = key_base + j * kTileN;
+        const int key0 = key_base + j * key_step;
         uint32_t r[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
@@ -653,13 +754,34 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 
       if (ok && my_tiles > 0) ok = mbar_wait(o_done(t), items_done++ & 1u, abort_word, 114 + t);
       const Segment seg = place->segment;
-      const int first_token = (2 * seg.pair + t) * p.tile_tokens;       // of the tile, within the sequence
-      const bool tile_used = first_token < seg.count;
-      const bool whole = seg.t0 == 0 && seg.t1 == seg.steps;
-      if (ok && tile_used && whole) {
+      const int first_token = (2 * seg.pair + (seg.halved ? 0 : t)) * p.tile_tokens;       // of the tile, within the sequence
+      const bool joined = seg.halved && seg.whole;
+      if (ok && joined && t == 1) {
+        // The second half of a halved item: the first tile's warp of the same TMEM lanes reads the accumulator itself.
+        *reinterpret_cast<float2 *>(smem + L::kOutOff + (warp - 4) * kOutStageBytes + lane * 8) = make_float2(m_ref, l_run);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(half_ready(quarter));
+        ok = mbar_wait(half_read(quarter), joins++ & 1u, abort_word, 116);
+      } else if (ok && seg.whole) {
+        float scale0 = 1.f, scale1 = 0.f;              // of the two halves
+        bool second_half = false;
+        if (joined) {
+          ok = mbar_wait(half_ready(quarter), joins++ & 1u, abort_word, 117);
+          if (!ok) break;
+          const float2 other = *reinterpret_cast<const float2 *>(smem + L::kOutOff + warp * kOutStageBytes + lane * 8);   // of warp + 4
+          second_half = seg.of(1) > 0;
+          const float top = fmaxf(l_run > 0.f ? m_ref : -INFINITY, other.y > 0.f ? other.x : -INFINITY);
+          scale0 = l_run > 0.f ? ex2_approx(m_ref - top) : 0.f;
+          scale1 = other.y > 0.f ? ex2_approx(other.x - top) : 0.f;
+          l_run = l_run * scale0 + other.y * scale1;
+          m_ref = top;
+        }
         tc_fence_after();
         const bool empty = l_run == 0.f;
         const float coefficient = empty ? 0.f : 1.0f / l_run;
+        scale0 *= coefficient;
+        scale1 *= coefficient;
         const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
         // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes.
 #pragma unroll 1
@@ -673,13 +795,25 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 #pragma unroll
             for (int i = 0; i < 64; ++i) r[i] = 0u;
           }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale0);
+          if (second_half) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_addr + 128 + half * 64 + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[32 * c + i] = __float_as_uint(fmaf(__uint_as_float(o[i]), scale1, __uint_as_float(r[32 * c + i])));
+            }
+          }
           __syncwarp();                              // the stage's previous contents have been read
 #pragma unroll
           for (int i = 0; i < 64; i += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]) * coefficient, __uint_as_float(r[i + 2 * k + 1]) * coefficient);
+              w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]));
               if (empty) w[k] = filled;
             }
             st_shared_v4(out_stage + lane * 128 + (((i >> 3) ^ (lane & 7)) << 4), w);
@@ -698,11 +832,16 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             }
           }
         }
+        if (joined) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half_read(quarter));
+        }
         const int at = row_in_tile / p.group, token = first_token + at;
         if (p.a.lse && at < p.tile_tokens && token < seg.count)
           p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + seg.kv_head * p.group + row_in_tile - at * p.group] =
               empty ? -INFINITY : m_ref * 0.69314718055994530942f + logf(l_run);
-      } else if (ok && tile_used) {
+      } else if (ok && first_token < seg.count) {
         // A part of an item: the state as it is, four columns of 32 rows to a store.
         tc_fence_after();
         float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (seg.t0 == 0 ? 1 : 0)) * 2 + t) * L::kRecordFloats;
@@ -747,12 +886,18 @@ __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(cons
   pdl_wait();
   pdl_launch_dependents();
   const ChunkSplit split = p.splits[blockIdx.x];
-  const int t = blockIdx.y, row = threadIdx.x;
+  const int t = blockIdx.y, row = threadIdx.x;       // a halved item's second tile has no rows of its own
   const int at = row / p.group, token = (2 * split.pair + t) * p.tile_tokens + at;
   if (split.records == 0 || at >= p.tile_tokens || token >= split.count) return;
-  auto record = [&](int i) { return p.records + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * 2 + t) * L::kRecordFloats; };
+  // A halved item's halves are records of their own.
+  const int halves = split.halved ? 2 : 1, records = split.records * halves;
+  auto record = [&](int i) {
+    const int share = split.halved ? i >> 1 : i;
+    return p.records + ((static_cast<int64_t>(blockIdx.x + share) * 2 + (share == 0 ? 1 : 0)) * 2 + (split.halved ? i & 1 : t)) * L::kRecordFloats;
+  };
   float top = -INFINITY;
-  for (int i = 0; i < split.records; ++i) {
+#pragma unroll 4
+  for (int i = 0; i < records; ++i) {
     const float2 ml = *reinterpret_cast<const float2 *>(record(i) + kTileM * kHd + 2 * row);
     if (ml.y > 0.f) top = fmaxf(top, ml.x);
   }
@@ -760,7 +905,8 @@ __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(cons
   float l = 0.f, acc[32];
 #pragma unroll
   for (int e = 0; e < 32; ++e) acc[e] = 0.f;
-  for (int i = 0; i < split.records; ++i) {
+#pragma unroll 2
+  for (int i = 0; i < records; ++i) {
     const float *r = record(i);
     const float2 ml = *reinterpret_cast<const float2 *>(r + kTileM * kHd + 2 * row);
     const float weight = ml.y > 0.f ? ex2_approx(ml.x - m_exp) : 0.f;

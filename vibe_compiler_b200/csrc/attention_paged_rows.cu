@@ -456,50 +456,53 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
   if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
 }
 
-// Folds the records of the unit that starts in share blockIdx.x and goes on in the shares behind it, a warp per row.
+// Folds the records of the unit that starts in share blockIdx.x and goes on in the shares behind it: row blockIdx.y, a thread
+// per element. Every warp weighs 32 records at a time with a lane each; the records' elements are loaded eight at a time.
 template <bool kBf16, int kD, bool kNarrow>
-__global__ void __launch_bounds__(kWarps * 32) attention_paged_fold_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kD) attention_paged_fold_kernel(const __grid_constant__ RowsParams p) {
   using S = RowsShape<kD>;
   constexpr int kRows = kNarrow ? 8 : 16;
   pdl_wait();
   pdl_launch_dependents();
   const RowsSplit split = p.splits[blockIdx.x];
-  if (split.records == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = split.tile * kRows;
-  for (int r = warp; r < kRows; r += kWarps) {
-    const int packed = row0 + r, token = packed / p.group;
-    if (token >= split.count) break;
-    // record i: the start (slot 1) of the first share, the ends (slot 0) of the others
-    auto record = [&](int i) { return p.records + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + r) * S::kRecord; };
-    float top = -INFINITY;
-    for (int i = lane; i < split.records; i += 32) top = fmaxf(top, record(i)[kD]);
+  const int lane = threadIdx.x & 31, r = blockIdx.y;
+  const int packed = split.tile * kRows + r, token = packed / p.group;
+  if (split.records == 0 || token >= split.count) return;
+  // record 0: the start (slot 1) of the first share; the others: the ends (slot 0) of the shares behind it
+  const float *base = p.records + (static_cast<int64_t>(blockIdx.x) * 2 * kRows + r) * S::kRecord;
+  auto record = [&](int i) { return base + (i == 0 ? kRows * S::kRecord : static_cast<int64_t>(i) * 2 * kRows * S::kRecord); };
+  float top = -INFINITY, l = 0.f, sum = 0.f;          // l: this lane's share
+  for (int first = 0; first < split.records; first += 32) {
+    const int count = min(32, split.records - first);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < count) ml = *reinterpret_cast<const float2 *>(record(first + lane) + kD);
+    float next = fmaxf(top, ml.x);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float m_exp = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    Slice<kD> sum = {};
-    for (int base = 0; base < split.records; base += 32) {
-      float weight = 0.f;
-      if (base + lane < split.records) {
-        const float2 ml = *reinterpret_cast<const float2 *>(record(base + lane) + kD);
-        weight = exp2_fast(ml.x - m_exp);
-        l = fmaf(ml.y, weight, l);
-      }
-      const int count = min(32, split.records - base);
-#pragma unroll 4
-      for (int i = 0; i < count; ++i) {
-        Slice<kD> part;
-        part.load(record(base + i), lane);
-        const float w = __shfl_sync(0xffffffffu, weight, i);
+    for (int off = 16; off > 0; off >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, off));
+    const float m_exp = next == -INFINITY ? 0.f : next, alpha = exp2_fast(top - m_exp), weight = exp2_fast(ml.x - m_exp);
+    top = next;
+    l = fmaf(l, alpha, ml.y * weight);
+    sum *= alpha;
+    for (int i = 0; i < count; i += 8) {
+      float v[8];
 #pragma unroll
-        for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(part.v[e], w, sum.v[e]);
+      for (int u = 0; u < 8; ++u) v[u] = i + u < count ? record(first + i + u)[threadIdx.x] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __shfl_sync(0xffffffffu, weight, (i + u) & 31);
+        sum = i + u < count ? fmaf(v[u], w, sum) : sum;
       }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    write_row<kBf16, kD>(p.a, split.begin + token, split.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
   }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  const bool empty = l == 0.f;
+  const int head = split.kv_head * p.group + packed - token * p.group;
+  const int64_t row = static_cast<int64_t>(split.begin) + token;
+  uint32_t bits = pack2<kBf16>(sum * (empty ? 0.f : 1.0f / l), 0.f);
+  if (empty) bits = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc0u : 0x7e00u);
+  static_cast<uint16_t *>(p.a.out)[row * p.a.out_token + head * p.a.out_head + threadIdx.x] = static_cast<uint16_t>(bits);
+  if (p.a.lse && threadIdx.x == 0) p.a.lse[row * p.a.q_heads + head] = empty ? -INFINITY : top * 0.69314718055994530942f + logf(l);
 }
 
 using RowsKernel = void (*)(const RowsParams);
@@ -560,7 +563,7 @@ wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int rows_l
   const unsigned grid = static_cast<unsigned>(sm_count * kCtasPerSm);
   WB200_CUDA_CHECK(launch_dependent(kRowsKernels[wide][narrow][bf16][a.cache.page_size % kTileKeys == 0], grid, kWarps * 32,
                                     wide ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes, stream, p));
-  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], grid, kWarps * 32, 0, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], dim3(grid, narrow ? 8 : 16), a.cache.head_dim, 0, stream, p));
   return WB200_OK;
 }
 

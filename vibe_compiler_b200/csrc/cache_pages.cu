@@ -18,7 +18,7 @@ namespace wb200 {
 namespace {
 
 constexpr int kCluster = 8;
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ int ld_cluster_i32(uint32_t cluster_addr) {
@@ -65,33 +65,45 @@ __device__ int block_prefix(int count, int *prefix, int *warp_sums, Value value)
   return base;
 }
 
-// The pages of the cache are cut over the cluster's warps in order, in whole groups of 32: each warp counts the pages of its
-// part for which `flag` holds; *before is the count in front of the warp's part, the result the count of all. `parts` is this
-// CTA's word in the exchange. One cluster barrier.
+// The pages of the cache are cut over the cluster's warps in order, in groups of 128: a lane looks at four neighbours at a time.
 struct PagePart {
   int begin, end;
 };
 __device__ __forceinline__ PagePart page_part(int pages) {
   const int rank = static_cast<int>(cluster_cta_rank()) * kWarps + (threadIdx.x >> 5);
-  const int groups = (pages + 31) / 32, workers = kCluster * kWarps;
-  const int begin = static_cast<int>(static_cast<long long>(groups) * rank / workers) * 32;
-  const int end = static_cast<int>(static_cast<long long>(groups) * (rank + 1) / workers) * 32;
-  return {min(begin, pages), min(end, pages)};
+  const int groups = (pages - 1) / 128 + 1, workers = kCluster * kWarps;
+  const int begin = static_cast<int>(static_cast<long long>(groups) * rank / workers), end = static_cast<int>(static_cast<long long>(groups) * (rank + 1) / workers);
+  return {begin * 128, static_cast<int>(min(static_cast<long long>(end) * 128, static_cast<long long>(pages)))};
 }
+// The counts of pages page .. page + 3, `behind` for those from `end` on.
+__device__ __forceinline__ void load_four(const int *refs, int page, int end, int behind, int (&v)[4]) {
+  if (page + 3 < end && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
+    const int4 w = *reinterpret_cast<const int4 *>(refs + page);
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = page + k < end ? refs[page + k] : behind;
+  }
+}
+// Counts the pages for which flag(page, count) holds, each warp those of its part; *before is the number in front of the warp's
+// part, the result that of all. `cta_total` is this CTA's word in the exchange. One cluster barrier.
 template <typename Flag>
-__device__ int cluster_count(PagePart part, int *warp_counts, int *cta_total, int *before, Flag flag) {
+__device__ int cluster_count(const int *refs, int behind, PagePart part, int *warp_counts, int *cta_total, int *before, Flag flag) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int mine = 0;
-  for (int page = part.begin + lane; page < part.end; page += 32) mine += flag(page) ? 1 : 0;
+#pragma unroll 2
+  for (int start = part.begin; start < part.end; start += 128) {
+    int v[4];
+    load_four(refs, start + 4 * lane, part.end, behind, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mine += start + 4 * lane + k < part.end && flag(start + 4 * lane + k, v[k]) ? 1 : 0;
+  }
   mine = __reduce_add_sync(0xffffffffu, mine);
   if (lane == 0) warp_counts[warp] = mine;
   __syncthreads();
-  int in_front = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) in_front += warp_counts[w];
-    total += warp_counts[w];
-  }
+  const int value = warp_counts[lane];               // kWarps == 32
+  const int total = __reduce_add_sync(0xffffffffu, value);
+  int in_front = __reduce_add_sync(0xffffffffu, lane < warp ? value : 0);
   if (threadIdx.x == 0) *cta_total = total;
   cluster_sync_all();
   const int rank = static_cast<int>(cluster_cta_rank());
@@ -106,16 +118,51 @@ __device__ int cluster_count(PagePart part, int *warp_counts, int *cta_total, in
   *before = in_front;
   return all;
 }
-// Walks a warp's part in order and calls take(page, rank) for each page with the flag, rank counted from `before`.
+static_assert(kWarps == 32, "a lane per warp's count");
+// Walks a warp's part in order, as far as ranks below `limit` go, and calls take(page, count, is, rank) for every page: rank is
+// the number of flagged pages in front of it, counted from `before`.
 template <typename Flag, typename Take>
-__device__ void for_each_ranked(PagePart part, int before, Flag flag, Take take) {
+__device__ void for_each_ranked(const int *refs, int behind, PagePart part, int before, int limit, Flag flag, Take take) {
   const int lane = threadIdx.x & 31;
-  for (int start = part.begin; start < part.end; start += 32) {
-    const int page = start + lane;
-    const bool is = page < part.end && flag(page);
-    const unsigned int mask = __ballot_sync(0xffffffffu, is);
-    if (is) take(page, before + __popc(mask & ((1u << lane) - 1u)));
-    before += __popc(mask);
+  for (int start = part.begin; start < part.end && before < limit; start += 128) {
+    const int page = start + 4 * lane;
+    int v[4], own = 0;
+    load_four(refs, page, part.end, behind, v);
+    bool is[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      is[k] = page + k < part.end && flag(page + k, v[k]);
+      own += is[k] ? 1 : 0;
+    }
+    int inclusive = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, inclusive, off);
+      if (lane >= off) inclusive += other;
+    }
+    int rank = before + inclusive - own;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (page + k < part.end) take(page + k, v[k], is[k], rank);
+      rank += is[k] ? 1 : 0;
+    }
+    before += __shfl_sync(0xffffffffu, inclusive, 31);
+  }
+}
+// refs_out as refs, each warp its part.
+__device__ void copy_refs(const PageTablesArgs &p, PagePart part) {
+  if (p.refs_out == p.refs) return;
+  for (int start = part.begin; start < part.end; start += 128) {
+    const int page = start + 4 * (threadIdx.x & 31);
+    int v[4];
+    load_four(p.refs, page, part.end, 0, v);
+    if (page + 3 < part.end && (reinterpret_cast<uintptr_t>(p.refs_out) & 15u) == 0) {
+      *reinterpret_cast<int4 *>(p.refs_out + page) = make_int4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (page + k < part.end) p.refs_out[page + k] = v[k];
+    }
   }
 }
 // The last i with prefix[i] <= rank (prefix ascending, prefix[0] = 0 <= rank < prefix[count]): the holder of a rank.
@@ -139,16 +186,21 @@ __device__ __forceinline__ int held_tokens(const PageTablesArgs &p, int s) {
   raise_status(p.refused, kRefusedLength);
   return -1;
 }
-// Every row of the table as it is, except the elements for which skip(row, column) holds.
+// Every row of the table as it is, a warp per row, except columns [from, to) of a row as skip(row, from, to) sets them.
 template <typename Skip>
 __device__ void copy_table(const PageTablesArgs &p, Skip skip) {
   if (p.table_out == p.table) return;
   const int warp = cluster_thread() >> 5, lane = threadIdx.x & 31;
   for (int s = warp; s < p.sequences; s += kClusterThreads / 32) {
-    const int *from = p.table + s * p.table_stride;
-    int *to = p.table_out + s * p.table_out_stride;
-    for (int j = lane; j < p.table_width; j += 32)
-      if (!skip(s, j)) to[j] = from[j];
+    int from = 0, to = 0;
+    skip(s, from, to);
+    const int *src = p.table + s * p.table_stride;
+    int *dst = p.table_out + s * p.table_out_stride;
+#pragma unroll 8
+    for (int j = lane; j < p.table_width; j += 32) {
+      const int page = src[j];
+      if (j < from || j >= to) dst[j] = page;
+    }
   }
 }
 
@@ -167,20 +219,23 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pag
     return need - pages_of(held, p.page_size);
   });
   const PagePart part = page_part(p.pages);
-  auto is_free = [&](int page) { return p.refs[page] == 0; };
+  auto is_free = [](int, int count) { return count == 0; };
   int before;
-  const int free_pages = cluster_count(part, warp_sums, &cta_total, &before, is_free);   // its barrier: all inputs that decide are read
+  const int free_pages = cluster_count(p.refs, 1, part, warp_sums, &cta_total, &before, is_free);   // its barrier: all inputs that decide are read
   const int outcome = too_wide ? -1 : max(0, extra - free_pages);
   const bool done = outcome == 0;
   if (cluster_thread() == 0) *result = outcome;
   // Lengths last of all inputs are overwritten: held_tokens() of the rows below still reads them.
-  copy_table(p, [&](int s, int j) { return done && first[s + 1] > first[s] && j >= have_of(s) && j < have_of(s) + (first[s + 1] - first[s]); });
-  if (p.refs_out != p.refs)
-    for (int page = part.begin + (threadIdx.x & 31); page < part.end; page += 32) p.refs_out[page] = p.refs[page];
+  copy_table(p, [&](int s, int &from, int &to) {
+    if (!done || first[s + 1] == first[s]) return;
+    from = have_of(s);
+    to = from + first[s + 1] - first[s];
+  });
+  copy_refs(p, part);
   __syncwarp();
-  if (done && extra > 0 && before < extra)
-    for_each_ranked(part, before, is_free, [&](int page, int rank) {
-      if (rank >= extra) return;
+  if (done)
+    for_each_ranked(p.refs, 1, part, before, extra, is_free, [&](int page, int, bool is, int rank) {
+      if (!is || rank >= extra) return;
       const int s = holder_of(first, p.sequences, rank);
       p.table_out[s * p.table_out_stride + have_of(s) + rank - first[s]] = page;
       p.refs_out[page] = 1;
@@ -216,19 +271,18 @@ pages_fork_kernel(const PageTablesArgs p, int count, const int *parents, const i
   for (int i = threadIdx.x; i < count; i += kThreads)
     if (in_table(parents[i]) && (named[parents[i] >> 5] >> (parents[i] & 31) & 1u)) wrong = 1;   // a parent that is a child
   const PagePart part = page_part(p.pages);
-  auto is_free = [&](int page) { return p.refs[page] == 0; };
+  auto is_free = [](int, int count) { return count == 0; };
   int before;
-  const int free_pages = cluster_count(part, warp_sums, &cta_total, &before, is_free);
+  const int free_pages = cluster_count(p.refs, 1, part, warp_sums, &cta_total, &before, is_free);
   const int outcome = wrong ? -1 : max(0, extra - free_pages);
   const bool done = outcome == 0;
   if (cluster_thread() == 0) *result = outcome;
-  copy_table(p, [&](int s, int) { return done && (named[s >> 5] >> (s & 31) & 1u); });
-  for (int page = part.begin + (threadIdx.x & 31); page < part.end; page += 32)
-    if (p.refs_out != p.refs) p.refs_out[page] = p.refs[page];
+  copy_table(p, [&](int s, int &, int &to) { to = done && (named[s >> 5] >> (s & 31) & 1u) ? p.table_width : 0; });
+  copy_refs(p, part);
   __syncwarp();
-  if (done && extra > 0 && before < extra)
-    for_each_ranked(part, before, is_free, [&](int page, int rank) {
-      if (rank >= extra) return;
+  if (done)
+    for_each_ranked(p.refs, 1, part, before, extra, is_free, [&](int page, int, bool is, int rank) {
+      if (!is || rank >= extra) return;
       const int i = holder_of(first, count, rank);
       p.table_out[children[i] * p.table_out_stride + held_tokens(p, parents[i]) / p.page_size] = page;
       p.refs_out[page] = 1;
@@ -271,9 +325,8 @@ pages_fork_kernel(const PageTablesArgs p, int count, const int *parents, const i
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pages_free_kernel(const PageTablesArgs p, int count, const int *sequences) {
   pdl_wait();
   pdl_launch_dependents();
-  copy_table(p, [](int, int) { return false; });
-  if (p.refs_out != p.refs)
-    for (int page = cluster_thread(); page < p.pages; page += kClusterThreads) p.refs_out[page] = p.refs[page];
+  copy_table(p, [](int, int &, int &) {});
+  copy_refs(p, page_part(p.pages));
   if (p.lengths_out != p.lengths)
     for (int s = cluster_thread(); s < p.sequences; s += kClusterThreads) p.lengths_out[s] = p.lengths[s];
   cluster_sync_all();
@@ -317,27 +370,16 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pag
   pdl_wait();
   pdl_launch_dependents();
   const PagePart part = page_part(p.pages);
-  auto in_use = [&](int page) { return p.refs[page] > 0; };
   int before, front_before;
-  const int live = cluster_count(part, warp_counts, &cta_totals[0], &before, in_use);
-  __syncthreads();   // the warps' counts have been read
-  const int in_front = cluster_count(part, warp_counts, &cta_totals[1], &front_before, [&](int page) { return page < live && p.refs[page] > 0; });
+  const int live = cluster_count(p.refs, 0, part, warp_counts, &cta_totals[0], &before, [](int, int count) { return count > 0; });
+  const int in_front = cluster_count(p.refs, 0, part, warp_counts, &cta_totals[1], &front_before, [&](int page, int count) { return page < live && count > 0; });
   const int moves = live - in_front;      // used pages behind the first `live`, and free ones among them
-  for_each_ranked(part, before, in_use, [&](int page, int rank) {
-    if (page >= live) sources[rank - in_front] = page;
+  for_each_ranked(p.refs, 0, part, before, live + 1, [](int, int count) { return count > 0; }, [&](int page, int, bool used, int rank) {
+    if (used && page >= live) sources[rank - in_front] = page;
+    if (!used && page < live) destinations[page - rank] = page;      // the pages in front of it less the used ones
   });
-  // Free pages among the first `live`: their rank is the page less the used pages in front of it.
-  int used_before = before;
-  for (int start = part.begin; start < part.end && start < live; start += 32) {
-    const int lane = threadIdx.x & 31, page = start + lane;
-    const bool used = page < part.end && in_use(page);
-    const unsigned int mask = __ballot_sync(0xffffffffu, used);
-    if (page < part.end && page < live && !used) destinations[page - used_before - __popc(mask & ((1u << lane) - 1u))] = page;
-    used_before += __popc(mask);
-  }
   for (int i = moves + cluster_thread(); i < p.pages / 2; i += kClusterThreads) sources[i] = destinations[i] = -1;
-  if (p.refs_out != p.refs)
-    for (int page = part.begin + (threadIdx.x & 31); page < part.end; page += 32) p.refs_out[page] = p.refs[page];
+  copy_refs(p, part);
   cluster_sync_all();
   // A moved page's count goes along, and in its place stands, until the table is done, where the page went.
   for (int i = cluster_thread(); i < moves; i += kClusterThreads) {
@@ -351,13 +393,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pag
     const int used = pages_of(max(held_tokens(p, s), 0), p.page_size);
     const int *from = p.table + s * p.table_stride;
     int *to = p.table_out + s * p.table_out_stride;
-    for (int j = lane; j < p.table_width; j += 32) {
+    const int width = p.table_out == p.table ? used : p.table_width;
+#pragma unroll 4
+    for (int j = lane; j < width; j += 32) {
       int page = from[j];
       if (j < used) {
         if (page < 0 || page >= p.pages) raise_status(p.refused, kRefusedPage);
         else if (page >= live && p.refs_out[page] < 0 && -1 - p.refs_out[page] < live) page = -1 - p.refs_out[page];
       }
-      if (j < used || p.table_out != p.table) to[j] = page;
+      to[j] = page;
     }
   }
   if (p.lengths_out && p.lengths_out != p.lengths)

@@ -40,61 +40,72 @@ __device__ __forceinline__ float2 sin_cos_of_turns(unsigned long long phase) {
   return make_float2((quadrant & 2u) ? -sine : sine, (quadrant == 1u || quadrant == 2u) ? -cosine : cosine);
 }
 
-// kVec elements of storage type kFormat.
+// kVec elements of storage type kFormat, as they are stored: elements that are only copied keep their bits.
 template <int kFormat, int kVec>
 struct Elements {
-  static constexpr int kBytes = (kFormat == WB200_F32 ? 4 : 2) * kVec;
-  float v[kVec];
-  __device__ __forceinline__ void load(const void *base, int64_t element) {
-    if constexpr (kFormat == WB200_F32) {
-      const float *p = static_cast<const float *>(base) + element;
-      if constexpr (kVec == 4) {
-        const float4 w = *reinterpret_cast<const float4 *>(p);
-        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-      } else {
-        v[0] = *p;
-      }
-    } else {
-      const uint16_t *p = static_cast<const uint16_t *>(base) + element;
-      if constexpr (kVec == 8) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t bits[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = widen_bits(bits[i] & 0xffffu, kFormat); v[2 * i + 1] = widen_bits(bits[i] >> 16, kFormat); }
-      } else {
-        v[0] = widen_bits(*p, kFormat);
-      }
-    }
+  static constexpr int kWords = kFormat == WB200_F32 ? kVec : (kVec + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void *p) {
+    if constexpr (kVec > 1) *reinterpret_cast<uint4 *>(w) = *static_cast<const uint4 *>(p);
+    else if constexpr (kFormat == WB200_F32) w[0] = *static_cast<const uint32_t *>(p);
+    else w[0] = *static_cast<const uint16_t *>(p);
   }
-  __device__ __forceinline__ void store(void *base, int64_t element) const {
-    if constexpr (kFormat == WB200_F32) {
-      float *p = static_cast<float *>(base) + element;
-      if constexpr (kVec == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-      else *p = v[0];
-    } else {
-      uint16_t *p = static_cast<uint16_t *>(base) + element;
-      if constexpr (kVec == 8) {
-        uint32_t bits[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bits[i] = narrow(v[2 * i]) | (narrow(v[2 * i + 1]) << 16);
-        *reinterpret_cast<uint4 *>(p) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
-      } else {
-        *p = static_cast<uint16_t>(narrow(v[0]));
-      }
-    }
+  __device__ __forceinline__ void store(void *p) const {
+    if constexpr (kVec > 1) *static_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(w);
+    else if constexpr (kFormat == WB200_F32) *static_cast<uint32_t *>(p) = w[0];
+    else *static_cast<uint16_t *>(p) = static_cast<uint16_t>(w[0]);
   }
-  static __device__ __forceinline__ uint32_t narrow(float x) {
-    if constexpr (kFormat == WB200_BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-    else return __half_as_ushort(__float2half_rn(x));
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (kFormat == WB200_F32) return __uint_as_float(w[i]);
+    else return widen_bits(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu, kFormat);
+  }
+  // Elements i (even) and i + 1; the last of an odd count by itself.
+  __device__ __forceinline__ void set(int i, float lo, float hi) {
+    if constexpr (kFormat == WB200_F32) {
+      w[i] = __float_as_uint(lo);
+      if constexpr (kVec > 1) w[i + 1] = __float_as_uint(hi);
+    } else if constexpr (kFormat == WB200_BF16) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+      w[i >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+      const __half2 v = __floats2half2_rn(lo, hi);
+      w[i >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+    }
   }
 };
-// Elements that are only copied keep their bits.
-template <int kBytes>
-__device__ __forceinline__ void copy_bits(const void *from, void *to) {
-  if constexpr (kBytes == 16) *static_cast<uint4 *>(to) = *static_cast<const uint4 *>(from);
-  else if constexpr (kBytes == 4) *static_cast<uint32_t *>(to) = *static_cast<const uint32_t *>(from);
-  else *static_cast<uint16_t *>(to) = *static_cast<const uint16_t *>(from);
-}
+// One item of one head: two vectors, where they go, and the rotation of their pairs.
+template <int kFormat, int kVec>
+struct Row {
+  bool live, rotates, has1;
+  int token;
+  uint8_t *to0, *to1;
+  Elements<kFormat, kVec> v0, v1;
+  // turns[i] = (sin, cos) of pair i of the item. Half layout: (v0[i], v1[i]). Interleaved: neighbours.
+  __device__ __forceinline__ void turn(const float2 *turns, int interleaved) {
+    if constexpr (kVec == 1) {
+      const float x = v0.get(0), y = v1.get(0);
+      const float2 u = turns[0];
+      v0.set(0, fmaf(x, u.y, -(y * u.x)), 0.f);
+      v1.set(0, fmaf(y, u.y, x * u.x), 0.f);
+    } else if (interleaved) {
+#pragma unroll
+      for (int i = 0; i < kVec; i += 2) {
+        const float2 u = turns[i / 2], w = turns[kVec / 2 + i / 2];
+        const float x = v0.get(i), y = v0.get(i + 1), z = v1.get(i), q = v1.get(i + 1);
+        v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(y, u.y, x * u.x));
+        v1.set(i, fmaf(z, w.y, -(q * w.x)), fmaf(q, w.y, z * w.x));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; i += 2) {
+        const float2 u = turns[i], w = turns[i + 1];
+        const float x = v0.get(i), y = v1.get(i), z = v0.get(i + 1), q = v1.get(i + 1);
+        v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(z, w.y, -(q * w.x)));
+        v1.set(i, fmaf(y, u.y, x * u.x), fmaf(q, w.y, z * w.x));
+      }
+    }
+  }
+};
 
 // A block takes `tokens_per_block` tokens; an item is 2 * kVec elements of one head: kVec pairs, or elements that are copied.
 template <int kFormat, int kVec, bool kAppend>
@@ -153,75 +164,64 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     angles[i] = make_float2(sc.x * c.magnitude, sc.y * c.magnitude);
   }
   __syncthreads();
-  const int items_per_token = a.heads * p.items;
-  for (int i = threadIdx.x; i < count * items_per_token; i += kThreads) {
-    const int t = i / items_per_token, in_token = i - t * items_per_token;
-    const int head = in_token / p.items, item = in_token - head * p.items;
-    const int64_t src = (first + t) * a.x_token + head * a.x_head;
-    void *base = a.out;
-    int64_t dst;
-    bool rotates = item * kVec < c.pairs;
-    int first_copied = 2 * c.pairs;       // where this head's copied elements begin
-    int copy_item = item - c.pairs / kVec;
-    if constexpr (kAppend) {
-      if (!state_of[t]) continue;
-      if (head < p.q_heads) {
-        dst = (first + t) * a.out_token + head * a.out_head;
-      } else if (head < p.q_heads + p.cache.kv_heads) {
-        base = p.cache.k;
-        dst = k_row[t] + (head - p.q_heads) * p.cache.k_head;
-      } else {
-        base = p.cache.v;
-        dst = v_row[t] + (head - p.q_heads - p.cache.kv_heads) * p.cache.v_head;
-        rotates = false;
-        first_copied = 0;
-        copy_item = item;
-      }
-    } else {
-      dst = (first + t) * a.out_token + head * a.out_head;
-    }
-    if (rotates) {
-      const int pair = item * kVec;
-      const float2 *turn = angles + t * c.pairs + pair;
-      Elements<kFormat, kVec> lo, hi;
-      if (a.interleaved) {
-        lo.load(a.x, src + 2 * pair);
-        hi.load(a.x, src + 2 * pair + kVec);
-        if constexpr (kVec == 1) {
-          const float x = lo.v[0], y = hi.v[0];
-          lo.v[0] = fmaf(x, turn[0].y, -(y * turn[0].x));
-          hi.v[0] = fmaf(y, turn[0].y, x * turn[0].x);
-        } else {
+  // A thread keeps to one item of the head (or every lanes-th) and takes every groups-th head of the block's tokens, two at a
+  // time so that their loads are in flight together; nothing is divided in the loop.
+  const int lanes = min(p.items, kThreads), groups = kThreads / lanes, group = static_cast<int>(threadIdx.x) / lanes;
+  if (group >= groups) return;
+  for (int item = static_cast<int>(threadIdx.x) - group * lanes; item < p.items; item += lanes) {
+    const bool in_pairs = item * kVec < c.pairs;
+    Row<kFormat, kVec> row[2];
+    int t = 0, head = group;
+    auto settle = [&]() { while (head >= a.heads) { head -= a.heads; ++t; } };
+    settle();
+    while (t < count) {
 #pragma unroll
-          for (int e = 0; e < kVec / 2; ++e) {
-            const float2 u = turn[e], w = turn[kVec / 2 + e];
-            const float x = lo.v[2 * e], y = lo.v[2 * e + 1], z = hi.v[2 * e], q = hi.v[2 * e + 1];
-            lo.v[2 * e] = fmaf(x, u.y, -(y * u.x));
-            lo.v[2 * e + 1] = fmaf(y, u.y, x * u.x);
-            hi.v[2 * e] = fmaf(z, w.y, -(q * w.x));
-            hi.v[2 * e + 1] = fmaf(q, w.y, z * w.x);
+      for (int u = 0; u < 2; ++u) {
+        row[u].live = t < count;
+        if (row[u].live) {
+          row[u].token = t;
+          int64_t src = (first + t) * a.x_token + head * a.x_head, dst = (first + t) * a.out_token + head * a.out_head;
+          void *base = a.out;
+          row[u].rotates = in_pairs;
+          if constexpr (kAppend) {
+            row[u].live = state_of[t] != 0;
+            if (head >= p.q_heads + p.cache.kv_heads) {
+              base = p.cache.v;
+              dst = v_row[t] + (head - p.q_heads - p.cache.kv_heads) * p.cache.v_head;
+              row[u].rotates = false;
+            } else if (head >= p.q_heads) {
+              base = p.cache.k;
+              dst = k_row[t] + (head - p.q_heads) * p.cache.k_head;
+            }
+          }
+          // The item's two vectors: of the pairs, or the 2 kVec elements in their place where they are copied.
+          int d0, d1;
+          if (row[u].rotates) {
+            d0 = a.interleaved ? 2 * item * kVec : item * kVec;
+            d1 = a.interleaved ? d0 + kVec : d0 + c.pairs;
+          } else {
+            d0 = 2 * item * kVec;
+            d1 = d0 + kVec;
+          }
+          row[u].to0 = static_cast<uint8_t *>(base) + (dst + d0) * kElementBytes;
+          row[u].to1 = static_cast<uint8_t *>(base) + (dst + d1) * kElementBytes;
+          row[u].has1 = d1 + kVec <= a.head_dim;
+          const uint8_t *x = static_cast<const uint8_t *>(a.x) + src * kElementBytes;
+          if (row[u].live) {
+            row[u].v0.load(x + static_cast<int64_t>(d0) * kElementBytes);
+            if (row[u].has1) row[u].v1.load(x + static_cast<int64_t>(d1) * kElementBytes);
           }
         }
-        lo.store(base, dst + 2 * pair);
-        hi.store(base, dst + 2 * pair + kVec);
-      } else {
-        lo.load(a.x, src + pair);
-        hi.load(a.x, src + c.pairs + pair);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float x = lo.v[e], y = hi.v[e];
-          lo.v[e] = fmaf(x, turn[e].y, -(y * turn[e].x));
-          hi.v[e] = fmaf(y, turn[e].y, x * turn[e].x);
-        }
-        lo.store(base, dst + pair);
-        hi.store(base, dst + c.pairs + pair);
+        head += groups;
+        settle();
       }
-    } else {
-      const int d = first_copied + 2 * kVec * copy_item;
-      const uint8_t *from = static_cast<const uint8_t *>(a.x) + (src + d) * kElementBytes;
-      uint8_t *to = static_cast<uint8_t *>(base) + (dst + d) * kElementBytes;
-      if (d + kVec <= a.head_dim) copy_bits<kElementBytes * kVec>(from, to);
-      if (d + 2 * kVec <= a.head_dim) copy_bits<kElementBytes * kVec>(from + kElementBytes * kVec, to + kElementBytes * kVec);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (!row[u].live) continue;
+        if (row[u].rotates) row[u].turn(angles + row[u].token * c.pairs + item * kVec, a.interleaved);
+        row[u].v0.store(row[u].to0);
+        if (row[u].has1) row[u].v1.store(row[u].to1);
+      }
     }
   }
 }
@@ -234,12 +234,13 @@ wb200_status launch(RotaryParams p, const RotaryConstants &c, bool aligned, cuda
   const bool wide = aligned && c.pairs % vec == 0 && a.head_dim % vec == 0;
   const int step = 2 * (wide ? vec : 1);
   p.items = (a.head_dim + step - 1) / step;   // rotated pairs fill whole items
-  // Tokens of few heads share a block, once there are blocks for every SM: 512 items keep its threads busy.
-  const int items_per_token = a.heads * p.items;
-  int per_block = (512 + items_per_token - 1) / items_per_token;
+  // A block's threads pass over its heads eight times where that leaves eight blocks to an SM, to spread what a block costs
+  // before its first load (positions, angles); few tokens get a block each.
+  const int groups = p.items < kThreads ? kThreads / p.items : 1;
+  int per_block = (8 * groups + a.heads - 1) / a.heads;
   if (per_block > kMaxTokensPerBlock) per_block = kMaxTokensPerBlock;
   if (c.pairs > 0 && per_block > kMaxAnglesPerBlock / c.pairs) per_block = kMaxAnglesPerBlock / c.pairs;
-  while (per_block > 1 && a.tokens / per_block < 592) --per_block;
+  while (per_block > 1 && a.tokens / per_block < 148 * 8) --per_block;
   p.tokens_per_block = per_block;
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + per_block - 1) / per_block);
   void (*kernel)(const RotaryParams, const RotaryConstants);
