@@ -566,7 +566,7 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
  * has no part in: pages are taken lowest index first, sequence by sequence. The keys themselves are moved by
  * wb200_pages_copy with the page numbers that fork and compact return, once per layer or for many layers in one call. */
 typedef struct wb200_page_tables {
-  uint32_t sequences, table_width, pages, page_size;   /* at most 32768 sequences */
+  uint32_t sequences, table_width, pages, page_size;   /* at most 16384 sequences */
   const int32_t *table, *lengths, *refs;               /* [sequences, table_width] at table_stride, [sequences], [pages] */
   int32_t *table_out, *lengths_out, *refs_out;         /* table_out at table_out_stride */
   int64_t table_stride, table_out_stride;

@@ -181,7 +181,7 @@ def test_append_refuses(changes, status):
 
 
 @pytest.mark.parametrize("changes,status", [
-    (dict(sequences=0), INVALID), (dict(sequences=40000), LIMIT), (dict(pages=0), INVALID), (dict(page_size=1 << 30), LIMIT), (dict(table=None), INVALID),
+    (dict(sequences=0), INVALID), (dict(sequences=16385), LIMIT), (dict(pages=0), INVALID), (dict(page_size=1 << 30), LIMIT), (dict(table=None), INVALID),
     (dict(refs_out=None), INVALID), (dict(lengths_out=None), INVALID), (dict(table_stride=3), INVALID), (dict(table_out_stride=8), INVALID)])
 def test_page_calls_refuse(changes, status):
     lib, word = abi.load(), 4 << 20

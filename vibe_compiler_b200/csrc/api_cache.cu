@@ -133,7 +133,7 @@ wb200_status make_page_tables(wb200_backend *backend, const wb200_page_tables *t
   if (!backend || !t) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
   if (t->sequences == 0 || t->table_width == 0 || t->pages == 0 || t->page_size == 0)
     return fail(WB200_ERR_INVALID_ARGUMENT, "page table extents must be positive");
-  if (t->sequences > static_cast<uint32_t>(kMaxPagedSequences)) return fail(WB200_ERR_LIMIT, "more than 32768 sequences in one page table");
+  if (t->sequences > static_cast<uint32_t>(kMaxPagedSequences)) return fail(WB200_ERR_LIMIT, "more than 16384 sequences in one page table");
   if (t->pages > 0x7fffffffu || t->page_size > 0x7fffffffu || static_cast<uint64_t>(t->sequences) * t->table_width > (1ull << 30) ||
       static_cast<uint64_t>(t->table_width) * t->page_size > 0x7fffffffull)
     return fail(WB200_ERR_LIMIT, "page table extents too large");

@@ -27,6 +27,9 @@ __device__ __forceinline__ int ld_cluster_i32(uint32_t cluster_addr) {
   return v;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // Exclusive sum over the block's threads; *total is the sum of all. Ends with a barrier.
 __device__ __forceinline__ int block_exclusive_sum(int value, int *warp_sums, int *total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -149,22 +152,6 @@ __device__ void for_each_ranked(const int *refs, int behind, PagePart part, int 
     before += __shfl_sync(0xffffffffu, inclusive, 31);
   }
 }
-// refs_out as refs, each warp its part.
-__device__ void copy_refs(const PageTablesArgs &p, PagePart part) {
-  if (p.refs_out == p.refs) return;
-  for (int start = part.begin; start < part.end; start += 128) {
-    const int page = start + 4 * (threadIdx.x & 31);
-    int v[4];
-    load_four(p.refs, page, part.end, 0, v);
-    if (page + 3 < part.end && (reinterpret_cast<uintptr_t>(p.refs_out) & 15u) == 0) {
-      *reinterpret_cast<int4 *>(p.refs_out + page) = make_int4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (page + k < part.end) p.refs_out[page + k] = v[k];
-    }
-  }
-}
 // The last i with prefix[i] <= rank (prefix ascending, prefix[0] = 0 <= rank < prefix[count]): the holder of a rank.
 __device__ __forceinline__ int holder_of(const int *prefix, int count, int rank) {
   int low = 0, high = count;
@@ -186,65 +173,72 @@ __device__ __forceinline__ int held_tokens(const PageTablesArgs &p, int s) {
   raise_status(p.refused, kRefusedLength);
   return -1;
 }
-// Every row of the table as it is, a warp per row, except columns [from, to) of a row as skip(row, from, to) sets them.
-template <typename Skip>
-__device__ void copy_table(const PageTablesArgs &p, Skip skip) {
+// The output arrays as the inputs are, where they are not the inputs themselves.
+__device__ void copy_ints(const int *from, int *to, int64_t count) {
+  int64_t done = 0;
+  if (((reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) & 15u) == 0) {
+    const int64_t quads = count / 4;
+#pragma unroll 4
+    for (int64_t i = cluster_thread(); i < quads; i += kClusterThreads) reinterpret_cast<int4 *>(to)[i] = reinterpret_cast<const int4 *>(from)[i];
+    done = quads * 4;
+  }
+  for (int64_t i = done + cluster_thread(); i < count; i += kClusterThreads) to[i] = from[i];
+}
+__device__ void copy_tables(const PageTablesArgs &p) {
+  if (p.refs_out != p.refs) copy_ints(p.refs, p.refs_out, p.pages);
+  if (p.lengths_out != p.lengths) copy_ints(p.lengths, p.lengths_out, p.sequences);
   if (p.table_out == p.table) return;
+  if (p.sequences == 1 || (p.table_stride == p.table_width && p.table_out_stride == p.table_width)) {
+    copy_ints(p.table, p.table_out, static_cast<int64_t>(p.sequences) * p.table_width);
+    return;
+  }
   const int warp = cluster_thread() >> 5, lane = threadIdx.x & 31;
   for (int s = warp; s < p.sequences; s += kClusterThreads / 32) {
-    int from = 0, to = 0;
-    skip(s, from, to);
-    const int *src = p.table + s * p.table_stride;
-    int *dst = p.table_out + s * p.table_out_stride;
+    const int *from = p.table + s * p.table_stride;
+    int *to = p.table_out + s * p.table_out_stride;
 #pragma unroll 8
-    for (int j = lane; j < p.table_width; j += 32) {
-      const int page = src[j];
-      if (j < from || j >= to) dst[j] = page;
-    }
+    for (int j = lane; j < p.table_width; j += 32) to[j] = from[j];
   }
 }
 
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pages_reserve_kernel(const PageTablesArgs p, const int *wanted, int *result) {
-  extern __shared__ int first[];          // [sequences + 1]: rank of a sequence's first new page
+  extern __shared__ int shared[];
+  int *first = shared, *have = shared + p.sequences + 1;   // [sequences + 1]: rank of a sequence's first new page; [sequences]: pages it has
   __shared__ int warp_sums[kWarps], cta_total;
   __shared__ int too_wide;
   pdl_wait();
   pdl_launch_dependents();
   if (threadIdx.x == 0) too_wide = 0;
   __syncthreads();
-  auto have_of = [&](int s) { return pages_of(max(held_tokens(p, s), 0), p.page_size); };
+  copy_tables(p);
   const int extra = block_prefix(p.sequences, first, warp_sums, [&](int s) {
     const int held = held_tokens(p, s), need = pages_of(max(max(held, wanted[s]), 0), p.page_size);
+    have[s] = pages_of(max(held, 0), p.page_size);
     if (held < 0 || need > p.table_width) { too_wide = 1; return 0; }
-    return need - pages_of(held, p.page_size);
+    return need - have[s];
   });
   const PagePart part = page_part(p.pages);
   auto is_free = [](int, int count) { return count == 0; };
   int before;
-  const int free_pages = cluster_count(p.refs, 1, part, warp_sums, &cta_total, &before, is_free);   // its barrier: all inputs that decide are read
+  // The barrier of the count stands between everything that decides what is done, and the copies, and the changes.
+  const int free_pages = cluster_count(p.refs, 1, part, warp_sums, &cta_total, &before, is_free);
+  cluster_arrive();
   const int outcome = too_wide ? -1 : max(0, extra - free_pages);
-  const bool done = outcome == 0;
   if (cluster_thread() == 0) *result = outcome;
-  // Lengths last of all inputs are overwritten: held_tokens() of the rows below still reads them.
-  copy_table(p, [&](int s, int &from, int &to) {
-    if (!done || first[s + 1] == first[s]) return;
-    from = have_of(s);
-    to = from + first[s + 1] - first[s];
-  });
-  copy_refs(p, part);
-  __syncwarp();
-  if (done)
+  if (outcome == 0) {
+    int s = -1;                                    // the sequence that the lane's last page went to
     for_each_ranked(p.refs, 1, part, before, extra, is_free, [&](int page, int, bool is, int rank) {
       if (!is || rank >= extra) return;
-      const int s = holder_of(first, p.sequences, rank);
-      p.table_out[s * p.table_out_stride + have_of(s) + rank - first[s]] = page;
+      if (s < 0 || rank >= first[s + 1]) s = holder_of(first, p.sequences, rank);
+      p.table_out[s * p.table_out_stride + have[s] + rank - first[s]] = page;
       p.refs_out[page] = 1;
     });
-  cluster_sync_all();   // every CTA has read the lengths, and the others' totals
-  for (int s = cluster_thread(); s < p.sequences; s += kClusterThreads) {
-    const int tokens = p.lengths[s];
-    p.lengths_out[s] = done ? max(tokens, wanted[s]) : tokens;
+    for (int i = cluster_thread(); i < p.sequences; i += kClusterThreads) {
+      const int held = p.lengths[i], tokens = max(held, wanted[i]);
+      if (tokens != held) p.lengths_out[i] = tokens;
+    }
   }
+  cluster_wait();   // every CTA has read the others' totals
 }
 
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
@@ -259,6 +253,7 @@ pages_fork_kernel(const PageTablesArgs p, int count, const int *parents, const i
   if (threadIdx.x == 0) wrong = 0;
   for (int i = threadIdx.x; i < (p.sequences + 31) / 32; i += kThreads) named[i] = 0u;
   __syncthreads();
+  copy_tables(p);
   auto in_table = [&](int s) { return s >= 0 && s < p.sequences; };
   const int extra = block_prefix(count, first, warp_sums, [&](int i) {
     const int parent = parents[i], child = children[i];
@@ -274,61 +269,52 @@ pages_fork_kernel(const PageTablesArgs p, int count, const int *parents, const i
   auto is_free = [](int, int count) { return count == 0; };
   int before;
   const int free_pages = cluster_count(p.refs, 1, part, warp_sums, &cta_total, &before, is_free);
+  cluster_arrive();
   const int outcome = wrong ? -1 : max(0, extra - free_pages);
-  const bool done = outcome == 0;
   if (cluster_thread() == 0) *result = outcome;
-  copy_table(p, [&](int s, int &, int &to) { to = done && (named[s >> 5] >> (s & 31) & 1u) ? p.table_width : 0; });
-  copy_refs(p, part);
-  __syncwarp();
-  if (done)
+  const int warp = cluster_thread() >> 5, lane = threadIdx.x & 31;
+  if (outcome == 0) {
+    // Parents are no children and children hold nothing, so what is read here is written by nobody; free pages and shared ones
+    // are different pages, and a count that is raised meanwhile was not 0.
     for_each_ranked(p.refs, 1, part, before, extra, is_free, [&](int page, int, bool is, int rank) {
       if (!is || rank >= extra) return;
       const int i = holder_of(first, count, rank);
-      p.table_out[children[i] * p.table_out_stride + held_tokens(p, parents[i]) / p.page_size] = page;
+      p.table_out[children[i] * p.table_out_stride + p.lengths[parents[i]] / p.page_size] = page;
       p.refs_out[page] = 1;
       destinations[i] = page;
     });
-  // The counts are in place before the shared pages are counted, and every CTA has read the totals and the free pages. Lengths
-  // of parents stay as they are; those of children are read by nobody from here on.
-  cluster_sync_all();
-  if (p.lengths_out != p.lengths)
-    for (int s = cluster_thread(); s < p.sequences; s += kClusterThreads)
-      if (!done || !(named[s >> 5] >> (s & 31) & 1u)) p.lengths_out[s] = p.lengths[s];
-  const int warp = cluster_thread() >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < count; i += kClusterThreads / 32) {
-    if (!done) {
-      if (lane == 0) sources[i] = destinations[i] = -1;
-      continue;
-    }
-    const int parent = parents[i], child = children[i], tokens = held_tokens(p, parent), full = tokens / p.page_size;
-    const bool partial = tokens % p.page_size != 0;
-    const int *from = p.table + parent * p.table_stride;
-    int *to = p.table_out + child * p.table_out_stride;
-    for (int j = lane; j < p.table_width; j += 32) {
-      if (j < full) {
-        const int page = from[j];
-        to[j] = page;
-        if (page >= 0 && page < p.pages) atomicAdd(p.refs_out + page, 1);
-        else raise_status(p.refused, kRefusedPage);
-      } else if (j != full || !partial) {
-        to[j] = -1;
+    for (int i = warp; i < count; i += kClusterThreads / 32) {
+      const int parent = parents[i], child = children[i], tokens = p.lengths[parent], full = tokens / p.page_size;
+      const bool partial = tokens % p.page_size != 0;
+      const int *from = p.table + parent * p.table_stride;
+      int *to = p.table_out + child * p.table_out_stride;
+#pragma unroll 4
+      for (int j = lane; j < p.table_width; j += 32) {
+        if (j < full) {
+          const int page = from[j];
+          to[j] = page;
+          if (page >= 0 && page < p.pages) atomicAdd(p.refs_out + page, 1);
+          else raise_status(p.refused, kRefusedPage);
+        } else if (j != full || !partial) {
+          to[j] = -1;
+        }
+      }
+      if (lane == 0) {
+        sources[i] = partial ? from[full] : -1;
+        if (!partial) destinations[i] = -1;
+        p.lengths_out[child] = tokens;
       }
     }
-    if (lane == 0) {
-      sources[i] = partial ? from[full] : -1;
-      if (!partial) destinations[i] = -1;
-      p.lengths_out[child] = tokens;
-    }
+  } else {
+    for (int i = cluster_thread(); i < count; i += kClusterThreads) sources[i] = destinations[i] = -1;
   }
+  cluster_wait();   // every CTA has read the others' totals
 }
 
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pages_free_kernel(const PageTablesArgs p, int count, const int *sequences) {
   pdl_wait();
   pdl_launch_dependents();
-  copy_table(p, [](int, int &, int &) {});
-  copy_refs(p, page_part(p.pages));
-  if (p.lengths_out != p.lengths)
-    for (int s = cluster_thread(); s < p.sequences; s += kClusterThreads) p.lengths_out[s] = p.lengths[s];
+  copy_tables(p);
   cluster_sync_all();
   const int warp = cluster_thread() >> 5, lane = threadIdx.x & 31;
   for (int i = warp; i < count; i += kClusterThreads / 32) {
@@ -379,7 +365,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) pag
     if (!used && page < live) destinations[page - rank] = page;      // the pages in front of it less the used ones
   });
   for (int i = moves + cluster_thread(); i < p.pages / 2; i += kClusterThreads) sources[i] = destinations[i] = -1;
-  copy_refs(p, part);
+  if (p.refs_out != p.refs) copy_ints(p.refs, p.refs_out, p.pages);
   cluster_sync_all();
   // A moved page's count goes along, and in its place stands, until the table is done, where the page went.
   for (int i = cluster_thread(); i < moves; i += kClusterThreads) {
@@ -471,7 +457,7 @@ wb200_status check_launch(const char *what, cudaError_t error) {
   return WB200_OK;
 }
 
-constexpr size_t kMostShared = (kMaxPagedSequences + 1 + kMaxPagedSequences / 32) * sizeof(int);
+constexpr size_t kMostShared = (2 * kMaxPagedSequences + 1) * sizeof(int);
 wb200_status allow_shared() {
   static PerDeviceOnce attributes;
   return attributes.run([]() -> wb200_status {
@@ -486,7 +472,7 @@ wb200_status allow_shared() {
 wb200_status launch_pages_reserve(const PageTablesArgs &args, const int *wanted, int *result, cudaStream_t stream) {
   wb200_status st = allow_shared();
   if (st != WB200_OK) return st;
-  return check_launch("pages_reserve", launch_dependent(pages_reserve_kernel, kCluster, kThreads, (static_cast<size_t>(args.sequences) + 1) * sizeof(int),
+  return check_launch("pages_reserve", launch_dependent(pages_reserve_kernel, kCluster, kThreads, (2 * static_cast<size_t>(args.sequences) + 1) * sizeof(int),
                                                         stream, args, wanted, result));
 }
 

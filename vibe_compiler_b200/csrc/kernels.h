@@ -353,7 +353,7 @@ struct PageTablesArgs {
   int64_t table_stride, table_out_stride;
   int *refused;
 };
-constexpr int kMaxPagedSequences = 32768;
+constexpr int kMaxPagedSequences = 16384;
 wb200_status launch_pages_reserve(const PageTablesArgs &args, const int *wanted, int *result, cudaStream_t stream);
 wb200_status launch_pages_fork(const PageTablesArgs &args, int count, const int *parents, const int *children, int *sources, int *destinations,
                                int *result, cudaStream_t stream);
