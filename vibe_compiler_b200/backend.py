@@ -542,33 +542,32 @@ class B200TargetModelBackend:
         return out
 
     # ------------------------------------------------------------------ serving from a paged KV cache (CUDA tensors)
+    # A step of a few tokens takes less time on the device than a careless wrapper takes here: tensors are checked by one
+    # condition each, and outputs come from the cheapest of torch's allocation calls.
     def _stream_of(self, stream: Optional[int]) -> int:
         """The stream a paged call runs on: the given one, or the current one of the backend's device."""
         return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else stream
 
-    def _empty(self, shape, dtype, stream: int):
-        """Memory of the backend's device that belongs to `stream`: what the call writes there is ordered behind what the
-        memory's last holder did, also when `stream` is not the current one."""
-        device = torch.device("cuda", self.device)
+    def _empty(self, like, shape, stream: int, dtype=None):
+        """Memory of `like`'s device that belongs to `stream`: what the call writes there is ordered behind what the memory's
+        last holder did, also when `stream` is not the current one."""
         if stream == torch._C._cuda_getCurrentRawStream(self.device):
-            return torch.empty(shape, dtype=dtype, device=device)
+            return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+        device = torch.device("cuda", self.device)
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)):
-            return torch.empty(shape, dtype=dtype, device=device)
+            return torch.empty(shape, dtype=dtype or like.dtype, device=device)
 
-    def _rows(self, name: str, t, heads: Optional[int] = None, head_dim: Optional[int] = None, tokens: Optional[int] = None, dtype=None):
-        """Checks a [tokens, heads, head_dim] tensor of this device."""
-        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous rows")
-        if (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim) or \
-                (tokens is not None and t.shape[0] != tokens) or (dtype is not None and t.dtype != dtype):
-            raise ValueError(f"{name} does not match the shape or type of the other tensors")
-        if t.device.type != "cuda" or t.device.index != self.device:
-            raise ValueError(f"{name} must be on the backend's device")
+    def _check_rows(self, name: str, t, shape: tuple, dtype):
+        """A [tokens, heads, head_dim] tensor of this device with contiguous rows."""
+        if t.dtype != dtype or t.shape != shape or t.get_device() != self.device or (t.stride(2) != 1 and shape[2] > 1):
+            if t.get_device() != self.device:
+                raise ValueError(f"{name} must be on the backend's device")
+            raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} with contiguous rows")
 
-    def _positions(self, positions, tokens: int):
-        if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
+    def _check_positions(self, positions, tokens: int):
+        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,) or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 or int64 tensor with one entry per token")
-        if positions.device.type != "cuda" or positions.device.index != self.device:
+        if positions.get_device() != self.device:
             raise ValueError("positions must be on the backend's device")
 
     def rope(self, x, positions, table, *, interleaved: bool = False, backward: bool = False, out=None, stream: Optional[int] = None):
@@ -576,26 +575,24 @@ class B200TargetModelBackend:
         positions[t]: pairs (i, i + R/2) of the first R = table.rotary_dim elements, or (2i, 2i + 1) when `interleaved`, the
         rest copied. `table`: a paged_cache.RotaryTable. `backward` applies the transposed map: x is the gradient of the
         rotated rows, the result the gradient of the rows. `out` may be x."""
-        self._rows("x", x)
-        if x.dtype not in _TORCH_FORMATS:
-            raise ValueError("x must be bfloat16, float16 or float32")
-        tokens, heads, head_dim = x.shape
-        self._positions(positions, tokens)
-        stream = self._stream_of(stream)
+        dtype, shape = x.dtype, x.shape
+        if dtype not in _TORCH_FORMATS or len(shape) != 3:
+            raise ValueError("x must be a [tokens, heads, head_dim] tensor of bfloat16, float16 or float32")
+        self._check_rows("x", x, shape, dtype)
+        self._check_positions(positions, shape[0])
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(self.device)
         if out is None:
-            out = self._empty((tokens, heads, head_dim), x.dtype, stream)
+            out = self._empty(x, shape, stream)
         else:
-            self._rows("out", out, heads, head_dim, tokens, x.dtype)
+            self._check_rows("out", out, shape, dtype)
+        x_strides, out_strides = x.stride(), out.stride()
         p = abi.RopeParams.from_buffer_copy(_ROPE_PACK(
-            tokens, heads, head_dim, _TORCH_FORMATS[x.dtype], bool(interleaved), bool(backward), positions.element_size(),
+            shape[0], shape[1], shape[2], _TORCH_FORMATS[dtype], bool(interleaved), bool(backward), positions.element_size(),
             table.rotary_dim, table.magnitude, table._address, positions.data_ptr(), x.data_ptr(), out.data_ptr(),
-            x.stride(0), x.stride(1), out.stride(0), out.stride(1), stream))
+            x_strides[0], x_strides[1], out_strides[0], out_strides[1], stream))
         self._check(self._lib.wb200_rope(self._handle, C.byref(p)))
         return out
-
-    def _paged(self, cache, batch):
-        if cache.device_index != self.device or batch.device_index != self.device:
-            raise ValueError("the cache and the batch must be on the backend's device")
 
     def rope_append(self, qkv, cache, batch, table, *, q_heads: int, interleaved: bool = False, positions=None, out=None,
                     stream: Optional[int] = None):
@@ -604,25 +601,27 @@ class B200TargetModelBackend:
         `cache` (a paged_cache.PagedCache). `batch`: a paged_cache.PagedBatch whose pages are reserved. `table` None rotates
         nothing. `positions` replace the cache positions in the rotation. Rows of tokens that belong to no sequence are not
         written."""
-        self._paged(cache, batch)
-        kv_heads, head_dim, dtype = cache.k.shape[2], cache.k.shape[3], cache.k.dtype
-        if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.dtype != dtype or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        device, dtype = self.device, cache.k.dtype
+        _, _, kv_heads, head_dim = cache.k.shape
+        if cache.device_index != device or batch.device_index != device or qkv.get_device() != device:
+            raise ValueError("qkv, the cache and the batch must be on the backend's device")
+        if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.dtype != dtype or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
             raise ValueError("qkv must be [tokens, (q_heads + 2 kv_heads) head_dim] of the cache's type with contiguous rows")
-        if qkv.device.type != "cuda" or qkv.device.index != self.device:
-            raise ValueError("qkv must be on the backend's device")
         tokens = qkv.shape[0]
         if positions is not None:
-            self._positions(positions, tokens)
-        stream = self._stream_of(stream)
+            self._check_positions(positions, tokens)
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(device)
         if out is None:
-            out = self._empty((tokens, q_heads, head_dim), dtype, stream)
+            out = self._empty(qkv, (tokens, q_heads, head_dim), stream)
         else:
-            self._rows("out", out, q_heads, head_dim, tokens, dtype)
+            self._check_rows("out", out, (tokens, q_heads, head_dim), dtype)
+        strides = out.stride()
         p = abi.RopeAppendParams.from_buffer_copy(_APPEND_PACK(
             q_heads, bool(interleaved), positions.element_size() if positions is not None else 4,
             table.rotary_dim if table is not None else 0, table.magnitude if table is not None else 1.0,
             table._address if table is not None else 0, positions.data_ptr() if positions is not None else 0, qkv.data_ptr(), out.data_ptr(),
-            qkv.stride(0), out.stride(0), out.stride(1), stream))
+            qkv.stride(0), strides[0], strides[1], stream))
         self._check(self._lib.wb200_rope_append(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
         return out
 
@@ -632,51 +631,54 @@ class B200TargetModelBackend:
         (grouped queries; with `causal` up to the token's own position). `lse` [tokens, q_heads] f32 receives the
         log-sum-exp. Rows of tokens that belong to no sequence are not written. Scratch memory comes from torch's allocator,
         per call and stream, so calls may overlap and be captured into CUDA graphs."""
-        self._paged(cache, batch)
-        self._rows("q", q, head_dim=cache.k.shape[3], dtype=cache.k.dtype)
-        tokens, q_heads, head_dim = q.shape
-        stream = self._stream_of(stream)
+        device, dtype, shape = self.device, cache.k.dtype, q.shape
+        if cache.device_index != device or batch.device_index != device:
+            raise ValueError("the cache and the batch must be on the backend's device")
+        if len(shape) != 3 or shape[2] != cache.k.shape[3]:
+            raise ValueError("q must be [tokens, q_heads, head_dim] with the cache's head dimension")
+        self._check_rows("q", q, shape, dtype)
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(device)
         if out is None:
-            out = self._empty((tokens, q_heads, head_dim), q.dtype, stream)
+            out = self._empty(q, shape, stream)
         else:
-            self._rows("out", out, q_heads, head_dim, tokens, q.dtype)
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous() or lse.device != q.device):
+            self._check_rows("out", out, shape, dtype)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous() or lse.get_device() != device):
             raise ValueError("lse must be a contiguous float32 [tokens, q_heads] tensor on the same device")
-        desc = batch._desc(tokens)
-        fields = (q_heads, bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
-                  lse.data_ptr() if lse is not None else 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1))
-        p = abi.AttentionPagedParams.from_buffer_copy(_PAGED_PACK(*fields, 0, 0, stream))
-        needed = self._lib.wb200_attention_paged_workspace_bytes(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p))
-        workspace = self._empty(needed, torch.uint8, stream)
-        p.workspace, p.workspace_bytes = workspace.data_ptr(), needed
-        self._check(self._lib.wb200_attention_paged(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
+        desc, q_strides, out_strides = batch._desc(shape[0]), q.stride(), out.stride()
+        p = abi.AttentionPagedParams.from_buffer_copy(_PAGED_PACK(
+            shape[1], bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
+            lse.data_ptr() if lse is not None else 0, q_strides[0], q_strides[1], out_strides[0], out_strides[1], 0, 0, stream))
+        arguments = self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)
+        needed = self._lib.wb200_attention_paged_workspace_bytes(*arguments)
+        if needed:
+            workspace = self._empty(q, needed, stream, torch.uint8)
+            p.workspace, p.workspace_bytes = workspace.data_ptr(), needed
+        self._check(self._lib.wb200_attention_paged(*arguments))
         return out
 
-    def _tables(self, table, lengths, refs, page_size, out, stream, with_lengths=True):
+    def _page_tables(self, table, lengths, refs, page_size, out, stream, with_lengths=True):
         """Checks the page arrays and makes the outputs; returns the C form and the outputs."""
-        for name, t, dims in (("table", table, 2), ("lengths", lengths, 1), ("refs", refs, 1)):
-            if t.dtype != torch.int32 or t.dim() != dims or t.device.type != "cuda" or t.device.index != self.device:
-                raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s) on the backend's device")
-            if t.shape[-1] > 1 and t.stride(-1) != 1:
-                raise ValueError(f"rows of {name} must be contiguous")
-        if lengths.shape[0] != table.shape[0]:
-            raise ValueError("table and lengths must describe the same sequences")
+        i32, device = torch.int32, self.device
+        if not (table.dtype == lengths.dtype == refs.dtype == i32 and table.get_device() == lengths.get_device() == refs.get_device() == device and
+                table.dim() == 2 and (table.stride(1) == 1 or table.shape[1] <= 1) and lengths.dim() == refs.dim() == 1 and
+                lengths.is_contiguous() and refs.is_contiguous() and lengths.shape[0] == table.shape[0]):
+            raise ValueError("table [sequences, width], lengths [sequences] and refs [pages] must be int32 tensors on the backend's device with contiguous rows")
         inputs = (table, lengths, refs) if with_lengths else (table, refs)
         if out is None:
-            out = tuple(self._empty(t.shape, torch.int32, stream) for t in inputs)
+            out = tuple([self._empty(t, t.shape, stream) for t in inputs])
         else:
             out = tuple(out)
-            if len(out) != len(inputs) or any(o.shape != t.shape or o.dtype != torch.int32 or o.device != t.device or
-                                              (o.shape[-1] > 1 and o.stride(-1) != 1) for o, t in zip(out, inputs)):
+            if len(out) != len(inputs) or any(o.shape != t.shape or o.dtype != i32 or o.get_device() != device for o, t in zip(out, inputs)) or \
+                    (out[0].stride(1) != 1 and table.shape[1] > 1) or not all(o.is_contiguous() for o in out[1:]):
                 raise ValueError("out must be tensors like the page arrays")
         desc = abi.PageTablesDesc.from_buffer_copy(_TABLES_PACK(
             table.shape[0], table.shape[1], refs.shape[0], page_size, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
             out[0].data_ptr(), out[1].data_ptr() if with_lengths else 0, out[-1].data_ptr(), table.stride(0), out[0].stride(0), stream))
         return desc, out
 
-    def _indices(self, name, t, count=None):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.device or \
-                (count is not None and t.shape[0] != count):
+    def _check_indices(self, name, t, count=None):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != self.device or (count is not None and t.shape[0] != count):
             raise ValueError(f"{name} must be a contiguous int32 vector of matching length on the backend's device")
 
     def pages_reserve(self, table, lengths, refs, wanted, page_size: int, *, out=None, stream: Optional[int] = None):
@@ -685,9 +687,9 @@ class B200TargetModelBackend:
         free ones of lowest index, sequence by sequence. result[0]: 0 done, n > 0 pages too few, -1 a sequence outgrows the
         table; unless 0, the arrays come out as they went in. `out`: (table, lengths, refs) to write, may be the inputs."""
         stream = self._stream_of(stream)
-        self._indices("wanted", wanted, table.shape[0])
-        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
-        result = self._empty(1, torch.int32, stream)
+        desc, out = self._page_tables(table, lengths, refs, page_size, out, stream)
+        self._check_indices("wanted", wanted, table.shape[0])
+        result = self._empty(lengths, 1, stream)
         self._check(self._lib.wb200_pages_reserve(self._handle, C.byref(desc), wanted.data_ptr(), result.data_ptr()))
         return (*out, result)
 
@@ -697,12 +699,11 @@ class B200TargetModelBackend:
         destinations)` copies (-1 where there is none). result[0]: 0 done, n > 0 pages too few, -1 indices that cannot be
         forked; unless 0, the arrays come out as they went in."""
         stream = self._stream_of(stream)
-        self._indices("parents", parents)
-        self._indices("children", children, parents.shape[0])
-        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
+        self._check_indices("parents", parents)
         count = parents.shape[0]
-        lists = self._empty(2 * count + 1, torch.int32, stream)
-        sources, destinations, result = lists[:count], lists[count:2 * count], lists[2 * count:]
+        self._check_indices("children", children, count)
+        desc, out = self._page_tables(table, lengths, refs, page_size, out, stream)
+        sources, destinations, result = self._empty(parents, count, stream), self._empty(parents, count, stream), self._empty(parents, 1, stream)
         self._check(self._lib.wb200_pages_fork(self._handle, C.byref(desc), count, parents.data_ptr(), children.data_ptr(), sources.data_ptr(),
                                                destinations.data_ptr(), result.data_ptr()))
         return (*out, sources, destinations, result)
@@ -710,8 +711,8 @@ class B200TargetModelBackend:
     def pages_free(self, table, lengths, refs, sequences, page_size: int, *, out=None, stream: Optional[int] = None):
         """The listed sequences give their pages back: (table, lengths, refs). Negative entries are passed over."""
         stream = self._stream_of(stream)
-        self._indices("sequences", sequences)
-        desc, out = self._tables(table, lengths, refs, page_size, out, stream)
+        self._check_indices("sequences", sequences)
+        desc, out = self._page_tables(table, lengths, refs, page_size, out, stream)
         self._check(self._lib.wb200_pages_free(self._handle, C.byref(desc), sequences.shape[0], sequences.data_ptr()))
         return out
 
@@ -719,9 +720,9 @@ class B200TargetModelBackend:
         """The pages in use to the front of the cache: (table, refs, sources, destinations), the moves for `pages_copy` with
         -1 behind the last. `out`: (table, refs)."""
         stream = self._stream_of(stream)
-        desc, out = self._tables(table, lengths, refs, page_size, out, stream, with_lengths=False)
-        moves = self._empty((2, refs.shape[0] // 2), torch.int32, stream)
-        sources, destinations = moves[0], moves[1]
+        desc, out = self._page_tables(table, lengths, refs, page_size, out, stream, with_lengths=False)
+        half = refs.shape[0] // 2
+        sources, destinations = self._empty(refs, half, stream), self._empty(refs, half, stream)
         self._check(self._lib.wb200_pages_compact(self._handle, C.byref(desc), sources.data_ptr(), destinations.data_ptr()))
         return (*out, sources, destinations)
 
@@ -731,9 +732,9 @@ class B200TargetModelBackend:
         source and a destination."""
         caches = (caches,) if hasattr(caches, "_desc") else caches
         stream = self._stream_of(stream)
-        self._indices("sources", sources)
-        self._indices("destinations", destinations, sources.shape[0])
-        if any(c.device_index != self.device for c in caches):
+        self._check_indices("sources", sources)
+        self._check_indices("destinations", destinations, sources.shape[0])
+        if any([c.device_index != self.device for c in caches]):
             raise ValueError("the caches must be on the backend's device")
         descs = (abi.PagedCacheDesc * len(caches))(*[c._desc for c in caches])
         self._check(self._lib.wb200_pages_copy(self._handle, descs, len(caches), sources.shape[0], sources.data_ptr(), destinations.data_ptr(), stream))

@@ -131,21 +131,23 @@ class PagedBatch:
     __slots__ = ("page_table", "key_lengths", "query_starts", "max_query", "device_index", "_fields")
 
     def __init__(self, page_table: torch.Tensor, key_lengths: torch.Tensor, query_starts: torch.Tensor, max_query: int = 0):
-        if not (page_table.dtype == key_lengths.dtype == query_starts.dtype == torch.int32):
+        if not page_table.dtype == key_lengths.dtype == query_starts.dtype == torch.int32:
             raise ValueError("page_table, key_lengths and query_starts must be int32")
         sequences = key_lengths.shape[0] if key_lengths.dim() == 1 else -1
-        if page_table.dim() != 2 or query_starts.dim() != 1 or page_table.shape[0] != sequences or query_starts.shape[0] != sequences + 1:
+        if page_table.dim() != 2 or query_starts.shape != (sequences + 1,) or page_table.shape[0] != sequences:
             raise ValueError("page_table is [sequences, width], key_lengths [sequences], query_starts [sequences + 1]")
-        if not page_table.is_cuda or not (page_table.device == key_lengths.device == query_starts.device):
+        device = page_table.get_device()
+        if device < 0 or device != key_lengths.get_device() or device != query_starts.get_device():
             raise ValueError("page_table, key_lengths and query_starts must be CUDA tensors of one device")
         width = page_table.shape[1]
-        if (width > 1 and page_table.stride(1) != 1) or not key_lengths.is_contiguous() or not query_starts.is_contiguous():
+        stride = page_table.stride()
+        if (stride[1] != 1 and width > 1) or not key_lengths.is_contiguous() or not query_starts.is_contiguous():
             raise ValueError("rows of page_table, key_lengths and query_starts must be contiguous")
         if max_query < 0:
             raise ValueError("max_query must not be negative")
         self.page_table, self.key_lengths, self.query_starts, self.max_query = page_table, key_lengths, query_starts, max_query
-        self.device_index = page_table.device.index
-        self._fields = (sequences, width, int(max_query), page_table.data_ptr(), key_lengths.data_ptr(), query_starts.data_ptr(), page_table.stride(0))
+        self.device_index = device
+        self._fields = (sequences, width, int(max_query), page_table.data_ptr(), key_lengths.data_ptr(), query_starts.data_ptr(), stride[0])
 
     def _desc(self, tokens: int) -> abi.PagedBatchDesc:
         sequences, width, max_query, table, lengths, starts, stride = self._fields
