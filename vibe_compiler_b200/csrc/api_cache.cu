@@ -107,26 +107,21 @@ wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cach
   return WB200_OK;
 }
 
-// Which kernels a call takes, from what the host knows: sizes, alignment and the caller's word on the longest chunk. Any
-// choice is right for any lengths. A sequence of up to kRowsBesideChunks packed rows is streamed by the rows kernel (one tile
-// of its MMA), which HBM bounds; a row tile of the chunk kernel takes as long for one row as for 128.
-constexpr int kRowsBesideChunks = 16;
-struct PagedPlan {
-  bool rows, chunk;
-  uint64_t workspace, rows_at;
-};
-PagedPlan plan_attention_paged(const AttentionPagedArgs &a, int sm_count) {
-  PagedPlan plan = {attention_paged_rows_supports(a), false, 0, 0};
-  if (!plan.rows) return plan;                     // the general kernel
+// Which kernel a call takes, from what the host knows: sizes, alignment and the caller's word on the longest chunk. Any choice
+// is right for any lengths. Where a sequence has at most kRowsAtMost packed rows (one tile of its MMA) the rows kernel streams
+// the keys, which HBM bounds; a row tile of the chunk kernel takes as long for one row as for 128.
+constexpr int kRowsAtMost = 16;
+enum class PagedKernel { general, rows, chunk };
+PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
+  if (!attention_paged_rows_supports(a)) return PagedKernel::general;
   int64_t longest = a.batch.max_query > 0 ? a.batch.max_query : (a.batch.tokens <= a.batch.sequences ? 1 : a.batch.tokens);
   if (longest > a.batch.tokens) longest = a.batch.tokens;
-  plan.chunk = longest * (a.q_heads / a.cache.kv_heads) > (getenv("XLIM") ? atoi(getenv("XLIM")) : kRowsBesideChunks) && attention_paged_chunk_supports(a);
-  if (plan.chunk) {
-    plan.rows = a.batch.sequences > 1 && !getenv("XCHUNK");
-    plan.rows_at = (attention_paged_chunk_workspace(sm_count) + 255) / 256 * 256;
-  }
-  plan.workspace = plan.rows_at + (plan.rows ? attention_paged_rows_workspace(sm_count) : 0);
-  return plan;
+  static const int lim = getenv("XLIM") ? atoi(getenv("XLIM")) : kRowsAtMost;
+  return longest * (a.q_heads / a.cache.kv_heads) > lim && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
+}
+uint64_t attention_paged_workspace(PagedKernel kernel, int sm_count) {
+  if (kernel == PagedKernel::general) return 0;
+  return kernel == PagedKernel::rows ? attention_paged_rows_workspace(sm_count) : attention_paged_chunk_workspace(sm_count);
 }
 
 wb200_status make_page_tables(wb200_backend *backend, const wb200_page_tables *t, bool lengths_out, PageTablesArgs *a) {
@@ -216,7 +211,7 @@ uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, con
   if (!backend || !cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
   AttentionPagedArgs a{};
   if (make_attention_paged(nullptr, cache, batch, p, &a) != WB200_OK) return 0;
-  return plan_attention_paged(a, backend->sm_count).workspace;
+  return attention_paged_workspace(choose_attention_paged(a), backend->sm_count);
 }
 
 wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
@@ -229,26 +224,17 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   if (!a.q || !a.out) return fail(WB200_ERR_INVALID_ARGUMENT, "q and out must not be null");
   if (!output_rows_apart(a.cache.head_dim, a.out_token, a.out_head, a.batch.tokens, a.q_heads))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
-  const PagedPlan plan = plan_attention_paged(a, backend->sm_count);
-  if (plan.workspace > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < plan.workspace))
+  const PagedKernel kernel = choose_attention_paged(a);
+  const uint64_t workspace = attention_paged_workspace(kernel, backend->sm_count);
+  if (workspace > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < workspace))
     return fail(WB200_ERR_INVALID_ARGUMENT, "the workspace must be 256-byte aligned and hold wb200_attention_paged_workspace_bytes() bytes");
   DeviceGuard guard(backend->device);
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
-  if (!plan.rows && !plan.chunk) {
-    if ((st = launch_attention_paged_general(a, stream)) == WB200_OK) backend->launches += 1;
-    return st;
-  }
-  const int limit = plan.rows && plan.chunk ? kRowsBesideChunks : 0;
-  if (plan.chunk) {
-    if ((st = launch_attention_paged_chunk(a, limit, backend->sm_count, stream)) != WB200_OK) return st;
-    backend->launches += 2;
-    a.workspace = static_cast<uint8_t *>(a.workspace) + plan.rows_at;
-  }
-  if (plan.rows) {
-    if ((st = launch_attention_paged_rows(a, limit, backend->sm_count, stream)) != WB200_OK) return st;
-    backend->launches += 2;
-  }
-  return WB200_OK;
+  if (kernel == PagedKernel::general) st = launch_attention_paged_general(a, stream);
+  else if (kernel == PagedKernel::rows) st = launch_attention_paged_rows(a, backend->sm_count, stream);
+  else st = launch_attention_paged_chunk(a, backend->sm_count, stream);
+  if (st == WB200_OK) backend->launches += kernel == PagedKernel::general ? 1 : 2;
+  return st;
 }
 
 wb200_status wb200_pages_reserve(wb200_backend *backend, const wb200_page_tables *tables, const int32_t *wanted, int32_t *result) {

@@ -7,9 +7,9 @@
 //            head r % group, 128 / group tokens to a tile. A chunk of 64 tokens of a group of 4 fills the two tiles of an item,
 //            which then reads its keys once instead of four times; Q comes in by one TMA box per tile and half.
 //   keys     A 128-key tile is one TMA box per page part of 2^n rows that divides both (whole tiles of 128-row pages, sixteen
-//            boxes at 8). The loader's lanes look up and issue a box each; page numbers are looked up one tile ahead.
+//            boxes at 8). K and V have a loader warp each, whose lanes look up a page each, one tile ahead.
 //   tails    Rows behind a sequence's last key are not masked by TMA's fill, as the page goes on, and 0 * v is not 0 for what a
-//            stale row may hold. A warp of its own zeroes those rows of V in shared memory before the products see them.
+//            stale row may hold. The V loader zeroes those rows in shared memory before the products see them.
 //   halves   An item is two row tiles of one KV head of one sequence, so that one tile's products run under the other's softmax.
 //            Where the sequence has rows for one tile only, its odd key tiles take the second tile's place, and the two halves
 //            of the state are joined at the end: a step of one row tile costs half of one of two instead of nearly all of it.
@@ -29,17 +29,21 @@ constexpr int kTileM = 128;                     // packed rows per Q tile (TMEM 
 constexpr int kTileN = 128;                     // keys per tile
 constexpr int kBlockBytes = 128 * 128;          // [128 rows][128 B], swizzled
 constexpr int kOutStageBytes = 32 * 128;        // a softmax warp's 32 rows x 64 columns of output
-constexpr int kPlaceBytes = 96;                 // of a softmax warp's place in its share
-constexpr int kThreads = 384;                   // warps: loader, MMA, cleaner, idle, 2 x 4 softmax
+constexpr int kThreads = 384;                   // warps: Q and K loader, MMA, V loader, scheduler, 2 x 4 softmax
+constexpr int kSegments = 4;                    // segments handed out and not yet taken in by every warp
+constexpr int kReaders = 11;                    // warps that take them
 constexpr int kPParts = 2;
 constexpr int kFirstChunks = 3;                 // 32-key chunks of the first part of P, of 4
 constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
 constexpr int kMaxSequences = 4096;             // staged in shared memory
-// Work, in half key tiles' time of two row tiles: a key tile of two row tiles, of one, and what an item costs by itself (its Q,
-// the first scores, the write-out: about one step of two tiles).
-constexpr int kPairWork = 2, kSingleWork = 1, kItemWork = 2;
-constexpr int kLeastWork = 4;                   // no share is made smaller
-constexpr int kLeastCut = 2;                    // a cut this near to an end of an item moves there
+// Work, in fifths of a step of two row tiles (about 3400 clocks): a key tile of two row tiles, of one, and what an item costs by
+// itself (its Q, the first scores, the write-out).
+constexpr int kPairWork = 5, kSingleWork = 3, kItemWork = 8;
+constexpr int kLeastWork = 10;                  // no share is made smaller
+constexpr int kLeastCut = 5;                    // a cut this near to an end of an item moves there
+// What cutting items costs a launch: the records' write-out, one more item to begin in each CTA, and the fold behind the last
+// CTA, about 11 us or six steps of two tiles.
+constexpr int kCutWork = 30;
 
 template <int kHd>
 struct Shape {
@@ -50,11 +54,11 @@ struct Shape {
   static constexpr int kRingOff = 2 * kTileBytes;
   static constexpr int kOutOff = kRingOff + kSlots * kTileBytes;
   static constexpr int kBarOff = kOutOff + 8 * kOutStageBytes;
-  static constexpr int kWalkOff = kBarOff + 512;             // where the softmax warps keep their place in the share
-  static constexpr size_t kBytes = kWalkOff + 8 * kPlaceBytes + 1024;
+  static constexpr int kSegmentOff = kBarOff + 512;
+  static constexpr size_t kBytes = kSegmentOff + kSegments * 64 + 1024;
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
   static constexpr int kRecordFloats = kTileM * kHd + 2 * kTileM;   // acc as [kHd / 4][128 rows][4], then (m, l) per row
-  static_assert(kMaxSequences * 16 <= kSlots * kTileBytes, "the staged lengths must fit the ring");
+  static_assert(kMaxSequences * 24 <= kSlots * kTileBytes, "the staged lengths must fit the ring");
 };
 
 // What the fold has to know about the item that a CTA's share ends inside of; `records` 0: none.
@@ -65,9 +69,9 @@ struct ChunkSplit {
 struct ChunkParams {
   AttentionPagedArgs a;
   int group, tile_tokens;          // query heads per KV head; tokens per Q tile
+  unsigned long long by_group;     // 2^32 / group + 1: row / group = row * by_group >> 32 for the rows of a tile
   int box_rows;                    // keys per TMA box
   int rows_inside;                 // the cache's tensor maps have rows inside heads
-  int rows_limit;                  // sequences with at most this many packed rows are another kernel's
   float scale_log2;
   float *records;                  // [grid][2][2 tiles][kRecordFloats]: a share's end of an item (0), its start of one (1)
   ChunkSplit *splits;              // [grid]
@@ -132,6 +136,15 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
@@ -143,6 +156,8 @@ __device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&v)[4]) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
 }
 
+// Token of a packed row, within its tile.
+__device__ __forceinline__ int token_of(const ChunkParams &p, int row) { return static_cast<int>(row * p.by_group >> 32); }
 // 128-key tiles that Q tile (or pair) whose last token is `last` visits.
 __device__ __forceinline__ int tiles_to(int keys, int count, int causal, int last) {
   int visible = keys;
@@ -176,7 +191,7 @@ __device__ __forceinline__ int cut_tile(const Item &item, int x, int least_cut) 
 struct Place {
   int sequence, kv_head, pair, tile;
 };
-// One CTA's part of an item: key tiles [t0, t1) of its steps.
+// One CTA's part of an item: key tiles [t0, t1) of its steps; t1 0 behind the last.
 struct Segment {
   int begin, count, keys;          // the sequence
   int sequence, kv_head, pair;
@@ -189,15 +204,15 @@ struct Segment {
   }
   __device__ __forceinline__ int tiles() const { return halved ? max(0, min(n0, t1) - t0) : max(of(0), of(1)); }
 };
-// Walks a CTA's share: the same segments in every warp.
+static_assert(sizeof(Segment) <= 64, "the segments' area");
+// The scheduler's walk through its CTA's share.
 struct ShareWalk {
   Place at, end;                   // at.sequence == the batch's: done
-  int begin, count, keys, pairs;   // of the current sequence; count 0: another kernel's, or empty
+  int begin, count, keys, pairs;   // of the current sequence
 
   __device__ __forceinline__ void look_up(const ChunkParams &p) {
     const PagedSequence s = paged_sequence(p.a.batch, p.a.cache, at.sequence, p.a.refused, false);
-    const bool mine = static_cast<long long>(s.count) * p.group > p.rows_limit;
-    begin = s.begin; count = mine ? s.count : 0; keys = s.keys;
+    begin = s.begin; count = s.count; keys = s.keys;
     pairs = (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
   }
   __device__ __forceinline__ bool next(const ChunkParams &p, Segment &out) {
@@ -222,20 +237,9 @@ struct ShareWalk {
     }
     return false;
   }
-  // The next segment with keys to visit.
-  __device__ __forceinline__ bool next_working(const ChunkParams &p, Segment &out) {
-    while (next(p, out))
-      if (out.tiles() > 0) return true;
-    return false;
-  }
 };
-
-// A softmax warp's place in its share, in shared memory: its threads need their registers for the scores.
-struct WarpPlace {
-  ShareWalk walk;
-  Segment segment;
-};
-static_assert(sizeof(WarpPlace) <= kPlaceBytes, "the places' area");
+// floor(a / b) for 0 <= a, 0 < b with a b < 2^53 / 2^8: the quotient's fraction is at least 1 / b away from an integer it misses.
+__device__ __forceinline__ long long floor_ratio(long long a, long long b) { return static_cast<long long>(static_cast<double>(a) / static_cast<double>(b)); }
 
 template <bool kBf16, int kHd>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -259,10 +263,13 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   const uint32_t q_empty = bar_base + 8u * (kFixed + 5 + 2 * kPParts);
   auto half_ready = [&](int quarter) { return bar_base + 8u * (kFixed + 6 + 2 * kPParts + quarter); };   // tile 1's half may be read
   auto half_read = [&](int quarter) { return bar_base + 8u * (kFixed + 10 + 2 * kPParts + quarter); };   // and has been
+  auto segment_full = [&](int i) { return bar_base + 8u * (kFixed + 14 + 2 * kPParts + i); };
+  auto segment_empty = [&](int i) { return bar_base + 8u * (kFixed + 14 + 2 * kPParts + kSegments + i); };
   uint8_t *bar_ptr = smem + L::kBarOff;
-  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 14 + 2 * kPParts));
-  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 15 + 2 * kPParts));
-  static_assert(8 * (kFixed + 16 + 2 * kPParts) <= 512, "the barriers must fit their area");
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 14 + 2 * kPParts + 2 * kSegments));
+  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 15 + 2 * kPParts + 2 * kSegments));
+  Segment *const segments = reinterpret_cast<Segment *>(smem + L::kSegmentOff);
+  static_assert(8 * (kFixed + 16 + 2 * kPParts + 2 * kSegments) <= 512, "the barriers must fit their area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -283,6 +290,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       mbar_init(half_ready(quarter), 1);
       mbar_init(half_read(quarter), 1);
     }
+    for (int i = 0; i < kSegments; ++i) {
+      mbar_init(segment_full(i), 1);
+      mbar_init(segment_empty(i), kReaders);
+    }
     *abort_word = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_q);
@@ -301,30 +312,45 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   pdl_launch_dependents();
 
   // ---- this CTA's share of all work; the lengths are staged in the ring's memory
-  ShareWalk walk;
+  __shared__ Place cuts[2];
+  __shared__ int last_share, item_count, most_work;
   {
-    int2 *staged = reinterpret_cast<int2 *>(smem + L::kRingOff);                                       // (count, keys)
-    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int2));   // inclusive sums of work
+    int4 *staged = reinterpret_cast<int4 *>(smem + L::kRingOff);                                       // begin, count, keys
+    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int4));   // inclusive sums of work
     const int sequences = p.a.batch.sequences;
+    if (threadIdx.x == 0) item_count = most_work = 0;
     for (int s = threadIdx.x; s < sequences; s += kThreads) {
       const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, s, p.a.refused, blockIdx.x == 0);
-      staged[s] = make_int2(static_cast<long long>(q.count) * p.group > p.rows_limit ? q.count : 0, q.keys);
+      staged[s] = make_int4(q.begin, q.count, q.keys, 0);
     }
     __syncthreads();
-    auto pairs_of = [&](int2 s) { return (s.x + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
-    auto pair_work = [&](int2 s, int pair) { return static_cast<long long>(item_work(make_item(p, s.x, s.y, pair))); };
+    auto pairs_of = [&](const int4 &s) { return (s.y + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
+    auto pair_work = [&](const int4 &s, int pair) { return item_work(make_item(p, s.y, s.z, pair)); };
+#pragma unroll 1
     for (int s = warp; s < sequences; s += kThreads / 32) {
-      const int2 q = staged[s];
+      const int4 q = staged[s];
       const int pairs = pairs_of(q);
       long long work = 0;
-      for (int pair = lane; pair < pairs; pair += 32) work += pair_work(q, pair);
+      int most = 0;
+#pragma unroll 1
+      for (int pair = lane; pair < pairs; pair += 32) {
+        const int mine = pair_work(q, pair);
+        work += mine;
+        most = max(most, mine);
+      }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) work += __shfl_xor_sync(0xffffffffu, work, off);
-      if (lane == 0) prefix[s] = work * p.a.cache.kv_heads;
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) {
+        prefix[s] = work * p.a.cache.kv_heads;
+        atomicAdd(&item_count, pairs * p.a.cache.kv_heads);
+        atomicMax(&most_work, most);
+      }
     }
     __syncthreads();
     if (warp == 0) {
       long long base = 0;
+#pragma unroll 1
       for (int start = 0; start < sequences; start += 32) {
         long long value = start + lane < sequences ? prefix[start + lane] : 0;
 #pragma unroll
@@ -337,142 +363,192 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       }
     }
     __syncthreads();
-    const long long total = sequences > 0 ? prefix[sequences - 1] : 0;
-    long long shares = total / kLeastWork;
-    shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
-    const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(total / shares / 32, 1ll << 20)));
-    // Where the cut in front of share `index` falls; also the item it falls on, and the work in front of that.
-    auto cut = [&](long long index, Item &item, long long &item_at) {
-      const long long x = total * index / shares;
+    // Warp 0 places the cut in front of the CTA's share, warp 1 the one behind it.
+    if (warp < 2) {
+      const long long total = sequences > 0 ? prefix[sequences - 1] : 0;
+      const long long shares = max(1ll, min(floor_ratio(total, kLeastWork), static_cast<long long>(gridDim.x)));
+      const long long share = floor_ratio(total, shares);
+      // Items are left whole where the CTA with the most of them ends before one with an equal share and the cost of cuts: items
+      // much alike by counting, others by what a share can grow by.
+      const long long counted = static_cast<long long>((item_count + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x)) * most_work;
+      const bool alike = 10ll * most_work * item_count <= 13ll * total;
+      const bool whole = (alike ? counted : share + most_work) <= share + kCutWork;
+      const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(share >> 5, 1ll << 20)));
+      const long long index = blockIdx.x + warp, x = floor_ratio(total * index, shares);
       Place place = {sequences, 0, 0, 0};
-      if (x >= total) return place;
-      int low = 0, high = sequences - 1;             // first sequence whose sum is beyond x
-      while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (prefix[mid] > x) high = mid;
-        else low = mid + 1;
-      }
-      const long long before = low > 0 ? prefix[low - 1] : 0, per_head = (prefix[low] - before) / p.a.cache.kv_heads;
-      const int2 q = staged[low];
-      const int pairs = pairs_of(q);
-      place.sequence = low;
-      place.kv_head = static_cast<int>((x - before) / per_head);
-      long long rest = x - before - place.kv_head * per_head;
-      for (int start = 0;; start += 32) {            // the pair of row tiles that work `rest` of the head lies in
-        const int pair = start + lane;
-        long long sum = pair < pairs ? pair_work(q, pair) : 0;
+      int last = 0;
+      if (index <= shares && x < total) {
+        int low = 0, high = sequences - 1;             // first sequence whose sum is beyond x
+        while (low < high) {
+          const int mid = (low + high) >> 1;
+          if (prefix[mid] > x) high = mid;
+          else low = mid + 1;
+        }
+        const long long before = low > 0 ? prefix[low - 1] : 0, per_head = floor_ratio(prefix[low] - before, p.a.cache.kv_heads);
+        const int4 q = staged[low];
+        const int pairs = pairs_of(q);
+        place.sequence = low;
+        place.kv_head = static_cast<int>(floor_ratio(x - before, per_head));
+        long long rest = x - before - place.kv_head * per_head;
+#pragma unroll 1
+        for (int start = 0;; start += 32) {            // the pair of row tiles that work `rest` of the head lies in
+          const int pair = start + lane;
+          long long sum = pair < pairs ? pair_work(q, pair) : 0;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const long long other = __shfl_up_sync(0xffffffffu, sum, off);
-          if (lane >= off) sum += other;
+          for (int off = 1; off < 32; off <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += other;
+          }
+          const unsigned int beyond = __ballot_sync(0xffffffffu, sum > rest);
+          if (beyond || start + 32 >= pairs) {
+            const int found = beyond ? __ffs(beyond) - 1 : 31;
+            const long long in_front = __shfl_sync(0xffffffffu, sum, max(found - 1, 0));
+            place.pair = start + found;
+            if (found > 0) rest -= in_front;
+            break;
+          }
+          rest -= __shfl_sync(0xffffffffu, sum, 31);
         }
-        const unsigned int beyond = __ballot_sync(0xffffffffu, sum > rest);
-        if (beyond || start + 32 >= pairs) {
-          const int found = beyond ? __ffs(beyond) - 1 : 31;
-          const long long in_front = found > 0 ? __shfl_sync(0xffffffffu, sum, found - 1) : 0;
-          place.pair = start + found;
-          rest -= in_front;
-          break;
-        }
-        rest -= __shfl_sync(0xffffffffu, sum, 31);
+        const Item item = make_item(p, q.y, q.z, place.pair);
+        const int all = item_work(item);
+        place.tile = whole ? (2 * rest < all ? 0 : item.steps) : cut_tile(item, static_cast<int>(rest), least_cut);
+        // The item goes on in the shares behind this cut, up to the last whose cut does not move to its end.
+        last = static_cast<int>(floor_ratio((x - rest + all - least_cut + 1) * shares - 1, total));
       }
-      item = make_item(p, q.x, q.y, place.pair);
-      item_at = x - rest;
-      place.tile = cut_tile(item, static_cast<int>(rest), least_cut);
-      return place;
-    };
-    walk.at = walk.end = {sequences, 0, 0, 0};
-    walk.begin = walk.count = walk.keys = walk.pairs = 0;
-    ChunkSplit split = {};
-    if (static_cast<long long>(blockIdx.x) < shares && total > 0) {
-      Item item;
-      long long item_at = 0;
-      walk.at = cut(blockIdx.x, item, item_at);
-      walk.end = cut(blockIdx.x + 1, item, item_at);
-      walk.look_up(p);
-      const Place &e = walk.end;
-      const bool starts_here = !(walk.at.sequence == e.sequence && walk.at.kv_head == e.kv_head && walk.at.pair == e.pair && walk.at.tile > 0);
-      if (e.sequence < sequences && e.tile > 0 && e.tile < item.steps && starts_here) {
-        // The item goes on in the shares behind this one, up to the last whose cut does not move to its end.
-        const long long last = ((item_at + item_work(item) - least_cut + 1) * shares - 1) / total;
-        const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, e.sequence, p.a.refused, false);
-        split = {static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1, q.begin, q.count, e.pair, e.kv_head, item.halved, {}};
+      if (lane == 0) {
+        cuts[warp] = place;
+        if (warp == 1) last_share = last;
       }
     }
-    if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
   }
   fence_proxy_async_smem();      // the staged lengths give way to tiles
   __syncthreads();
+
+  // The segments as the scheduler hands them out: every other warp takes them in turn.
+  int segment_at = 0;
+  uint32_t segment_phase = 0;
+  auto take = [&](Segment &seg) {              // false behind the last, or when a wait gave up
+    if (!__all_sync(0xffffffffu, mbar_wait(segment_full(segment_at), segment_phase, abort_word, 103))) return false;
+    seg = segments[segment_at];
+    return seg.t1 > 0;
+  };
+  auto give_back = [&]() {                     // this warp has no more need of the segment in shared memory
+    __syncwarp();
+    if (lane == 0) mbar_arrive(segment_empty(segment_at));
+    if (++segment_at == kSegments) { segment_at = 0; segment_phase ^= 1u; }
+  };
+  auto take_working = [&](Segment &seg) {      // the next one with keys to visit, given back
+    while (take(seg)) {
+      give_back();
+      if (seg.tiles() > 0) return true;
+    }
+    return false;
+  };
 
   // setmaxnreg.inc waits until the CTA's own register pool can supply the request: the totals must fit the launch's.
   static_assert(128 * 104 + 256 * 200 <= kThreads * 168, "setmaxnreg totals exceed the launch allocation");
   if (warp < 4) {
   setmaxnreg_dec<104>();
-  if (warp == 0) {
-    // ------------------------------------------------------------ loader: one box per lane
-    int slot = 0;
-    uint32_t phase = 0, q_loads = 0;
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------ loaders: Q and K by warp 0, V by warp 2. Either walks as a whole
+    // warp and one elected lane issues; a box costs its issuer more than 100 clocks, so two warps share them.
+    const bool is_v = warp == 2;
+    const CUtensorMap *map = is_v ? &tmap_v : &tmap_k;
+    uint32_t position = 0;                           // of the segment's first tile in the ring's order: slot position % kSlots
+    uint32_t q_loads = 0, tail_phases = 0;           // bit s: parity of the next tail in slot s
     bool ok = true;
     Segment seg;
-    const int boxes = kTileN / p.box_rows;           // of 64 columns, per tile and half
-    const int box = lane / L::kHalves, half = lane % L::kHalves;
-    const bool has_box = box < boxes;
+    const int boxes = kTileN / p.box_rows;           // per tile, of 64 columns each
+    const int page_size = p.a.cache.page_size;
+    const int box_slot = lane * p.box_rows / page_size, box_row = lane * p.box_rows % page_size;   // lane i: box i of a tile
+    const int tile_slots = kTileN / page_size, tile_rows = kTileN % page_size;
+    const uint32_t box_bytes = p.box_rows * 128;
     const int q_bytes = p.tile_tokens * p.group * 128 * L::kHalves;
-    while (ok && walk.next_working(p, seg)) {
-      if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (q_loads - 1) & 1u, abort_word, 101))) break;
-      ++q_loads;
+    while (ok && take_working(seg)) {
       const int tiles = seg.tiles();
-      const int token0 = seg.begin + seg.pair * 2 * p.tile_tokens, token1 = token0 + p.tile_tokens;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, seg.halved ? q_bytes : 2 * q_bytes);
-        for (int c = 0; c < L::kHalves; ++c) {
-          tma_load_3d(smem_base + L::kQOff + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token0);
-          if (!seg.halved) tma_load_3d(smem_base + L::kQOff + L::kTileBytes + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token1);
+      if (!is_v) {
+        if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (q_loads - 1) & 1u, abort_word, 101))) break;
+        ++q_loads;
+        const int token0 = seg.begin + seg.pair * 2 * p.tile_tokens, token1 = token0 + p.tile_tokens;
+        if (elect_one_sync()) {
+          mbar_arrive_expect_tx(q_full, seg.halved ? q_bytes : 2 * q_bytes);
+          for (int c = 0; c < L::kHalves; ++c) {
+            tma_load_3d(smem_base + L::kQOff + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token0);
+            if (!seg.halved) tma_load_3d(smem_base + L::kQOff + L::kTileBytes + c * kBlockBytes, &tmap_q, q_full, c * 64, seg.kv_head * p.group, token1);
+          }
         }
+        __syncwarp();
       }
       const int *pages = p.a.batch.page_table + seg.sequence * p.a.batch.table_stride;
-      auto key_of = [&](int j) { return (seg.t0 + j) * kTileN + box * p.box_rows; };
-      auto look_up = [&](int j) { return has_box && j < tiles && key_of(j) < seg.keys ? __ldg(pages + key_of(j) / p.a.cache.page_size) : -1; };
-      auto load = [&](int j, int page, bool is_v) {
-        const int key = key_of(j);
-        const bool loads = has_box && key < seg.keys;
-        if (loads && !is_v && (page < 0 || page >= p.a.cache.pages)) raise_status(p.a.refused, kRefusedPage);   // the box is filled with zeros
-        const int in_page = loads ? key % p.a.cache.page_size : 0;
-        const int y = p.rows_inside ? in_page : seg.kv_head, z = p.rows_inside ? seg.kv_head : in_page;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, loads)) * p.box_rows * 128;
-        if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), phase ^ 1u, abort_word, 102))) { ok = false; return; }
-        const uint32_t bar = is_v && (seg.t0 + j + 1) * kTileN > seg.keys ? tail_full(slot) : kv_full(slot);
-        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-        __syncwarp();
-        if (loads)
-          tma_load_4d(smem_base + L::kRingOff + slot * L::kTileBytes + half * kBlockBytes + box * p.box_rows * 128, is_v ? &tmap_v : &tmap_k, bar,
-                      half * 64, y, z, page);
-        if (++slot == L::kSlots) { slot = 0; phase ^= 1u; }
-      };
-      // The order in which the MMA warp takes them: K of the first tile of each row tile, then V of a tile and K of the next
-      // one of the same row tile in turn.
-      if (!seg.halved) {
-        int page = look_up(0);
-        for (int j = 0; j < tiles && ok; ++j) {
-          const int next_page = look_up(j + 1);
-          load(j, page, false);
-          if (ok) load(j, page, true);
-          page = next_page;
-        }
-      } else {
-        int even = look_up(0), odd = look_up(1);
-        load(0, even, false);
-        if (ok && tiles > 1) load(1, odd, false);
-        for (int j = 0; j < tiles && ok; j += 2) {
-          const int next_even = look_up(j + 2), next_odd = look_up(j + 3);
-          load(j, even, true);
-          if (ok && j + 2 < tiles) load(j + 2, next_even, false);
-          if (ok && j + 1 < tiles) load(j + 1, odd, true);
-          if (ok && j + 3 < tiles) load(j + 3, next_odd, false);
-          even = next_even;
-          odd = next_odd;
-        }
+      // Where the keys of lane i's box of a tile lie: entry of the page table, row in the page. The page is looked up a tile ahead.
+      int at_slot, at_row, page;
+      {
+        const int first = seg.t0 * kTileN / page_size;
+        at_slot = first + box_slot;
+        at_row = seg.t0 * kTileN - first * page_size + box_row;
+        if (at_row >= page_size) { at_row -= page_size; ++at_slot; }
       }
+      int keys_left = seg.keys - seg.t0 * kTileN;
+      auto look_up = [&](int left, int entry) { return lane < boxes && lane * p.box_rows < left ? __ldg(pages + entry) : -1; };
+      page = look_up(keys_left, at_slot);
+      for (int j = 0; j < tiles && ok; ++j, keys_left -= kTileN) {
+        const int row = at_row;
+        at_slot += tile_slots;
+        at_row += tile_rows;
+        if (at_row >= page_size) { at_row -= page_size; ++at_slot; }
+        const int next_page = j + 1 < tiles ? look_up(keys_left - kTileN, at_slot) : -1;
+        const int count = min(boxes, (keys_left + p.box_rows - 1) / p.box_rows);    // boxes that hold a key
+        if (!is_v && lane < count && (page < 0 || page >= p.a.cache.pages)) raise_status(p.a.refused, kRefusedPage);   // zeros come in for it
+        // The order of the ring is that in which the MMA warp takes the tiles: K and V in turn, or, halved, K of the first two
+        // tiles, then V of a tile and K of the next one of its half in turn.
+        uint32_t at = position;
+        if (!seg.halved) at += 2 * j + (is_v ? 1 : 0);
+        else if (is_v) at += j < tiles - 1 ? 2 * j + 2 : 2 * tiles - 1;
+        else at += j < 2 ? j : 2 * j - 1;
+        const int slot = at % L::kSlots;
+        if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), ((at / L::kSlots) & 1u) ^ 1u, abort_word, 102))) { ok = false; break; }
+        const bool tail = is_v && keys_left < kTileN;
+        const uint32_t bar = tail ? tail_full(slot) : kv_full(slot);
+        uint32_t dst = smem_base + L::kRingOff + slot * L::kTileBytes;
+        if (elect_one_sync()) mbar_arrive_expect_tx(bar, count * box_bytes * L::kHalves);
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < count; i += 4, dst += 4 * box_bytes) {     // the operands of four boxes first, then their copies in one go
+          int box_page[4], box_at[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            box_page[u] = __shfl_sync(0xffffffffu, page, (i + u) & 31);
+            box_at[u] = __shfl_sync(0xffffffffu, row, (i + u) & 31);
+          }
+          if (elect_one_sync()) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (i + u >= count) break;
+              const int y = p.rows_inside ? box_at[u] : seg.kv_head, z = p.rows_inside ? seg.kv_head : box_at[u];
+#pragma unroll
+              for (int c = 0; c < L::kHalves; ++c) tma_load_4d(dst + u * box_bytes + c * kBlockBytes, map, bar, c * 64, y, z, box_page[u]);
+            }
+          }
+          __syncwarp();
+        }
+        if (tail) {
+          // V rows behind the sequence's last key give way to zeros before the products see them.
+          if (!__all_sync(0xffffffffu, mbar_wait(bar, (tail_phases >> slot) & 1u, abort_word, 105))) { ok = false; break; }
+          tail_phases ^= 1u << slot;
+          const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+          const uint32_t from = smem_base + L::kRingOff + slot * L::kTileBytes + keys_left * 128;
+#pragma unroll 1
+          for (int i = lane; i < (kTileN - keys_left) * 8; i += 32) {
+#pragma unroll
+            for (int c = 0; c < L::kHalves; ++c) st_shared_v4(from + c * kBlockBytes + i * 16, zero);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv_full(slot));
+        }
+        page = next_page;
+      }
+      position += 2 * tiles;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (the whole warp walks, one elected lane issues)
@@ -529,7 +605,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       Segment seg;
       using Tile0 = std::integral_constant<int, 0>;
       using Tile1 = std::integral_constant<int, 1>;
-      while (ok && walk.next_working(p, seg)) {
+      while (ok && take_working(seg)) {
         const int n0 = seg.of(0), n1 = seg.of(1);
         const int n_max = max(n0, n1);
         ok = mbar_wait(q_full, q_count & 1u, abort_word);
@@ -615,32 +691,29 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         base1 += n1;
       }
     }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------ cleaner: zeroes V rows behind a sequence's last key
-    int slot = 0;
-    uint32_t phases = 0;                             // bit s: parity of the next tail in slot s
-    bool ok = true;
-    Segment seg;
-    while (ok && walk.next_working(p, seg)) {
-      const int tiles = seg.tiles();
-      const int end = seg.t0 + tiles;
-      const int v_slot = (slot + 2 * tiles - 1) % L::kSlots;    // the last tile's V
-      if (end * kTileN > seg.keys) {
-        if (!__all_sync(0xffffffffu, mbar_wait(tail_full(v_slot), (phases >> v_slot) & 1u, abort_word, 105))) { ok = false; break; }
-        phases ^= 1u << v_slot;
-        const int valid = seg.keys - (end - 1) * kTileN;
-        const uint32_t zero[4] = {0u, 0u, 0u, 0u};
-        const int chunks = (kTileN - valid) * 8;     // of 16 bytes, per half
-#pragma unroll
-        for (int h = 0; h < L::kHalves; ++h)
-          for (int i = lane; i < chunks; i += 32)
-            st_shared_v4(smem_base + L::kRingOff + v_slot * L::kTileBytes + h * kBlockBytes + valid * 128 + i * 16, zero);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kv_full(v_slot));
+  } else {
+    // ------------------------------------------------------------ scheduler
+    ShareWalk walk;
+    walk.at = cuts[0];
+    walk.end = cuts[1];
+    walk.begin = walk.count = walk.keys = walk.pairs = 0;
+    if (walk.at.sequence < p.a.batch.sequences) walk.look_up(p);
+    ChunkSplit split = {};
+    bool more = true;
+    while (more) {
+      Segment seg;
+      more = walk.next(p, seg);
+      if (!more) seg = {};
+      // The share ends inside an item that it begins: the fold will want the records of the shares behind it.
+      if (more && seg.t0 == 0 && !seg.whole) split = {last_share - static_cast<int>(blockIdx.x) + 1, seg.begin, seg.count, seg.pair, seg.kv_head, seg.halved, {}};
+      if (!__all_sync(0xffffffffu, mbar_wait(segment_empty(segment_at), segment_phase ^ 1u, abort_word, 104))) break;
+      if (lane == 0) {
+        segments[segment_at] = seg;
+        mbar_arrive(segment_full(segment_at));
       }
-      slot = (slot + 2 * tiles) % L::kSlots;
+      if (++segment_at == kSegments) { segment_at = 0; segment_phase ^= 1u; }
     }
+    if (lane == 0) p.splits[blockIdx.x] = split;
   }
   } else {
     setmaxnreg_inc<200>();
@@ -654,19 +727,11 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     uint32_t tiles_done = 0, items_done = 0, joins = 0;
     bool ok = true;
     const uint32_t out_stage = smem_base + L::kOutOff + (warp - 4) * kOutStageBytes;
-    WarpPlace *place = reinterpret_cast<WarpPlace *>(smem + L::kWalkOff + (warp - 4) * kPlaceBytes);
-    if (lane == 0) place->walk = walk;
-    __syncwarp();
     while (ok) {
       int my_tiles, row_limit, masked_from, key_base, key_step;     // keys from masked_from on are hidden from some row of the tile
       {
-        ShareWalk at = place->walk;
         Segment seg;
-        const bool more = at.next(p, seg);
-        __syncwarp();
-        if (lane == 0) { place->walk = at; place->segment = seg; }
-        __syncwarp();
-        if (!more) break;
+        if (!take(seg)) break;
         my_tiles = seg.of(t);
         key_base = (seg.t0 + (seg.halved ? t : 0)) * kTileN;
         key_step = (seg.halved ? 2 : 1) * kTileN;
@@ -674,7 +739,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         masked_from = seg.keys;
         if (p.a.causal) {                                   // token i sees keys up to keys - count + i
           const int first = seg.keys - seg.count + (2 * seg.pair + (seg.halved ? 0 : t)) * p.tile_tokens;
-          row_limit = min(row_limit, first + row_in_tile / p.group);
+          row_limit = min(row_limit, first + token_of(p, row_in_tile));
           masked_from = min(masked_from, first + 1);
         }
       }
@@ -753,7 +818,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       }
 
       if (ok && my_tiles > 0) ok = mbar_wait(o_done(t), items_done++ & 1u, abort_word, 114 + t);
-      const Segment seg = place->segment;
+      const Segment seg = segments[segment_at];
       const int first_token = (2 * seg.pair + (seg.halved ? 0 : t)) * p.tile_tokens;       // of the tile, within the sequence
       const bool joined = seg.halved && seg.whole;
       if (ok && joined && t == 1) {
@@ -783,46 +848,46 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         scale0 *= coefficient;
         scale1 *= coefficient;
         const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
-        // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes.
+        // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes. The
+        // loops stay rolled: code that runs once per item comes from L2, eight instructions a line.
 #pragma unroll 1
         for (int half = 0; half < L::kHalves; ++half) {
-          uint32_t r[64];
-          if (my_tiles > 0) {
+          __syncwarp();                              // the stage's previous contents have been read
+#pragma unroll 1
+          for (int c = half * 64; c < half * 64 + 64; c += 16) {
+            uint32_t r[16];
+            if (my_tiles > 0) {
+              tmem_ld_32x16(o_addr + c, r);
+              tmem_wait_ld();
+            } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) tmem_ld_32x32(o_addr + half * 64 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
-            tmem_wait_ld();
-          } else {
+              for (int i = 0; i < 16; ++i) r[i] = 0u;
+            }
 #pragma unroll
-            for (int i = 0; i < 64; ++i) r[i] = 0u;
-          }
-#pragma unroll
-          for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale0);
-          if (second_half) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_addr + 128 + half * 64 + c * 32, o);
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale0);
+            if (second_half) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_addr + 128 + c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) r[32 * c + i] = __float_as_uint(fmaf(__uint_as_float(o[i]), scale1, __uint_as_float(r[32 * c + i])));
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), scale1, __uint_as_float(r[i])));
             }
-          }
-          __syncwarp();                              // the stage's previous contents have been read
 #pragma unroll
-          for (int i = 0; i < 64; i += 8) {
-            uint32_t w[4];
+            for (int i = 0; i < 16; i += 8) {
+              uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]));
-              if (empty) w[k] = filled;
+              for (int k = 0; k < 4; ++k) {
+                w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]));
+                if (empty) w[k] = filled;
+              }
+              st_shared_v4(out_stage + lane * 128 + (((((c & 63) + i) >> 3) ^ (lane & 7)) << 4), w);
             }
-            st_shared_v4(out_stage + lane * 128 + (((i >> 3) ^ (lane & 7)) << 4), w);
           }
           __syncwarp();
-#pragma unroll
+#pragma unroll 2
           for (int i = 0; i < 8; ++i) {
             const int r_out = i * 4 + (lane >> 3), chunk = lane & 7;
-            const int packed = quarter * 32 + r_out, at = packed / p.group, token_out = first_token + at;
+            const int packed = quarter * 32 + r_out, at = token_of(p, packed), token_out = first_token + at;
             if (at < p.tile_tokens && token_out < seg.count) {
               uint32_t w[4];
               ld_shared_v4(out_stage + r_out * 128 + ((chunk ^ (r_out & 7)) << 4), w);
@@ -837,7 +902,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
           __syncwarp();
           if (lane == 0) mbar_arrive(half_read(quarter));
         }
-        const int at = row_in_tile / p.group, token = first_token + at;
+        const int at = token_of(p, row_in_tile), token = first_token + at;
         if (p.a.lse && at < p.tile_tokens && token < seg.count)
           p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + seg.kv_head * p.group + row_in_tile - at * p.group] =
               empty ? -INFINITY : m_ref * 0.69314718055994530942f + logf(l_run);
@@ -846,23 +911,24 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         tc_fence_after();
         float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (seg.t0 == 0 ? 1 : 0)) * 2 + t) * L::kRecordFloats;
 #pragma unroll 1
-        for (int part = 0; part < kHd / 32; ++part) {
-          uint32_t r[32];
+        for (int c = 0; c < kHd; c += 16) {
+          uint32_t r[16];
           if (my_tiles > 0) {
-            tmem_ld_32x32(o_addr + part * 32, r);
+            tmem_ld_32x16(o_addr + c, r);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 0u;
+            for (int i = 0; i < 16; ++i) r[i] = 0u;
           }
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4 *>(record + ((part * 8 + (i >> 2)) * kTileM + row_in_tile) * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4 *>(record + (((c + i) >> 2) * kTileM + row_in_tile) * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
         *reinterpret_cast<float2 *>(record + kTileM * kHd + 2 * row_in_tile) = make_float2(m_ref, l_run);
       }
       // The accumulator has been read before this warp lets the next segment's first product over it, by its next arrival.
       tc_fence_before();
+      give_back();
     }
   }
 
@@ -879,7 +945,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   }
 }
 
-// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is the Q tile, blockIdx.z 32 columns, a thread a row.
+// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is the Q tile, blockIdx.z sixteen columns, a thread
+// a row. Two records' elements are on their way together with all their statistics.
 template <bool kBf16, int kHd>
 __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
   using L = Shape<kHd>;
@@ -887,46 +954,50 @@ __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(cons
   pdl_launch_dependents();
   const ChunkSplit split = p.splits[blockIdx.x];
   const int t = blockIdx.y, row = threadIdx.x;       // a halved item's second tile has no rows of its own
-  const int at = row / p.group, token = (2 * split.pair + t) * p.tile_tokens + at;
+  const int at = token_of(p, row), token = (2 * split.pair + t) * p.tile_tokens + at;
   if (split.records == 0 || at >= p.tile_tokens || token >= split.count) return;
   // A halved item's halves are records of their own.
-  const int halves = split.halved ? 2 : 1, records = split.records * halves;
+  const int records = split.records * (split.halved ? 2 : 1);
   auto record = [&](int i) {
     const int share = split.halved ? i >> 1 : i;
     return p.records + ((static_cast<int64_t>(blockIdx.x + share) * 2 + (share == 0 ? 1 : 0)) * 2 + (split.halved ? i & 1 : t)) * L::kRecordFloats;
   };
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < records; ++i) {
-    const float2 ml = *reinterpret_cast<const float2 *>(record(i) + kTileM * kHd + 2 * row);
-    if (ml.y > 0.f) top = fmaxf(top, ml.x);
-  }
-  const float m_exp = top == -INFINITY ? 0.f : top;
-  float l = 0.f, acc[32];
+  float top = -INFINITY, l = 0.f, acc[16];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) acc[e] = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < records; ++i) {
-    const float *r = record(i);
-    const float2 ml = *reinterpret_cast<const float2 *>(r + kTileM * kHd + 2 * row);
-    const float weight = ml.y > 0.f ? ex2_approx(ml.x - m_exp) : 0.f;
-    l = fmaf(ml.y, weight, l);
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < records; i += 2) {
+    const bool both = i + 1 < records;
+    const float *r[2] = {record(i), record(both ? i + 1 : i)};
+    float2 ml[2];
+    float4 v[2][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float4 v = *reinterpret_cast<const float4 *>(r + ((blockIdx.z * 8 + e) * kTileM + row) * 4);
-      acc[4 * e] = fmaf(v.x, weight, acc[4 * e]);
-      acc[4 * e + 1] = fmaf(v.y, weight, acc[4 * e + 1]);
-      acc[4 * e + 2] = fmaf(v.z, weight, acc[4 * e + 2]);
-      acc[4 * e + 3] = fmaf(v.w, weight, acc[4 * e + 3]);
+    for (int u = 0; u < 2; ++u) {
+      ml[u] = *reinterpret_cast<const float2 *>(r[u] + kTileM * kHd + 2 * row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[u][e] = *reinterpret_cast<const float4 *>(r[u] + ((blockIdx.z * 4 + e) * kTileM + row) * 4);
+    }
+    if (!both) ml[1].y = 0.f;
+    const float next = fmaxf(top, fmaxf(ml[0].y > 0.f ? ml[0].x : -INFINITY, ml[1].y > 0.f ? ml[1].x : -INFINITY));
+    const float m_exp = next == -INFINITY ? 0.f : next, alpha = ex2_approx(top - m_exp);
+    const float w0 = ml[0].y > 0.f ? ex2_approx(ml[0].x - m_exp) : 0.f, w1 = ml[1].y > 0.f ? ex2_approx(ml[1].x - m_exp) : 0.f;
+    top = next;
+    l = l * alpha + (ml[0].y * w0 + ml[1].y * w1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[4 * e] = acc[4 * e] * alpha + (v[0][e].x * w0 + v[1][e].x * w1);
+      acc[4 * e + 1] = acc[4 * e + 1] * alpha + (v[0][e].y * w0 + v[1][e].y * w1);
+      acc[4 * e + 2] = acc[4 * e + 2] * alpha + (v[0][e].z * w0 + v[1][e].z * w1);
+      acc[4 * e + 3] = acc[4 * e + 3] * alpha + (v[0][e].w * w0 + v[1][e].w * w1);
     }
   }
   const bool empty = l == 0.f;
   const float coefficient = empty ? 0.f : 1.0f / l;
   const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
   const int head = split.kv_head * p.group + row - at * p.group;
-  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.z * 32;
+  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.z * 16;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 2; ++e) {
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -988,13 +1059,13 @@ bool attention_paged_chunk_supports(const AttentionPagedArgs &a) {
 
 size_t attention_paged_chunk_workspace(int sm_count) { return chunk_record_bytes(sm_count) + static_cast<size_t>(sm_count) * sizeof(ChunkSplit); }
 
-wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int rows_limit, int sm_count, cudaStream_t stream) {
+wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int sm_count, cudaStream_t stream) {
   ChunkParams p{};
   p.a = a;
   p.group = a.q_heads / a.cache.kv_heads;
   p.tile_tokens = kTileM / p.group;
+  p.by_group = (1ull << 32) / p.group + 1;
   p.box_rows = box_rows_of(a.cache.page_size);
-  p.rows_limit = rows_limit;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.records = static_cast<float *>(a.workspace);
   p.splits = reinterpret_cast<ChunkSplit *>(static_cast<uint8_t *>(a.workspace) + chunk_record_bytes(sm_count));
@@ -1030,7 +1101,7 @@ wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int rows_
   });
   if (st != WB200_OK) return st;
   WB200_CUDA_CHECK(launch_dependent(kernel, sm_count, kThreads, wide ? Shape<128>::kBytes : Shape<64>::kBytes, stream, tq, tk, tv, p));
-  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, 2, a.cache.head_dim / 32), kTileM, 0, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, 2, a.cache.head_dim / 16), kTileM, 0, stream, p));
   return WB200_OK;
 }
 

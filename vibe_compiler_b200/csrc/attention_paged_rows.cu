@@ -42,7 +42,6 @@ struct RowsSplit {
 struct RowsParams {
   AttentionPagedArgs a;
   int group;                        // query heads per KV head
-  int rows_limit;                   // sequences of more packed rows are another kernel's; 0: none are
   int least_steps;                  // no share is made smaller than this many steps
   float scale_log2;
   float *records;                   // [grid][2][rows per tile][kRecord]: a share's end of a unit (0), its start of one (1)
@@ -139,7 +138,7 @@ struct RowsUnits {
 };
 template <int kRows>
 __device__ __forceinline__ RowsUnits rows_units(const RowsParams &p, const PagedSequence &s) {
-  if (s.count == 0 || (p.rows_limit > 0 && static_cast<long long>(s.count) * p.group > p.rows_limit)) return {1, 0};
+  if (s.count == 0) return {1, 0};
   const int steps = s.keys == 0 ? 1 : (s.keys - 1) / kStepKeys + 1;
   const long long tiles = (static_cast<long long>(s.count) * p.group + kRows - 1) / kRows;
   return {steps, tiles * p.a.cache.kv_heads * steps};
@@ -537,17 +536,16 @@ bool attention_paged_rows_supports(const AttentionPagedArgs &a) {
 
 size_t attention_paged_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kCtasPerSm * sizeof(RowsSplit); }
 
-wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int rows_limit, int sm_count, cudaStream_t stream) {
+wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_count, cudaStream_t stream) {
   RowsParams p{};
   p.a = a;
   p.group = a.q_heads / a.cache.kv_heads;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.rows_limit = rows_limit;
   p.least_steps = 2;
   p.records = static_cast<float *>(a.workspace);
   p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
-  // Tiles of 8 rows where a sequence's rows fit one, as far as the caller says; beside chunks, most of the others bring one token.
-  const bool narrow = static_cast<int64_t>(p.group) * (a.batch.max_query > 0 && rows_limit == 0 ? a.batch.max_query : 1) <= 8;
+  // Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
+  const bool narrow = static_cast<int64_t>(p.group) * (a.batch.max_query > 0 ? a.batch.max_query : 1) <= 8;
   const int wide = a.cache.head_dim == 128 ? 1 : 0, bf16 = a.cache.format == WB200_BF16 ? 1 : 0;
   static PerDeviceOnce attributes;
   const wb200_status st = attributes.run([]() -> wb200_status {

@@ -338,13 +338,11 @@ wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cuda
 // Few rows per KV head (attention_paged_rows.cu): two launches.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
 size_t attention_paged_rows_workspace(int sm_count);
-wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int rows_limit, int sm_count, cudaStream_t stream);
-// Chunks of tokens on tcgen05 tensor cores (attention_paged_chunk.cu): two launches. `rows_limit` cuts a batch between the two:
-// sequences of at most that many (token, query head of a group) rows are the rows kernel's (0 there: all are), the others the
-// chunk kernel's (0 there: all are).
+wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int sm_count, cudaStream_t stream);
+// Chunks of tokens on tcgen05 tensor cores (attention_paged_chunk.cu): two launches.
 bool attention_paged_chunk_supports(const AttentionPagedArgs &args);
 size_t attention_paged_chunk_workspace(int sm_count);
-wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &args, int rows_limit, int sm_count, cudaStream_t stream);
+wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &args, int sm_count, cudaStream_t stream);
 
 struct PageTablesArgs {
   int sequences, table_width, pages, page_size;
