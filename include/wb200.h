@@ -541,7 +541,8 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
  * zero_fully_masked) and its lse -inf. Cache rows behind key_lengths[s] may hold anything; a NaN or infinite V element of a
  * key inside the length reaches the rows that do not see the key too, as 0 * v does.
  * head_dim is a multiple of 8 up to 256. `workspace` needs wb200_attention_paged_workspace_bytes() bytes, 256-byte
- * aligned, of any content; calls that may run at the same time need one each. */
+ * aligned, of any content; calls that may run at the same time need one each. Without cache, batch and params that function
+ * returns what is enough for any call of the backend (about 40 MB). */
 typedef struct wb200_attention_paged_params {
   uint32_t q_heads;
   uint8_t causal, zero_fully_masked, reserved[2];

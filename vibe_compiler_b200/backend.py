@@ -160,6 +160,7 @@ class ResultPool:
 
 class B200TargetModelBackend:
     _results = ResultPool()   # shared by the backends of the process
+    _paged_workspace: Optional[int] = None   # bytes that are enough for any attention_paged call
 
     def __init__(self, device: int = 0):
         self._lib = abi.load()
@@ -649,12 +650,11 @@ class B200TargetModelBackend:
         p = abi.AttentionPagedParams.from_buffer_copy(_PAGED_PACK(
             shape[1], bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
             lse.data_ptr() if lse is not None else 0, q_strides[0], q_strides[1], out_strides[0], out_strides[1], 0, 0, stream))
-        arguments = self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)
-        needed = self._lib.wb200_attention_paged_workspace_bytes(*arguments)
-        if needed:
-            workspace = self._empty(q, needed, stream, torch.uint8)
-            p.workspace, p.workspace_bytes = workspace.data_ptr(), needed
-        self._check(self._lib.wb200_attention_paged(*arguments))
+        if self._paged_workspace is None:
+            self._paged_workspace = int(self._lib.wb200_attention_paged_workspace_bytes(self._handle, None, None, None))
+        workspace = self._empty(q, self._paged_workspace, stream, torch.uint8)
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), self._paged_workspace
+        self._check(self._lib.wb200_attention_paged(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
         return out
 
     def _page_tables(self, table, lengths, refs, page_size, out, stream, with_lengths=True):
@@ -666,7 +666,10 @@ class B200TargetModelBackend:
             raise ValueError("table [sequences, width], lengths [sequences] and refs [pages] must be int32 tensors on the backend's device with contiguous rows")
         inputs = (table, lengths, refs) if with_lengths else (table, refs)
         if out is None:
-            out = tuple([self._empty(t, t.shape, stream) for t in inputs])
+            if stream == torch._C._cuda_getCurrentRawStream(device):
+                out = tuple([torch.empty_like(t) for t in inputs])
+            else:
+                out = tuple([self._empty(t, t.shape, stream) for t in inputs])
         else:
             out = tuple(out)
             if len(out) != len(inputs) or any(o.shape != t.shape or o.dtype != i32 or o.get_device() != device for o, t in zip(out, inputs)) or \

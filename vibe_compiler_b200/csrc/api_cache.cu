@@ -116,8 +116,7 @@ PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
   if (!attention_paged_rows_supports(a)) return PagedKernel::general;
   int64_t longest = a.batch.max_query > 0 ? a.batch.max_query : (a.batch.tokens <= a.batch.sequences ? 1 : a.batch.tokens);
   if (longest > a.batch.tokens) longest = a.batch.tokens;
-  static const int lim = getenv("XLIM") ? atoi(getenv("XLIM")) : kRowsAtMost;
-  return longest * (a.q_heads / a.cache.kv_heads) > lim && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
+  return longest * (a.q_heads / a.cache.kv_heads) > kRowsAtMost && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
 }
 uint64_t attention_paged_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;
@@ -208,7 +207,12 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
 
 uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
                                                const wb200_attention_paged_params *p) {
-  if (!backend || !cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
+  if (!backend) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
+  if (!cache && !batch && !p) {
+    const uint64_t rows = attention_paged_rows_workspace(backend->sm_count), chunk = attention_paged_chunk_workspace(backend->sm_count);
+    return rows > chunk ? rows : chunk;
+  }
+  if (!cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
   AttentionPagedArgs a{};
   if (make_attention_paged(nullptr, cache, batch, p, &a) != WB200_OK) return 0;
   return attention_paged_workspace(choose_attention_paged(a), backend->sm_count);

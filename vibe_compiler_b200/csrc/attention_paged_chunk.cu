@@ -36,14 +36,14 @@ constexpr int kPParts = 2;
 constexpr int kFirstChunks = 3;                 // 32-key chunks of the first part of P, of 4
 constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
 constexpr int kMaxSequences = 4096;             // staged in shared memory
-// Work, in fifths of a step of two row tiles (about 3400 clocks): a key tile of two row tiles, of one, and what an item costs by
-// itself (its Q, the first scores, the write-out).
-constexpr int kPairWork = 5, kSingleWork = 3, kItemWork = 8;
-constexpr int kLeastWork = 10;                  // no share is made smaller
-constexpr int kLeastCut = 5;                    // a cut this near to an end of an item moves there
+// Work, in twelfths of a step of two row tiles (3250 clocks): a key tile of two row tiles, of one (1820 clocks), and what an item
+// costs by itself (its Q, the first scores, the write-out: 4700).
+constexpr int kPairWork = 12, kSingleWork = 7, kItemWork = 18;
+constexpr int kLeastWork = 24;                  // no share is made smaller
+constexpr int kLeastCut = 12;                   // a cut this near to an end of an item moves there
 // What cutting items costs a launch: the records' write-out, one more item to begin in each CTA, and the fold behind the last
 // CTA, about 11 us or six steps of two tiles.
-constexpr int kCutWork = 30;
+constexpr int kCutWork = 72;
 
 template <int kHd>
 struct Shape {
@@ -373,7 +373,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       const long long counted = static_cast<long long>((item_count + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x)) * most_work;
       const bool alike = 10ll * most_work * item_count <= 13ll * total;
       const bool whole = (alike ? counted : share + most_work) <= share + kCutWork;
-      const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(share >> 5, 1ll << 20)));
+      const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(share >> 6, 1ll << 20)));
       const long long index = blockIdx.x + warp, x = floor_ratio(total * index, shares);
       Place place = {sequences, 0, 0, 0};
       int last = 0;

@@ -73,43 +73,36 @@ struct Elements {
     }
   }
 };
-// One item of one head: two vectors, where they go, and the rotation of their pairs.
+// Turns the pairs of two vectors by (sin, cos) of turns[i]: (v0[i], v1[i]) in the half layout, neighbours when interleaved.
 template <int kFormat, int kVec>
-struct Row {
-  bool live, rotates, has1;
-  int token;
-  uint8_t *to0, *to1;
-  Elements<kFormat, kVec> v0, v1;
-  // turns[i] = (sin, cos) of pair i of the item. Half layout: (v0[i], v1[i]). Interleaved: neighbours.
-  __device__ __forceinline__ void turn(const float2 *turns, int interleaved) {
-    if constexpr (kVec == 1) {
-      const float x = v0.get(0), y = v1.get(0);
-      const float2 u = turns[0];
-      v0.set(0, fmaf(x, u.y, -(y * u.x)), 0.f);
-      v1.set(0, fmaf(y, u.y, x * u.x), 0.f);
-    } else if (interleaved) {
+__device__ __forceinline__ void turn(Elements<kFormat, kVec> &v0, Elements<kFormat, kVec> &v1, const float2 *turns, int interleaved) {
+  if constexpr (kVec == 1) {
+    const float x = v0.get(0), y = v1.get(0);
+    const float2 u = turns[0];
+    v0.set(0, fmaf(x, u.y, -(y * u.x)), 0.f);
+    v1.set(0, fmaf(y, u.y, x * u.x), 0.f);
+  } else if (interleaved) {
 #pragma unroll
-      for (int i = 0; i < kVec; i += 2) {
-        const float2 u = turns[i / 2], w = turns[kVec / 2 + i / 2];
-        const float x = v0.get(i), y = v0.get(i + 1), z = v1.get(i), q = v1.get(i + 1);
-        v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(y, u.y, x * u.x));
-        v1.set(i, fmaf(z, w.y, -(q * w.x)), fmaf(q, w.y, z * w.x));
-      }
-    } else {
+    for (int i = 0; i < kVec; i += 2) {
+      const float2 u = turns[i / 2], w = turns[kVec / 2 + i / 2];
+      const float x = v0.get(i), y = v0.get(i + 1), z = v1.get(i), q = v1.get(i + 1);
+      v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(y, u.y, x * u.x));
+      v1.set(i, fmaf(z, w.y, -(q * w.x)), fmaf(q, w.y, z * w.x));
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < kVec; i += 2) {
-        const float2 u = turns[i], w = turns[i + 1];
-        const float x = v0.get(i), y = v1.get(i), z = v0.get(i + 1), q = v1.get(i + 1);
-        v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(z, w.y, -(q * w.x)));
-        v1.set(i, fmaf(y, u.y, x * u.x), fmaf(q, w.y, z * w.x));
-      }
+    for (int i = 0; i < kVec; i += 2) {
+      const float2 u = turns[i], w = turns[i + 1];
+      const float x = v0.get(i), y = v1.get(i), z = v0.get(i + 1), q = v1.get(i + 1);
+      v0.set(i, fmaf(x, u.y, -(y * u.x)), fmaf(z, w.y, -(q * w.x)));
+      v1.set(i, fmaf(y, u.y, x * u.x), fmaf(q, w.y, z * w.x));
     }
   }
-};
+}
 
 // A block takes `tokens_per_block` tokens; an item is 2 * kVec elements of one head: kVec pairs, or elements that are copied.
 template <int kFormat, int kVec, bool kAppend>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ RotaryConstants c) {
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ RotaryConstants c) {
   constexpr int kElementBytes = kFormat == WB200_F32 ? 4 : 2;
   __shared__ float2 angles[kMaxAnglesPerBlock];
   __shared__ int64_t k_row[kMaxTokensPerBlock], v_row[kMaxTokensPerBlock];   // element offsets of the tokens' cache rows
@@ -164,64 +157,42 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     angles[i] = make_float2(sc.x * c.magnitude, sc.y * c.magnitude);
   }
   __syncthreads();
-  // A thread keeps to one item of the head (or every lanes-th) and takes every groups-th head of the block's tokens, two at a
-  // time so that their loads are in flight together; nothing is divided in the loop.
+  // A thread keeps to one item of the head (or every lanes-th) and takes every groups-th head of the block's tokens; nothing is
+  // divided in the loop.
   const int lanes = min(p.items, kThreads), groups = kThreads / lanes, group = static_cast<int>(threadIdx.x) / lanes;
   if (group >= groups) return;
   for (int item = static_cast<int>(threadIdx.x) - group * lanes; item < p.items; item += lanes) {
-    const bool in_pairs = item * kVec < c.pairs;
-    Row<kFormat, kVec> row[2];
     int t = 0, head = group;
-    auto settle = [&]() { while (head >= a.heads) { head -= a.heads; ++t; } };
-    settle();
-    while (t < count) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        row[u].live = t < count;
-        if (row[u].live) {
-          row[u].token = t;
-          int64_t src = (first + t) * a.x_token + head * a.x_head, dst = (first + t) * a.out_token + head * a.out_head;
-          void *base = a.out;
-          row[u].rotates = in_pairs;
-          if constexpr (kAppend) {
-            row[u].live = state_of[t] != 0;
-            if (head >= p.q_heads + p.cache.kv_heads) {
-              base = p.cache.v;
-              dst = v_row[t] + (head - p.q_heads - p.cache.kv_heads) * p.cache.v_head;
-              row[u].rotates = false;
-            } else if (head >= p.q_heads) {
-              base = p.cache.k;
-              dst = k_row[t] + (head - p.q_heads) * p.cache.k_head;
-            }
-          }
-          // The item's two vectors: of the pairs, or the 2 kVec elements in their place where they are copied.
-          int d0, d1;
-          if (row[u].rotates) {
-            d0 = a.interleaved ? 2 * item * kVec : item * kVec;
-            d1 = a.interleaved ? d0 + kVec : d0 + c.pairs;
-          } else {
-            d0 = 2 * item * kVec;
-            d1 = d0 + kVec;
-          }
-          row[u].to0 = static_cast<uint8_t *>(base) + (dst + d0) * kElementBytes;
-          row[u].to1 = static_cast<uint8_t *>(base) + (dst + d1) * kElementBytes;
-          row[u].has1 = d1 + kVec <= a.head_dim;
-          const uint8_t *x = static_cast<const uint8_t *>(a.x) + src * kElementBytes;
-          if (row[u].live) {
-            row[u].v0.load(x + static_cast<int64_t>(d0) * kElementBytes);
-            if (row[u].has1) row[u].v1.load(x + static_cast<int64_t>(d1) * kElementBytes);
-          }
+    while (true) {
+      while (head >= a.heads) { head -= a.heads; ++t; }
+      if (t >= count) break;
+      int64_t dst = (first + t) * a.out_token + head * a.out_head;
+      uint8_t *base = static_cast<uint8_t *>(a.out);
+      bool rotates = item * kVec < c.pairs, live = true;
+      if constexpr (kAppend) {
+        live = state_of[t] != 0;
+        if (head >= p.q_heads + p.cache.kv_heads) {
+          base = static_cast<uint8_t *>(p.cache.v);
+          dst = v_row[t] + (head - p.q_heads - p.cache.kv_heads) * p.cache.v_head;
+          rotates = false;
+        } else if (head >= p.q_heads) {
+          base = static_cast<uint8_t *>(p.cache.k);
+          dst = k_row[t] + (head - p.q_heads) * p.cache.k_head;
         }
-        head += groups;
-        settle();
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (!row[u].live) continue;
-        if (row[u].rotates) row[u].turn(angles + row[u].token * c.pairs + item * kVec, a.interleaved);
-        row[u].v0.store(row[u].to0);
-        if (row[u].has1) row[u].v1.store(row[u].to1);
+      if (live) {
+        // The item's two vectors: of the pairs, or the 2 kVec elements in their place where they are copied.
+        const int d0 = (rotates && !a.interleaved ? 1 : 2) * item * kVec, d1 = d0 + (rotates && !a.interleaved ? c.pairs : kVec);
+        const bool has1 = d1 + kVec <= a.head_dim;
+        const uint8_t *x = static_cast<const uint8_t *>(a.x) + ((first + t) * a.x_token + head * a.x_head) * kElementBytes;
+        Elements<kFormat, kVec> v0, v1;
+        v0.load(x + static_cast<int64_t>(d0) * kElementBytes);
+        if (has1) v1.load(x + static_cast<int64_t>(d1) * kElementBytes);
+        if (rotates) turn(v0, v1, angles + t * c.pairs + item * kVec, a.interleaved);
+        v0.store(base + (dst + d0) * kElementBytes);
+        if (has1) v1.store(base + (dst + d1) * kElementBytes);
       }
+      head += groups;
     }
   }
 }
@@ -234,10 +205,12 @@ wb200_status launch(RotaryParams p, const RotaryConstants &c, bool aligned, cuda
   const bool wide = aligned && c.pairs % vec == 0 && a.head_dim % vec == 0;
   const int step = 2 * (wide ? vec : 1);
   p.items = (a.head_dim + step - 1) / step;   // rotated pairs fill whole items
-  // A block's threads pass over its heads eight times where that leaves eight blocks to an SM, to spread what a block costs
-  // before its first load (positions, angles); few tokens get a block each.
+  // A block's threads pass over its tokens' heads about twice, so that the eight blocks of an SM overlap one another's positions,
+  // angles, loads and stores; few tokens get a block each. Gradient of 16384 x 40 x 128 bf16 (336 MB, 51 us at the copy rate) and
+  // prompts of 13 thousand tokens x 48 heads: 60 / 73 us; four passes 61 / 74, eight 61 / 76, sixteen 72 / 88; two heads of a thread
+  // in flight 65 / 84 (58 registers, four blocks to an SM); blocks of 128 threads 67 / 84, of 512 70 / 78.
   const int groups = p.items < kThreads ? kThreads / p.items : 1;
-  int per_block = (8 * groups + a.heads - 1) / a.heads;
+  int per_block = (2 * groups + a.heads - 1) / a.heads;
   if (per_block > kMaxTokensPerBlock) per_block = kMaxTokensPerBlock;
   if (c.pairs > 0 && per_block > kMaxAnglesPerBlock / c.pairs) per_block = kMaxAnglesPerBlock / c.pairs;
   while (per_block > 1 && a.tokens / per_block < 148 * 8) --per_block;
