@@ -468,7 +468,8 @@ wb200_status wb200_decoder_layer_timeline(wb200_backend *backend, float *ms, uin
  * per invocation. All buffers are device buffers of the backend's device; every call enqueues its kernels on `stream`,
  * allocates nothing and returns without synchronising, so calls can be captured into CUDA graphs. What the kernels find
  * wrong in device data (a page outside the cache, lengths outside the table, an index twice) they leave out, never reading
- * or writing outside the given buffers, and the next wb200_backend_poll() returns WB200_ERR_INVALID_ARGUMENT. */
+ * or writing outside the given buffers, and the next wb200_backend_poll() returns WB200_ERR_INVALID_ARGUMENT; the results of
+ * the sequences concerned have no meaning. One row of a page table covers at most 2^30 tokens. */
 
 /* Rotary positions: for a token at position p and pair i < rotary_dim / 2 of a head,
  *   (y_a, y_b) = magnitude * (x_a cos t - x_b sin t, x_b cos t + x_a sin t),   t = 2 pi p turns_i
@@ -546,7 +547,7 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
 typedef struct wb200_attention_paged_params {
   uint32_t q_heads;
   uint8_t causal, zero_fully_masked, reserved[2];
-  float scale;              /* > 0 */
+  float scale;              /* > 0, at most 1e38 */
   uint32_t reserved2;
   const void *q;            /* [tokens, q_heads, head_dim] at q_token_stride, q_head_stride; cache's format */
   void *out;                /* likewise */

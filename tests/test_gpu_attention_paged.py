@@ -85,6 +85,71 @@ def test_layouts_and_strides(backend, layout, lengths, news):
     backend.poll()
 
 
+@pytest.mark.parametrize("lengths,news", [([300, 1000], [1, 1]), ([300, 1000], [200, 150])])
+@pytest.mark.parametrize("order", ["queries off 16 bytes", "output off 16 bytes", "heads outside tokens", "V in another order than K",
+                                   "pages inside rows", "cache off 16 bytes"])
+def test_orders_that_need_another_kernel(backend, lengths, news, order):
+    size, hq, hk, d = 32, 8, 2, 128
+    cache = make_cache(50, size, hk, d, torch.float16, "rows", 1)
+    batch, tokens = make_batch(lengths, news, size, 50, 2)
+    q = torch.randn(tokens, hq, d, generator=torch.Generator().manual_seed(5)).half().cuda()
+
+    def apart(t, shift):                              # the same values, `shift` elements into a buffer
+        buffer = torch.zeros(t.numel() + shift, dtype=t.dtype, device="cuda")
+        view = buffer[shift:].view(t.shape)
+        view.copy_(t)
+        return view
+    out = None
+    if order == "queries off 16 bytes":
+        q = apart(q, 3)
+    elif order == "output off 16 bytes":
+        out = apart(torch.zeros_like(q), 1)
+    elif order == "heads outside tokens":
+        q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    elif order == "V in another order than K":
+        cache = PagedCache(cache.k, cache.v.transpose(1, 2).contiguous().transpose(1, 2))
+    elif order == "pages inside rows":
+        cache = PagedCache(*(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (cache.k, cache.v)))
+    else:
+        cache = PagedCache(apart(cache.k, 4), apart(cache.v, 4))
+    want, _, bound, _ = ref.attention(q, cache.k, cache.v, batch.page_table, batch.key_lengths, batch.query_starts, 0.1)
+    got = backend.attention_paged(q, cache, batch, 0.1, out=out)
+    backend.poll()
+    assert bool(((got.double() - want).abs() <= bound).all())
+
+
+def test_more_sequences_than_a_block_stages(backend):
+    count = 5000
+    news = [0] * count
+    news[17], news[4999], news[3000] = 40, 1, 9
+    lengths = [0] * count
+    lengths[17], lengths[4999], lengths[3000], lengths[4] = 70, 33, 9, 16
+    cache = make_cache(20, 16, 2, 128, torch.bfloat16, "rows", 1)
+    batch, tokens = make_batch(lengths, news, 16, 20, 2)
+    agree(backend, torch.randn(tokens, 8, 128, device="cuda").bfloat16(), cache, batch, 0.1)
+    few = PagedBatch(batch.page_table[:4000], batch.key_lengths[:4000].contiguous(), batch.query_starts[:4001].contiguous())
+    agree(backend, torch.randn(tokens, 8, 128, device="cuda").bfloat16(), cache, few, 0.1)
+
+
+def test_one_page_in_many_places(backend):
+    # a sequence may list a page more than once: 40 thousand keys over three pages
+    cache = make_cache(3, 128, 2, 128, torch.bfloat16, "rows", 1)
+    table = torch.arange(320, dtype=torch.int32, device="cuda")[None, :] % 3
+    for n in (1, 70):
+        batch = PagedBatch(table, torch.tensor([40900], dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+        agree(backend, torch.randn(n, 8, 128, device="cuda").bfloat16(), cache, batch, 0.1)
+
+
+def test_empty_calls(backend):
+    cache = make_cache(4, 16, 2, 128, torch.bfloat16, "rows", 1)
+    batch, _ = make_batch([20, 0], [0, 0], 16, 4, 2)
+    assert backend.attention_paged(torch.empty(0, 8, 128, dtype=torch.bfloat16, device="cuda"), cache, batch, 0.1).shape == (0, 8, 128)
+    untouched = torch.full((3, 8, 128), 2.0, dtype=torch.bfloat16, device="cuda")
+    backend.attention_paged(torch.zeros_like(untouched), cache, batch, 0.1, out=untouched)
+    backend.poll()
+    assert bool((untouched == 2.0).all())
+
+
 @pytest.mark.parametrize("lengths,news", [([90, 40], [1, 1]), ([90, 40, 10], [60, 50, 30])])
 def test_rows_without_keys(backend, lengths, news):
     # more new tokens than keys: the first ones stand in front of key 0

@@ -66,8 +66,8 @@ wb200_status make_cache(const wb200_paged_cache *c, bool f32_too, PagedCacheArgs
 wb200_status make_batch(const wb200_paged_batch *b, const PagedCacheArgs &c, PagedBatchArgs *a) {
   if (b->sequences > 0x7ffffffeu || b->tokens > 0x7fffffffu || b->table_width > 0x7fffffffu || b->max_query > 0x7fffffffu)
     return fail(WB200_ERR_LIMIT, "paged batch extents too large");
-  if (static_cast<uint64_t>(b->table_width) * static_cast<uint64_t>(c.page_size) > 0x7fffffffull)
-    return fail(WB200_ERR_LIMIT, "a row of the page table covers more than 2^31 - 1 tokens");
+  if (static_cast<uint64_t>(b->table_width) * static_cast<uint64_t>(c.page_size) > (1ull << 30))
+    return fail(WB200_ERR_LIMIT, "a row of the page table covers more than 2^30 tokens");
   if (b->sequences != 0 && b->tokens != 0) {
     if (!b->key_lengths || !b->query_starts || (b->table_width != 0 && !b->page_table))
       return fail(WB200_ERR_INVALID_ARGUMENT, "page_table, key_lengths and query_starts must not be null");
@@ -94,7 +94,7 @@ wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cach
     return fail(WB200_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
   if (cache->head_dim % 8 != 0 || cache->head_dim > 256) return fail(WB200_ERR_UNSUPPORTED, "paged attention takes head dimensions that are multiples of 8, up to 256");
   if (static_cast<uint64_t>(batch->tokens) * p->q_heads > 0x7fffffffull) return fail(WB200_ERR_LIMIT, "more than 2^31 - 1 rows in one paged attention");
-  if (!(p->scale > 0.f) || p->scale > 3.402823466e38f) return fail(WB200_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (!(p->scale > 0.f) || !(p->scale <= 1e38f)) return fail(WB200_ERR_INVALID_ARGUMENT, "scale must be positive and at most 1e38");
   a->q_heads = static_cast<int>(p->q_heads);
   a->causal = p->causal ? 1 : 0;
   a->zero_fully_masked = p->zero_fully_masked ? 1 : 0;
@@ -129,7 +129,7 @@ wb200_status make_page_tables(wb200_backend *backend, const wb200_page_tables *t
     return fail(WB200_ERR_INVALID_ARGUMENT, "page table extents must be positive");
   if (t->sequences > static_cast<uint32_t>(kMaxPagedSequences)) return fail(WB200_ERR_LIMIT, "more than 16384 sequences in one page table");
   if (t->pages > 0x7fffffffu || t->page_size > 0x7fffffffu || static_cast<uint64_t>(t->sequences) * t->table_width > (1ull << 30) ||
-      static_cast<uint64_t>(t->table_width) * t->page_size > 0x7fffffffull)
+      static_cast<uint64_t>(t->table_width) * t->page_size > (1ull << 30))
     return fail(WB200_ERR_LIMIT, "page table extents too large");
   if (!t->table || !t->lengths || !t->refs || !t->table_out || !t->refs_out || (lengths_out && !t->lengths_out))
     return fail(WB200_ERR_INVALID_ARGUMENT, "page table, lengths and refs must not be null");

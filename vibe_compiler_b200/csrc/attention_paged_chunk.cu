@@ -489,7 +489,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         if (at_row >= page_size) { at_row -= page_size; ++at_slot; }
       }
       int keys_left = seg.keys - seg.t0 * kTileN;
-      auto look_up = [&](int left, int entry) { return lane < boxes && lane * p.box_rows < left ? __ldg(pages + entry) : -1; };
+      auto look_up = [&](int left, int entry) { return lane < boxes && lane * p.box_rows < left ? pages[entry] : -1; };
       page = look_up(keys_left, at_slot);
       for (int j = 0; j < tiles && ok; ++j, keys_left -= kTileN) {
         const int row = at_row;
@@ -1053,8 +1053,8 @@ bool attention_paged_chunk_supports(const AttentionPagedArgs &a) {
   if (!attention_paged_rows_supports(a) || group > kTileM || a.batch.sequences > kMaxSequences) return false;
   if (box_rows_of(a.cache.page_size) < 8) return false;      // a box covers whole 8-row groups of the swizzle
   CacheMap map;
-  return make_cache_map(a.cache, &map) &&
-         (a.q_heads == 1 || a.batch.tokens == 1 || a.q_token >= static_cast<int64_t>(a.q_heads - 1) * a.q_head + a.cache.head_dim);   // tokens outside heads
+  return make_cache_map(a.cache, &map) && (a.q_heads == 1 || a.q_head >= a.cache.head_dim) &&
+         (a.q_heads == 1 || a.batch.tokens == 1 || a.q_token >= a.q_heads * a.q_head);   // tokens outside heads
 }
 
 size_t attention_paged_chunk_workspace(int sm_count) { return chunk_record_bytes(sm_count) + static_cast<size_t>(sm_count) * sizeof(ChunkSplit); }

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
     auto look_up = [&](int tile) {
       const int key = first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
-      return tile < tiles && key < key_end ? __ldg(pages + key / a.cache.page_size) : -1;
+      return tile < tiles && key < key_end ? pages[key / a.cache.page_size] : -1;
     };
     auto issue_tile = [&](int tile, int slot, int page) {
       if (tile < tiles) {
