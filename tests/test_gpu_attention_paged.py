@@ -192,7 +192,8 @@ def test_bad_device_data_is_left_out_and_reported(backend, news, fault):
     cache = make_cache(30, 16, 2, 128, torch.bfloat16, "rows", 1)
     batch, tokens = make_batch([200, 150], news, 16, 30, 2)
     q = torch.randn(tokens, 8, 128, device="cuda").bfloat16()
-    want = backend.attention_paged(q, cache, batch, 0.1)
+    # The other sequence's rows are right; where its keys are cut, and so the order of its sums, follows what is left of the batch.
+    want, _, bound, _ = ref.attention(q, cache.k, cache.v, batch.page_table, batch.key_lengths, batch.query_starts, 0.1)
     if fault.startswith("page"):
         batch.page_table[1, 3] = 30 if fault == "page too large" else -7
     elif fault.startswith("length"):
@@ -202,7 +203,7 @@ def test_bad_device_data_is_left_out_and_reported(backend, news, fault):
     got = backend.attention_paged(q, cache, batch, 0.1)
     with pytest.raises(WB200Error):
         backend.poll()
-    assert torch.equal(got[:news[0]], want[:news[0]])
+    assert bool(((got.double() - want).abs() <= bound)[:news[0]].all())
     backend.poll()
 
 

@@ -27,4 +27,8 @@ __device__ __forceinline__ int paged_visible(const PagedSequence &s, int index, 
   return last < 0 ? 0 : last;
 }
 
+// floor(a / b) for whole 0 <= a < 2^53 and 0 < b < 2^53: a quotient that is not whole is at least 1 / b away from the next whole
+// number, more than the division's rounding.
+__device__ __forceinline__ long long floor_ratio(long long a, long long b) { return static_cast<long long>(static_cast<double>(a) / static_cast<double>(b)); }
+
 }  // namespace wb200

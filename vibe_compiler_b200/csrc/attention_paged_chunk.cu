@@ -238,9 +238,6 @@ struct ShareWalk {
     return false;
   }
 };
-// floor(a / b) for 0 <= a, 0 < b with a b < 2^53 / 2^8: the quotient's fraction is at least 1 / b away from an integer it misses.
-__device__ __forceinline__ long long floor_ratio(long long a, long long b) { return static_cast<long long>(static_cast<double>(a) / static_cast<double>(b)); }
-
 template <bool kBf16, int kHd>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,

@@ -29,9 +29,10 @@ struct RowsShape {
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
   static constexpr int kStages = kD == 128 ? 3 : 6;          // 24 KiB of copies in flight per warp either way
   static constexpr int kRingBytes = kStages * 2 * kTileBytes;
-  static constexpr int kSmemBytes = kWarps * kRingBytes;
   static constexpr int kRecord = kD + 4;                     // floats: acc[D], m, l and padding to 16 bytes
-  static_assert(kWarps * 16 * kRecord * 4 <= kSmemBytes, "the warps' records must fit the rings");
+  static constexpr int kRecordsOff = kWarps * kRingBytes;    // the warps' records of eight rows
+  static constexpr int kSmemBytes = kRecordsOff + kWarps * 8 * kRecord * 4;
+  static_assert(2 * (kSmemBytes + 512 + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
 // What the fold has to know about the unit that a CTA's share ends inside of; `records` 0: no such unit.
@@ -42,7 +43,6 @@ struct RowsSplit {
 struct RowsParams {
   AttentionPagedArgs a;
   int group;                        // query heads per KV head
-  int least_steps;                  // no share is made smaller than this many steps
   float scale_log2;
   float *records;                   // [grid][2][rows per tile][kRecord]: a share's end of a unit (0), its start of one (1)
   RowsSplit *splits;                // [grid]
@@ -131,7 +131,12 @@ __device__ __forceinline__ void write_row(const AttentionPagedArgs &a, int token
   if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * a.q_heads + head] = empty ? -INFINITY : m * 0.69314718055994530942f + logf(l);
 }
 
-// Steps of a sequence: tiles of rows x KV heads x steps of keys (at least one, so that rows without keys are written).
+// Work is counted in steps; a unit by itself (its queries, the first copies, the fold over the warps) counts as three, and a cut
+// this near behind its beginning falls on it. 40 sequences of 50 to 8000 keys (107 us at the copy rate) with 0 / 1 / 2 / 3 / 5
+// steps: 130 / 124 / 119 / 117 / 116 us, 100 sequences of 20 to 1000 keys (35 us) 60 / 52 / 47 / 47 / 47.
+constexpr int kUnitSteps = 3;
+constexpr int kLeastSteps = 3;      // no share is made smaller: small batches are latency, and more CTAs shorten it
+// A sequence's units: tiles of rows x KV heads, each of `steps` steps of keys (at least one, so that rows without keys are written).
 struct RowsUnits {
   int steps;
   long long weight;
@@ -141,7 +146,7 @@ __device__ __forceinline__ RowsUnits rows_units(const RowsParams &p, const Paged
   if (s.count == 0) return {1, 0};
   const int steps = s.keys == 0 ? 1 : (s.keys - 1) / kStepKeys + 1;
   const long long tiles = (static_cast<long long>(s.count) * p.group + kRows - 1) / kRows;
-  return {steps, tiles * p.a.cache.kv_heads * steps};
+  return {steps, tiles * p.a.cache.kv_heads * (steps + kUnitSteps)};
 }
 
 template <bool kBf16, int kD, bool kNarrow, bool kAligned>
@@ -183,12 +188,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     if (w < warp) before += warp_totals[w];
     total += warp_totals[w];
   }
-  long long shares = total / p.least_steps;
+  long long shares = floor_ratio(total, kLeastSteps);
   shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
   const long long index = blockIdx.x;
-  auto boundary = [&](long long c) { return total * c / shares; };
-  long long at = index < shares ? boundary(index) : total;
-  const long long share_end = index < shares ? boundary(index + 1) : total;
+  long long at = index < shares ? floor_ratio(total * index, shares) : total;
+  const long long share_end = index < shares ? floor_ratio(total * (index + 1), shares) : total;
   if (at < share_end && before <= at && at < before + mine) {
     long long prefix = before;
     for (int s = first_mine; s < end_mine; ++s) {
@@ -207,70 +211,102 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
   long long prefix = s >= 0 ? start_prefix : 0;
   RowsSplit split = {};
 
-  uint8_t *ring = smem + warp * S::kRingBytes;
-  const uint32_t ring_addr = smem_u32(ring);
-  float *records = reinterpret_cast<float *>(smem);   // [warp][kRows][kRecord], over the rings once they are read
+  const uint32_t ring_addr = smem_u32(smem + warp * S::kRingBytes);
+  float *records = reinterpret_cast<float *>(smem + S::kRecordsOff);   // [warp][8][kRecord]
 
-  while (s >= 0 && at < share_end) {
-    const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
-    const RowsUnits units = rows_units<kRows>(p, sequence);
-    if (at >= prefix + units.weight) {                 // on to the next sequence that has rows
-      prefix += units.weight;
-      if (++s >= a.batch.sequences) break;
-      continue;
-    }
-    const long long unit = (at - prefix) / units.steps;
-    const int step0 = static_cast<int>(at - prefix - unit * units.steps);
-    const int step1 = static_cast<int>(min(static_cast<long long>(units.steps), step0 + (share_end - at)));
-    const int kv_head = static_cast<int>(unit % a.cache.kv_heads), row_tile = static_cast<int>(unit / a.cache.kv_heads);
-    const int row0 = row_tile * kRows;                 // first packed row
-    const int rows_here = static_cast<int>(min(static_cast<long long>(sequence.count) * p.group - row0, static_cast<long long>(kRows)));
-    // keys that the tile's last token sees bound what is read
-    const int tile_keys = min(sequence.keys, paged_visible(sequence, (row0 + rows_here - 1) / p.group, a.causal));
-    const int key_begin = step0 * kStepKeys, key_end = min(tile_keys, step1 * kStepKeys);
-    const int first_key = key_begin + warp * kTileKeys;
-    const int tiles = key_end > first_key ? (key_end - first_key + kStepKeys - 1) / kStepKeys : 0;
-
-    const uint16_t *k_base = static_cast<const uint16_t *>(a.cache.k) + kv_head * a.cache.k_head;
-    const uint16_t *v_base = static_cast<const uint16_t *>(a.cache.v) + kv_head * a.cache.v_head;
-    const int *pages = a.batch.page_table + s * a.batch.table_stride;
-    // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
-    auto look_up = [&](int tile) {
-      const int key = first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
-      return tile < tiles && key < key_end ? pages[key / a.cache.page_size] : -1;
-    };
-    auto issue_tile = [&](int tile, int slot, int page) {
-      if (tile < tiles) {
-        const int key0 = first_key + tile * kStepKeys;
-        const uint32_t k_dst = ring_addr + slot * (2 * S::kTileBytes), v_dst = k_dst + S::kTileBytes;
-        const int own_key = key0 + (lane & 15);
-        const bool inside = page >= 0 && page < a.cache.pages;
-        if (!inside && own_key < key_end) raise_status(a.refused, kRefusedPage);
-        const unsigned int seen = __ballot_sync(0xffffffffu, inside && own_key < key_end) & 0xffffu;
-        if (lane == 0) seen_keys[warp][slot] = static_cast<int>(seen);
-        const int in_page = (kAligned ? key0 : own_key) % a.cache.page_size;
-        const int64_t k_row = (inside ? page : 0) * a.cache.k_page + in_page * a.cache.k_row;
-        const int64_t v_row = (inside ? page : 0) * a.cache.v_page + in_page * a.cache.v_row;
-        constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
-#pragma unroll
-        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
-          const int r = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
-          int64_t k_at, v_at;
-          if constexpr (kAligned) {
-            k_at = k_row + r * a.cache.k_row;
-            v_at = v_row + r * a.cache.v_row;
-          } else {
-            k_at = __shfl_sync(0xffffffffu, k_row, r);
-            v_at = __shfl_sync(0xffffffffu, v_row, r);
-          }
-          const bool reads = (seen >> r) & 1u;         // other rows are zeros
-          cp_async16(k_dst + tile_offset<S::kRowBytes>(r, c), k_base + (reads ? k_at + c * 8 : 0), reads ? 16u : 0u);
-          cp_async16(v_dst + tile_offset<S::kRowBytes>(r, c), v_base + (reads ? v_at + c * 8 : 0), reads ? 16u : 0u);
-        }
+  // The part of a unit that lies in the share: steps [step0, step1) of `steps`, of which this warp takes every fourth tile.
+  struct Part {
+    PagedSequence sequence;
+    int kv_head, row_tile, row0, rows;     // first packed row, rows there are
+    int step0, step1, steps, left;         // left: work of the unit behind the share
+    int first_key, key_end, tiles;         // this warp's
+  } part;
+  const int *pages = nullptr;
+  const uint16_t *k_base = nullptr, *v_base = nullptr;
+  auto next_part = [&]() {
+    while (s >= 0 && at < share_end) {
+      part.sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
+      const RowsUnits units = rows_units<kRows>(p, part.sequence);
+      if (at >= prefix + units.weight) {               // on to the next sequence that has rows
+        prefix += units.weight;
+        if (++s >= a.batch.sequences) return false;
+        continue;
       }
-      cp_async_commit();
-    };
+      const int all = units.steps + kUnitSteps, unit = static_cast<int>(floor_ratio(at - prefix, all));
+      const int begin = static_cast<int>(at - prefix - static_cast<long long>(unit) * all);
+      const int end = static_cast<int>(min(static_cast<long long>(all), begin + (share_end - at)));
+      at += end - begin;
+      part.left = all - end;
+      part.steps = units.steps;
+      part.step0 = max(begin - kUnitSteps, 0);
+      part.step1 = max(end - kUnitSteps, 0);
+      if (part.step1 == part.step0) continue;
+      part.row_tile = unit / a.cache.kv_heads;
+      part.kv_head = unit - part.row_tile * a.cache.kv_heads;
+      part.row0 = part.row_tile * kRows;
+      part.rows = static_cast<int>(min(static_cast<long long>(part.sequence.count) * p.group - part.row0, static_cast<long long>(kRows)));
+      // keys that the tile's last token sees bound what is read
+      const int tile_keys = min(part.sequence.keys, paged_visible(part.sequence, (part.row0 + part.rows - 1) / p.group, a.causal));
+      part.key_end = min(tile_keys, part.step1 * kStepKeys);
+      part.first_key = part.step0 * kStepKeys + warp * kTileKeys;
+      part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
+      pages = a.batch.page_table + s * a.batch.table_stride;
+      k_base = static_cast<const uint16_t *>(a.cache.k) + part.kv_head * a.cache.k_head;
+      v_base = static_cast<const uint16_t *>(a.cache.v) + part.kv_head * a.cache.v_head;
+      return true;
+    }
+    return false;
+  };
+  // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
+  auto look_up = [&](int tile) {
+    const int key = part.first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
+    return tile < part.tiles && key < part.key_end ? pages[key / a.cache.page_size] : -1;
+  };
+  auto issue_tile = [&](int tile, int slot, int page) {
+    if (tile < part.tiles) {
+      const int key0 = part.first_key + tile * kStepKeys;
+      const uint32_t k_dst = ring_addr + slot * (2 * S::kTileBytes), v_dst = k_dst + S::kTileBytes;
+      const int own_key = key0 + (lane & 15);
+      const bool inside = page >= 0 && page < a.cache.pages;
+      if (!inside && own_key < part.key_end) raise_status(a.refused, kRefusedPage);
+      const unsigned int seen = __ballot_sync(0xffffffffu, inside && own_key < part.key_end) & 0xffffu;
+      if (lane == 0) seen_keys[warp][slot] = static_cast<int>(seen);
+      const int in_page = (kAligned ? key0 : own_key) % a.cache.page_size;
+      const int64_t k_row = (inside ? page : 0) * a.cache.k_page + in_page * a.cache.k_row;
+      const int64_t v_row = (inside ? page : 0) * a.cache.v_page + in_page * a.cache.v_row;
+      constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
+#pragma unroll
+      for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+        const int r = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
+        int64_t k_at, v_at;
+        if constexpr (kAligned) {
+          k_at = k_row + r * a.cache.k_row;
+          v_at = v_row + r * a.cache.v_row;
+        } else {
+          k_at = __shfl_sync(0xffffffffu, k_row, r);
+          v_at = __shfl_sync(0xffffffffu, v_row, r);
+        }
+        const bool reads = (seen >> r) & 1u;         // other rows are zeros
+        cp_async16(k_dst + tile_offset<S::kRowBytes>(r, c), k_base + (reads ? k_at + c * 8 : 0), reads ? 16u : 0u);
+        cp_async16(v_dst + tile_offset<S::kRowBytes>(r, c), v_base + (reads ? v_at + c * 8 : 0), reads ? 16u : 0u);
+      }
+    }
+    cp_async_commit();
+  };
+  int page = -1;                                       // of the next tile to be issued
+  auto fill_ring = [&]() {
+    page = look_up(0);
+#pragma unroll 1
+    for (int i = 0; i < S::kStages; ++i) {
+      const int next = look_up(i + 1);
+      issue_tile(i, i, page);
+      page = next;
+    }
+  };
 
+  bool more = next_part();
+  if (more) fill_ring();
+  while (more) {
     constexpr int kHalves = kNarrow ? 1 : 2;           // softmax rows per lane: g (and g + 8)
     constexpr int kAccs = kNarrow ? kD / 16 : kD / 8;  // fragments: 16 elements x 8 rows, or 16 rows x 8 elements
     float m_run[kHalves], l_run[kHalves], acc[kAccs][4];
@@ -279,28 +315,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     for (int h = 0; h < kHalves; ++h) {
       m_run[h] = -INFINITY;
       l_run[h] = 0.f;
-      last_key[h] = paged_visible(sequence, (row0 + g + 8 * h) / p.group, a.causal) - 1;
+      last_key[h] = paged_visible(part.sequence, (part.row0 + g + 8 * h) / p.group, a.causal) - 1;
     }
 #pragma unroll
     for (int j = 0; j < kAccs; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-
-    int page = look_up(0);
-#pragma unroll 1
-    for (int i = 0; i < S::kStages; ++i) {
-      const int next = look_up(i + 1);
-      issue_tile(i, i, page);
-      page = next;
-    }
     // The tile's rows as A fragments (rows behind the last are zero).
     uint32_t q_frag[kD / 16][4];
     {
       const uint32_t *rows[2] = {nullptr, nullptr};
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        const int packed = row0 + g + 8 * h, token = packed / p.group;
-        if (g + 8 * h < rows_here)
-          rows[h] = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + static_cast<int64_t>(sequence.begin + token) * a.q_token +
-                                                       (kv_head * p.group + packed - token * p.group) * a.q_head) + t;
+        const int packed = part.row0 + g + 8 * h, token = packed / p.group;
+        if (g + 8 * h < part.rows)
+          rows[h] = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + static_cast<int64_t>(part.sequence.begin + token) * a.q_token +
+                                                       (part.kv_head * p.group + packed - token * p.group) * a.q_head) + t;
       }
 #pragma unroll
       for (int ks = 0; ks < kD / 16; ++ks) {
@@ -313,21 +341,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
 
     int slot = 0;
 #pragma unroll 1
-    for (int tile = 0; tile < tiles; ++tile) {
+    for (int tile = 0; tile < part.tiles; ++tile) {
       const int next = look_up(tile + S::kStages + 1);
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint32_t k_src = ring_addr + slot * (2 * S::kTileBytes), v_src = k_src + S::kTileBytes;
-      const int key0 = first_key + tile * kStepKeys + 2 * t;
+      const int key0 = part.first_key + tile * kStepKeys + 2 * t;
       const unsigned int seen = static_cast<unsigned int>(seen_keys[warp][slot]) >> (2 * t);
-      float part[2][2][4] = {};                        // even and odd k-steps apart: four short chains
+      float dot[2][2][4] = {};                         // even and odd k-steps apart: four short chains
 #pragma unroll
       for (int ks = 0; ks < kD / 16; ++ks) {
         const int mi = lane >> 3;
         uint32_t bfrag[4];
         ldmatrix_x4(k_src + tile_offset<S::kRowBytes>((mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), bfrag);
-        mma_16816<kBf16>(part[ks & 1][0], q_frag[ks], bfrag[0], bfrag[1]);
-        mma_16816<kBf16>(part[ks & 1][1], q_frag[ks], bfrag[2], bfrag[3]);
+        mma_16816<kBf16>(dot[ks & 1][0], q_frag[ks], bfrag[0], bfrag[1]);
+        mma_16816<kBf16>(dot[ks & 1][1], q_frag[ks], bfrag[2], bfrag[3]);
       }
       float alpha[kHalves], pr[kHalves][4];            // keys 2t, 2t + 1, 8 + 2t, 9 + 2t
 #pragma unroll
@@ -336,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int offset = (i >> 1) * 8 + (i & 1);
-          sc[i] = (part[0][i >> 1][2 * h + (i & 1)] + part[1][i >> 1][2 * h + (i & 1)]) * p.scale_log2;
+          sc[i] = (dot[0][i >> 1][2 * h + (i & 1)] + dot[1][i >> 1][2 * h + (i & 1)]) * p.scale_log2;
           if (!((seen >> offset) & 1u) || key0 + offset > last_key[h]) sc[i] = -INFINITY;
         }
         float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
@@ -387,71 +415,71 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
       page = next;
       if (++slot == S::kStages) slot = 0;
     }
-    cp_async_wait<0>();
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
       l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
     }
-    __syncthreads();   // the rings are free
-    {
-      float *mine_records = records + warp * (kRows * S::kRecord);
+    // The next part's first tiles are on their way while this one's state is put together. (The ring's groups of copies have all
+    // been waited for but the empty ones behind the last tile.)
+    const Part done = part;
+    more = next_part();
+    if (more) fill_ring();
+    const bool whole = done.step0 == 0 && done.step1 == done.steps;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {                // eight rows at a time
+      __syncthreads();                                 // the records of the rows before have been read
+      float *mine_records = records + warp * (8 * S::kRecord);
       if constexpr (kNarrow) {
 #pragma unroll
         for (int j = 0; j < kAccs; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mine_records[(2 * t + (i & 1)) * S::kRecord + j * 16 + g + 8 * (i >> 1)] = acc[j][i];
-      }
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        float *row = mine_records + (g + 8 * h) * S::kRecord;
-        if constexpr (!kNarrow) {
-#pragma unroll
-          for (int j = 0; j < kAccs; ++j) *reinterpret_cast<float2 *>(row + j * 8 + 2 * t) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-        }
-        if (t == 0) *reinterpret_cast<float2 *>(row + kD) = make_float2(m_run[h], l_run[h]);
-      }
-    }
-    __syncthreads();
-    // Fold over the warps, a warp per row, with the row's maximum as the common exponent reference.
-    const bool whole = step0 == 0 && step1 == units.steps;
-    for (int r = warp; r < rows_here; r += kWarps) {
-      float2 ml[kWarps];
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        ml[w] = *reinterpret_cast<const float2 *>(records + (w * kRows + r) * S::kRecord + kD);
-        top = fmaxf(top, ml[w].x);
-      }
-      const float m_exp = top == -INFINITY ? 0.f : top;
-      float l = 0.f;
-      Slice<kD> sum = {};
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float weight = exp2_fast(ml[w].x - m_exp);
-        Slice<kD> part;
-        part.load(records + (w * kRows + r) * S::kRecord, lane);
-        l = fmaf(ml[w].y, weight, l);
-#pragma unroll
-        for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(part.v[e], weight, sum.v[e]);
-      }
-      if (whole) {
-        const int packed = row0 + r, token = packed / p.group;
-        write_row<kBf16, kD>(a, sequence.begin + token, kv_head * p.group + packed - token * p.group, lane, top, l, sum);
       } else {
-        float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (step0 == 0 ? 1 : 0)) * kRows + r) * S::kRecord;
-        sum.store(record, lane);
-        if (lane == 0) *reinterpret_cast<float2 *>(record + kD) = make_float2(top, l);
+#pragma unroll
+        for (int j = 0; j < kAccs; ++j) *reinterpret_cast<float2 *>(mine_records + g * S::kRecord + j * 8 + 2 * t) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+      }
+      if (t == 0) *reinterpret_cast<float2 *>(mine_records + g * S::kRecord + kD) = make_float2(m_run[h], l_run[h]);
+      __syncthreads();
+      // Fold over the warps, a warp per row, with the row's maximum as the common exponent reference.
+      for (int r = warp; r < 8 && r + 8 * h < done.rows; r += kWarps) {
+        float2 ml[kWarps];
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          ml[w] = *reinterpret_cast<const float2 *>(records + (w * 8 + r) * S::kRecord + kD);
+          top = fmaxf(top, ml[w].x);
+        }
+        const float m_exp = top == -INFINITY ? 0.f : top;
+        float l = 0.f;
+        Slice<kD> sum = {};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float weight = exp2_fast(ml[w].x - m_exp);
+          Slice<kD> slice;
+          slice.load(records + (w * 8 + r) * S::kRecord, lane);
+          l = fmaf(ml[w].y, weight, l);
+#pragma unroll
+          for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(slice.v[e], weight, sum.v[e]);
+        }
+        const int row = r + 8 * h;
+        if (whole) {
+          const int packed = done.row0 + row, token = packed / p.group;
+          write_row<kBf16, kD>(a, done.sequence.begin + token, done.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+        } else {
+          float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (done.step0 == 0 ? 1 : 0)) * kRows + row) * S::kRecord;
+          sum.store(record, lane);
+          if (lane == 0) *reinterpret_cast<float2 *>(record + kD) = make_float2(top, l);
+        }
       }
     }
-    at += step1 - step0;
-    if (step0 == 0 && step1 < units.steps) {           // the unit starts here and goes on in the CTAs behind this one
-      const long long unit_end = at + (units.steps - step1);
-      const long long last = (unit_end * shares - 1) / total;   // the last share that begins in front of the unit's end
-      split = {1 + static_cast<int>(last - index), sequence.begin, sequence.count, row_tile, kv_head, {}};
+    if (done.step0 == 0 && !whole) {
+      // The unit ends the share and goes on in the CTAs behind this one, up to the last share that begins in front of its end.
+      const long long last = floor_ratio((share_end + done.left) * shares - 1, total);
+      split = {1 + static_cast<int>(last - index), done.sequence.begin, done.sequence.count, done.row_tile, done.kv_head, {}};
     }
-    __syncthreads();   // the records have been read before the rings are written again
   }
+  cp_async_wait<0>();
   if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
 }
 
@@ -541,7 +569,6 @@ wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_cou
   p.a = a;
   p.group = a.q_heads / a.cache.kv_heads;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.least_steps = 2;
   p.records = static_cast<float *>(a.workspace);
   p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
   // Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
