@@ -61,8 +61,9 @@ def test_attention_matches_float64(backend, dtype, causal, lengths, news, size, 
     batch, tokens = make_batch(lengths, news, size, pages, 2, spare_rows=3)
     spoil_unused(cache, batch, size)
     q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
-    for max_query in (0, 1, max(news)):              # a hint: right, wrong or missing
-        hinted = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query)
+    wide, _ = make_batch(lengths, news, size, pages, 2, width=65536 // size + 2)     # room for longer sequences
+    for max_query, table in ((0, batch.page_table), (1, batch.page_table), (max(news), batch.page_table), (1, wide.page_table), (0, wide.page_table)):
+        hinted = PagedBatch(table, batch.key_lengths, batch.query_starts, max_query=max_query)      # a hint: right, wrong or missing
         agree(backend, q, cache, hinted, head_dim ** -0.5, causal=causal, zero_fully_masked=max_query == 1)
 
 

@@ -237,7 +237,8 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   if (kernel == PagedKernel::general) st = launch_attention_paged_general(a, stream);
   else if (kernel == PagedKernel::rows) st = launch_attention_paged_rows(a, backend->sm_count, stream);
   else st = launch_attention_paged_chunk(a, backend->sm_count, stream);
-  if (st == WB200_OK) backend->launches += kernel == PagedKernel::general ? 1 : 2;
+  const bool one = kernel == PagedKernel::general || (kernel == PagedKernel::rows && attention_paged_rows_clustered(a, backend->sm_count));
+  if (st == WB200_OK) backend->launches += one ? 1 : 2;
   return st;
 }
 

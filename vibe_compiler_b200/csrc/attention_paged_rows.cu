@@ -22,6 +22,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTileKeys = 16;
 constexpr int kStepKeys = kWarps * kTileKeys;
+constexpr int kCluster = 8;         // the portable cluster size
 
 template <int kD>
 struct RowsShape {
@@ -107,6 +108,15 @@ struct Slice {
       v[0] = w.x; v[1] = w.y;
     }
   }
+  __device__ __forceinline__ void load_cluster(uint32_t row, int lane) {     // of a CTA of the cluster
+    if constexpr (kPer == 4) {
+      const float4 w = ld_cluster_f32x4(row + 16 * lane);
+      v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+      const float2 w = ld_cluster_f32x2(row + 8 * lane);
+      v[0] = w.x; v[1] = w.y;
+    }
+  }
   __device__ __forceinline__ void store(float *row, int lane) const {
     if constexpr (kPer == 4) *reinterpret_cast<float4 *>(row + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
     else *reinterpret_cast<float2 *>(row + 2 * lane) = make_float2(v[0], v[1]);
@@ -149,7 +159,9 @@ __device__ __forceinline__ RowsUnits rows_units(const RowsParams &p, const Paged
   return {steps, tiles * p.a.cache.kv_heads * (steps + kUnitSteps)};
 }
 
-template <bool kBf16, int kD, bool kNarrow, bool kAligned>
+// kClustered: a cluster of kCluster CTAs takes a whole unit (blockIdx.y), an equal part of its keys each, and its first CTA folds
+// their states through distributed shared memory: one launch and no records, for batches of few units.
+template <bool kBf16, int kD, bool kNarrow, bool kAligned, bool kClustered>
 __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(const __grid_constant__ RowsParams p) {
   using S = RowsShape<kD>;
   constexpr int kRows = kNarrow ? 8 : 16;
@@ -160,55 +172,59 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
   const AttentionPagedArgs &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const bool reports = blockIdx.x == 0;
   pdl_wait();
   pdl_launch_dependents();
 
-  // This CTA's share of all steps. A thread sums up a run of consecutive sequences.
-  const int per_thread = (a.batch.sequences + kWarps * 32 - 1) / (kWarps * 32);
-  const int first_mine = min(a.batch.sequences, static_cast<int>(threadIdx.x) * per_thread), end_mine = min(a.batch.sequences, first_mine + per_thread);
-  long long mine = 0;
-  for (int s = first_mine; s < end_mine; ++s) {
-    const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, reports);
-    mine += rows_units<kRows>(p, sequence).weight;
-  }
-  long long before = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, before, off);
-    if (lane >= off) before += other;
-  }
-  if (lane == 31) warp_totals[warp] = before;
-  if (threadIdx.x == 0) start_sequence = -1;
-  __syncthreads();
-  long long total = 0;
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += warp_totals[w];
-    total += warp_totals[w];
-  }
-  long long shares = floor_ratio(total, kLeastSteps);
-  shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
+  // This CTA's share of all steps: at .. share_end, from sequence s on, in front of which `prefix` steps lie.
+  int s = -1, next_tile = 0;
+  long long total = 0, shares = 1, at = 0, share_end = 0, prefix = 0;
   const long long index = blockIdx.x;
-  long long at = index < shares ? floor_ratio(total * index, shares) : total;
-  const long long share_end = index < shares ? floor_ratio(total * (index + 1), shares) : total;
-  if (at < share_end && before <= at && at < before + mine) {
-    long long prefix = before;
-    for (int s = first_mine; s < end_mine; ++s) {
-      const PagedSequence sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
-      const long long weight = rows_units<kRows>(p, sequence).weight;
-      if (at < prefix + weight) {
-        start_sequence = s;
-        start_prefix = prefix;
-        break;
-      }
-      prefix += weight;
+  if constexpr (!kClustered) {
+    // A thread sums up a run of consecutive sequences.
+    const int per_thread = (a.batch.sequences + kWarps * 32 - 1) / (kWarps * 32);
+    const int first_mine = min(a.batch.sequences, static_cast<int>(threadIdx.x) * per_thread), end_mine = min(a.batch.sequences, first_mine + per_thread);
+    long long mine = 0;
+    for (int i = first_mine; i < end_mine; ++i) {
+      const PagedSequence sequence = paged_sequence(a.batch, a.cache, i, a.refused, blockIdx.x == 0);
+      mine += rows_units<kRows>(p, sequence).weight;
     }
+    long long before = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, before, off);
+      if (lane >= off) before += other;
+    }
+    if (lane == 31) warp_totals[warp] = before;
+    if (threadIdx.x == 0) start_sequence = -1;
+    __syncthreads();
+    before -= mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_totals[w];
+      total += warp_totals[w];
+    }
+    shares = floor_ratio(total, kLeastSteps);
+    shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
+    at = index < shares ? floor_ratio(total * index, shares) : total;
+    share_end = index < shares ? floor_ratio(total * (index + 1), shares) : total;
+    if (at < share_end && before <= at && at < before + mine) {
+      for (int i = first_mine; i < end_mine; ++i) {
+        const PagedSequence sequence = paged_sequence(a.batch, a.cache, i, a.refused, false);
+        const long long weight = rows_units<kRows>(p, sequence).weight;
+        if (at < before + weight) {
+          start_sequence = i;
+          start_prefix = before;
+          break;
+        }
+        before += weight;
+      }
+    }
+    __syncthreads();
+    s = start_sequence;
+    prefix = s >= 0 ? start_prefix : 0;
+  } else {
+    s = static_cast<int>(blockIdx.y) / a.cache.kv_heads;
   }
-  __syncthreads();
-  int s = start_sequence;
-  long long prefix = s >= 0 ? start_prefix : 0;
   RowsSplit split = {};
 
   const uint32_t ring_addr = smem_u32(smem + warp * S::kRingBytes);
@@ -220,42 +236,58 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     int kv_head, row_tile, row0, rows;     // first packed row, rows there are
     int step0, step1, steps, left;         // left: work of the unit behind the share
     int first_key, key_end, tiles;         // this warp's
-  } part;
+  } part = {};
   const int *pages = nullptr;
   const uint16_t *k_base = nullptr, *v_base = nullptr;
+  auto settle_part = [&]() {
+    part.row0 = part.row_tile * kRows;
+    part.rows = static_cast<int>(min(static_cast<long long>(part.sequence.count) * p.group - part.row0, static_cast<long long>(kRows)));
+    // keys that the tile's last token sees bound what is read
+    const int tile_keys = min(part.sequence.keys, paged_visible(part.sequence, (part.row0 + part.rows - 1) / p.group, a.causal));
+    part.key_end = min(tile_keys, part.step1 * kStepKeys);
+    part.first_key = part.step0 * kStepKeys + warp * kTileKeys;
+    part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
+    pages = a.batch.page_table + s * a.batch.table_stride;
+    k_base = static_cast<const uint16_t *>(a.cache.k) + part.kv_head * a.cache.k_head;
+    v_base = static_cast<const uint16_t *>(a.cache.v) + part.kv_head * a.cache.v_head;
+  };
   auto next_part = [&]() {
-    while (s >= 0 && at < share_end) {
-      part.sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
-      const RowsUnits units = rows_units<kRows>(p, part.sequence);
-      if (at >= prefix + units.weight) {               // on to the next sequence that has rows
-        prefix += units.weight;
-        if (++s >= a.batch.sequences) return false;
-        continue;
-      }
-      const int all = units.steps + kUnitSteps, unit = static_cast<int>(floor_ratio(at - prefix, all));
-      const int begin = static_cast<int>(at - prefix - static_cast<long long>(unit) * all);
-      const int end = static_cast<int>(min(static_cast<long long>(all), begin + (share_end - at)));
-      at += end - begin;
-      part.left = all - end;
-      part.steps = units.steps;
-      part.step0 = max(begin - kUnitSteps, 0);
-      part.step1 = max(end - kUnitSteps, 0);
-      if (part.step1 == part.step0) continue;
-      part.row_tile = unit / a.cache.kv_heads;
-      part.kv_head = unit - part.row_tile * a.cache.kv_heads;
-      part.row0 = part.row_tile * kRows;
-      part.rows = static_cast<int>(min(static_cast<long long>(part.sequence.count) * p.group - part.row0, static_cast<long long>(kRows)));
-      // keys that the tile's last token sees bound what is read
-      const int tile_keys = min(part.sequence.keys, paged_visible(part.sequence, (part.row0 + part.rows - 1) / p.group, a.causal));
-      part.key_end = min(tile_keys, part.step1 * kStepKeys);
-      part.first_key = part.step0 * kStepKeys + warp * kTileKeys;
-      part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
-      pages = a.batch.page_table + s * a.batch.table_stride;
-      k_base = static_cast<const uint16_t *>(a.cache.k) + part.kv_head * a.cache.k_head;
-      v_base = static_cast<const uint16_t *>(a.cache.v) + part.kv_head * a.cache.v_head;
+    if constexpr (kClustered) {
+      // The next tile of rows of the sequence; every CTA of the cluster has a part of it, be it empty.
+      part.kv_head = static_cast<int>(blockIdx.y) - s * a.cache.kv_heads;
+      part.sequence = paged_sequence(a.batch, a.cache, s, a.refused, blockIdx.x == 0 && part.kv_head == 0);
+      if (static_cast<long long>(next_tile) * kRows >= static_cast<long long>(part.sequence.count) * p.group) return false;
+      part.row_tile = next_tile++;
+      part.steps = rows_units<kRows>(p, part.sequence).steps;
+      part.step0 = static_cast<int>(static_cast<long long>(part.steps) * blockIdx.x / kCluster);
+      part.step1 = static_cast<int>(static_cast<long long>(part.steps) * (blockIdx.x + 1) / kCluster);
+      settle_part();
       return true;
+    } else {
+      while (s >= 0 && at < share_end) {
+        part.sequence = paged_sequence(a.batch, a.cache, s, a.refused, false);
+        const RowsUnits units = rows_units<kRows>(p, part.sequence);
+        if (at >= prefix + units.weight) {               // on to the next sequence that has rows
+          prefix += units.weight;
+          if (++s >= a.batch.sequences) return false;
+          continue;
+        }
+        const int all = units.steps + kUnitSteps, unit = static_cast<int>(floor_ratio(at - prefix, all));
+        const int begin = static_cast<int>(at - prefix - static_cast<long long>(unit) * all);
+        const int end = static_cast<int>(min(static_cast<long long>(all), begin + (share_end - at)));
+        at += end - begin;
+        part.left = all - end;
+        part.steps = units.steps;
+        part.step0 = max(begin - kUnitSteps, 0);
+        part.step1 = max(end - kUnitSteps, 0);
+        if (part.step1 == part.step0) continue;
+        part.row_tile = unit / a.cache.kv_heads;
+        part.kv_head = unit - part.row_tile * a.cache.kv_heads;
+        settle_part();
+        return true;
+      }
+      return false;
     }
-    return false;
   };
   // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
   auto look_up = [&](int tile) {
@@ -463,7 +495,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
           for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(slice.v[e], weight, sum.v[e]);
         }
         const int row = r + 8 * h;
-        if (whole) {
+        if constexpr (kClustered) {                    // over the first warp's record, which this warp has read
+          sum.store(records + r * S::kRecord, lane);
+          if (lane == 0) *reinterpret_cast<float2 *>(records + r * S::kRecord + kD) = make_float2(top, l);
+        } else if (whole) {
           const int packed = done.row0 + row, token = packed / p.group;
           write_row<kBf16, kD>(a, done.sequence.begin + token, done.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
         } else {
@@ -472,15 +507,44 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
           if (lane == 0) *reinterpret_cast<float2 *>(record + kD) = make_float2(top, l);
         }
       }
+      if constexpr (kClustered) {
+        cluster_sync_all();                            // the CTAs' states are in their shared memory
+        if (blockIdx.x == 0) {
+          for (int r = warp; r < 8 && r + 8 * h < done.rows; r += kWarps) {
+            const uint32_t local = smem_u32(records + r * S::kRecord);
+            float2 ml = make_float2(-INFINITY, 0.f);   // of CTA `lane`
+            if (lane < kCluster) ml = ld_cluster_f32x2(cluster_map_shared(local + kD * 4, lane));
+            float top = ml.x;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float weight = exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
+            float l = ml.y * weight;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            Slice<kD> sum = {};
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) {
+              Slice<kD> slice;
+              slice.load_cluster(cluster_map_shared(local, c), lane);
+              const float w = __shfl_sync(0xffffffffu, weight, c);
+#pragma unroll
+              for (int e = 0; e < Slice<kD>::kPer; ++e) sum.v[e] = fmaf(slice.v[e], w, sum.v[e]);
+            }
+            const int packed = done.row0 + r + 8 * h, token = packed / p.group;
+            write_row<kBf16, kD>(a, done.sequence.begin + token, done.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+          }
+        }
+        cluster_sync_all();                            // and are kept until they have been read
+      }
     }
-    if (done.step0 == 0 && !whole) {
+    if (!kClustered && done.step0 == 0 && !whole) {
       // The unit ends the share and goes on in the CTAs behind this one, up to the last share that begins in front of its end.
       const long long last = floor_ratio((share_end + done.left) * shares - 1, total);
       split = {1 + static_cast<int>(last - index), done.sequence.begin, done.sequence.count, done.row_tile, done.kv_head, {}};
     }
   }
   cp_async_wait<0>();
-  if (threadIdx.x == 0) p.splits[blockIdx.x] = split;
+  if (!kClustered && threadIdx.x == 0) p.splits[blockIdx.x] = split;
 }
 
 // Folds the records of the unit that starts in share blockIdx.x and goes on in the shares behind it: row blockIdx.y, a thread
@@ -533,15 +597,16 @@ __global__ void __launch_bounds__(kD) attention_paged_fold_kernel(const __grid_c
 }
 
 using RowsKernel = void (*)(const RowsParams);
-template <bool kBf16, int kD, bool kNarrow>
+template <bool kBf16, int kD, bool kNarrow, bool kClustered>
 constexpr RowsKernel rows_kernel(bool aligned) {
-  return aligned ? attention_paged_rows_kernel<kBf16, kD, kNarrow, true> : attention_paged_rows_kernel<kBf16, kD, kNarrow, false>;
+  return aligned ? attention_paged_rows_kernel<kBf16, kD, kNarrow, true, kClustered> : attention_paged_rows_kernel<kBf16, kD, kNarrow, false, kClustered>;
 }
-#define WB200_ROWS_KERNELS(D, NARROW)                                                                               \
-  {{rows_kernel<false, D, NARROW>(false), rows_kernel<false, D, NARROW>(true)},                                     \
-   {rows_kernel<true, D, NARROW>(false), rows_kernel<true, D, NARROW>(true)}}
-const RowsKernel kRowsKernels[2][2][2][2] = {   // [head_dim 128][narrow][bf16][aligned]
-    {WB200_ROWS_KERNELS(64, false), WB200_ROWS_KERNELS(64, true)}, {WB200_ROWS_KERNELS(128, false), WB200_ROWS_KERNELS(128, true)}};
+#define WB200_ROWS_KERNELS(D, NARROW, CLUSTERED)                                                                          \
+  {{rows_kernel<false, D, NARROW, CLUSTERED>(false), rows_kernel<false, D, NARROW, CLUSTERED>(true)},                     \
+   {rows_kernel<true, D, NARROW, CLUSTERED>(false), rows_kernel<true, D, NARROW, CLUSTERED>(true)}}
+const RowsKernel kRowsKernels[2][2][2][2][2] = {   // [clustered][head_dim 128][narrow][bf16][aligned]
+    {{WB200_ROWS_KERNELS(64, false, false), WB200_ROWS_KERNELS(64, true, false)}, {WB200_ROWS_KERNELS(128, false, false), WB200_ROWS_KERNELS(128, true, false)}},
+    {{WB200_ROWS_KERNELS(64, false, true), WB200_ROWS_KERNELS(64, true, true)}, {WB200_ROWS_KERNELS(128, false, true), WB200_ROWS_KERNELS(128, true, true)}}};
 const RowsKernel kFoldKernels[2][2][2] = {      // [head_dim 128][narrow][bf16]
     {{attention_paged_fold_kernel<false, 64, false>, attention_paged_fold_kernel<true, 64, false>},
      {attention_paged_fold_kernel<false, 64, true>, attention_paged_fold_kernel<true, 64, true>}},
@@ -562,6 +627,18 @@ bool attention_paged_rows_supports(const AttentionPagedArgs &a) {
   return (bits & 15u) == 0;     // rows begin on 16 bytes
 }
 
+// Clusters where all units' are resident at once (clusters of eight leave a part of every GPC unused) and, at the longest the
+// page table can hold, an eighth of a unit's keys through one CTA (39 bytes / ns) does not take longer than all keys through the
+// whole GPU (6500 bytes / ns) and the second launch (4 us). One launch and two, head_dim 128, 16-row pages, per call in a graph:
+// 1 x 8 KV heads, 500 / 2000 / 4000 / 16000 keys 5.6 / 7.7 / 11.0 / 31.8 and 10.0 / 9.7 / 11.0 / 20.5 us; 4 x 8, 1000 / 4000 / 32000
+// keys 7.2 / 16.4 / 84.7 and 11.0 / 19.2 / 87.0 us.
+bool attention_paged_rows_clustered(const AttentionPagedArgs &a, int sm_count) {
+  const int64_t units = static_cast<int64_t>(a.batch.sequences) * a.cache.kv_heads;
+  if (units * kCluster > sm_count * kCtasPerSm * 7 / 8) return false;
+  const double unit_bytes = 4.0 * a.cache.head_dim * a.cache.page_size * a.batch.table_width;
+  return unit_bytes / kCluster / 39.0 <= static_cast<double>(units) * unit_bytes / 6500.0 + 4000.0;
+}
+
 size_t attention_paged_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kCtasPerSm * sizeof(RowsSplit); }
 
 wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_count, cudaStream_t stream) {
@@ -580,14 +657,32 @@ wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_cou
       for (int n = 0; n < 2; ++n)
         for (int b = 0; b < 2; ++b)
           for (int al = 0; al < 2; ++al)
-            WB200_CUDA_CHECK(cudaFuncSetAttribute(kRowsKernels[d][n][b][al], cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  d ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes));
+            for (int c = 0; c < 2; ++c)
+              WB200_CUDA_CHECK(cudaFuncSetAttribute(kRowsKernels[c][d][n][b][al], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                    d ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes));
     return WB200_OK;
   });
   if (st != WB200_OK) return st;
+  const size_t smem = wide ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes;
+  const bool aligned = a.cache.page_size % kTileKeys == 0;
+  if (attention_paged_rows_clustered(a, sm_count)) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(kCluster, static_cast<unsigned>(a.batch.sequences) * a.cache.kv_heads);
+    config.blockDim = dim3(kWarps * 32);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes_of[2];
+    attributes_of[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes_of[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes_of[1].id = cudaLaunchAttributeClusterDimension;
+    attributes_of[1].val.clusterDim.x = kCluster; attributes_of[1].val.clusterDim.y = 1; attributes_of[1].val.clusterDim.z = 1;
+    config.attrs = attributes_of;
+    config.numAttrs = 2;
+    WB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kRowsKernels[1][wide][narrow][bf16][aligned], p));
+    return WB200_OK;
+  }
   const unsigned grid = static_cast<unsigned>(sm_count * kCtasPerSm);
-  WB200_CUDA_CHECK(launch_dependent(kRowsKernels[wide][narrow][bf16][a.cache.page_size % kTileKeys == 0], grid, kWarps * 32,
-                                    wide ? RowsShape<128>::kSmemBytes : RowsShape<64>::kSmemBytes, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(kRowsKernels[0][wide][narrow][bf16][aligned], grid, kWarps * 32, smem, stream, p));
   WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], dim3(grid, narrow ? 8 : 16), a.cache.head_dim, 0, stream, p));
   return WB200_OK;
 }

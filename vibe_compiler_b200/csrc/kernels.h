@@ -335,8 +335,9 @@ struct AttentionPagedArgs {
   int *status;        // bounded waits
 };
 wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cudaStream_t stream);
-// Few rows per KV head (attention_paged_rows.cu): two launches.
+// Few rows per KV head (attention_paged_rows.cu): one launch where `clustered`, else two.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
+bool attention_paged_rows_clustered(const AttentionPagedArgs &args, int sm_count);
 size_t attention_paged_rows_workspace(int sm_count);
 wb200_status launch_attention_paged_rows(const AttentionPagedArgs &args, int sm_count, cudaStream_t stream);
 // Chunks of tokens on tcgen05 tensor cores (attention_paged_chunk.cu): two launches.
