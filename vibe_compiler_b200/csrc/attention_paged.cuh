@@ -27,6 +27,17 @@ __device__ __forceinline__ int paged_visible(const PagedSequence &s, int index, 
   return last < 0 ? 0 : last;
 }
 
+// The first sequence from s on that brings tokens, or the number of sequences; by a whole warp, 32 sequences at a look.
+__device__ __forceinline__ int next_with_tokens(const PagedBatchArgs &b, int s) {
+  const int lane = threadIdx.x & 31;
+  for (; s < b.sequences; s += 32) {
+    const int i = s + lane;
+    const unsigned int found = __ballot_sync(0xffffffffu, i < b.sequences && b.query_starts[i + 1] > b.query_starts[i]);
+    if (found) return s + __ffs(found) - 1;
+  }
+  return b.sequences;
+}
+
 // floor(a / b) for whole 0 <= a < 2^53 and 0 < b < 2^53: a quotient that is not whole is at least 1 / b away from the next whole
 // number, more than the division's rounding.
 __device__ __forceinline__ long long floor_ratio(long long a, long long b) { return static_cast<long long>(static_cast<double>(a) / static_cast<double>(b)); }

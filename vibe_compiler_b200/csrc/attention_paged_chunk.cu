@@ -222,7 +222,7 @@ struct ShareWalk {
   __device__ __forceinline__ bool next(const ChunkParams &p, Segment &out) {
     while (at.sequence < p.a.batch.sequences) {
       if (count == 0 || at.kv_head == p.a.cache.kv_heads) {
-        at = {at.sequence + 1, 0, 0, 0};
+        at = {next_with_tokens(p.a.batch, at.sequence + 1), 0, 0, 0};
         if (at.sequence < p.a.batch.sequences) look_up(p);
         continue;
       }
@@ -320,31 +320,50 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int4));   // inclusive sums of work
     const int sequences = p.a.batch.sequences;
     if (threadIdx.x == 0) item_count = most_work = 0;
-    for (int s = threadIdx.x; s < sequences; s += kThreads) {
-      const PagedSequence q = paged_sequence(p.a.batch, p.a.cache, s, p.a.refused, blockIdx.x == 0);
-      staged[s] = make_int4(q.begin, q.count, q.keys, 0);
-    }
     __syncthreads();
-    auto pairs_of = [&](const int4 &s) { return (s.y + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
-    auto pair_work = [&](const int4 &s, int pair) { return item_work(make_item(p, s.y, s.z, pair)); };
+    auto pairs_of = [&](int count) { return (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
+    auto pair_work = [&](int count, int keys, int pair) { return item_work(make_item(p, count, keys, pair)); };
+    // A lane per sequence; those of more than four items by the whole warp.
 #pragma unroll 1
-    for (int s = warp; s < sequences; s += kThreads / 32) {
-      const int4 q = staged[s];
-      const int pairs = pairs_of(q);
+    for (int start = warp * 32; start < sequences; start += kThreads) {
+      const int s = start + lane;
+      PagedSequence q = {0, 0, 0};
+      if (s < sequences) {
+        q = paged_sequence(p.a.batch, p.a.cache, s, p.a.refused, blockIdx.x == 0);
+        staged[s] = make_int4(q.begin, q.count, q.keys, 0);
+      }
+      const int pairs = pairs_of(q.count);
       long long work = 0;
       int most = 0;
+      if (pairs <= 4) {
 #pragma unroll 1
-      for (int pair = lane; pair < pairs; pair += 32) {
-        const int mine = pair_work(q, pair);
-        work += mine;
-        most = max(most, mine);
+        for (int pair = 0; pair < pairs; ++pair) {
+          const int mine = pair_work(q.count, q.keys, pair);
+          work += mine;
+          most = max(most, mine);
+        }
       }
+      unsigned int long_ones = __ballot_sync(0xffffffffu, pairs > 4);
+      while (long_ones) {
+        const int from = __ffs(long_ones) - 1;
+        long_ones &= long_ones - 1;
+        const int count = __shfl_sync(0xffffffffu, q.count, from), keys = __shfl_sync(0xffffffffu, q.keys, from), all = pairs_of(count);
+        long long sum = 0;
+#pragma unroll 1
+        for (int pair = lane; pair < all; pair += 32) {
+          const int mine = pair_work(count, keys, pair);
+          sum += mine;
+          most = max(most, mine);
+        }
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) work += __shfl_xor_sync(0xffffffffu, work, off);
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == from) work = sum;
+      }
+      if (s < sequences) prefix[s] = work * p.a.cache.kv_heads;
+      const int items = __reduce_add_sync(0xffffffffu, pairs) * p.a.cache.kv_heads;
       most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0) {
-        prefix[s] = work * p.a.cache.kv_heads;
-        atomicAdd(&item_count, pairs * p.a.cache.kv_heads);
+      if (lane == 0 && items > 0) {
+        atomicAdd(&item_count, items);
         atomicMax(&most_work, most);
       }
     }
@@ -387,14 +406,14 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         }
         const long long before = low > 0 ? prefix[low - 1] : 0, per_head = floor_ratio(prefix[low] - before, p.a.cache.kv_heads);
         const int4 q = staged[low];
-        const int pairs = pairs_of(q);
+        const int pairs = pairs_of(q.y);
         place.sequence = low;
         place.kv_head = static_cast<int>(floor_ratio(x - before, per_head));
         long long rest = x - before - place.kv_head * per_head;
 #pragma unroll 1
         for (int start = 0;; start += 32) {            // the pair of row tiles that work `rest` of the head lies in
           const int pair = start + lane;
-          long long sum = pair < pairs ? pair_work(q, pair) : 0;
+          long long sum = pair < pairs ? pair_work(q.y, q.z, pair) : 0;
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) {
             const long long other = __shfl_up_sync(0xffffffffu, sum, off);

@@ -188,10 +188,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     const int per_thread = (a.batch.sequences + kWarps * 32 - 1) / (kWarps * 32);
     const int first_mine = min(a.batch.sequences, static_cast<int>(threadIdx.x) * per_thread), end_mine = min(a.batch.sequences, first_mine + per_thread);
     long long mine = 0;
-    for (int i = first_mine; i < end_mine; ++i) {
-      const PagedSequence sequence = paged_sequence(a.batch, a.cache, i, a.refused, blockIdx.x == 0);
-      mine += rows_units<kRows>(p, sequence).weight;
-    }
+#pragma unroll 4
+    for (int i = first_mine; i < end_mine; ++i) mine += rows_units<kRows>(p, paged_sequence(a.batch, a.cache, i, a.refused, false)).weight;
+    if (blockIdx.x == 0)
+      for (int i = first_mine; i < end_mine; ++i) paged_sequence(a.batch, a.cache, i, a.refused, true);
     long long before = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
         const RowsUnits units = rows_units<kRows>(p, part.sequence);
         if (at >= prefix + units.weight) {               // on to the next sequence that has rows
           prefix += units.weight;
-          if (++s >= a.batch.sequences) return false;
+          s = next_with_tokens(a.batch, s + 1);
+          if (s >= a.batch.sequences) return false;
           continue;
         }
         const int all = units.steps + kUnitSteps, unit = static_cast<int>(floor_ratio(at - prefix, all));
