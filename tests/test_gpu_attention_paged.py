@@ -319,3 +319,44 @@ def test_a_serving_run(backend):
         whole = layer.forward(text[None])[0, :len(got)]
         # both round every stage to bf16 on the way; the suite's bound for the layer
         assert (got.double() - whole.double()).abs().max().item() <= 1e-2 * whole.double().abs().max().item()
+
+
+@pytest.mark.parametrize("sequences", [3, 40])
+def test_a_captured_serving_step(backend, sequences):
+    """One decoding step - room, cache writes, attention, the layer around them - captured once and replayed: each replay takes
+    the next token of every sequence, as the lengths, tables and page counts on the device go on."""
+    from vibe_compiler_b200.decoder_layer import LayerConfig, ShardedDecoderLayer, random_weights
+    cfg = LayerConfig(d_model=512, q_heads=8, kv_heads=2, head_dim=128, ffn=768)
+    layer = ShardedDecoderLayer(backend, cfg, random_weights(cfg))
+    size, steps, pages = 16, 20, 8 * sequences
+    g = torch.Generator().manual_seed(3)
+    prompts = [int(n) for n in torch.randint(1, 90, (sequences,), generator=g)]
+    texts = [torch.randn(n + steps, 512, generator=g).bfloat16().cuda() for n in prompts]
+
+    def begin():
+        tables, cache = PageTables(backend, sequences, 40, pages, size), PagedCache.zeros(pages, size, 2, 128)
+        assert int(tables.reserve(torch.tensor(prompts, dtype=torch.int32).cuda())) == 0
+        starts = torch.tensor([0] + prompts, dtype=torch.int32).cumsum(0).int().cuda()
+        layer.forward_paged(torch.cat([t[:n] for t, n in zip(texts, prompts)]), cache, PagedBatch(tables.table, tables.lengths, starts, max_query=max(prompts)))
+        return tables, cache
+
+    one_each = torch.arange(sequences + 1, dtype=torch.int32, device="cuda")
+
+    def step(tables, cache, x):
+        result = tables.reserve(tables.lengths + 1)
+        return layer.forward_paged(x, cache, PagedBatch(tables.table, tables.lengths, one_each, max_query=1)), result
+    tokens = [torch.stack([t[n + i] for t, n in zip(texts, prompts)]) for i in range(steps)]
+    state = begin()
+    want = [step(*state, x)[0].clone() for x in tokens]
+    warm = begin()
+    step(*warm, tokens[0])
+    state, x = begin(), tokens[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, result = step(*state, x)
+    for i in range(steps):
+        x.copy_(tokens[i])
+        graph.replay()
+        assert int(result) == 0 and torch.equal(y, want[i])
+    backend.poll()
+    assert state[0].lengths.tolist() == [n + steps for n in prompts]
