@@ -130,7 +130,11 @@ class ShardedDecoderLayer:
                 from .paged_cache import RotaryTable
                 self._rotary = RotaryTable(cfg.head_dim, theta=cfg.rope_theta)
             rotary = self._rotary
+        if x.dim() != 2 or not x.is_contiguous():
+            raise ValueError("x must be a contiguous [tokens, d_model] tensor")
         tokens = x.shape[0]
+        if tokens == 0:
+            return torch.empty_like(x)
         if tokens % 8:                         # the GEMMs take rows by eights; the rows behind belong to no sequence
             x = torch.nn.functional.pad(x, (0, 0, 0, 8 - tokens % 8))
         qkv = be.gemm_epilogue(be.rmsnorm(x, self.norm1, cfg.eps), self.wqkv)
