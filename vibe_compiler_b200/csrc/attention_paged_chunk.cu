@@ -965,19 +965,24 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   }
 }
 
-// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is the Q tile, blockIdx.z sixteen columns, a thread
-// a row. Two records' elements are on their way together with all their statistics.
+// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is sixteen columns, a thread a row of either Q tile, or,
+// of a halved item, a row and every second group of four records. Four records' elements are on their way together: a long cache
+// of few rows leaves many records (an item of 9000 keys about 40), of which two at a time, by a thread per row, took 20 us.
 template <bool kBf16, int kHd>
-__global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
   using L = Shape<kHd>;
+  constexpr int kAtOnce = 4;
+  __shared__ float joined[18][kTileM];               // of the second thread of a halved item's row
   pdl_wait();
   pdl_launch_dependents();
   const ChunkSplit split = p.splits[blockIdx.x];
-  const int t = blockIdx.y, row = threadIdx.x;       // a halved item's second tile has no rows of its own
+  if (split.records == 0) return;
+  const int row = threadIdx.x % kTileM, second = threadIdx.x / kTileM;
+  const int t = split.halved ? 0 : second, groups = split.halved ? 2 : 1, group = split.halved ? second : 0;
   const int at = token_of(p, row), token = (2 * split.pair + t) * p.tile_tokens + at;
-  if (split.records == 0 || at >= p.tile_tokens || token >= split.count) return;
+  const bool used = at < p.tile_tokens && token < split.count;
   // A halved item's halves are records of their own.
-  const int records = split.records * (split.halved ? 2 : 1);
+  const int records = used ? split.records * (split.halved ? 2 : 1) : 0;
   auto record = [&](int i) {
     const int share = split.halved ? i >> 1 : i;
     return p.records + ((static_cast<int64_t>(blockIdx.x + share) * 2 + (share == 0 ? 1 : 0)) * 2 + (split.halved ? i & 1 : t)) * L::kRecordFloats;
@@ -985,37 +990,63 @@ __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(cons
   float top = -INFINITY, l = 0.f, acc[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll 1
-  for (int i = 0; i < records; i += 2) {
-    const bool both = i + 1 < records;
-    const float *r[2] = {record(i), record(both ? i + 1 : i)};
-    float2 ml[2];
-    float4 v[2][4];
+  auto add = [&](const float (&m)[kAtOnce], const float (&sum)[kAtOnce], const float (&v)[kAtOnce][16]) {
+    float next = top;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      ml[u] = *reinterpret_cast<const float2 *>(r[u] + kTileM * kHd + 2 * row);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[u][e] = *reinterpret_cast<const float4 *>(r[u] + ((blockIdx.z * 4 + e) * kTileM + row) * 4);
-    }
-    if (!both) ml[1].y = 0.f;
-    const float next = fmaxf(top, fmaxf(ml[0].y > 0.f ? ml[0].x : -INFINITY, ml[1].y > 0.f ? ml[1].x : -INFINITY));
+    for (int u = 0; u < kAtOnce; ++u) next = fmaxf(next, sum[u] > 0.f ? m[u] : -INFINITY);
     const float m_exp = next == -INFINITY ? 0.f : next, alpha = ex2_approx(top - m_exp);
-    const float w0 = ml[0].y > 0.f ? ex2_approx(ml[0].x - m_exp) : 0.f, w1 = ml[1].y > 0.f ? ex2_approx(ml[1].x - m_exp) : 0.f;
     top = next;
-    l = l * alpha + (ml[0].y * w0 + ml[1].y * w1);
+    l *= alpha;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[4 * e] = acc[4 * e] * alpha + (v[0][e].x * w0 + v[1][e].x * w1);
-      acc[4 * e + 1] = acc[4 * e + 1] * alpha + (v[0][e].y * w0 + v[1][e].y * w1);
-      acc[4 * e + 2] = acc[4 * e + 2] * alpha + (v[0][e].z * w0 + v[1][e].z * w1);
-      acc[4 * e + 3] = acc[4 * e + 3] * alpha + (v[0][e].w * w0 + v[1][e].w * w1);
+    for (int e = 0; e < 16; ++e) acc[e] *= alpha;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float w = sum[u] == 0.f ? 0.f : ex2_approx(m[u] - m_exp);
+      l = fmaf(sum[u], w, l);
+      if (sum[u] == 0.f) continue;                   // a part that saw no key
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = fmaf(v[u][e], w, acc[e]);
+    }
+  };
+#pragma unroll 1
+  for (int i = group * kAtOnce; i < records; i += groups * kAtOnce) {
+    float m[kAtOnce], sum[kAtOnce], v[kAtOnce][16];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      m[u] = sum[u] = 0.f;
+      if (i + u < records) {
+        const float *r = record(i + u);
+        const float2 ml = *reinterpret_cast<const float2 *>(r + kTileM * kHd + 2 * row);
+        m[u] = ml.x;
+        sum[u] = ml.y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float4 *>(&v[u][4 * e]) = *reinterpret_cast<const float4 *>(r + ((blockIdx.y * 4 + e) * kTileM + row) * 4);
+      }
+    }
+    add(m, sum, v);
+  }
+  if (split.halved) {
+    if (group > 0) {
+      joined[0][row] = top;
+      joined[1][row] = l;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) joined[2 + e][row] = acc[e];
+    }
+    __syncthreads();
+    if (group > 0) return;
+    if (used) {
+      float m[kAtOnce] = {joined[0][row]}, sum[kAtOnce] = {joined[1][row]}, v[kAtOnce][16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[0][e] = joined[2 + e][row];
+      add(m, sum, v);
     }
   }
+  if (!used) return;
   const bool empty = l == 0.f;
   const float coefficient = empty ? 0.f : 1.0f / l;
   const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
   const int head = split.kv_head * p.group + row - at * p.group;
-  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.z * 16;
+  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.y * 16;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     uint32_t w[4];
@@ -1026,7 +1057,7 @@ __global__ void __launch_bounds__(kTileM) attention_paged_chunk_fold_kernel(cons
     }
     *reinterpret_cast<uint4 *>(dst + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (p.a.lse && blockIdx.z == 0)
+  if (p.a.lse && blockIdx.y == 0)
     p.a.lse[static_cast<int64_t>(split.begin + token) * p.a.q_heads + head] = empty ? -INFINITY : top * 0.69314718055994530942f + logf(l);
 }
 
@@ -1121,7 +1152,7 @@ wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int sm_co
   });
   if (st != WB200_OK) return st;
   WB200_CUDA_CHECK(launch_dependent(kernel, sm_count, kThreads, wide ? Shape<128>::kBytes : Shape<64>::kBytes, stream, tq, tk, tv, p));
-  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, 2, a.cache.head_dim / 16), kTileM, 0, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, a.cache.head_dim / 16), 2 * kTileM, 0, stream, p));
   return WB200_OK;
 }
 
