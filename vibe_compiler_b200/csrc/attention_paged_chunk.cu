@@ -74,6 +74,7 @@ struct ChunkParams {
   AttentionPagedArgs a;
   int group, tile_tokens;          // query heads per KV head; tokens per Q tile
   unsigned long long by_group;     // 2^32 / group + 1: row / group = row * by_group >> 32 for the rows of a tile
+  unsigned long long by_grid;      // floor((2^64 - 1) / grid) + 1: n / grid = n * by_grid >> 64 for n < 2^56
   int box_rows;                    // keys per TMA box
   int rows_inside;                 // the cache's tensor maps have rows inside heads
   float scale_log2;
@@ -216,7 +217,10 @@ struct ShareWalk {
 
   __device__ __forceinline__ void look_up(const ChunkParams &p) {
     const PagedSequence s = paged_sequence(p.a.batch, p.a.cache, at.sequence, p.a.refused, false);
-    begin = s.begin; count = s.count; keys = s.keys;
+    enter(p, s.begin, s.count, s.keys);
+  }
+  __device__ __forceinline__ void enter(const ChunkParams &p, int sequence_begin, int sequence_count, int sequence_keys) {
+    begin = sequence_begin; count = sequence_count; keys = sequence_keys;
     pairs = (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
   }
   __device__ __forceinline__ bool next(const ChunkParams &p, Segment &out) {
@@ -315,9 +319,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   // ---- this CTA's share of all work; the lengths are staged in the ring's memory
   __shared__ Place cuts[2];
   __shared__ int last_share, item_count, most_work;
+  __shared__ int4 first_staged;
   {
     int4 *staged = reinterpret_cast<int4 *>(smem + L::kRingOff);                                       // begin, count, keys
-    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int4));   // inclusive sums of work
+    long long *prefix = reinterpret_cast<long long *>(smem + L::kRingOff + kMaxSequences * sizeof(int4));   // inclusive sums of a head's work
     const int sequences = p.a.batch.sequences;
     if (threadIdx.x == 0) item_count = most_work = 0;
     __syncthreads();
@@ -359,7 +364,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         if (lane == from) work = sum;
       }
-      if (s < sequences) prefix[s] = work * p.a.cache.kv_heads;
+      if (s < sequences) prefix[s] = work;
       const int items = __reduce_add_sync(0xffffffffu, pairs) * p.a.cache.kv_heads;
       most = __reduce_max_sync(0xffffffffu, most);
       if (lane == 0 && items > 0) {
@@ -383,35 +388,50 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       }
     }
     __syncthreads();
-    // Warp 0 places the cut in front of the CTA's share, warp 1 the one behind it.
+    // Warp 0 places the cut in front of the CTA's share, warp 1 the one behind it. Code that runs once costs what its fetch costs:
+    // with whole-number divisions by way of f64 and a search by halves this took 1.7 to 2.6 us of a launch.
     if (warp < 2) {
-      const long long total = sequences > 0 ? prefix[sequences - 1] : 0;
-      const long long shares = max(1ll, min(floor_ratio(total, kLeastWork), static_cast<long long>(gridDim.x)));
-      const long long share = floor_ratio(total, shares);
+      const int heads = p.a.cache.kv_heads, grid = static_cast<int>(gridDim.x);
+      const long long total = sequences > 0 ? prefix[sequences - 1] * heads : 0;
+      const int shares = total >= static_cast<long long>(kLeastWork) * grid ? grid : max(1, static_cast<int>(total) / kLeastWork);
+      // Where share i begins: total * i / shares. Totals of fewer shares than CTAs are small.
+      auto cut_at = [&](int i) {
+        const unsigned long long n = static_cast<unsigned long long>(total) * static_cast<unsigned>(i);
+        return static_cast<long long>(shares == grid ? __umul64hi(n, p.by_grid) : static_cast<unsigned>(n) / static_cast<unsigned>(shares));
+      };
       // Items are left whole where the CTA with the most of them ends before one with an equal share and the cost of cuts: items
       // much alike by counting, others by what a share can grow by.
-      const long long counted = static_cast<long long>((item_count + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x)) * most_work;
+      const long long counted = static_cast<long long>(__umul64hi(item_count + grid - 1, p.by_grid)) * most_work;
       const bool alike = 10ll * most_work * item_count <= 13ll * total;
-      const bool whole = (alike ? counted : share + most_work) <= share + kCutWork;
-      const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(share >> 6, 1ll << 20)));
-      const long long index = blockIdx.x + warp, x = floor_ratio(total * index, shares);
+      const bool whole = alike ? (counted - kCutWork) * shares <= total : most_work <= kCutWork;
+      const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(cut_at(1) >> 6, 1ll << 20)));
+      const int index = static_cast<int>(blockIdx.x) + warp;
+      const long long x = cut_at(index);
       Place place = {sequences, 0, 0, 0};
       int last = 0;
       if (index <= shares && x < total) {
-        int low = 0, high = sequences - 1;             // first sequence whose sum is beyond x
-        while (low < high) {
-          const int mid = (low + high) >> 1;
-          if (prefix[mid] > x) high = mid;
-          else low = mid + 1;
+        int low = 0, span = sequences;                 // the first sequence whose sum is beyond x lies in [low, low + span)
+#pragma unroll 1
+        while (span > 1) {
+          const int step = (span + 31) >> 5;
+          const int found = __ffs(__ballot_sync(0xffffffffu, prefix[low + min((lane + 1) * step, span) - 1] * heads > x)) - 1;
+          low += found * step;
+          span = min(step, span - found * step);
         }
-        const long long before = low > 0 ? prefix[low - 1] : 0, per_head = floor_ratio(prefix[low] - before, p.a.cache.kv_heads);
+        const long long before = low > 0 ? prefix[low - 1] : 0, per_head = prefix[low] - before;
         const int4 q = staged[low];
         const int pairs = pairs_of(q.y);
         place.sequence = low;
-        place.kv_head = static_cast<int>(floor_ratio(x - before, per_head));
-        long long rest = x - before - place.kv_head * per_head;
+        long long rest = x - before * heads;
 #pragma unroll 1
-        for (int start = 0;; start += 32) {            // the pair of row tiles that work `rest` of the head lies in
+        for (int start = 1;; start += 32) {            // how many whole heads lie in front
+          const unsigned int whole_heads = __ballot_sync(0xffffffffu, start + lane < heads && (start + lane) * per_head <= rest);
+          place.kv_head += __popc(whole_heads);
+          if (whole_heads != 0xffffffffu) break;
+        }
+        rest -= place.kv_head * per_head;
+#pragma unroll 1
+        for (int start = 0; pairs > 1; start += 32) {  // the pair of row tiles that work `rest` of the head lies in
           const int pair = start + lane;
           long long sum = pair < pairs ? pair_work(q.y, q.z, pair) : 0;
 #pragma unroll
@@ -432,8 +452,19 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const Item item = make_item(p, q.y, q.z, place.pair);
         const int all = item_work(item);
         place.tile = whole ? (2 * rest < all ? 0 : item.steps) : cut_tile(item, static_cast<int>(rest), least_cut);
-        // The item goes on in the shares behind this cut, up to the last whose cut does not move to its end.
-        last = static_cast<int>(floor_ratio((x - rest + all - least_cut + 1) * shares - 1, total));
+        if (warp == 0) {
+          if (lane == 0) first_staged = q;
+        } else if (place.tile > 0 && place.tile < item.steps) {
+          // The item goes on in the shares behind this cut, up to the last whose cut does not move to its end.
+          const long long end = x - rest + all - least_cut;
+          last = index;
+#pragma unroll 1
+          for (int start = index + 1;; start += 32) {
+            const unsigned int inside = __ballot_sync(0xffffffffu, start + lane < shares && cut_at(start + lane) <= end);
+            last += __popc(inside);
+            if (inside != 0xffffffffu) break;
+          }
+        }
       }
       if (lane == 0) {
         cuts[warp] = place;
@@ -717,7 +748,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     walk.at = cuts[0];
     walk.end = cuts[1];
     walk.begin = walk.count = walk.keys = walk.pairs = 0;
-    if (walk.at.sequence < p.a.batch.sequences) walk.look_up(p);
+    if (walk.at.sequence < p.a.batch.sequences) walk.enter(p, first_staged.x, first_staged.y, first_staged.z);
     ChunkSplit split = {};
     bool more = true;
     while (more) {
@@ -1116,6 +1147,7 @@ wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int sm_co
   p.group = a.q_heads / a.cache.kv_heads;
   p.tile_tokens = kTileM / p.group;
   p.by_group = (1ull << 32) / p.group + 1;
+  p.by_grid = ~0ull / static_cast<unsigned>(sm_count) + 1;
   p.box_rows = box_rows_of(a.cache.page_size);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.records = static_cast<float *>(a.workspace);
