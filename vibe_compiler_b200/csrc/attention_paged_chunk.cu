@@ -899,6 +899,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         scale0 *= coefficient;
         scale1 *= coefficient;
         const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
+        const int at = token_of(p, row_in_tile), token = first_token + at, head = seg.kv_head * p.group + row_in_tile - at * p.group;
+        const bool used = at < p.tile_tokens && token < seg.count;
+        // Where the lane's row of the output begins; -1: not a row.
+        const long long row_at = used ? static_cast<int64_t>(seg.begin + token) * p.a.out_token + head * p.a.out_head : -1;
         // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes. The
         // loops stay rolled: code that runs once per item comes from L2, eight instructions a line.
 #pragma unroll 1
@@ -935,17 +939,20 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             }
           }
           __syncwarp();
-#pragma unroll 2
-          for (int i = 0; i < 8; ++i) {
-            const int r_out = i * 4 + (lane >> 3), chunk = lane & 7;
-            const int packed = quarter * 32 + r_out, at = token_of(p, packed), token_out = first_token + at;
-            if (at < p.tile_tokens && token_out < seg.count) {
-              uint32_t w[4];
-              ld_shared_v4(out_stage + r_out * 128 + ((chunk ^ (r_out & 7)) << 4), w);
-              uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(seg.begin + token_out) * p.a.out_token +
-                              (seg.kv_head * p.group + packed - at * p.group) * p.a.out_head + half * 64 + chunk * 8;
-              *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll 1
+          for (int i = 0; i < 32; i += 16) {         // four loads on their way together
+            uint32_t w[4][4];
+            long long to[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int r_out = i + 4 * u + (lane >> 3);
+              to[u] = __shfl_sync(0xffffffffu, row_at, r_out);
+              ld_shared_v4(out_stage + r_out * 128 + (((lane ^ r_out) & 7) << 4), w[u]);
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (to[u] >= 0)
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.a.out) + to[u] + half * 64 + (lane & 7) * 8) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
           }
         }
         if (joined) {
@@ -953,9 +960,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
           __syncwarp();
           if (lane == 0) mbar_arrive(half_read(quarter));
         }
-        const int at = token_of(p, row_in_tile), token = first_token + at;
-        if (p.a.lse && at < p.tile_tokens && token < seg.count)
-          p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + seg.kv_head * p.group + row_in_tile - at * p.group] =
+        if (p.a.lse && used)
+          p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + head] =
               empty ? -INFINITY : m_ref * 0.69314718055994530942f + logf(l_run);
       } else if (ok && first_token < seg.count) {
         // A part of an item: the state as it is, four columns of 32 rows to a store.
