@@ -266,15 +266,14 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   auto p_part = [&](int t, int part) { return bar_base + 8u * (kFixed + 3 + kPParts * t + part); };
   auto o_done = [&](int t) { return bar_base + 8u * (kFixed + 3 + 2 * kPParts + t); };
   const uint32_t q_empty = bar_base + 8u * (kFixed + 5 + 2 * kPParts);
-  auto half_ready = [&](int quarter) { return bar_base + 8u * (kFixed + 6 + 2 * kPParts + quarter); };   // tile 1's half may be read
-  auto half_read = [&](int quarter) { return bar_base + 8u * (kFixed + 10 + 2 * kPParts + quarter); };   // and has been
-  auto segment_full = [&](int i) { return bar_base + 8u * (kFixed + 14 + 2 * kPParts + i); };
-  auto segment_empty = [&](int i) { return bar_base + 8u * (kFixed + 14 + 2 * kPParts + kSegments + i); };
+  auto paired = [&](int quarter) { return bar_base + 8u * (kFixed + 6 + 2 * kPParts + quarter); };   // the two tiles' warps of the same TMEM lanes
+  auto segment_full = [&](int i) { return bar_base + 8u * (kFixed + 10 + 2 * kPParts + i); };
+  auto segment_empty = [&](int i) { return bar_base + 8u * (kFixed + 10 + 2 * kPParts + kSegments + i); };
   uint8_t *bar_ptr = smem + L::kBarOff;
-  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 14 + 2 * kPParts + 2 * kSegments));
-  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 15 + 2 * kPParts + 2 * kSegments));
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bar_ptr + 8 * (kFixed + 10 + 2 * kPParts + 2 * kSegments));
+  volatile int *abort_word = reinterpret_cast<volatile int *>(bar_ptr + 8 * (kFixed + 11 + 2 * kPParts + 2 * kSegments));
   Segment *const segments = reinterpret_cast<Segment *>(smem + L::kSegmentOff);
-  static_assert(8 * (kFixed + 16 + 2 * kPParts + 2 * kSegments) <= 512, "the barriers must fit their area");
+  static_assert(8 * (kFixed + 12 + 2 * kPParts + 2 * kSegments) <= 512, "the barriers must fit their area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -291,10 +290,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       for (int part = 0; part < kPParts; ++part) mbar_init(p_part(t, part), kTileM / 32);
       mbar_init(o_done(t), 1);
     }
-    for (int quarter = 0; quarter < 4; ++quarter) {
-      mbar_init(half_ready(quarter), 1);
-      mbar_init(half_read(quarter), 1);
-    }
+    for (int quarter = 0; quarter < 4; ++quarter) mbar_init(paired(quarter), 2);
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(segment_full(i), 1);
       mbar_init(segment_empty(i), kReaders);
@@ -775,7 +771,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_sel + kColS0 + t * 128;
     const uint32_t o_addr = tmem_base + lane_sel + kColO0 + t * 128;
-    uint32_t tiles_done = 0, items_done = 0, joins = 0;
+    uint32_t tiles_done = 0, items_done = 0, meets = 0;
     bool ok = true;
     const uint32_t out_stage = smem_base + L::kOutOff + (warp - 4) * kOutStageBytes;
     while (ok) {
@@ -872,26 +868,32 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       const Segment seg = segments[segment_at];
       const int first_token = (2 * seg.pair + (seg.halved ? 0 : t)) * p.tile_tokens;       // of the tile, within the sequence
       const bool joined = seg.halved && seg.whole;
-      if (ok && joined && t == 1) {
-        // The second half of a halved item: the first tile's warp of the same TMEM lanes reads the accumulator itself.
-        *reinterpret_cast<float2 *>(smem + L::kOutOff + (warp - 4) * kOutStageBytes + lane * 8) = make_float2(m_ref, l_run);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(half_ready(quarter));
-        ok = mbar_wait(half_read(quarter), joins++ & 1u, abort_word, 116);
-      } else if (ok && seg.whole) {
-        float scale0 = 1.f, scale1 = 0.f;              // of the two halves
-        bool second_half = false;
+      if (ok && seg.whole) {
+        // Of a halved item the two tiles' warps of the same TMEM lanes join their states and write half of the columns each.
+        const int columns = joined ? kHd / 2 : kHd, c0 = joined ? t * columns : 0;
+        const uint32_t other_addr = o_addr + (t ? -128 : 128);
+        auto arrive_pair = [&]() {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(paired(quarter));
+        };
+        auto wait_pair = [&]() { return mbar_wait(paired(quarter), meets++ & 1u, abort_word, 116); };
+        float scale0 = 1.f, scale1 = 0.f;              // of this warp's state and the other's
+        bool other_half = false;
         if (joined) {
-          ok = mbar_wait(half_ready(quarter), joins++ & 1u, abort_word, 117);
-          if (!ok) break;
-          const float2 other = *reinterpret_cast<const float2 *>(smem + L::kOutOff + warp * kOutStageBytes + lane * 8);   // of warp + 4
-          second_half = seg.of(1) > 0;
+          float2 *const states = reinterpret_cast<float2 *>(smem + L::kOutOff);
+          states[(warp - 4) * (kOutStageBytes / 8) + lane] = make_float2(m_ref, l_run);
+          tc_fence_before();
+          arrive_pair();
+          if (!(ok = wait_pair())) break;
+          const float2 other = states[((warp - 4) ^ 4) * (kOutStageBytes / 8) + lane];
+          arrive_pair();
+          other_half = seg.of(1 - t) > 0;
           const float top = fmaxf(l_run > 0.f ? m_ref : -INFINITY, other.y > 0.f ? other.x : -INFINITY);
           scale0 = l_run > 0.f ? ex2_approx(m_ref - top) : 0.f;
           scale1 = other.y > 0.f ? ex2_approx(other.x - top) : 0.f;
           l_run = l_run * scale0 + other.y * scale1;
           m_ref = top;
+          if (!(ok = wait_pair())) break;              // the stages' states have been read
         }
         tc_fence_after();
         const bool empty = l_run == 0.f;
@@ -903,16 +905,17 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const bool used = at < p.tile_tokens && token < seg.count;
         // Where the lane's row of the output begins; -1: not a row.
         const long long row_at = used ? static_cast<int64_t>(seg.begin + token) * p.a.out_token + head * p.a.out_head : -1;
-        // Through shared memory, 32 rows x 64 columns at a time, so that a store instruction covers four rows' 128 bytes. The
-        // loops stay rolled: code that runs once per item comes from L2, eight instructions a line.
+        // Through shared memory, 32 rows x 64 columns at a time (32 columns of a half at head_dim 64), so that a store instruction
+        // covers rows' 128 (64) bytes. The loops stay rolled: code that runs once per item comes from L2, eight instructions a line.
+        const int by_row = columns < 64 ? 2 : 3;       // 2^n lanes store a row
 #pragma unroll 1
-        for (int half = 0; half < L::kHalves; ++half) {
+        for (int pass = c0; pass < c0 + columns; pass += 64) {
           __syncwarp();                              // the stage's previous contents have been read
 #pragma unroll 1
-          for (int c = half * 64; c < half * 64 + 64; c += 16) {
+          for (int c = 0; c < min(columns, 64); c += 16) {
             uint32_t r[16];
             if (my_tiles > 0) {
-              tmem_ld_32x16(o_addr + c, r);
+              tmem_ld_32x16(o_addr + pass + c, r);
               tmem_wait_ld();
             } else {
 #pragma unroll
@@ -920,9 +923,9 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale0);
-            if (second_half) {
+            if (other_half) {
               uint32_t o[16];
-              tmem_ld_32x16(o_addr + 128 + c, o);
+              tmem_ld_32x16(other_addr + pass + c, o);
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), scale1, __uint_as_float(r[i])));
@@ -935,34 +938,36 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                 w[k] = pack2<kBf16>(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]));
                 if (empty) w[k] = filled;
               }
-              st_shared_v4(out_stage + lane * 128 + (((((c & 63) + i) >> 3) ^ (lane & 7)) << 4), w);
+              st_shared_v4(out_stage + lane * 128 + ((((c + i) >> 3) ^ (lane & 7)) << 4), w);
             }
           }
-          __syncwarp();
+          if (joined) {                              // one pass: both accumulators have been read
+            tc_fence_before();
+            arrive_pair();
+          } else {
+            __syncwarp();
+          }
+          const int chunk = lane & ((1 << by_row) - 1);
 #pragma unroll 1
-          for (int i = 0; i < 32; i += 16) {         // four loads on their way together
+          for (int i = lane >> by_row; i < 32; i += 128 >> by_row) {         // four loads on their way together
             uint32_t w[4][4];
             long long to[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-              const int r_out = i + 4 * u + (lane >> 3);
+              const int r_out = i + u * (32 >> by_row);
               to[u] = __shfl_sync(0xffffffffu, row_at, r_out);
-              ld_shared_v4(out_stage + r_out * 128 + (((lane ^ r_out) & 7) << 4), w[u]);
+              ld_shared_v4(out_stage + r_out * 128 + (((chunk ^ r_out) & 7) << 4), w[u]);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
               if (to[u] >= 0)
-                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.a.out) + to[u] + half * 64 + (lane & 7) * 8) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.a.out) + to[u] + pass + chunk * 8) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
           }
         }
-        if (joined) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(half_read(quarter));
-        }
-        if (p.a.lse && used)
+        if (p.a.lse && used && !(joined && t))
           p.a.lse[static_cast<int64_t>(seg.begin + token) * p.a.q_heads + head] =
               empty ? -INFINITY : m_ref * 0.69314718055994530942f + logf(l_run);
+        if (joined) ok = wait_pair();
       } else if (ok && first_token < seg.count) {
         // A part of an item: the state as it is, four columns of 32 rows to a store.
         tc_fence_after();
