@@ -49,6 +49,7 @@ struct RowsParams {
   AttentionPagedArgs a;
   int group;                        // query heads per KV head
   float scale_log2;
+  unsigned long long by_grid;       // floor((2^64 - 1) / grid) + 1: n / grid = n * by_grid >> 64 for n < 2^55
   float *records;                   // [grid][2][rows per tile][kRecord]: a share's end of a unit (0), its start of one (1)
   RowsSplit *splits;                // [grid]
 };
@@ -181,8 +182,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
 
   // This CTA's share of all steps: at .. share_end, from sequence s on, in front of which `prefix` steps lie.
   int s = -1, next_tile = 0;
-  long long total = 0, shares = 1, at = 0, share_end = 0, prefix = 0;
-  const long long index = blockIdx.x;
+  long long total = 0, at = 0, share_end = 0, prefix = 0;
+  const int index = static_cast<int>(blockIdx.x), grid = static_cast<int>(gridDim.x);
+  int shares = 1;
+  // Where share i begins: total * i / shares. Totals of fewer shares than CTAs are small.
+  auto cut_at = [&](int i) {
+    const unsigned long long n = static_cast<unsigned long long>(total) * static_cast<unsigned>(i);
+    return static_cast<long long>(shares == grid ? __umul64hi(n, p.by_grid) : static_cast<unsigned>(n) / static_cast<unsigned>(shares));
+  };
   if constexpr (!kClustered) {
     // A thread sums up a run of consecutive sequences.
     const int per_thread = (a.batch.sequences + kWarps * 32 - 1) / (kWarps * 32);
@@ -207,10 +214,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
       if (w < warp) before += warp_totals[w];
       total += warp_totals[w];
     }
-    shares = floor_ratio(total, kLeastSteps);
-    shares = shares < 1 ? 1 : (shares > gridDim.x ? gridDim.x : shares);
-    at = index < shares ? floor_ratio(total * index, shares) : total;
-    share_end = index < shares ? floor_ratio(total * (index + 1), shares) : total;
+    shares = total >= static_cast<long long>(kLeastSteps) * grid ? grid : max(1, static_cast<int>(total) / kLeastSteps);
+    at = index < shares ? cut_at(index) : total;
+    share_end = index < shares ? cut_at(index + 1) : total;
     if (at < share_end && before <= at && at < before + mine) {
       for (int i = first_mine; i < end_mine; ++i) {
         const PagedSequence sequence = paged_sequence(a.batch, a.cache, i, a.refused, false);
@@ -277,8 +283,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
           if (s >= a.batch.sequences) return false;
           continue;
         }
-        const int all = units.steps + kUnitSteps, unit = static_cast<int>(floor_ratio(at - prefix, all));
-        const int begin = static_cast<int>(at - prefix - static_cast<long long>(unit) * all);
+        const long long into = at - prefix;
+        const int all = units.steps + kUnitSteps;
+        const int unit = into >> 32 ? static_cast<int>(floor_ratio(into, all)) : static_cast<int>(static_cast<unsigned>(into) / static_cast<unsigned>(all));
+        const int begin = static_cast<int>(into - static_cast<long long>(unit) * all);
         const int end = static_cast<int>(min(static_cast<long long>(all), begin + (share_end - at)));
         at += end - begin;
         part.left = all - end;
@@ -544,8 +552,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
     }
     if (!kClustered && done.step0 == 0 && !whole) {
       // The unit ends the share and goes on in the CTAs behind this one, up to the last share that begins in front of its end.
-      const long long last = floor_ratio((share_end + done.left) * shares - 1, total);
-      split = {1 + static_cast<int>(last - index), done.sequence.begin, done.sequence.count, done.row_tile, done.kv_head, {}};
+      int behind = 0;
+#pragma unroll 1
+      for (int start = index + 1;; start += 32) {
+        const unsigned int inside = __ballot_sync(0xffffffffu, start + lane < shares && cut_at(start + lane) < share_end + done.left);
+        behind += __popc(inside);
+        if (inside != 0xffffffffu) break;
+      }
+      split = {1 + behind, done.sequence.begin, done.sequence.count, done.row_tile, done.kv_head, {}};
     }
   }
   cp_async_wait<0>();
@@ -651,6 +665,7 @@ wb200_status launch_attention_paged_rows(const AttentionPagedArgs &a, int sm_cou
   p.a = a;
   p.group = a.q_heads / a.cache.kv_heads;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.by_grid = ~0ull / static_cast<unsigned>(sm_count * kCtasPerSm) + 1;
   p.records = static_cast<float *>(a.workspace);
   p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
   // Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
