@@ -38,8 +38,12 @@ __device__ __forceinline__ int next_with_tokens(const PagedBatchArgs &b, int s) 
   return b.sequences;
 }
 
-// floor(a / b) for whole 0 <= a < 2^53 and 0 < b < 2^53: a quotient that is not whole is at least 1 / b away from the next whole
-// number, more than the division's rounding.
-__device__ __forceinline__ long long floor_ratio(long long a, long long b) { return static_cast<long long>(static_cast<double>(a) / static_cast<double>(b)); }
+// The L2 policy of a sequence's keys: those that are read once give way first to what is read again.
+__device__ __forceinline__ uint64_t l2_policy(bool read_again) {
+  uint64_t normal, first;
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  return read_again ? normal : first;
+}
 
 }  // namespace wb200

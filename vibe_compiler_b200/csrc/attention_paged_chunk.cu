@@ -150,11 +150,11 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&v)[4]) {
@@ -526,6 +526,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         }
         __syncwarp();
       }
+      // Keys of one pair of row tiles: 40 sequences of 5 tokens 131 -> 125 us, beside chunks 271 -> 268.
+      const uint64_t policy = l2_policy(seg.count > 2 * p.tile_tokens);
       const int *pages = p.a.batch.page_table + seg.sequence * p.a.batch.table_stride;
       // Where the keys of lane i's box of a tile lie: entry of the page table, row in the page. The page is looked up a tile ahead.
       int at_slot, at_row, page;
@@ -573,7 +575,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
               if (i + u >= count) break;
               const int y = p.rows_inside ? box_at[u] : seg.kv_head, z = p.rows_inside ? seg.kv_head : box_at[u];
 #pragma unroll
-              for (int c = 0; c < L::kHalves; ++c) tma_load_4d(dst + u * box_bytes + c * kBlockBytes, map, bar, c * 64, y, z, box_page[u]);
+              for (int c = 0; c < L::kHalves; ++c) tma_load_4d(dst + u * box_bytes + c * kBlockBytes, map, bar, c * 64, y, z, box_page[u], policy);
             }
           }
           __syncwarp();
