@@ -360,3 +360,23 @@ def test_a_captured_serving_step(backend, sequences):
         assert int(result) == 0 and torch.equal(y, want[i])
     backend.poll()
     assert state[0].lengths.tolist() == [n + steps for n in prompts]
+
+
+# (sequences, most new tokens, most keys in front, KV heads, group, head_dim): more heads than a warp's lanes, more sequences than a
+# look at every 32nd finds in one go, no work in front of and between the sequences, fewer shares than SMs, one item for all SMs.
+@pytest.mark.parametrize("sequences,news,front,hk,group,head_dim", [
+    (5, 30, 200, 33, 1, 64), (3, 20, 90, 70, 1, 64), (1500, 9, 20, 2, 4, 64), (1100, 3, 40, 1, 8, 128), (2, 9, 30, 1, 4, 64),
+    (1, 40, 12000, 1, 8, 128), (1, 2, 20000, 1, 2, 64), (40, 70, 600, 3, 5, 128)])
+def test_work_is_shared_out_whole(backend, sequences, news, front, hk, group, head_dim):
+    rng = torch.Generator().manual_seed(sequences)
+    new = torch.randint(0, news + 1, (sequences,), generator=rng).tolist()
+    new[0], new[-1] = (0 if sequences > 2 else news), news
+    lengths = [n + int(torch.randint(0, front + 1, (1,), generator=rng)) if n else 0 for n in new]
+    lengths[-1] = front + news
+    size = 16
+    pages = sum(-(-n // size) for n in lengths) + 3
+    cache = make_cache(pages, size, hk, head_dim, torch.bfloat16, "rows", 1)
+    batch, tokens = make_batch(lengths, new, size, pages, 2, spare_rows=3)
+    q = torch.randn(tokens, hk * group, head_dim, generator=rng).bfloat16().cuda()
+    for max_query in (0, 1, news):
+        agree(backend, q, cache, PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query), head_dim ** -0.5)

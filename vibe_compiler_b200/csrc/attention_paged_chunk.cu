@@ -1009,14 +1009,16 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   }
 }
 
-// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is sixteen columns, a thread a row of either Q tile, or,
+// Folds the records of the item that starts in share blockIdx.x: blockIdx.y is eight columns, a thread a row of either Q tile, or,
 // of a halved item, a row and every second group of four records. Four records' elements are on their way together: a long cache
-// of few rows leaves many records (an item of 9000 keys about 40), of which two at a time, by a thread per row, took 20 us.
+// of few rows leaves many records (an item of 9000 keys about 40), of which two at a time, by a thread per row, took 20 us. Eight
+// columns to a thread leave room for three blocks on an SM, sixteen for two: 100 tokens over 20000 keys of one KV head 30.6 / 33.0 us.
+constexpr int kColumns = 8;
 template <bool kBf16, int kHd>
-__global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(2 * kTileM, 3) attention_paged_chunk_fold_kernel(const __grid_constant__ ChunkParams p) {
   using L = Shape<kHd>;
   constexpr int kAtOnce = 4;
-  __shared__ float joined[18][kTileM];               // of the second thread of a halved item's row
+  __shared__ float joined[2 + kColumns][kTileM];               // of the second thread of a halved item's row
   pdl_wait();
   pdl_launch_dependents();
   const ChunkSplit split = p.splits[blockIdx.x];
@@ -1031,10 +1033,10 @@ __global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(
     const int share = split.halved ? i >> 1 : i;
     return p.records + ((static_cast<int64_t>(blockIdx.x + share) * 2 + (share == 0 ? 1 : 0)) * 2 + (split.halved ? i & 1 : t)) * L::kRecordFloats;
   };
-  float top = -INFINITY, l = 0.f, acc[16];
+  float top = -INFINITY, l = 0.f, acc[kColumns];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  auto add = [&](const float (&m)[kAtOnce], const float (&sum)[kAtOnce], const float (&v)[kAtOnce][16]) {
+  for (int e = 0; e < kColumns; ++e) acc[e] = 0.f;
+  auto add = [&](const float (&m)[kAtOnce], const float (&sum)[kAtOnce], const float (&v)[kAtOnce][kColumns]) {
     float next = top;
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) next = fmaxf(next, sum[u] > 0.f ? m[u] : -INFINITY);
@@ -1042,19 +1044,19 @@ __global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(
     top = next;
     l *= alpha;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] *= alpha;
+    for (int e = 0; e < kColumns; ++e) acc[e] *= alpha;
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       const float w = sum[u] == 0.f ? 0.f : ex2_approx(m[u] - m_exp);
       l = fmaf(sum[u], w, l);
       if (sum[u] == 0.f) continue;                   // a part that saw no key
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] = fmaf(v[u][e], w, acc[e]);
+      for (int e = 0; e < kColumns; ++e) acc[e] = fmaf(v[u][e], w, acc[e]);
     }
   };
 #pragma unroll 1
   for (int i = group * kAtOnce; i < records; i += groups * kAtOnce) {
-    float m[kAtOnce], sum[kAtOnce], v[kAtOnce][16];
+    float m[kAtOnce], sum[kAtOnce], v[kAtOnce][kColumns];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       m[u] = sum[u] = 0.f;
@@ -1064,7 +1066,7 @@ __global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(
         m[u] = ml.x;
         sum[u] = ml.y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<float4 *>(&v[u][4 * e]) = *reinterpret_cast<const float4 *>(r + ((blockIdx.y * 4 + e) * kTileM + row) * 4);
+        for (int e = 0; e < kColumns / 4; ++e) *reinterpret_cast<float4 *>(&v[u][4 * e]) = *reinterpret_cast<const float4 *>(r + ((blockIdx.y * (kColumns / 4) + e) * kTileM + row) * 4);
       }
     }
     add(m, sum, v);
@@ -1074,14 +1076,14 @@ __global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(
       joined[0][row] = top;
       joined[1][row] = l;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) joined[2 + e][row] = acc[e];
+      for (int e = 0; e < kColumns; ++e) joined[2 + e][row] = acc[e];
     }
     __syncthreads();
     if (group > 0) return;
     if (used) {
-      float m[kAtOnce] = {joined[0][row]}, sum[kAtOnce] = {joined[1][row]}, v[kAtOnce][16];
+      float m[kAtOnce] = {joined[0][row]}, sum[kAtOnce] = {joined[1][row]}, v[kAtOnce][kColumns];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[0][e] = joined[2 + e][row];
+      for (int e = 0; e < kColumns; ++e) v[0][e] = joined[2 + e][row];
       add(m, sum, v);
     }
   }
@@ -1090,9 +1092,9 @@ __global__ void __launch_bounds__(2 * kTileM) attention_paged_chunk_fold_kernel(
   const float coefficient = empty ? 0.f : 1.0f / l;
   const uint32_t filled = p.a.zero_fully_masked ? 0u : (kBf16 ? 0x7fc07fc0u : 0x7e007e00u);
   const int head = split.kv_head * p.group + row - at * p.group;
-  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.y * 16;
+  uint16_t *dst = static_cast<uint16_t *>(p.a.out) + static_cast<int64_t>(split.begin + token) * p.a.out_token + head * p.a.out_head + blockIdx.y * kColumns;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
+  for (int e = 0; e < kColumns / 8; ++e) {
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -1197,7 +1199,7 @@ wb200_status launch_attention_paged_chunk(const AttentionPagedArgs &a, int sm_co
   });
   if (st != WB200_OK) return st;
   WB200_CUDA_CHECK(launch_dependent(kernel, sm_count, kThreads, wide ? Shape<128>::kBytes : Shape<64>::kBytes, stream, tq, tk, tv, p));
-  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, a.cache.head_dim / 16), 2 * kTileM, 0, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(fold, dim3(sm_count, a.cache.head_dim / kColumns), 2 * kTileM, 0, stream, p));
   return WB200_OK;
 }
 
