@@ -12,8 +12,8 @@
 //            stale row may hold. The V loader zeroes those rows in shared memory before the products see them.
 //   halves   An item is two row tiles of one KV head of one sequence, so that one tile's products run under the other's softmax.
 //            Where the sequence has rows for one tile only, its odd key tiles take the second tile's place, and the two halves
-//            of the state are joined at the end: a step of one row tile takes 1820 clocks instead of nearly the 3250 of
-//            two.
+//            of the state are joined at the end, by both tiles' warps, half of the columns each: a step of one row tile takes
+//            1820 clocks instead of nearly the 3250 of two.
 //   shares   All items lie one behind the other on one axis of work, cut into equal shares for the CTAs, so ragged batches and
 //            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A cut near the end of
 //            an item moves to it; others leave f32 records of the item's parts, folded by a second kernel.
@@ -21,7 +21,7 @@
 // Bound: the chain S -> softmax -> P V of a step (see attention_fa.cu), 4 * head_dim flop per visible (row, key) pair. A step of two
 // row tiles takes 3250 clocks, of which its products are 2048. 4096 tokens behind 32768 cached ones, 32/8 heads: 1.9 ms back to
 // back in a graph (1.2 PFLOP/s), 2.2 ms among other work (the clock gives way to the power cap); 8 chunks of 256 tokens at 4096 keys
-// 133 us, the tensor pipe 54 % busy, of which about 10 us are the start, the cuts' records and their fold.
+// 132 us, the tensor pipe 54 % busy, of which about 9 us are the start, the cuts' records and their fold.
 #include <type_traits>
 
 #include "attention_paged.cuh"
