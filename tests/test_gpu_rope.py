@@ -184,3 +184,41 @@ def test_append_leaves_out_rows_without_a_place(backend, fault):
     assert torch.equal(now[:17], good[:17]) and not torch.equal(now[17:], good[17:])
     changed = (cache.v != before[1]).flatten(1).any(1).nonzero().flatten().tolist()
     assert set(changed) <= set(batch.page_table[0, :2].tolist()) | ({int(batch.page_table[1, 0])} if fault.startswith("more") else set())
+
+
+@pytest.mark.parametrize("fault", ["a range ends behind the rows", "a range begins in front of the rows", "ranges wholly behind the rows", "keys beyond the table"])
+def test_append_leaves_out_whole_sequences_that_do_not_fit(backend, fault):
+    """A token range or a length outside the buffers says nothing about any of its tokens: none of them is written, as attention
+    reads none of them."""
+    cache = make_cache(16, 16, 2, 64, torch.float16, "rows", 1)
+    batch, tokens = make_batch([20, 150], [3, 2], 16, 16, 2)
+    spare = (set(range(16)) - set(batch.page_table.flatten().tolist())).pop()
+    batch.page_table[1, 11] = spare                   # a page for the table's last entry
+    qkv = torch.randn(tokens, 8 * 64, device="cuda").half()
+    if fault == "a range ends behind the rows":       # would put the rows of keys 148 and 149 at 108 and 109
+        batch.query_starts[2] = tokens + 40
+    elif fault == "a range begins in front of the rows":
+        batch.query_starts[0] = -2
+    elif fault == "ranges wholly behind the rows":
+        batch.query_starts += tokens
+    else:
+        batch.key_lengths[1] = 12 * 16 + 1            # its first new token would still have a place
+    before = cache.k.clone(), cache.v.clone()
+    out = torch.full((tokens, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    backend.rope_append(qkv, cache, batch, None, q_heads=4, out=out)
+    with pytest.raises(WB200Error, match="left out"):
+        backend.poll()
+    backend.poll()
+    rows, good = qkv.view(tokens, 8, 64), slice(0, 0)
+    if fault in ("a range ends behind the rows", "keys beyond the table"):
+        good, at = slice(0, 3), torch.arange(17, 20)
+        pages = batch.page_table[0].cpu().long()[at // 16]
+        before[0][pages, at % 16], before[1][pages, at % 16] = rows[:3, 4:6], rows[:3, 6:]
+    elif fault == "a range begins in front of the rows":
+        good, at = slice(3, 5), torch.arange(148, 150)
+        pages = batch.page_table[1].cpu().long()[at // 16]
+        before[0][pages, at % 16], before[1][pages, at % 16] = rows[3:, 4:6], rows[3:, 6:]
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
+    want = torch.full_like(out, 7.0)
+    want[good] = rows[good, :4]
+    assert torch.equal(out, want)

@@ -9,8 +9,7 @@
 // computes them once, into shared memory.
 //
 // Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below.
-#include "kernels.h"
-#include "ptx_sm100.cuh"
+#include "attention_paged.cuh"
 
 namespace wb200 {
 namespace {
@@ -114,24 +113,30 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   pdl_wait();
   pdl_launch_dependents();
   if constexpr (kAppend) {
-    // The tokens' sequences: every thread compares some sequences' token ranges with the block's tokens.
+    // The tokens' sequences: every thread compares some sequences' token ranges with the block's tokens. A range that is not one of
+    // the rows' is reported whether or not a token of the block lies in it.
     if (threadIdx.x < count) sequence_of[threadIdx.x] = -1;
     __syncthreads();
     for (int s = threadIdx.x; s < p.batch.sequences; s += kThreads) {
-      const int begin = max(p.batch.query_starts[s], first), end = min(p.batch.query_starts[s + 1], first + count);
-      for (int t = begin; t < end; ++t) sequence_of[t - first] = s;
+      const int begin = p.batch.query_starts[s], end = p.batch.query_starts[s + 1];
+      if (begin < end && (begin < 0 || end > a.tokens)) {
+        raise_status(p.refused, kRefusedLength);
+        continue;
+      }
+      for (int t = max(begin, first); t < min(end, first + count); ++t) sequence_of[t - first] = s;
     }
     __syncthreads();
     if (threadIdx.x < count) {
       const int s = sequence_of[threadIdx.x], token = first + static_cast<int>(threadIdx.x);
       int state = 0;
-      if (s >= 0) {
-        const int begin = p.batch.query_starts[s], end = p.batch.query_starts[s + 1];
-        const long long position = static_cast<long long>(p.batch.key_lengths[s]) - (static_cast<long long>(end) - token);
-        if (position < 0 || position >= static_cast<long long>(p.batch.table_width) * p.cache.page_size || begin < 0) {
+      // What attention would leave out as a whole is not written here in part: its positions mean nothing.
+      const PagedSequence sequence = s >= 0 ? paged_sequence(p.batch, p.cache, s, p.refused, true) : PagedSequence{0, 0, 0};
+      if (sequence.count > 0) {
+        const int position = sequence.keys - sequence.count + (token - sequence.begin);      // less than keys, which the table holds
+        if (position < 0) {
           raise_status(p.refused, kRefusedLength);
         } else {
-          const int slot = static_cast<int>(position / p.cache.page_size), row = static_cast<int>(position - static_cast<long long>(slot) * p.cache.page_size);
+          const int slot = position / p.cache.page_size, row = position - slot * p.cache.page_size;
           const int page = p.batch.page_table[s * p.batch.table_stride + slot];
           if (page < 0 || page >= p.cache.pages) {
             raise_status(p.refused, kRefusedPage);
