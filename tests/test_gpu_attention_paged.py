@@ -380,3 +380,13 @@ def test_work_is_shared_out_whole(backend, sequences, news, front, hk, group, he
     q = torch.randn(tokens, hk * group, head_dim, generator=rng).bfloat16().cuda()
     for max_query in (0, 1, news):
         agree(backend, q, cache, PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query), head_dim ** -0.5)
+
+
+@pytest.mark.parametrize("stride", [0, 64, 128])
+@pytest.mark.parametrize("news", [[9, 3], [200, 70]])
+def test_one_query_head_of_any_token_stride(backend, news, stride):
+    # queries that share memory, all of one row or half of the one before, are read like any others
+    cache = make_cache(50, 32, 1, 128, torch.bfloat16, "rows", 1)
+    batch, tokens = make_batch([300, 500], news, 32, 50, 2)
+    buffer = torch.randn(tokens * 128, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    agree(backend, buffer.as_strided((tokens, 1, 128), (stride, 128, 1)), cache, batch, 0.1)

@@ -1151,7 +1151,7 @@ bool attention_paged_chunk_supports(const AttentionPagedArgs &a) {
   if (box_rows_of(a.cache.page_size) < 8) return false;      // a box covers whole 8-row groups of the swizzle
   CacheMap map;
   return make_cache_map(a.cache, &map) && (a.q_heads == 1 || a.q_head >= a.cache.head_dim) &&
-         (a.q_heads == 1 || a.batch.tokens == 1 || a.q_token >= a.q_heads * a.q_head);   // tokens outside heads
+         (a.batch.tokens == 1 || a.q_token >= (a.q_heads == 1 ? a.cache.head_dim : a.q_heads * a.q_head));   // tokens outside heads
 }
 
 size_t attention_paged_chunk_workspace(int sm_count) { return chunk_record_bytes(sm_count) + static_cast<size_t>(sm_count) * sizeof(ChunkSplit); }
