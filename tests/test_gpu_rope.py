@@ -222,3 +222,21 @@ def test_append_leaves_out_whole_sequences_that_do_not_fit(backend, fault):
     want = torch.full_like(out, 7.0)
     want[good] = rows[good, :4]
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("position", [1, 2, 7, 10, -1, -3])
+def test_slow_pairs_keep_their_sine(backend, position):
+    """(1, 0) turns into (cos t, sin t): a small sine (slow pairs, and pairs near half a turn) is right to a few units in its own
+    last place: the angle is rounded once (2^-24), sincospi is off by one unit in the last place (2^-23), and the product with
+    the sine is one rounding more (2^-24)."""
+    slowest = RotaryTable(128, theta=500000.0, scaling="linear", factor=8.0).frequencies[-1]
+    table = RotaryTable.from_frequencies([slowest, 1e-9, 3e-12, 1e-6, math.pi * (1 + 1e-7), 2 * math.pi * (1 - 1e-8), 0.3])
+    n = len(table.frequencies)
+    x = torch.zeros(1, 1, 2 * n, device="cuda")
+    x[..., :n] = 1.0
+    got = backend.rope(x, torch.tensor([position], device="cuda"), table)[0, 0].cpu().double()
+    for i in range(n):
+        phase = position * table._turns[i] % 2 ** 64
+        half_turns, rest = divmod(phase + 2 ** 62, 2 ** 63)
+        want = (-1) ** half_turns * math.sin(2 * math.pi * ((rest - 2 ** 62) / 2.0 ** 64))
+        assert abs(got[n + i] - want) <= 4 * 2.0 ** -24 * abs(want), (i, got[n + i].item(), want)

@@ -5,8 +5,8 @@
 // The angle. A frequency is given in 2^-64 turns per position, so position * frequency in 64-bit integers IS the angle
 // modulo whole turns, for positions of either sign and any size; a product in f32 has lost the angle's fourth digit at
 // position 1000 and all of them at 10^6. Of the 64 bits the two highest (rounded) are the quadrant and the rest, within an
-// eighth of a turn, keeps 24 significant bits for sincospif. The sines and cosines of a token serve all its heads: a block
-// computes them once, into shared memory.
+// eighth of a turn, is rounded to 24 significant bits of its own for sincospif, so that the small sines of slow pairs are as
+// right as any. The sines and cosines of a token serve all its heads: a block computes them once, into shared memory.
 //
 // Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below.
 #include "attention_paged.cuh"
@@ -34,7 +34,7 @@ __device__ __forceinline__ float2 sin_cos_of_turns(unsigned long long phase) {
   const unsigned int quadrant = static_cast<unsigned int>((phase + (1ull << 61)) >> 62) & 3u;
   const long long rest = static_cast<long long>(phase - (static_cast<unsigned long long>(quadrant) << 62));   // +- 2^61
   float s, c;
-  sincospif(static_cast<float>(static_cast<int>(rest >> 30)) * 0x1p-33f, &s, &c);   // half turns
+  sincospif(static_cast<float>(rest) * 0x1p-63f, &s, &c);   // half turns
   const float sine = (quadrant & 1u) ? c : s, cosine = (quadrant & 1u) ? s : c;
   return make_float2((quadrant & 2u) ? -sine : sine, (quadrant == 1u || quadrant == 2u) ? -cosine : cosine);
 }
