@@ -632,7 +632,8 @@ wb200_status wb200_switch_sum(wb200_backend *backend, const wb200_switch_sum_par
 
 /* Reads and clears the device status word of asynchronous (WB200_MEM_DEVICE) calls after
  * synchronising `stream`. Returns WB200_ERR_DEVICE_TIMEOUT if a kernel gave up a bounded wait, WB200_ERR_INVALID_ARGUMENT if
- * one of the paged-cache kernels found device data it had to leave out. */
+ * one of the paged-cache kernels found device data it had to leave out; with both pending the first, and the other at the next
+ * call. */
 wb200_status wb200_backend_poll(wb200_backend *backend, void *stream);
 
 /* Self-test of the bounded device-side waits: launches a kernel that waits, for at most `cycle_limit` SM clocks, on a

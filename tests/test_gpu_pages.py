@@ -225,3 +225,15 @@ def test_page_tables_in_place(backend):
     tables.compact([cache])
     assert tables.table[1, :3].tolist() == [2, 0, 1] and tables.refs[:6].tolist() == [1, 1, 1, 0, 0, 0] and bool((cache.k[1] == 3.0).all())
     backend.poll()
+
+
+def test_poll_reports_one_thing_after_the_other(backend):
+    """A wait that gave up and refused data, both pending: neither report is lost."""
+    table, lengths, refs = state(12, 6, 100, 8, 3, fill=0.5)
+    backend.pages_free(table, lengths, refs, torch.tensor([12], dtype=torch.int32).cuda(), 8)
+    backend.selftest_bounded_wait(100_000)
+    with pytest.raises(WB200Error, match="wait"):
+        backend.poll()
+    with pytest.raises(WB200Error, match="left out"):
+        backend.poll()
+    backend.poll()

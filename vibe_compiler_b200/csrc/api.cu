@@ -74,10 +74,12 @@ wb200_status wb200_backend_poll(wb200_backend *backend, void *stream) {
   if (!backend) return fail(WB200_ERR_INVALID_ARGUMENT, "backend is null");
   DeviceGuard guard(backend->device);
   const wb200_status st = read_device_status(backend, static_cast<cudaStream_t>(stream), nullptr);
+  if (st != WB200_OK) return st;                       // what else there is to report waits for the next poll
   volatile int *refused = backend->h_status + 2;
   const int code = *refused;
-  if (code != 0) *refused = 0;
-  return st != WB200_OK || code == 0 ? st : fail(WB200_ERR_INVALID_ARGUMENT, refused_data_message(code));
+  if (code == 0) return WB200_OK;
+  *refused = 0;
+  return fail(WB200_ERR_INVALID_ARGUMENT, refused_data_message(code));
 }
 
 wb200_status wb200_physical_geometry(const wb200_tensor_desc *desc, wb200_geometry *out) {
