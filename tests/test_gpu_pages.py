@@ -237,3 +237,19 @@ def test_poll_reports_one_thing_after_the_other(backend):
     with pytest.raises(WB200Error, match="left out"):
         backend.poll()
     backend.poll()
+
+
+@pytest.mark.parametrize("page", [-1, 100])
+def test_fork_reports_a_last_page_outside_the_cache(backend, page):
+    # the page that a child's own last page is to be copied from: without a report the child's rows would be whatever lies there
+    table, lengths, refs = state(12, 6, 100, 8, 3, fill=0.5)
+    lengths[0] = 0
+    parent = max(range(1, 12), key=lambda s: int(lengths[s]))
+    lengths[parent] = lengths[parent] // 8 * 8 - 3    # its last page holds five tokens
+    table[parent, int(lengths[parent]) // 8] = page
+    p, c = torch.tensor([parent], dtype=torch.int32).cuda(), torch.tensor([0], dtype=torch.int32).cuda()
+    got = backend.pages_fork(table, lengths, refs, p, c, 8)
+    assert int(got[5]) == 0 and got[3].tolist() == [-1]
+    with pytest.raises(WB200Error, match="page number"):
+        backend.poll()
+    backend.poll()

@@ -304,7 +304,12 @@ pages_fork_kernel(const PageTablesArgs p, int count, const int *parents, const i
         }
       }
       if (lane == 0) {
-        sources[i] = partial ? from[full] : -1;
+        int source = partial ? from[full] : -1;
+        if (partial && (source < 0 || source >= p.pages)) {        // nothing to copy the child's last rows from
+          raise_status(p.refused, kRefusedPage);
+          source = -1;
+        }
+        sources[i] = source;
         if (!partial) destinations[i] = -1;
         p.lengths_out[child] = tokens;
       }
