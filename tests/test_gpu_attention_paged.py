@@ -390,3 +390,26 @@ def test_one_query_head_of_any_token_stride(backend, news, stride):
     batch, tokens = make_batch([300, 500], news, 32, 50, 2)
     buffer = torch.randn(tokens * 128, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
     agree(backend, buffer.as_strided((tokens, 1, 128), (stride, 128, 1)), cache, batch, 0.1)
+
+
+def test_a_decoding_step_of_the_layer_takes_the_decoding_kernel(backend):
+    """Without the caller's word on the longest chunk, 3 tokens of 3 sequences are one each; a range that ends behind them is reported."""
+    from vibe_compiler_b200.decoder_layer import LayerConfig, ShardedDecoderLayer, random_weights
+    cfg = LayerConfig(d_model=512, q_heads=8, kv_heads=2, head_dim=128, ffn=768)
+    layer = ShardedDecoderLayer(backend, cfg, random_weights(cfg))
+    cache = make_cache(30, 16, 2, 128, torch.bfloat16, "rows", 1)
+    batch, tokens = make_batch([90, 40, 200], [1, 1, 1], 16, 30, 2)
+    x = torch.randn(tokens, 512, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    launches, results = [], []
+    for max_query in (1, 0):
+        before = backend.launch_count
+        hinted = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query)
+        results.append(layer.forward_paged(x, cache, hinted))
+        launches.append(backend.launch_count - before)
+    assert launches[0] == launches[1] and torch.equal(*results)
+    backend.poll()
+    batch.query_starts[3] += 2
+    layer.forward_paged(x, cache, batch)
+    with pytest.raises(WB200Error):
+        backend.poll()
+    backend.poll()

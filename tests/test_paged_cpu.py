@@ -217,3 +217,41 @@ def test_struct_layouts_match_the_header():
     assert C.sizeof(abi.RopeAppendParams) == 8 + 16 + 3 * 8 + 4 * 8
     assert C.sizeof(abi.AttentionPagedParams) == 16 + 3 * 8 + 4 * 8 + 3 * 8
     assert C.sizeof(abi.PageTablesDesc) == 16 + 6 * 8 + 3 * 8
+
+
+class RecordingBackend:
+    """The backend calls of a layer's step, as shapes."""
+    device = 0
+
+    def __init__(self):
+        self.rows = {}
+
+    def rmsnorm(self, x, weight, eps):
+        return x
+
+    def gemm_epilogue(self, x, weight, epilogue=None):
+        assert x.shape[0] % 8 == 0 and x.shape[1] == weight.shape[0] and x.is_contiguous()
+        return x.new_zeros(x.shape[0], weight.shape[1] // (2 if epilogue is not None else 1))
+
+    def rope_append(self, qkv, cache, batch, table, *, q_heads):
+        self.rows["append"] = qkv.shape[0]
+        return qkv.new_zeros(qkv.shape[0], q_heads, 16)
+
+    def attention_paged(self, q, cache, batch, scale, out=None):
+        self.rows["attention"] = q.shape[0]
+        return out.copy_(q) if out is not None else q.clone()
+
+    def residual_add(self, a, b):
+        return a + b
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 8, 33])
+def test_a_step_gives_its_tokens_and_no_more_to_the_paged_calls(tokens):
+    # the rows that fill up an eight for the GEMMs are no tokens: they would choose another kernel and hide ranges that end among them
+    from vibe_compiler_b200.decoder_layer import LayerConfig, ShardedDecoderLayer, random_weights
+    cfg = LayerConfig(d_model=32, q_heads=2, kv_heads=1, head_dim=16, ffn=32)
+    recorder = RecordingBackend()
+    layer = ShardedDecoderLayer(recorder, cfg, random_weights(cfg), device=torch.device("cpu"))
+    x = torch.randn(tokens, 32).bfloat16()
+    assert layer.forward_paged(x, None, None, RotaryTable(16)).shape == (tokens, 32)
+    assert recorder.rows == {"append": tokens, "attention": tokens}

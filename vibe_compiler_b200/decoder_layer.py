@@ -135,11 +135,13 @@ class ShardedDecoderLayer:
         tokens = x.shape[0]
         if tokens == 0:
             return torch.empty_like(x)
-        if tokens % 8:                         # the GEMMs take rows by eights; the rows behind belong to no sequence
+        if tokens % 8:                         # the GEMMs take rows by eights
             x = torch.nn.functional.pad(x, (0, 0, 0, 8 - tokens % 8))
         qkv = be.gemm_epilogue(be.rmsnorm(x, self.norm1, cfg.eps), self.wqkv)
-        q = be.rope_append(qkv, cache, batch, rotary, q_heads=self.hq)
-        attn = be.attention_paged(q, cache, batch, cfg.head_dim ** -0.5)
+        # The paged calls get the tokens alone: their number chooses the kernel, and a range that ends behind them is refused.
+        q = be.rope_append(qkv[:tokens], cache, batch, rotary, q_heads=self.hq)
+        attn = qkv.new_empty(x.shape[0], self.hq, cfg.head_dim)
+        be.attention_paged(q, cache, batch, cfg.head_dim ** -0.5, out=attn[:tokens])
         partial = self._all_reduce(be.gemm_epilogue(attn.view(x.shape[0], self.hq * cfg.head_dim), self.wo))   # sum over head shards
         x1 = be.residual_add(x, partial)
         return be.residual_add(x1, self._all_reduce(self.ffn_partial(x1)))[:tokens]                           # sum over FFN shards
