@@ -465,11 +465,12 @@ wb200_status wb200_decoder_layer_timeline(wb200_backend *backend, float *ms, uin
 /* ------------------------------------------------------------------ serving from a paged KV cache
  * A cache of K and V rows cut into pages of `page_size` tokens, a page table that says which pages a sequence's rows lie
  * in, and the operators that write, read and keep it. The reference has no counterpart: it decodes from one compact cache
- * per invocation. All buffers are device buffers of the backend's device; every call enqueues its kernels on `stream`,
- * allocates nothing and returns without synchronising, so calls can be captured into CUDA graphs. What the kernels find
- * wrong in device data (a page outside the cache, lengths outside the table, an index twice) they leave out, never reading
- * or writing outside the given buffers, and the next wb200_backend_poll() returns WB200_ERR_INVALID_ARGUMENT; the results of
- * the sequences concerned have no meaning. One row of a page table covers at most 2^30 tokens. */
+ * per invocation. All buffers are device buffers of the backend's device, aligned to their elements; every call enqueues
+ * its kernels on `stream`, allocates nothing and returns without synchronising, so calls can be captured into CUDA graphs.
+ * What the kernels find wrong in device data (a page outside the cache, lengths outside the table, an index twice) they leave
+ * out, never reading or writing outside the given buffers, and the next wb200_backend_poll() returns
+ * WB200_ERR_INVALID_ARGUMENT; the results of the sequences concerned have no meaning. One row of a page table covers at most
+ * 2^30 tokens. */
 
 /* Rotary positions: for a token at position p and pair i < rotary_dim / 2 of a head,
  *   (y_a, y_b) = magnitude * (x_a cos t - x_b sin t, x_b cos t + x_a sin t),   t = 2 pi p turns_i

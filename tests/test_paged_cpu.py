@@ -255,3 +255,45 @@ def test_a_step_gives_its_tokens_and_no_more_to_the_paged_calls(tokens):
     x = torch.randn(tokens, 32).bfloat16()
     assert layer.forward_paged(x, None, None, RotaryTable(16)).shape == (tokens, 32)
     assert recorder.rows == {"append": tokens, "attention": tokens}
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(x=(2 << 20) + 1), INVALID), (dict(out=(3 << 20) + 1), INVALID), (dict(positions=(1 << 20) + 4), INVALID),
+    (dict(positions=(1 << 20) + 2, position_bytes=4), INVALID), (dict(x=(2 << 20) + 2, format=abi.F32), INVALID)])
+def test_rope_refuses_addresses_off_its_elements(changes, status):
+    assert abi.load().wb200_rope(HANDLE, C.byref(rows(**changes))) == status
+
+
+@pytest.mark.parametrize("target,changes", [
+    (cache, dict(k=(1 << 20) + 1)), (cache, dict(v=(2 << 20) + 1)), (batch, dict(page_table=(1 << 20) + 2)), (batch, dict(key_lengths=(2 << 20) + 2)),
+    (batch, dict(query_starts=(3 << 20) + 1)), (attention, dict(q=(1 << 20) + 1)), (attention, dict(out=(2 << 20) + 1)), (attention, dict(lse=(3 << 20) + 2)),
+    (append, dict(qkv=(1 << 20) + 1)), (append, dict(q=(2 << 20) + 1)), (append, dict(positions=(1 << 20) + 4, position_bytes=8))])
+def test_paged_calls_refuse_addresses_off_their_elements(target, changes):
+    made = {f: f(**(changes if f is target else {})) for f in (cache, batch, attention, append)}
+    lib = abi.load()
+    if target is not append:
+        assert lib.wb200_attention_paged(HANDLE, C.byref(made[cache]), C.byref(made[batch]), C.byref(made[attention])) == INVALID
+    if target is not attention:
+        assert lib.wb200_rope_append(HANDLE, C.byref(made[cache]), C.byref(made[batch]), C.byref(made[append])) == INVALID
+    if target is cache:
+        one = (abi.PagedCacheDesc * 1)(made[cache])
+        assert lib.wb200_pages_copy(HANDLE, one, 1, 1, 4 << 20, 4 << 20, None) == INVALID
+
+
+def test_page_calls_refuse_addresses_off_their_elements():
+    lib, word, off = abi.load(), 4 << 20, (4 << 20) + 2
+    for name in ("table", "lengths", "refs", "table_out", "lengths_out", "refs_out"):
+        t = tables(**{name: (5 << 20) + 2})
+        assert lib.wb200_pages_reserve(HANDLE, C.byref(t), word, word) == INVALID
+        assert lib.wb200_pages_free(HANDLE, C.byref(t), 1, word) == INVALID
+        assert lib.wb200_pages_fork(HANDLE, C.byref(t), 1, word, word, word, word, word) == INVALID
+        assert lib.wb200_pages_compact(HANDLE, C.byref(t), word, word) == INVALID
+    t = tables()
+    for i in range(2):
+        assert lib.wb200_pages_reserve(HANDLE, C.byref(t), *[off if j == i else word for j in range(2)]) == INVALID
+        assert lib.wb200_pages_compact(HANDLE, C.byref(t), *[off if j == i else word for j in range(2)]) == INVALID
+        one = (abi.PagedCacheDesc * 1)(cache())
+        assert lib.wb200_pages_copy(HANDLE, one, 1, 1, *[off if j == i else word for j in range(2)], None) == INVALID
+    assert lib.wb200_pages_free(HANDLE, C.byref(t), 1, off) == INVALID
+    for i in range(5):
+        assert lib.wb200_pages_fork(HANDLE, C.byref(t), 1, *[off if j == i else word for j in range(5)]) == INVALID

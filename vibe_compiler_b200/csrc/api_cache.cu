@@ -18,6 +18,13 @@ const char *refused_data_message(int code) {
 
 namespace {
 
+// Addresses of elements of `bytes` bytes; null counts. The kernels load and store whole elements.
+template <typename... Pointers>
+bool on_elements(uint32_t bytes, const Pointers *...pointers) {
+  return ((reinterpret_cast<uintptr_t>(pointers) | ... | 0u) & (bytes - 1)) == 0;
+}
+wb200_status off_elements() { return fail(WB200_ERR_INVALID_ARGUMENT, "device arrays must be aligned to their elements"); }
+
 wb200_status make_rotary_constants(const wb200_rope_table &t, uint32_t head_dim, RotaryConstants *c) {
   if (t.rotary_dim % 2 != 0 || t.rotary_dim > head_dim || t.rotary_dim > 2 * kMaxRotaryPairs)
     return fail(WB200_ERR_INVALID_ARGUMENT, "rotary_dim must be even and at most head_dim and 512");
@@ -51,6 +58,7 @@ wb200_status make_cache(const wb200_paged_cache *c, bool f32_too, PagedCacheArgs
   if (c->pages > 0x7fffffffu || c->page_size > 0x7fffffffu || c->kv_heads > 0xffffu || c->head_dim > 0xffffu)
     return fail(WB200_ERR_LIMIT, "paged cache extents too large");
   if (!c->k || !c->v) return fail(WB200_ERR_INVALID_ARGUMENT, "k and v of the paged cache must not be null");
+  if (!on_elements(c->format == WB200_F32 ? 4 : 2, c->k, c->v)) return off_elements();
   const int64_t extent[3] = {c->pages, c->page_size, c->kv_heads};
   if (!rows_apart(c->head_dim, {c->k_page_stride, c->k_row_stride, c->k_head_stride}, extent) ||
       !rows_apart(c->head_dim, {c->v_page_stride, c->v_row_stride, c->v_head_stride}, extent))
@@ -73,6 +81,7 @@ wb200_status make_batch(const wb200_paged_batch *b, const PagedCacheArgs &c, Pag
       return fail(WB200_ERR_INVALID_ARGUMENT, "page_table, key_lengths and query_starts must not be null");
     if (b->sequences > 1 && b->table_stride < static_cast<int64_t>(b->table_width))
       return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the page table overlap");
+    if (!on_elements(4, b->page_table, b->key_lengths, b->query_starts)) return off_elements();
   }
   a->sequences = static_cast<int>(b->sequences); a->table_width = static_cast<int>(b->table_width);
   a->tokens = static_cast<int>(b->tokens); a->max_query = static_cast<int>(b->max_query);
@@ -133,6 +142,7 @@ wb200_status make_page_tables(wb200_backend *backend, const wb200_page_tables *t
     return fail(WB200_ERR_LIMIT, "page table extents too large");
   if (!t->table || !t->lengths || !t->refs || !t->table_out || !t->refs_out || (lengths_out && !t->lengths_out))
     return fail(WB200_ERR_INVALID_ARGUMENT, "page table, lengths and refs must not be null");
+  if (!on_elements(4, t->table, t->lengths, t->refs, t->table_out, t->lengths_out, t->refs_out)) return off_elements();
   if (t->sequences > 1 && (t->table_stride < static_cast<int64_t>(t->table_width) || t->table_out_stride < static_cast<int64_t>(t->table_width)))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the page table overlap");
   if (t->table == t->table_out && t->sequences > 1 && t->table_stride != t->table_out_stride)
@@ -162,6 +172,7 @@ wb200_status wb200_rope(wb200_backend *backend, const wb200_rope_params *p) {
   if (st != WB200_OK) return st;
   if (p->tokens == 0) return WB200_OK;
   if (!p->x || !p->out || !p->positions) return fail(WB200_ERR_INVALID_ARGUMENT, "x, out and positions must not be null");
+  if (!on_elements(p->format == WB200_F32 ? 4 : 2, p->x, p->out) || !on_elements(p->position_bytes, p->positions)) return off_elements();
   if (!output_rows_apart(p->head_dim, p->out_token_stride, p->out_head_stride, p->tokens, p->heads))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
   if (p->x == p->out && ((p->tokens > 1 && p->x_token_stride != p->out_token_stride) || (p->heads > 1 && p->x_head_stride != p->out_head_stride)))
@@ -192,6 +203,7 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
   if (p->positions && p->position_bytes != 4 && p->position_bytes != 8) return fail(WB200_ERR_INVALID_ARGUMENT, "positions are int32 or int64");
   if (b.tokens == 0 || b.sequences == 0) return WB200_OK;
   if (!p->qkv || (p->q_heads != 0 && !p->q)) return fail(WB200_ERR_INVALID_ARGUMENT, "qkv and q must not be null");
+  if (!on_elements(2, p->qkv, p->q) || (p->positions && !on_elements(p->position_bytes, p->positions))) return off_elements();
   if (p->q_heads != 0 && !output_rows_apart(cache->head_dim, p->q_token_stride, p->q_head_stride, b.tokens, p->q_heads))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
   RopeArgs a{};
@@ -226,6 +238,7 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   if (st != WB200_OK) return st;
   if (a.batch.tokens == 0 || a.batch.sequences == 0) return WB200_OK;
   if (!a.q || !a.out) return fail(WB200_ERR_INVALID_ARGUMENT, "q and out must not be null");
+  if (!on_elements(2, a.q, a.out) || !on_elements(4, a.lse)) return off_elements();
   if (!output_rows_apart(a.cache.head_dim, a.out_token, a.out_head, a.batch.tokens, a.q_heads))
     return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
   const PagedKernel kernel = choose_attention_paged(a);
@@ -247,6 +260,7 @@ wb200_status wb200_pages_reserve(wb200_backend *backend, const wb200_page_tables
   wb200_status st = make_page_tables(backend, tables, true, &a);
   if (st != WB200_OK) return st;
   if (!wanted || !result) return fail(WB200_ERR_INVALID_ARGUMENT, "wanted and result must not be null");
+  if (!on_elements(4, wanted, result)) return off_elements();
   DeviceGuard guard(backend->device);
   if ((st = launch_pages_reserve(a, wanted, result, static_cast<cudaStream_t>(tables->stream))) == WB200_OK) backend->launches += 1;
   return st;
@@ -260,6 +274,7 @@ wb200_status wb200_pages_fork(wb200_backend *backend, const wb200_page_tables *t
   if (count > tables->sequences) return fail(WB200_ERR_INVALID_ARGUMENT, "more forks than sequences");
   if (!result || (count != 0 && (!parents || !children || !sources || !destinations)))
     return fail(WB200_ERR_INVALID_ARGUMENT, "parents, children, sources, destinations and result must not be null");
+  if (!on_elements(4, parents, children, sources, destinations, result)) return off_elements();
   DeviceGuard guard(backend->device);
   st = launch_pages_fork(a, static_cast<int>(count), parents, children, sources, destinations, result, static_cast<cudaStream_t>(tables->stream));
   if (st == WB200_OK) backend->launches += 1;
@@ -272,6 +287,7 @@ wb200_status wb200_pages_free(wb200_backend *backend, const wb200_page_tables *t
   if (st != WB200_OK) return st;
   if (count > (1u << 30)) return fail(WB200_ERR_LIMIT, "more than 2^30 sequences to free");
   if (count != 0 && !sequences) return fail(WB200_ERR_INVALID_ARGUMENT, "sequences must not be null");
+  if (!on_elements(4, sequences)) return off_elements();
   DeviceGuard guard(backend->device);
   if ((st = launch_pages_free(a, static_cast<int>(count), sequences, static_cast<cudaStream_t>(tables->stream))) == WB200_OK) backend->launches += 1;
   return st;
@@ -282,6 +298,7 @@ wb200_status wb200_pages_compact(wb200_backend *backend, const wb200_page_tables
   wb200_status st = make_page_tables(backend, tables, false, &a);
   if (st != WB200_OK) return st;
   if (tables->pages >= 2 && (!sources || !destinations)) return fail(WB200_ERR_INVALID_ARGUMENT, "sources and destinations must not be null");
+  if (!on_elements(4, sources, destinations)) return off_elements();
   DeviceGuard guard(backend->device);
   if ((st = launch_pages_compact(a, sources, destinations, static_cast<cudaStream_t>(tables->stream))) == WB200_OK) backend->launches += 1;
   return st;
@@ -302,6 +319,7 @@ wb200_status wb200_pages_copy(wb200_backend *backend, const wb200_paged_cache *c
   }
   if (cache_count == 0 || count == 0) return WB200_OK;
   if (!sources || !destinations) return fail(WB200_ERR_INVALID_ARGUMENT, "sources and destinations must not be null");
+  if (!on_elements(4, sources, destinations)) return off_elements();
   DeviceGuard guard(backend->device);
   for (uint32_t first = 0; first < cache_count; first += kMaxCachesPerCopy) {
     PagedCacheArgs part[kMaxCachesPerCopy];
