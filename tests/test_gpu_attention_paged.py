@@ -413,3 +413,43 @@ def test_a_decoding_step_of_the_layer_takes_the_decoding_kernel(backend):
     with pytest.raises(WB200Error):
         backend.poll()
     backend.poll()
+
+
+# (keys, new tokens, query heads): units and items whole, halved, cut over CTAs, and taken by clusters; the last by the general kernel
+@pytest.mark.parametrize("lengths,news,hq,hk,head_dim", [
+    ([700, 90], [1, 1], 8, 2, 128), ([9000] * 12, [1] * 12, 8, 8, 64), ([300, 260], [200, 250], 4, 2, 128), ([500, 300], [40, 9], 4, 2, 64),
+    ([20000], [60], 4, 2, 128), ([9000], [500], 4, 1, 64), ([150, 90], [70, 1], 2, 1, 72)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_scores_that_are_no_numbers(backend, lengths, news, hq, hk, head_dim, value):
+    """A NaN or infinite score among the keys that a row sees makes what the definition makes of it: NaN, or for -inf a key without
+    weight. Rows that do not see it, of the same tile or of another sequence, keep their values."""
+    size = 16
+    cache = make_cache(sum(-(-n // size) for n in lengths) + 3, size, hk, head_dim, torch.bfloat16, "rows", 1)
+    batch, tokens = make_batch(lengths, news, size, cache.k.shape[0], 2)
+    q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    q[..., 0] = q[..., 0].abs() + 0.5                 # what meets the infinity is positive
+
+    def of(key):
+        return batch.page_table[0].long()[key // size], key % size
+    bad = lengths[0] - news[0] // 2 - 1               # half of the first sequence's tokens see this key
+    cache.k[(*of(torch.tensor(bad, device="cuda")), slice(None), 0)] = value
+    sees = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    sees[bad - (lengths[0] - news[0]):news[0]] = True
+    expected = ref.attention(q, cache.k, cache.v, batch.page_table, batch.key_lengths, batch.query_starts, 0.1)
+    if value == -float("inf"):
+        # for the rows that see it: the same without the key, those behind it one place further in front
+        k, v, fewer = cache.k.clone(), cache.v.clone(), batch.key_lengths.clone()
+        behind = torch.arange(bad + 1, lengths[0], device="cuda")
+        k[of(behind - 1)], v[of(behind - 1)] = cache.k[of(behind)], cache.v[of(behind)]
+        fewer[0] -= 1
+        for whole, seen in zip(expected, ref.attention(q, k, v, batch.page_table, fewer, batch.query_starts, 0.1)):
+            whole[sees] = seen[sees]
+    want, want_lse, bound, bound_lse = expected
+    for max_query in (0, 1, max(news)):
+        out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 5.0, device="cuda")
+        hinted = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query)
+        backend.attention_paged(q, cache, hinted, 0.1, out=out, lse=lse)
+        backend.poll()
+        rows = torch.ones_like(sees) if value == -float("inf") else ~sees
+        assert bool(((out.double() - want).abs() <= bound)[rows].all()) and bool(((lse.double() - want_lse).abs() <= bound_lse)[rows].all())
+        assert bool(out[~rows].isnan().all()) and not bool(lse[~rows].isfinite().any())

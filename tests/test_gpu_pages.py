@@ -253,3 +253,33 @@ def test_fork_reports_a_last_page_outside_the_cache(backend, page):
     with pytest.raises(WB200Error, match="page number"):
         backend.poll()
     backend.poll()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("pages,size", [(60, 8), (5000, 16), (70001, 4)])
+def test_reserve_with_exactly_enough_and_too_few_pages(backend, pages, size, in_place):
+    """Wants of all free pages and of three more, in pools of one and of many parts of the scan, spread over many sequences."""
+    sequences, width = 40, pages // 16
+    table, lengths, refs = state(sequences, width, pages, size, 5, fill=0.6)
+    free = int((refs == 0).sum())
+    for wanted_pages, outcome in ((free, 0), (free + 3, 3)):
+        plain = ref.Pages(table, lengths, refs, size)
+        have = [plain.count(s) for s in range(sequences)]
+        wanted, spread = lengths.tolist(), wanted_pages
+        for s in range(sequences):
+            more = min(spread, width - have[s])
+            if more:
+                wanted[s] = (have[s] + more) * size - (s % size)
+                spread -= more
+        assert spread == 0
+        wanted = torch.tensor(wanted, dtype=torch.int32).cuda()
+        before = table.clone(), lengths.clone(), refs.clone()
+        arrays = (table.clone(), lengths.clone(), refs.clone())
+        got = backend.pages_reserve(*arrays, wanted, size, out=arrays if in_place else None)
+        assert int(got[3]) == outcome
+        if outcome:
+            assert all(torch.equal(a, b) for a, b in zip(got[:3], before)) and all(torch.equal(a, b) for a, b in zip(arrays, before))
+        else:
+            assert plain.reserve(wanted) == 0 and int((got[2] == 0).sum()) == 0
+            agree(plain, *got[:3])
+    backend.poll()
