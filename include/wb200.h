@@ -467,17 +467,18 @@ wb200_status wb200_decoder_layer_timeline(wb200_backend *backend, float *ms, uin
  * in, and the operators that write, read and keep it. The reference has no counterpart: it decodes from one compact cache
  * per invocation. All buffers are device buffers of the backend's device, aligned to their elements; every call enqueues
  * its kernels on `stream`, allocates nothing and returns without synchronising, so calls can be captured into CUDA graphs.
- * What the kernels find wrong in device data (a page outside the cache, lengths outside the table, an index twice) they leave
- * out, never reading or writing outside the given buffers, and the next wb200_backend_poll() returns
- * WB200_ERR_INVALID_ARGUMENT; the results of the sequences concerned have no meaning. One row of a page table covers at most
- * 2^30 tokens. */
+ * What the kernels find wrong in device data (a page or a sequence outside its array, a token range outside the rows, a length
+ * outside the page table) they leave out, never reading or writing outside the given buffers, and the next
+ * wb200_backend_poll() returns WB200_ERR_INVALID_ARGUMENT; the results of the sequences concerned have no meaning. What an
+ * index named twice does stands at each call: poll does not report it. One row of a page table covers at most 2^30 tokens. */
 
 /* Rotary positions: for a token at position p and pair i < rotary_dim / 2 of a head,
  *   (y_a, y_b) = magnitude * (x_a cos t - x_b sin t, x_b cos t + x_a sin t),   t = 2 pi p turns_i
  * with (a, b) = (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; elements from rotary_dim on are copied.
  * `turns[i]` is the part of a full turn per position in units of 2^-64 turns. The product with the position wraps at whole
- * turns in 64-bit integers, so the angle is right to 2^-65 turns per position at any position. Arithmetic in f32, one
- * rounding to the storage format. */
+ * turns in 64-bit integers, so the angle is right to 2^-65 turns per position at any position; in front of sine and cosine its
+ * distance from the nearest quarter turn is rounded to 24 significant bits. Arithmetic in f32, one rounding to the storage
+ * format. */
 typedef struct wb200_rope_table {
   uint32_t rotary_dim;      /* even, at most 512 and the head dimension; 0 rotates nothing */
   float magnitude;          /* scale of the rotated elements */
@@ -539,12 +540,15 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
 /* Attention of every sequence's new tokens over its paged keys, grouped queries (q_heads % kv_heads == 0):
  *   s_j = scale q.k_j,   out = sum_j exp(s_j - lse) v_j,   lse = ln sum_j exp(s_j)
  * over the keys j < key_lengths[s], with `causal` those up to the token's own position. Statistics and sums are kept in
- * f32; probabilities may be rounded to the storage format in front of the product with V. A row without keys is NaN (0 with
- * zero_fully_masked) and its lse -inf. Cache rows behind key_lengths[s] may hold anything; a NaN or infinite V element of a
- * key inside the length reaches the rows that do not see the key too, as 0 * v does.
- * head_dim is a multiple of 8 up to 256. `workspace` needs wb200_attention_paged_workspace_bytes() bytes, 256-byte
- * aligned, of any content; calls that may run at the same time need one each. Without cache, batch and params that function
- * returns what is enough for any call of the backend (about 40 MB). */
+ * f32; probabilities, relative to about the row's largest, are rounded to the storage format in front of the product with V
+ * where head_dim is 64 or 128 and rows begin on 16 bytes (f16 ones up to 2^-25 vanish there, not from the sum), and kept in
+ * f32 elsewhere. A row without keys is NaN (0 with zero_fully_masked) and its lse -inf. Cache rows behind key_lengths[s] may
+ * hold anything; a NaN or infinite V element of a key inside the length reaches the rows that do not see the key too, as
+ * 0 * v does.
+ * head_dim is a multiple of 8 up to 256; 64 and 128, with rows that begin on 16 bytes, take the matrix kernels, others one that
+ * gives a warp to each row and is 8 to 33 times slower. `workspace` needs wb200_attention_paged_workspace_bytes() bytes,
+ * 256-byte aligned, of any content; calls that may run at the same time need one each. Without cache, batch and params that
+ * function returns what is enough for any call of the backend (about 40 MB). */
 typedef struct wb200_attention_paged_params {
   uint32_t q_heads;
   uint8_t causal, zero_fully_masked, reserved[2];
@@ -593,7 +597,7 @@ wb200_status wb200_pages_free(wb200_backend *backend, const wb200_page_tables *t
 wb200_status wb200_pages_compact(wb200_backend *backend, const wb200_page_tables *tables, int32_t *sources, int32_t *destinations);
 /* Whole pages of K and V, sources[i] -> destinations[i], in each of `caches` (same extents, strides and format). Entries with
  * a negative number are passed over. No page may be a destination twice, or a source and a destination: its content would be
- * undefined. */
+ * undefined, and nothing reports it. */
 wb200_status wb200_pages_copy(wb200_backend *backend, const wb200_paged_cache *caches, uint32_t cache_count, uint32_t count,
                               const int32_t *sources, const int32_t *destinations, void *stream);
 
