@@ -1,4 +1,6 @@
 """Attention over a paged KV cache against float64 (bounds: tests/paged_reference.attention)."""
+import copy
+
 import pytest
 import torch
 
@@ -453,3 +455,29 @@ def test_scores_that_are_no_numbers(backend, lengths, news, hq, hk, head_dim, va
         rows = torch.ones_like(sees) if value == -float("inf") else ~sees
         assert bool(((out.double() - want).abs() <= bound)[rows].all()) and bool(((lse.double() - want_lse).abs() <= bound_lse)[rows].all())
         assert bool(out[~rows].isnan().all()) and not bool(lse[~rows].isfinite().any())
+
+
+def test_copied_handles_describe_the_tensors_they_hold(backend):
+    """A copy, or an object sent to another process, has tensors of its own: the addresses that a call passes on have to be theirs."""
+    cache = make_cache(20, 16, 2, 128, torch.bfloat16, "rows", 1)
+    batch, _ = make_batch([90, 40], [1, 1], 16, 20, 2)
+    batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=7)
+    for again in (copy.copy, copy.deepcopy):
+        other, d = again(batch), again(batch)._desc(2)
+        for name in ("page_table", "key_lengths", "query_starts"):
+            assert torch.equal(getattr(other, name), getattr(batch, name)) and getattr(other._desc(2), name) == getattr(other, name).data_ptr()
+        assert (d.sequences, d.max_query, other.max_query) == (2, 7, 7)
+        other = again(cache)
+        assert (other._desc.k, other._desc.v) == (other.k.data_ptr(), other.v.data_ptr()) and torch.equal(other.k, cache.k)
+    for name in ("page_table", "key_lengths", "query_starts"):      # a tensor put in another's place is the one that is read
+        setattr(batch, name, getattr(batch, name).clone())
+        assert getattr(batch._desc(2), name) == getattr(batch, name).data_ptr()
+        with pytest.raises(ValueError):
+            setattr(batch, name, getattr(batch, name).long())
+    cache.k, cache.v, batch.max_query = cache.k.clone(), cache.v.clone(), 9
+    assert (cache._desc.k, cache._desc.v, batch._desc(2).max_query) == (cache.k.data_ptr(), cache.v.data_ptr(), 9)
+    before = batch.key_lengths.data_ptr()
+    batch.key_lengths += 1
+    assert batch.key_lengths.data_ptr() == before and batch.key_lengths.tolist() == [91, 41]
+    with pytest.raises(ValueError):
+        cache.k = cache.k[:10]

@@ -1,8 +1,10 @@
 """What serving from a paged cache decides on the host: the rotary tables' numbers, and every refusal, without a device.
 
 A refused call looks at no device state, so the library is given a block of zeros for its backend handle."""
+import copy
 import ctypes as C
 import math
+import pickle
 from fractions import Fraction
 
 import pytest
@@ -297,3 +299,11 @@ def test_page_calls_refuse_addresses_off_their_elements():
     assert lib.wb200_pages_free(HANDLE, C.byref(t), 1, off) == INVALID
     for i in range(5):
         assert lib.wb200_pages_fork(HANDLE, C.byref(t), 1, *[off if j == i else word for j in range(5)]) == INVALID
+
+
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda t: pickle.loads(pickle.dumps(t))])
+def test_a_copied_rotary_table_has_constants_of_its_own(again):
+    table = RotaryTable(64, theta=500000.0, scaling="yarn", factor=4.0, original_length=8192)
+    other = again(table)
+    assert (other.frequencies, other.magnitude, other.rotary_dim, list(other._turns)) == (table.frequencies, table.magnitude, 64, list(table._turns))
+    assert other._address == C.addressof(other._turns) != table._address

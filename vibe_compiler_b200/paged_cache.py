@@ -93,13 +93,16 @@ class RotaryTable:
         self._turns = (C.c_uint64 * max(1, len(frequencies)))(*[int(round(math.ldexp(f / (2.0 * math.pi), 64))) % (1 << 64) for f in frequencies])
         self._address = C.addressof(self._turns)
 
+    def __reduce__(self):                             # a copy's constants lie elsewhere
+        return type(self).from_frequencies, (self.frequencies, self.magnitude)
+
 
 class PagedCache:
     """One layer's K and V: tensors [pages, page_size, kv_heads, head_dim] on one GPU, bf16 or f16 (f32 for `pages_copy`
     only). Any strides with the head dimension innermost: a cache laid out [pages, kv_heads, page_size, head_dim] is passed
     as its transposed view."""
 
-    __slots__ = ("k", "v", "_desc", "device_index")
+    __slots__ = ("_k", "_v", "_desc", "device_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _FORMATS:
@@ -108,7 +111,7 @@ class PagedCache:
             raise ValueError("k and v must be CUDA tensors of one device")
         if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
             raise ValueError("the head dimension of k and v must be contiguous")
-        self.k, self.v, self.device_index = k, v, k.device.index
+        self._k, self._v, self.device_index = k, v, k.device.index
         self._desc = abi.PagedCacheDesc.from_buffer_copy(_CACHE_PACK(
             k.shape[0], k.shape[1], k.shape[2], k.shape[3], _FORMATS[k.dtype], 0, k.data_ptr(), v.data_ptr(),
             k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2)))
@@ -117,9 +120,16 @@ class PagedCache:
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16, device="cuda") -> "PagedCache":
         return cls(*(torch.zeros(pages, page_size, kv_heads, head_dim, dtype=dtype, device=device) for _ in range(2)))
 
+    # The calls pass on addresses, so a copy is made anew, and so is what they are taken from when another tensor is put in.
+    def __reduce__(self):
+        return type(self), (self._k, self._v)
+
+    k = property(lambda self: self._k, lambda self, k: self.__init__(k, self._v))
+    v = property(lambda self: self._v, lambda self, v: self.__init__(self._k, v))
+
     @property
     def page_size(self) -> int:
-        return self.k.shape[1]
+        return self._k.shape[1]
 
 
 class PagedBatch:
@@ -128,7 +138,7 @@ class PagedBatch:
     tensors: page_table [sequences, width], key_lengths [sequences], query_starts [sequences + 1]. `max_query`: the most new
     tokens of one sequence, if known (it chooses between kernels, the results do not depend on it)."""
 
-    __slots__ = ("page_table", "key_lengths", "query_starts", "max_query", "device_index", "_fields")
+    __slots__ = ("_tensors", "device_index", "_fields")
 
     def __init__(self, page_table: torch.Tensor, key_lengths: torch.Tensor, query_starts: torch.Tensor, max_query: int = 0):
         if not page_table.dtype == key_lengths.dtype == query_starts.dtype == torch.int32:
@@ -145,9 +155,22 @@ class PagedBatch:
             raise ValueError("rows of page_table, key_lengths and query_starts must be contiguous")
         if max_query < 0:
             raise ValueError("max_query must not be negative")
-        self.page_table, self.key_lengths, self.query_starts, self.max_query = page_table, key_lengths, query_starts, max_query
-        self.device_index = device
+        self._tensors, self.device_index = (page_table, key_lengths, query_starts), device
         self._fields = (sequences, width, int(max_query), page_table.data_ptr(), key_lengths.data_ptr(), query_starts.data_ptr(), stride[0])
+
+    # As for PagedCache.
+    def __reduce__(self):
+        return type(self), (*self._tensors, self.max_query)
+
+    def _with(self, at: int, value) -> None:
+        arguments = [*self._tensors, self.max_query]
+        arguments[at] = value
+        self.__init__(*arguments)
+
+    page_table = property(lambda self: self._tensors[0], lambda self, value: self._with(0, value))
+    key_lengths = property(lambda self: self._tensors[1], lambda self, value: self._with(1, value))
+    query_starts = property(lambda self: self._tensors[2], lambda self, value: self._with(2, value))
+    max_query = property(lambda self: self._fields[2], lambda self, value: self._with(3, value))
 
     def _desc(self, tokens: int) -> abi.PagedBatchDesc:
         sequences, width, max_query, table, lengths, starts, stride = self._fields
