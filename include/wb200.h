@@ -571,7 +571,9 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
  * page (0: free). The four calls below take them and write them to the *_out arrays, each of which may be the input itself;
  * table entries behind a sequence's pages keep their value unless said otherwise. Every result is one the order of threads
  * has no part in: pages are taken lowest index first, sequence by sequence. The keys themselves are moved by
- * wb200_pages_copy with the page numbers that fork and compact return, once per layer or for many layers in one call. */
+ * wb200_pages_copy with the page numbers that fork and compact return, once per layer or for many layers in one call.
+ * Lengths grow by reserve and end by free. A length lowered by other means leaves the pages behind it held by nobody's table,
+ * never to be free again; fork shares the pages that a length fills, whether their rows have been written or not. */
 typedef struct wb200_page_tables {
   uint32_t sequences, table_width, pages, page_size;   /* at most 16384 sequences */
   const int32_t *table, *lengths, *refs;               /* [sequences, table_width] at table_stride, [sequences], [pages] */
@@ -585,7 +587,8 @@ wb200_status wb200_pages_reserve(wb200_backend *backend, const wb200_page_tables
 /* Sequence children[i], which holds nothing, becomes a copy of parents[i]: full pages are shared, a last page that is not
  * full gets a page of its own, to which the caller copies its rows: sources[i] -> destinations[i] (-1, -1 where there is
  * none); the child's table entries behind its pages become -1. *result: 0 done; n > 0: n pages too few; -1: an index or
- * length out of range, a child that holds tokens, is named twice or is a parent too. Unless 0, the arrays come out as they went in, the lists -1. */
+ * length out of range, a child that holds tokens, is named twice or is a parent too. Unless 0, the arrays come out as they
+ * went in, the lists -1. */
 wb200_status wb200_pages_fork(wb200_backend *backend, const wb200_page_tables *tables, uint32_t count, const int32_t *parents,
                               const int32_t *children, int32_t *sources, int32_t *destinations, int32_t *result);
 /* The listed sequences give their pages back and hold nothing: length 0, the table entries of those that held something -1.

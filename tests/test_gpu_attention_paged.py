@@ -481,3 +481,31 @@ def test_copied_handles_describe_the_tensors_they_hold(backend):
     assert batch.key_lengths.data_ptr() == before and batch.key_lengths.tolist() == [91, 41]
     with pytest.raises(ValueError):
         cache.k = cache.k[:10]
+
+
+def test_rejected_drafts_are_written_over(backend):
+    """Two of five drafted tokens stay: the next ones go over the others' rows, their room reserved all along."""
+    size, hq, hk, d = 4, 4, 2, 64
+    tables, cache = PageTables(backend, 1, 20, 30, size), PagedCache.zeros(30, size, hk, d)
+    rows = torch.randn(60, (hq + 2 * hk) * d, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    keys, kept = torch.zeros(1, dtype=torch.int32, device="cuda"), []      # the true number of keys; the rows behind them
+
+    def step(new, stay):
+        keys.fill_(len(kept) + len(new))
+        assert int(tables.reserve(keys)) == 0
+        batch = PagedBatch(tables.table, keys, torch.tensor([0, len(new)], dtype=torch.int32, device="cuda"))
+        q = backend.rope_append(rows[new], cache, batch, None, q_heads=hq)
+        out = backend.attention_paged(q, cache, batch, 0.125)
+        seen = rows[kept + new].view(-1, hq + 2 * hk, d)
+        plain = PagedCache(*(t.contiguous()[None] for t in (seen[:, hq:hq + hk], seen[:, hq + hk:])))
+        one = PagedBatch(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), keys, batch.query_starts)
+        want, _, bound, _ = ref.attention(q, plain.k, plain.v, one.page_table, keys, batch.query_starts, 0.125)
+        assert bool(((out.double() - want).abs() <= bound).all())
+        kept.extend(new[:stay])
+
+    step(list(range(9)), 9)
+    step([10, 11, 12, 13, 14], 2)
+    step([20, 21], 1)
+    step([30, 31, 32, 33, 34, 35], 6)
+    backend.poll()
+    assert int(tables.refs.sum()) == -(-18 // size) and len(kept) == 18
