@@ -567,6 +567,54 @@ uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, con
 wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
                                    const wb200_attention_paged_params *params);
 
+/* K and V rows of the batch's tokens as they stand in the cache, out of their pages: what the append of the same batch wrote.
+ * Sequence s gives its last query_starts[s + 1] - query_starts[s] rows up to key_lengths[s], so query_starts that count up the key
+ * lengths read sequences whole. Rows of tokens that belong to no sequence, or whose page is refused, are not written. */
+typedef struct wb200_cache_read_params {
+  void *k, *v;              /* [tokens, kv_heads, head_dim] at the strides below, in elements; cache's format */
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  void *stream;
+} wb200_cache_read_params;
+wb200_status wb200_cache_read(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
+                              const wb200_cache_read_params *params);
+
+/* A paged cache held in four bits. A row of a KV head is cut into groups of 64 elements (the last takes what is left); of a
+ * group stand
+ *   low   its least element,  step  (its largest - low) / 15 in f32, rounded up,      both in `format`, and
+ *   codes (x - low) / step in f32, to the nearest of 0 .. 15 (ties to even),
+ * for the values low + code * step, each within half a step of its element. A group that holds an infinity or a NaN (or spans
+ * more than f32 does) is NaN as a whole. Element e of a row lies in byte e / 2 of its codes, an even one in the low half;
+ * group g's pair is word g of its steps, step in the low half. head_dim is a multiple of 8 up to 256. Attention and pages_copy
+ * read these and nothing else, so a cache may be filled by other means too. Rows of codes begin on 4 bytes; on 16, with
+ * head_dim 64 or 128, they take the matrix kernels. Rows of one head that lie one behind the other in a page ([pages, kv_heads,
+ * page_size, ...]) make the widest reads. */
+typedef struct wb200_quantized_rows {
+  void *codes, *steps;
+  int64_t codes_page_stride, codes_row_stride, codes_head_stride;   /* in bytes */
+  int64_t steps_page_stride, steps_row_stride, steps_head_stride;   /* in pairs */
+} wb200_quantized_rows;
+typedef struct wb200_quantized_cache {
+  uint32_t pages, page_size, kv_heads, head_dim;
+  uint32_t format;          /* WB200_BF16 or WB200_F16: of steps, queries, rows written and read */
+  uint32_t bits;            /* 4 */
+  wb200_quantized_rows k, v;
+} wb200_quantized_cache;
+/* wb200_rope_append with the K and V rows quantised as they are written. K is turned in f64 and rounded to f32 and to `format`,
+ * so that its codes are those of the definition but for angles' last bits. */
+wb200_status wb200_rope_append_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                         const wb200_rope_append_params *params);
+/* wb200_cache_read: the values low + code * step, rounded to `format`. */
+wb200_status wb200_cache_read_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                        const wb200_cache_read_params *params);
+/* wb200_attention_paged over the values low + code * step. */
+uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache,
+                                                   const wb200_paged_batch *batch, const wb200_attention_paged_params *params);
+wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                       const wb200_attention_paged_params *params);
+/* wb200_pages_copy of codes and steps. */
+wb200_status wb200_pages_copy_quantized(wb200_backend *backend, const wb200_quantized_cache *caches, uint32_t cache_count, uint32_t count,
+                                        const int32_t *sources, const int32_t *destinations, void *stream);
+
 /* The pages of a cache are kept in three arrays: page table, tokens held by each sequence, and how many sequences hold each
  * page (0: free). The four calls below take them and write them to the *_out arrays, each of which may be the input itself;
  * table entries behind a sequence's pages keep their value unless said otherwise. Every result is one the order of threads

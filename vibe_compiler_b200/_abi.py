@@ -157,6 +157,22 @@ class PagedCacheDesc(C.Structure):
                 ("v_page_stride", C.c_int64), ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64)]
 
 
+class QuantizedRows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("steps", C.c_void_p),
+                ("codes_page_stride", C.c_int64), ("codes_row_stride", C.c_int64), ("codes_head_stride", C.c_int64),
+                ("steps_page_stride", C.c_int64), ("steps_row_stride", C.c_int64), ("steps_head_stride", C.c_int64)]
+
+
+class QuantizedCacheDesc(C.Structure):
+    _fields_ = [("pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("format", C.c_uint32), ("bits", C.c_uint32), ("k", QuantizedRows), ("v", QuantizedRows)]
+
+
+class CacheReadParams(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("stream", C.c_void_p)]
+
+
 class PagedBatchDesc(C.Structure):
     _fields_ = [("sequences", C.c_uint32), ("table_width", C.c_uint32), ("tokens", C.c_uint32), ("max_query", C.c_uint32),
                 ("page_table", C.c_void_p), ("key_lengths", C.c_void_p), ("query_starts", C.c_void_p), ("table_stride", C.c_int64)]
@@ -247,6 +263,12 @@ SIGNATURES = {
     "wb200_rope_append": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(RopeAppendParams)]),
     "wb200_attention_paged_workspace_bytes": (C.c_uint64, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
     "wb200_attention_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
+    "wb200_cache_read": (C.c_int, [C.c_void_p, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(CacheReadParams)]),
+    "wb200_rope_append_quantized": (C.c_int, [C.c_void_p, C.POINTER(QuantizedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(RopeAppendParams)]),
+    "wb200_cache_read_quantized": (C.c_int, [C.c_void_p, C.POINTER(QuantizedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(CacheReadParams)]),
+    "wb200_attention_quantized_workspace_bytes": (C.c_uint64, [C.c_void_p, C.POINTER(QuantizedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
+    "wb200_attention_quantized": (C.c_int, [C.c_void_p, C.POINTER(QuantizedCacheDesc), C.POINTER(PagedBatchDesc), C.POINTER(AttentionPagedParams)]),
+    "wb200_pages_copy_quantized": (C.c_int, [C.c_void_p, C.POINTER(QuantizedCacheDesc), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "wb200_pages_reserve": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_void_p, C.c_void_p]),
     "wb200_pages_fork": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_uint32] + [C.c_void_p] * 5),
     "wb200_pages_free": (C.c_int, [C.c_void_p, C.POINTER(PageTablesDesc), C.c_uint32, C.c_void_p]),

@@ -40,9 +40,11 @@ _GEMM_PACK = struct.Struct("=3I6B6x5Q").pack
 _ROPE_PACK = struct.Struct("=3I4BIfQ3Q4qQ").pack
 _APPEND_PACK = struct.Struct("=IBBxxIfQ3Q3qQ").pack
 _PAGED_PACK = struct.Struct("=IBBxxfI3Q4q3Q").pack
+_READ_PACK = struct.Struct("=2Q4qQ").pack
 _TABLES_PACK = struct.Struct("=4I6Q2qQ").pack
 assert len(_ATTENTION_PACK(*[0] * 24)) == C.sizeof(abi.AttentionParams) and len(_GEMM_PACK(*[0] * 14)) == C.sizeof(abi.GemmEpilogueParams)
 assert len(_ROPE_PACK(*[0] * 18)) == C.sizeof(abi.RopeParams) and len(_APPEND_PACK(*[0] * 13)) == C.sizeof(abi.RopeAppendParams)
+assert len(_READ_PACK(*[0] * 7)) == C.sizeof(abi.CacheReadParams)
 assert len(_PAGED_PACK(*[0] * 15)) == C.sizeof(abi.AttentionPagedParams) and len(_TABLES_PACK(*[0] * 13)) == C.sizeof(abi.PageTablesDesc)
 
 
@@ -599,11 +601,11 @@ class B200TargetModelBackend:
                     stream: Optional[int] = None):
         """Rows [q heads | k heads | v heads] of the fused projection, qkv [tokens, (q_heads + 2 kv_heads) head_dim]: returns
         the rotated queries [tokens, q_heads, head_dim] and stores the rotated K and the V rows to their sequences' pages of
-        `cache` (a paged_cache.PagedCache). `batch`: a paged_cache.PagedBatch whose pages are reserved. `table` None rotates
-        nothing. `positions` replace the cache positions in the rotation. Rows of tokens that belong to no sequence are not
+        `cache` (a paged_cache.PagedCache, or a QuantizedCache, for which they are quantised on the way). `batch`: a
+        paged_cache.PagedBatch whose pages are reserved. `table` None rotates nothing. `positions` replace the cache positions in the rotation. Rows of tokens that belong to no sequence are not
         written."""
-        device, dtype = self.device, cache.k.dtype
-        _, _, kv_heads, head_dim = cache.k.shape
+        device, dtype = self.device, cache.dtype
+        _, _, kv_heads, head_dim = cache.shape
         if cache.device_index != device or batch.device_index != device or qkv.get_device() != device:
             raise ValueError("qkv, the cache and the batch must be on the backend's device")
         if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.dtype != dtype or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
@@ -623,19 +625,48 @@ class B200TargetModelBackend:
             table.rotary_dim if table is not None else 0, table.magnitude if table is not None else 1.0,
             table._address if table is not None else 0, positions.data_ptr() if positions is not None else 0, qkv.data_ptr(), out.data_ptr(),
             qkv.stride(0), strides[0], strides[1], stream))
-        self._check(self._lib.wb200_rope_append(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
+        call = self._lib.wb200_rope_append_quantized if cache.quantized else self._lib.wb200_rope_append
+        self._check(call(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
+        return out
+
+    def cache_read(self, cache, batch, tokens: int, *, out=None, stream: Optional[int] = None):
+        """K and V rows of the `tokens` tokens of `batch` as they stand in the pages of `cache` (a paged_cache.PagedCache or
+        QuantizedCache): two [tokens, kv_heads, head_dim] tensors of the cache's type, what `rope_append` of the same batch wrote.
+        Sequence s gives its last query_starts[s + 1] - query_starts[s] rows, so query_starts that count up the key lengths read
+        sequences whole. `out`: (k, v) to write. Rows of tokens that belong to no sequence are not written."""
+        device = self.device
+        if cache.device_index != device or batch.device_index != device:
+            raise ValueError("the cache and the batch must be on the backend's device")
+        if tokens < 0:
+            raise ValueError("tokens must not be negative")
+        shape, dtype = (tokens, *cache.shape[2:]), cache.dtype
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(device)
+        if out is None:
+            like = batch.key_lengths
+            out = self._empty(like, shape, stream, dtype), self._empty(like, shape, stream, dtype)
+        else:
+            out = tuple(out)
+            if len(out) != 2:
+                raise ValueError("out must be a pair (k, v)")
+            self._check_rows("out[0]", out[0], shape, dtype)
+            self._check_rows("out[1]", out[1], shape, dtype)
+        k, v = out
+        p = abi.CacheReadParams.from_buffer_copy(_READ_PACK(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], stream))
+        call = self._lib.wb200_cache_read_quantized if cache.quantized else self._lib.wb200_cache_read
+        self._check(call(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
         return out
 
     def attention_paged(self, q, cache, batch, scale: float, *, causal: bool = True, zero_fully_masked: bool = False, out=None,
                         lse=None, stream: Optional[int] = None):
-        """Attention of every sequence's new tokens, q [tokens, q_heads, head_dim], over its keys in the pages of `cache`
-        (grouped queries; with `causal` up to the token's own position). `lse` [tokens, q_heads] f32 receives the
+        """Attention of every sequence's new tokens, q [tokens, q_heads, head_dim], over its keys in the pages of `cache` (a
+        paged_cache.PagedCache or QuantizedCache; grouped queries; with `causal` up to the token's own position). `lse` [tokens, q_heads] f32 receives the
         log-sum-exp. Rows of tokens that belong to no sequence are not written. Scratch memory comes from torch's allocator,
         per call and stream, so calls may overlap and be captured into CUDA graphs."""
-        device, dtype, shape = self.device, cache.k.dtype, q.shape
+        device, dtype, shape = self.device, cache.dtype, q.shape
         if cache.device_index != device or batch.device_index != device:
             raise ValueError("the cache and the batch must be on the backend's device")
-        if len(shape) != 3 or shape[2] != cache.k.shape[3]:
+        if len(shape) != 3 or shape[2] != cache.shape[3]:
             raise ValueError("q must be [tokens, q_heads, head_dim] with the cache's head dimension")
         self._check_rows("q", q, shape, dtype)
         if stream is None:
@@ -651,10 +682,12 @@ class B200TargetModelBackend:
             shape[1], bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
             lse.data_ptr() if lse is not None else 0, q_strides[0], q_strides[1], out_strides[0], out_strides[1], 0, 0, stream))
         if self._paged_workspace is None:
-            self._paged_workspace = int(self._lib.wb200_attention_paged_workspace_bytes(self._handle, None, None, None))
+            self._paged_workspace = max(int(query(self._handle, None, None, None)) for query in
+                                        (self._lib.wb200_attention_paged_workspace_bytes, self._lib.wb200_attention_quantized_workspace_bytes))
         workspace = self._empty(q, self._paged_workspace, stream, torch.uint8)
         p.workspace, p.workspace_bytes = workspace.data_ptr(), self._paged_workspace
-        self._check(self._lib.wb200_attention_paged(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
+        call = self._lib.wb200_attention_quantized if cache.quantized else self._lib.wb200_attention_paged
+        self._check(call(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
         return out
 
     def _page_tables(self, table, lengths, refs, page_size, out, stream, with_lengths=True):
@@ -730,7 +763,7 @@ class B200TargetModelBackend:
         return (*out, sources, destinations)
 
     def pages_copy(self, caches, sources, destinations, *, stream: Optional[int] = None) -> None:
-        """Whole pages of every cache (a PagedCache or a sequence of them with one shape, strides and type): K and V of page
+        """Whole pages of every cache (a PagedCache or a QuantizedCache, or a sequence of one kind with one shape, strides and type): K and V of page
         sources[i] to page destinations[i]; negative entries are passed over. No page may be a destination twice, or both a
         source and a destination."""
         caches = (caches,) if hasattr(caches, "_desc") else caches
@@ -739,8 +772,12 @@ class B200TargetModelBackend:
         self._check_indices("destinations", destinations, sources.shape[0])
         if any([c.device_index != self.device for c in caches]):
             raise ValueError("the caches must be on the backend's device")
-        descs = (abi.PagedCacheDesc * len(caches))(*[c._desc for c in caches])
-        self._check(self._lib.wb200_pages_copy(self._handle, descs, len(caches), sources.shape[0], sources.data_ptr(), destinations.data_ptr(), stream))
+        quantized = len(caches) > 0 and caches[0].quantized
+        if any([c.quantized != quantized for c in caches]):
+            raise ValueError("the caches of one copy must be of one kind")
+        descs = ((abi.QuantizedCacheDesc if quantized else abi.PagedCacheDesc) * len(caches))(*[c._desc for c in caches])
+        call = self._lib.wb200_pages_copy_quantized if quantized else self._lib.wb200_pages_copy
+        self._check(call(self._handle, descs, len(caches), sources.shape[0], sources.data_ptr(), destinations.data_ptr(), stream))
 
     def decoder_layer(self, x, *, norm1, wqkv, wo, norm2, wgu, wdown, q_heads: int, kv_heads: int, head_dim: int, eps: float,
                       rope_theta: float, position_offset: int = 0, allreduce=None, workspace=None, out=None,

@@ -71,6 +71,36 @@ wb200_status make_cache(const wb200_paged_cache *c, bool f32_too, PagedCacheArgs
   return WB200_OK;
 }
 
+// A cache held in four bits: its extents and where its rows lie.
+wb200_status make_quantized(const wb200_quantized_cache *c, PagedCacheArgs *a, QuantizedRowsArgs *rows) {
+  if (c->format != WB200_BF16 && c->format != WB200_F16) return fail(WB200_ERR_UNSUPPORTED, "a quantized cache stands for bf16 or f16");
+  if (c->bits != 4) return fail(WB200_ERR_UNSUPPORTED, "a quantized cache holds codes of 4 bits");
+  if (c->pages == 0 || c->page_size == 0 || c->kv_heads == 0 || c->head_dim == 0)
+    return fail(WB200_ERR_INVALID_ARGUMENT, "paged cache extents must be positive");
+  if (c->head_dim % 8 != 0 || c->head_dim > static_cast<uint32_t>(kQuantMaxHeadDim))
+    return fail(WB200_ERR_UNSUPPORTED, "a quantized cache takes head dimensions that are multiples of 8, up to 256");
+  if (c->pages > 0x7fffffffu || c->page_size > 0x7fffffffu || c->kv_heads > 0xffffu) return fail(WB200_ERR_LIMIT, "paged cache extents too large");
+  *a = PagedCacheArgs{};
+  a->pages = static_cast<int>(c->pages); a->page_size = static_cast<int>(c->page_size);
+  a->kv_heads = static_cast<int>(c->kv_heads); a->head_dim = static_cast<int>(c->head_dim); a->format = static_cast<int>(c->format);
+  const int64_t extent[3] = {c->pages, c->page_size, c->kv_heads};
+  const int64_t groups = (c->head_dim + kQuantGroup - 1) / kQuantGroup;
+  const wb200_quantized_rows *from[2] = {&c->k, &c->v};
+  QuantizedRows *to[2] = {&rows->k, &rows->v};
+  for (int i = 0; i < 2; ++i) {
+    const wb200_quantized_rows &r = *from[i];
+    if (!r.codes || !r.steps) return fail(WB200_ERR_INVALID_ARGUMENT, "codes and steps of the quantized cache must not be null");
+    if (!on_elements(4, r.codes, r.steps) || ((r.codes_page_stride | r.codes_row_stride | r.codes_head_stride) & 3) != 0)
+      return fail(WB200_ERR_INVALID_ARGUMENT, "rows of codes and pairs of steps must begin on 4 bytes");
+    if (!rows_apart(c->head_dim / 2, {r.codes_page_stride, r.codes_row_stride, r.codes_head_stride}, extent) ||
+        !rows_apart(groups, {r.steps_page_stride, r.steps_row_stride, r.steps_head_stride}, extent))
+      return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the quantized cache overlap");
+    *to[i] = {static_cast<uint8_t *>(r.codes), static_cast<uint32_t *>(r.steps), r.codes_page_stride, r.codes_row_stride, r.codes_head_stride,
+              r.steps_page_stride, r.steps_row_stride, r.steps_head_stride};
+  }
+  return WB200_OK;
+}
+
 wb200_status make_batch(const wb200_paged_batch *b, const PagedCacheArgs &c, PagedBatchArgs *a) {
   if (b->sequences > 0x7ffffffeu || b->tokens > 0x7fffffffu || b->table_width > 0x7fffffffu || b->max_query > 0x7fffffffu)
     return fail(WB200_ERR_LIMIT, "paged batch extents too large");
@@ -94,14 +124,13 @@ bool output_rows_apart(int64_t head_dim, int64_t token_stride, int64_t head_stri
   return rows_apart(head_dim, {token_stride, head_stride, 1}, {tokens, heads, 1});
 }
 
-wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
-                                  const wb200_attention_paged_params *p, AttentionPagedArgs *a) {
-  wb200_status st = make_cache(cache, false, &a->cache);
+// `a->cache` is made already.
+wb200_status make_attention(wb200_backend *backend, const wb200_paged_batch *batch, const wb200_attention_paged_params *p, AttentionPagedArgs *a) {
+  wb200_status st = make_batch(batch, a->cache, &a->batch);
   if (st != WB200_OK) return st;
-  if ((st = make_batch(batch, a->cache, &a->batch)) != WB200_OK) return st;
-  if (p->q_heads == 0 || p->q_heads > 0xffffu || p->q_heads % cache->kv_heads != 0)
+  if (p->q_heads == 0 || p->q_heads > 0xffffu || p->q_heads % static_cast<uint32_t>(a->cache.kv_heads) != 0)
     return fail(WB200_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
-  if (cache->head_dim % 8 != 0 || cache->head_dim > 256) return fail(WB200_ERR_UNSUPPORTED, "paged attention takes head dimensions that are multiples of 8, up to 256");
+  if (a->cache.head_dim % 8 != 0 || a->cache.head_dim > 256) return fail(WB200_ERR_UNSUPPORTED, "paged attention takes head dimensions that are multiples of 8, up to 256");
   if (static_cast<uint64_t>(batch->tokens) * p->q_heads > 0x7fffffffull) return fail(WB200_ERR_LIMIT, "more than 2^31 - 1 rows in one paged attention");
   if (!(p->scale > 0.f) || !(p->scale <= 1e38f)) return fail(WB200_ERR_INVALID_ARGUMENT, "scale must be positive and at most 1e38");
   a->q_heads = static_cast<int>(p->q_heads);
@@ -114,6 +143,17 @@ wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cach
   a->refused = backend ? backend->d_status + 2 : nullptr;
   a->status = backend ? backend->d_status : nullptr;
   return WB200_OK;
+}
+
+wb200_status make_attention_paged(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
+                                  const wb200_attention_paged_params *p, AttentionPagedArgs *a) {
+  const wb200_status st = make_cache(cache, false, &a->cache);
+  return st != WB200_OK ? st : make_attention(backend, batch, p, a);
+}
+wb200_status make_attention_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                      const wb200_attention_paged_params *p, AttentionPagedArgs *a, QuantizedRowsArgs *rows) {
+  const wb200_status st = make_quantized(cache, &a->cache, rows);
+  return st != WB200_OK ? st : make_attention(backend, batch, p, a);
 }
 
 // Which kernel a call takes, from what the host knows: sizes, alignment and the caller's word on the longest chunk. Any choice
@@ -156,6 +196,71 @@ wb200_status make_page_tables(wb200_backend *backend, const wb200_page_tables *t
   return WB200_OK;
 }
 
+// The append onto either kind of cache, whose extents are in `c`; `rows` null: the 16-bit one.
+wb200_status rope_append(wb200_backend *backend, const PagedCacheArgs &c, const QuantizedRowsArgs *rows, const wb200_paged_batch *batch,
+                         const wb200_rope_append_params *p) {
+  PagedBatchArgs b;
+  RotaryConstants constants;
+  wb200_status st = make_batch(batch, c, &b);
+  if (st != WB200_OK) return st;
+  const uint32_t kv_heads = static_cast<uint32_t>(c.kv_heads), head_dim = static_cast<uint32_t>(c.head_dim);
+  if ((st = make_rotary_constants(p->table, head_dim, &constants)) != WB200_OK) return st;
+  if (p->q_heads > 0xffffu || (static_cast<uint64_t>(p->q_heads) + 2ull * kv_heads) * head_dim > (1u << 24))
+    return fail(WB200_ERR_LIMIT, "rope extents too large");
+  if (p->positions && p->position_bytes != 4 && p->position_bytes != 8) return fail(WB200_ERR_INVALID_ARGUMENT, "positions are int32 or int64");
+  if (b.tokens == 0 || b.sequences == 0) return WB200_OK;
+  if (!p->qkv || (p->q_heads != 0 && !p->q)) return fail(WB200_ERR_INVALID_ARGUMENT, "qkv and q must not be null");
+  if (!on_elements(2, p->qkv, p->q) || (p->positions && !on_elements(p->position_bytes, p->positions))) return off_elements();
+  if (p->q_heads != 0 && !output_rows_apart(head_dim, p->q_token_stride, p->q_head_stride, b.tokens, p->q_heads))
+    return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
+  RopeArgs a{};
+  a.tokens = b.tokens; a.heads = static_cast<int>(p->q_heads) + 2 * c.kv_heads; a.head_dim = c.head_dim; a.format = c.format;
+  a.interleaved = p->interleaved ? 1 : 0; a.position_bytes = p->position_bytes;
+  a.positions = p->positions; a.x = p->qkv; a.out = p->q;
+  a.x_token = p->qkv_token_stride; a.x_head = c.head_dim; a.out_token = p->q_token_stride; a.out_head = p->q_head_stride;
+  DeviceGuard guard(backend->device);
+  const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+  st = rows ? launch_rope_append_quantized(a, constants, c, *rows, b, backend->d_status + 2, stream)
+            : launch_rope_append(a, constants, c, b, backend->d_status + 2, stream);
+  if (st == WB200_OK) backend->launches += 1;
+  return st;
+}
+
+wb200_status cache_read(wb200_backend *backend, const PagedCacheArgs &c, const QuantizedRowsArgs *rows, const wb200_paged_batch *batch,
+                        const wb200_cache_read_params *p) {
+  PagedBatchArgs b;
+  wb200_status st = make_batch(batch, c, &b);
+  if (st != WB200_OK) return st;
+  if (static_cast<uint64_t>(c.kv_heads) * static_cast<uint64_t>(c.head_dim) > (1u << 23)) return fail(WB200_ERR_LIMIT, "rows of one token too large");
+  if (b.tokens == 0 || b.sequences == 0) return WB200_OK;
+  if (!p->k || !p->v) return fail(WB200_ERR_INVALID_ARGUMENT, "k and v must not be null");
+  if (!on_elements(2, p->k, p->v)) return off_elements();
+  if (!output_rows_apart(c.head_dim, p->k_token_stride, p->k_head_stride, b.tokens, c.kv_heads) ||
+      !output_rows_apart(c.head_dim, p->v_token_stride, p->v_head_stride, b.tokens, c.kv_heads))
+    return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
+  DeviceGuard guard(backend->device);
+  st = launch_cache_read({p->k, p->v, p->k_token_stride, p->k_head_stride, p->v_token_stride, p->v_head_stride}, c, rows, b, backend->d_status + 2,
+                         static_cast<cudaStream_t>(p->stream));
+  if (st == WB200_OK) backend->launches += 1;
+  return st;
+}
+
+// What attention needs beside its sizes, checked before any kernel is chosen; `done`: there is nothing to do.
+wb200_status check_attention_buffers(const AttentionPagedArgs &a, bool *done) {
+  *done = a.batch.tokens == 0 || a.batch.sequences == 0;
+  if (*done) return WB200_OK;
+  if (!a.q || !a.out) return fail(WB200_ERR_INVALID_ARGUMENT, "q and out must not be null");
+  if (!on_elements(2, a.q, a.out) || !on_elements(4, a.lse)) return off_elements();
+  if (!output_rows_apart(a.cache.head_dim, a.out_token, a.out_head, a.batch.tokens, a.q_heads))
+    return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
+  return WB200_OK;
+}
+wb200_status check_workspace(const wb200_attention_paged_params *p, uint64_t needed, const char *query) {
+  if (needed > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < needed))
+    return fail(WB200_ERR_INVALID_ARGUMENT, std::string("the workspace must be 256-byte aligned and hold ") + query + "() bytes");
+  return WB200_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -192,29 +297,33 @@ wb200_status wb200_rope_append(wb200_backend *backend, const wb200_paged_cache *
                                const wb200_rope_append_params *p) {
   if (!backend || !cache || !batch || !p) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
   PagedCacheArgs c;
-  PagedBatchArgs b;
-  RotaryConstants constants;
-  wb200_status st = make_cache(cache, false, &c);
-  if (st != WB200_OK) return st;
-  if ((st = make_batch(batch, c, &b)) != WB200_OK) return st;
-  if ((st = make_rotary_constants(p->table, cache->head_dim, &constants)) != WB200_OK) return st;
-  if (p->q_heads > 0xffffu || (static_cast<uint64_t>(p->q_heads) + 2ull * cache->kv_heads) * cache->head_dim > (1u << 24))
-    return fail(WB200_ERR_LIMIT, "rope extents too large");
-  if (p->positions && p->position_bytes != 4 && p->position_bytes != 8) return fail(WB200_ERR_INVALID_ARGUMENT, "positions are int32 or int64");
-  if (b.tokens == 0 || b.sequences == 0) return WB200_OK;
-  if (!p->qkv || (p->q_heads != 0 && !p->q)) return fail(WB200_ERR_INVALID_ARGUMENT, "qkv and q must not be null");
-  if (!on_elements(2, p->qkv, p->q) || (p->positions && !on_elements(p->position_bytes, p->positions))) return off_elements();
-  if (p->q_heads != 0 && !output_rows_apart(cache->head_dim, p->q_token_stride, p->q_head_stride, b.tokens, p->q_heads))
-    return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
-  RopeArgs a{};
-  a.tokens = b.tokens; a.heads = static_cast<int>(p->q_heads) + 2 * c.kv_heads; a.head_dim = c.head_dim; a.format = c.format;
-  a.interleaved = p->interleaved ? 1 : 0; a.position_bytes = p->position_bytes;
-  a.positions = p->positions; a.x = p->qkv; a.out = p->q;
-  a.x_token = p->qkv_token_stride; a.x_head = c.head_dim; a.out_token = p->q_token_stride; a.out_head = p->q_head_stride;
-  DeviceGuard guard(backend->device);
-  st = launch_rope_append(a, constants, c, b, backend->d_status + 2, static_cast<cudaStream_t>(p->stream));
-  if (st == WB200_OK) backend->launches += 1;
-  return st;
+  const wb200_status st = make_cache(cache, false, &c);
+  return st != WB200_OK ? st : rope_append(backend, c, nullptr, batch, p);
+}
+
+wb200_status wb200_rope_append_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                         const wb200_rope_append_params *p) {
+  if (!backend || !cache || !batch || !p) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
+  PagedCacheArgs c;
+  QuantizedRowsArgs rows;
+  const wb200_status st = make_quantized(cache, &c, &rows);
+  return st != WB200_OK ? st : rope_append(backend, c, &rows, batch, p);
+}
+
+wb200_status wb200_cache_read(wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch, const wb200_cache_read_params *p) {
+  if (!backend || !cache || !batch || !p) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
+  PagedCacheArgs c;
+  const wb200_status st = make_cache(cache, false, &c);
+  return st != WB200_OK ? st : cache_read(backend, c, nullptr, batch, p);
+}
+
+wb200_status wb200_cache_read_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                        const wb200_cache_read_params *p) {
+  if (!backend || !cache || !batch || !p) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
+  PagedCacheArgs c;
+  QuantizedRowsArgs rows;
+  const wb200_status st = make_quantized(cache, &c, &rows);
+  return st != WB200_OK ? st : cache_read(backend, c, &rows, batch, p);
 }
 
 uint64_t wb200_attention_paged_workspace_bytes(const wb200_backend *backend, const wb200_paged_cache *cache, const wb200_paged_batch *batch,
@@ -236,15 +345,10 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   AttentionPagedArgs a{};
   wb200_status st = make_attention_paged(backend, cache, batch, p, &a);
   if (st != WB200_OK) return st;
-  if (a.batch.tokens == 0 || a.batch.sequences == 0) return WB200_OK;
-  if (!a.q || !a.out) return fail(WB200_ERR_INVALID_ARGUMENT, "q and out must not be null");
-  if (!on_elements(2, a.q, a.out) || !on_elements(4, a.lse)) return off_elements();
-  if (!output_rows_apart(a.cache.head_dim, a.out_token, a.out_head, a.batch.tokens, a.q_heads))
-    return fail(WB200_ERR_INVALID_ARGUMENT, "rows of the output overlap");
+  bool done;
+  if ((st = check_attention_buffers(a, &done)) != WB200_OK || done) return st;
   const PagedKernel kernel = choose_attention_paged(a);
-  const uint64_t workspace = attention_paged_workspace(kernel, backend->sm_count);
-  if (workspace > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < workspace))
-    return fail(WB200_ERR_INVALID_ARGUMENT, "the workspace must be 256-byte aligned and hold wb200_attention_paged_workspace_bytes() bytes");
+  if ((st = check_workspace(p, attention_paged_workspace(kernel, backend->sm_count), "wb200_attention_paged_workspace_bytes")) != WB200_OK) return st;
   DeviceGuard guard(backend->device);
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   if (kernel == PagedKernel::general) st = launch_attention_paged_general(a, stream);
@@ -252,6 +356,28 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
   else st = launch_attention_paged_chunk(a, backend->sm_count, stream);
   const bool one = kernel == PagedKernel::general || (kernel == PagedKernel::rows && attention_paged_rows_clustered(a, backend->sm_count));
   if (st == WB200_OK) backend->launches += one ? 1 : 2;
+  return st;
+}
+
+uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                                   const wb200_attention_paged_params *p) {
+  if (!backend || ((cache || batch || p) && !(cache && batch && p))) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
+  return 0;
+}
+
+wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
+                                       const wb200_attention_paged_params *p) {
+  if (!backend || !cache || !batch || !p) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
+  AttentionPagedArgs a{};
+  QuantizedRowsArgs rows;
+  wb200_status st = make_attention_quantized(backend, cache, batch, p, &a, &rows);
+  if (st != WB200_OK) return st;
+  bool done;
+  if ((st = check_attention_buffers(a, &done)) != WB200_OK || done) return st;
+  DeviceGuard guard(backend->device);
+  const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+  st = launch_attention_quantized_general(a, rows, stream);
+  if (st == WB200_OK) backend->launches += 1;
   return st;
 }
 
@@ -302,6 +428,52 @@ wb200_status wb200_pages_compact(wb200_backend *backend, const wb200_page_tables
   DeviceGuard guard(backend->device);
   if ((st = launch_pages_compact(a, sources, destinations, static_cast<cudaStream_t>(tables->stream))) == WB200_OK) backend->launches += 1;
   return st;
+}
+
+// A quantized cache moves as two caches of words, its codes and its steps.
+wb200_status wb200_pages_copy_quantized(wb200_backend *backend, const wb200_quantized_cache *caches, uint32_t cache_count, uint32_t count,
+                                        const int32_t *sources, const int32_t *destinations, void *stream) {
+  if (!backend || (cache_count != 0 && !caches)) return fail(WB200_ERR_INVALID_ARGUMENT, "null argument");
+  if (count > 0x7fffffffu) return fail(WB200_ERR_LIMIT, "more than 2^31 - 1 pages to copy");
+  for (uint32_t i = 0; i < cache_count; ++i) {
+    PagedCacheArgs one;
+    QuantizedRowsArgs rows;
+    const wb200_status st = make_quantized(caches + i, &one, &rows);
+    if (st != WB200_OK) return st;
+    wb200_quantized_cache like = caches[i];
+    like.k.codes = caches[0].k.codes; like.k.steps = caches[0].k.steps;
+    like.v.codes = caches[0].v.codes; like.v.steps = caches[0].v.steps;
+    if (memcmp(&like, &caches[0], sizeof(like)) != 0)
+      return fail(WB200_ERR_INVALID_ARGUMENT, "the caches of one copy must have the same extents, strides and format");
+  }
+  if (cache_count == 0 || count == 0) return WB200_OK;
+  if (!sources || !destinations) return fail(WB200_ERR_INVALID_ARGUMENT, "sources and destinations must not be null");
+  if (!on_elements(4, sources, destinations)) return off_elements();
+  DeviceGuard guard(backend->device);
+  for (int steps = 0; steps < 2; ++steps) {
+    for (uint32_t first = 0; first < cache_count; first += kMaxCachesPerCopy) {
+      PagedCacheArgs part[kMaxCachesPerCopy];
+      const uint32_t n = cache_count - first < kMaxCachesPerCopy ? cache_count - first : kMaxCachesPerCopy;
+      for (uint32_t i = 0; i < n; ++i) {
+        QuantizedRowsArgs rows;
+        make_quantized(caches + first + i, part + i, &rows);
+        PagedCacheArgs &c = part[i];
+        c.format = WB200_F32;                                // words
+        c.head_dim = steps ? (c.head_dim + kQuantGroup - 1) / kQuantGroup : c.head_dim / 8;
+        c.k = steps ? static_cast<void *>(rows.k.steps) : rows.k.codes;
+        c.v = steps ? static_cast<void *>(rows.v.steps) : rows.v.codes;
+        const int64_t k[3] = {rows.k.codes_page, rows.k.codes_row, rows.k.codes_head}, v[3] = {rows.v.codes_page, rows.v.codes_row, rows.v.codes_head};
+        const int64_t ks[3] = {rows.k.steps_page, rows.k.steps_row, rows.k.steps_head}, vs[3] = {rows.v.steps_page, rows.v.steps_row, rows.v.steps_head};
+        c.k_page = steps ? ks[0] : k[0] / 4; c.k_row = steps ? ks[1] : k[1] / 4; c.k_head = steps ? ks[2] : k[2] / 4;
+        c.v_page = steps ? vs[0] : v[0] / 4; c.v_row = steps ? vs[1] : v[1] / 4; c.v_head = steps ? vs[2] : v[2] / 4;
+      }
+      const wb200_status st = launch_pages_copy(part, static_cast<int>(n), static_cast<int>(count), sources, destinations, backend->d_status + 2,
+                                                static_cast<cudaStream_t>(stream));
+      if (st != WB200_OK) return st;
+      backend->launches += 1;
+    }
+  }
+  return WB200_OK;
 }
 
 wb200_status wb200_pages_copy(wb200_backend *backend, const wb200_paged_cache *caches, uint32_t cache_count, uint32_t count,

@@ -1,7 +1,9 @@
 // Attention over a paged KV cache, the general kernel: any head dimension that is a multiple of 8, up to 256, any page size and
 // any strides. A warp takes one row (token, query head) and walks its keys 32 at a time: a lane scores one key, the warp
-// carries the running maximum and sum in f32, and every lane accumulates eight elements of the row.
+// carries the running maximum and sum in f32, and every lane accumulates eight elements of the row. Rows held in four bits are
+// widened where a 16-bit row is, eight elements of a word at a time.
 #include "attention_paged.cuh"
+#include "quantized_rows.cuh"
 
 namespace wb200 {
 namespace {
@@ -22,8 +24,26 @@ __device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
   for (int i = 0; i < 4; ++i) { v[2 * i] = widen_bits(w[i] & 0xffffu, kFormat); v[2 * i + 1] = widen_bits(w[i] >> 16, kFormat); }
 }
 
+// Where a key's row of K or V lies, 16-bit or quantised, and eight elements of it.
 template <int kFormat, bool kWide>
-__global__ void __launch_bounds__(kRows * 32) attention_paged_general_kernel(const __grid_constant__ AttentionPagedArgs a) {
+struct PlainRow {
+  const uint16_t *p;
+  __device__ __forceinline__ void load(int c, float (&v)[8]) const { load8<kFormat, kWide>(p + c, v); }
+};
+template <int kFormat>
+struct QuantizedRow {
+  const uint8_t *codes;
+  const uint32_t *steps;
+  __device__ __forceinline__ void load(int c, float (&v)[8]) const {
+    const uint32_t word = *reinterpret_cast<const uint32_t *>(codes + c / 2), pair = steps[c / kQuantGroup];
+    const float step = quant_step(pair, kFormat), low = quant_low(pair, kFormat);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = quant_value(word, i, step, low);
+  }
+};
+
+template <int kFormat, bool kWide, bool kQuantized>
+__global__ void __launch_bounds__(kRows * 32) attention_paged_general_kernel(const __grid_constant__ AttentionPagedArgs a, const __grid_constant__ QuantizedRowsArgs rows) {
   __shared__ float q_rows[kRows][kMaxHeadDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp;
@@ -48,26 +68,37 @@ __global__ void __launch_bounds__(kRows * 32) attention_paged_general_kernel(con
   __syncwarp();
   const float scale_log2 = a.scale * 1.4426950408889634f;
   const int *pages = a.batch.page_table + s * a.batch.table_stride;
-  const uint16_t *k = static_cast<const uint16_t *>(a.cache.k) + kv_head * a.cache.k_head;
-  const uint16_t *v = static_cast<const uint16_t *>(a.cache.v) + kv_head * a.cache.v_head;
+  auto row_at = [&](bool is_v, int page, int in_page) {
+    if constexpr (kQuantized) {
+      const QuantizedRows &r = is_v ? rows.v : rows.k;
+      return QuantizedRow<kFormat>{r.codes + page * r.codes_page + in_page * r.codes_row + kv_head * r.codes_head,
+                                   r.steps + page * r.steps_page + in_page * r.steps_row + kv_head * r.steps_head};
+    } else if (is_v) {
+      return PlainRow<kFormat, kWide>{static_cast<const uint16_t *>(a.cache.v) + page * a.cache.v_page + in_page * a.cache.v_row + kv_head * a.cache.v_head};
+    } else {
+      return PlainRow<kFormat, kWide>{static_cast<const uint16_t *>(a.cache.k) + page * a.cache.k_page + in_page * a.cache.k_row + kv_head * a.cache.k_head};
+    }
+  };
   float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
   for (int base = 0; base < visible; base += 32) {
     const int key = base + lane;
     float score = -INFINITY;
-    long long v_at = -1;
+    int page = -1, in_page = 0;
     if (key < visible) {
-      const int slot = key / a.cache.page_size, in_page = key - slot * a.cache.page_size, page = pages[slot];
+      const int slot = key / a.cache.page_size;
+      in_page = key - slot * a.cache.page_size;
+      page = pages[slot];
       if (page < 0 || page >= a.cache.pages) {
         raise_status(a.refused, kRefusedPage);
+        page = -1;
       } else {
-        const uint16_t *k_row = k + page * a.cache.k_page + in_page * a.cache.k_row;
-        v_at = page * a.cache.v_page + in_page * a.cache.v_row;
+        const auto k_row = row_at(false, page, in_page);
         float sum = 0.f;
         for (int c = 0; c < d; c += 8) {
           float x[8];
-          load8<kFormat, kWide>(k_row + c, x);
+          k_row.load(c, x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum = fmaf(x[e], q_rows[warp][c + e], sum);
         }
@@ -88,11 +119,11 @@ __global__ void __launch_bounds__(kRows * 32) attention_paged_general_kernel(con
     for (int e = 0; e < 8; ++e) acc[e] *= alpha;
     const int count = min(32, visible - base);
     for (int j = 0; j < count; ++j) {
-      const long long at = __shfl_sync(0xffffffffu, v_at, j);
+      const int v_page = __shfl_sync(0xffffffffu, page, j), v_row = __shfl_sync(0xffffffffu, in_page, j);
       const float weight = __shfl_sync(0xffffffffu, p, j);
-      if (at < 0 || 8 * lane >= d) continue;
+      if (v_page < 0 || 8 * lane >= d) continue;
       float x[8];
-      load8<kFormat, kWide>(v + at + 8 * lane, x);
+      row_at(true, v_page, v_row).load(8 * lane, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] = fmaf(weight, x[e], acc[e]);
     }
@@ -115,9 +146,16 @@ wb200_status launch_attention_paged_general(const AttentionPagedArgs &a, cudaStr
   const uint64_t bits = reinterpret_cast<uintptr_t>(a.cache.k) | reinterpret_cast<uintptr_t>(a.cache.v) |
                         static_cast<uint64_t>((a.cache.k_page | a.cache.k_row | a.cache.k_head | a.cache.v_page | a.cache.v_row | a.cache.v_head) * 2);
   const bool wide = (bits & 15u) == 0, bf16 = a.cache.format == WB200_BF16;
-  const auto kernel = wide ? (bf16 ? attention_paged_general_kernel<WB200_BF16, true> : attention_paged_general_kernel<WB200_F16, true>)
-                           : (bf16 ? attention_paged_general_kernel<WB200_BF16, false> : attention_paged_general_kernel<WB200_F16, false>);
-  WB200_CUDA_CHECK(launch_dependent(kernel, static_cast<unsigned>(blocks), kRows * 32, 0, stream, a));
+  const auto kernel = wide ? (bf16 ? attention_paged_general_kernel<WB200_BF16, true, false> : attention_paged_general_kernel<WB200_F16, true, false>)
+                           : (bf16 ? attention_paged_general_kernel<WB200_BF16, false, false> : attention_paged_general_kernel<WB200_F16, false, false>);
+  WB200_CUDA_CHECK(launch_dependent(kernel, static_cast<unsigned>(blocks), kRows * 32, 0, stream, a, QuantizedRowsArgs{}));
+  return WB200_OK;
+}
+
+wb200_status launch_attention_quantized_general(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows, cudaStream_t stream) {
+  const int64_t blocks = (static_cast<int64_t>(a.batch.tokens) * a.q_heads + kRows - 1) / kRows;
+  const auto kernel = a.cache.format == WB200_BF16 ? attention_paged_general_kernel<WB200_BF16, true, true> : attention_paged_general_kernel<WB200_F16, true, true>;
+  WB200_CUDA_CHECK(launch_dependent(kernel, static_cast<unsigned>(blocks), kRows * 32, 0, stream, a, rows));
   return WB200_OK;
 }
 

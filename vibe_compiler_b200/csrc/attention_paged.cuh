@@ -27,6 +27,43 @@ __device__ __forceinline__ int paged_visible(const PagedSequence &s, int index, 
   return last < 0 ? 0 : last;
 }
 
+// Where the rows of tokens [first, first + count) of a block lie: for each that belongs to a sequence whose lengths fit and whose page
+// is one of the cache's, place(index in the block, page, row of the page, position) is called by one thread, for the others nothing.
+// `sequence_of`: count words of shared memory. Ends with a barrier.
+template <typename Place>
+__device__ __forceinline__ void place_tokens(const PagedBatchArgs &b, const PagedCacheArgs &c, int first, int count, int *refused, int *sequence_of, Place place) {
+  // Every thread compares some sequences' token ranges with the block's tokens. A range that is not one of the rows' is reported
+  // whether or not a token of the block lies in it.
+  if (threadIdx.x < count) sequence_of[threadIdx.x] = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < b.sequences; s += blockDim.x) {
+    const int begin = b.query_starts[s], end = b.query_starts[s + 1];
+    if (begin < end && (begin < 0 || end > b.tokens)) {
+      raise_status(refused, kRefusedLength);
+      continue;
+    }
+    for (int t = max(begin, first); t < min(end, first + count); ++t) sequence_of[t - first] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x < count) {
+    const int s = sequence_of[threadIdx.x], token = first + static_cast<int>(threadIdx.x);
+    // What attention would leave out as a whole is not written here in part: its positions mean nothing.
+    const PagedSequence sequence = s >= 0 ? paged_sequence(b, c, s, refused, true) : PagedSequence{0, 0, 0};
+    if (sequence.count > 0) {
+      const int position = sequence.keys - sequence.count + (token - sequence.begin);      // less than keys, which the table holds
+      if (position < 0) {
+        raise_status(refused, kRefusedLength);
+      } else {
+        const int slot = position / c.page_size, row = position - slot * c.page_size;
+        const int page = b.page_table[s * b.table_stride + slot];
+        if (page < 0 || page >= c.pages) raise_status(refused, kRefusedPage);
+        else place(static_cast<int>(threadIdx.x), page, row, position);
+      }
+    }
+  }
+  __syncthreads();
+}
+
 // The first sequence from s on that brings tokens, or the number of sequences; by a whole warp, 32 sequences at a look.
 __device__ __forceinline__ int next_with_tokens(const PagedBatchArgs &b, int s) {
   const int lane = threadIdx.x & 31;

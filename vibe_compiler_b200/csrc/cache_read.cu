@@ -1,0 +1,125 @@
+// K and V rows of a batch's tokens out of the pages of a cache, as they stand there (wb200_cache_read*): the inverse of the append.
+// A row held in four bits is widened and rounded once to the cache's type.
+//
+// A thread keeps to its eight elements of the token's K and V heads and walks the block's tokens, four loads on their way together.
+// Bound: HBM, the rows read and the rows written.
+#include "attention_paged.cuh"
+#include "quantized_rows.cuh"
+
+namespace wb200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 16;
+constexpr int kAtOnce = 4;
+
+struct ReadParams {
+  CacheReadArgs a;
+  PagedCacheArgs cache;
+  QuantizedRowsArgs rows;
+  PagedBatchArgs batch;
+  int tokens_per_block;
+  int *refused;
+};
+
+// kWide: 16-byte accesses to every 16-bit row.
+template <int kFormat, bool kQuantized, bool kWide>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
+  __shared__ int page_of[kMaxTokens], row_of[kMaxTokens], sequence_of[kMaxTokens];
+  const int first = blockIdx.x * p.tokens_per_block, count = min(p.tokens_per_block, p.batch.tokens - first);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < kMaxTokens) page_of[threadIdx.x] = -1;
+  place_tokens(p.batch, p.cache, first, count, p.refused, sequence_of, [&](int t, int page, int row, int) {
+    page_of[t] = page;
+    row_of[t] = row;
+  });
+  const int chunks = (p.cache.head_dim + 7) / 8, items = 2 * p.cache.kv_heads * chunks;
+#pragma unroll 1
+  for (int item = threadIdx.x; item < items; item += kThreads) {
+    const int row_head = item / chunks, e0 = 8 * (item - row_head * chunks);
+    const bool is_v = row_head >= p.cache.kv_heads;
+    const int head = row_head - (is_v ? p.cache.kv_heads : 0);
+    uint16_t *const to = static_cast<uint16_t *>(is_v ? p.a.v : p.a.k) + head * (is_v ? p.a.v_head : p.a.k_head) + e0;
+    const int64_t to_token = is_v ? p.a.v_token : p.a.k_token;
+    const int width = min(8, p.cache.head_dim - e0);
+#pragma unroll 1
+    for (int t0 = 0; t0 < count; t0 += kAtOnce) {
+      uint32_t w[kAtOnce][kQuantized ? 2 : 4];
+      bool live[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int t = t0 + u;
+        live[u] = t < count && page_of[t] >= 0;
+        if (!live[u]) continue;
+        if constexpr (kQuantized) {
+          const QuantizedRows &r = is_v ? p.rows.v : p.rows.k;
+          w[u][0] = *reinterpret_cast<const uint32_t *>(r.codes + page_of[t] * r.codes_page + row_of[t] * r.codes_row + head * r.codes_head + e0 / 2);
+          w[u][1] = r.steps[page_of[t] * r.steps_page + row_of[t] * r.steps_row + head * r.steps_head + e0 / kQuantGroup];
+        } else {
+          const uint16_t *from = static_cast<const uint16_t *>(is_v ? p.cache.v : p.cache.k) + page_of[t] * (is_v ? p.cache.v_page : p.cache.k_page) +
+                                 row_of[t] * (is_v ? p.cache.v_row : p.cache.k_row) + head * (is_v ? p.cache.v_head : p.cache.k_head) + e0;
+          if constexpr (kWide) {
+            *reinterpret_cast<uint4 *>(w[u]) = *reinterpret_cast<const uint4 *>(from);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[u][i] = (2 * i < width ? from[2 * i] : 0u) | ((2 * i + 1 < width ? static_cast<uint32_t>(from[2 * i + 1]) : 0u) << 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (!live[u]) continue;
+        uint32_t out[4];
+        if constexpr (kQuantized) {
+          const float step = quant_step(w[u][1], kFormat), low = quant_low(w[u][1], kFormat);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            out[i] = narrow_bits(quant_value(w[u][0], 2 * i, step, low), kFormat) | (narrow_bits(quant_value(w[u][0], 2 * i + 1, step, low), kFormat) << 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[i] = w[u][i];
+        }
+        uint16_t *const dst = to + (first + t0 + u) * to_token;
+        if constexpr (kWide) {
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < width) dst[i] = static_cast<uint16_t>(out[i >> 1] >> (16 * (i & 1)));
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+
+wb200_status launch_cache_read(const CacheReadArgs &a, const PagedCacheArgs &cache, const QuantizedRowsArgs *rows, const PagedBatchArgs &batch,
+                               int *refused, cudaStream_t stream) {
+  ReadParams p{};
+  p.a = a;
+  p.cache = cache;
+  if (rows) p.rows = *rows;
+  p.batch = batch;
+  p.refused = refused;
+  // Few tokens get a block each.
+  p.tokens_per_block = kMaxTokens;
+  while (p.tokens_per_block > 1 && batch.tokens / p.tokens_per_block < 148 * 8) p.tokens_per_block >>= 1;
+  uint64_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | static_cast<uint64_t>((a.k_token | a.k_head | a.v_token | a.v_head) * 2) |
+                  static_cast<uint64_t>(cache.head_dim * 2);
+  if (!rows)
+    bits |= reinterpret_cast<uintptr_t>(cache.k) | reinterpret_cast<uintptr_t>(cache.v) |
+            static_cast<uint64_t>((cache.k_page | cache.k_row | cache.k_head | cache.v_page | cache.v_row | cache.v_head) * 2);
+  const bool wide = (bits & 15u) == 0, bf16 = cache.format == WB200_BF16;
+  void (*kernel)(const ReadParams);
+  if (!rows) kernel = wide ? cache_read_kernel<WB200_BF16, false, true> : cache_read_kernel<WB200_BF16, false, false>;     // copies bits of either type
+  else if (bf16) kernel = wide ? cache_read_kernel<WB200_BF16, true, true> : cache_read_kernel<WB200_BF16, true, false>;
+  else kernel = wide ? cache_read_kernel<WB200_F16, true, true> : cache_read_kernel<WB200_F16, true, false>;
+  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(batch.tokens) + p.tokens_per_block - 1) / p.tokens_per_block);
+  WB200_CUDA_CHECK(launch_dependent(kernel, blocks, kThreads, 0, stream, p));
+  return WB200_OK;
+}
+
+}  // namespace wb200

@@ -304,6 +304,19 @@ struct PagedCacheArgs {
   void *k, *v;
   int64_t k_page, k_row, k_head, v_page, v_row, v_head;   // strides in elements
 };
+// Rows of a KV head as codes of four bits and, for every kQuantGroup elements (the last group of a head takes what is left), the
+// pair (step, low) of the cache's type: the code c stands for low + c * step.
+constexpr int kQuantGroup = 64;
+constexpr int kQuantMaxHeadDim = 256;
+struct QuantizedRows {
+  uint8_t *codes;                              // head_dim / 2 bytes a row, the even element in the low half of a byte
+  uint32_t *steps;                             // step in the low half of a word, low in the high one
+  int64_t codes_page, codes_row, codes_head;   // strides in bytes, multiples of 4
+  int64_t steps_page, steps_row, steps_head;   // strides in words
+};
+struct QuantizedRowsArgs {
+  QuantizedRows k, v;
+};
 struct PagedBatchArgs {
   int sequences, table_width, tokens, max_query;
   const int *page_table, *key_lengths, *query_starts;
@@ -320,6 +333,16 @@ wb200_status launch_rope(const RopeArgs &args, const RotaryConstants &constants,
 // args: x the fused rows (heads = q_heads + 2 kv_heads, x_head = head_dim), out the rotated q heads.
 wb200_status launch_rope_append(const RopeArgs &args, const RotaryConstants &constants, const PagedCacheArgs &cache, const PagedBatchArgs &batch,
                                 int *refused, cudaStream_t stream);
+// The same with K and V quantised; `cache` gives the extents alone.
+wb200_status launch_rope_append_quantized(const RopeArgs &args, const RotaryConstants &constants, const PagedCacheArgs &cache,
+                                          const QuantizedRowsArgs &rows, const PagedBatchArgs &batch, int *refused, cudaStream_t stream);
+// K and V rows of the batch's tokens (cache_read.cu); `rows` null: those of the cache itself.
+struct CacheReadArgs {
+  void *k, *v;
+  int64_t k_token, k_head, v_token, v_head;
+};
+wb200_status launch_cache_read(const CacheReadArgs &args, const PagedCacheArgs &cache, const QuantizedRowsArgs *rows, const PagedBatchArgs &batch,
+                               int *refused, cudaStream_t stream);
 
 struct AttentionPagedArgs {
   PagedCacheArgs cache;
@@ -335,6 +358,8 @@ struct AttentionPagedArgs {
   int *status;        // bounded waits
 };
 wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cudaStream_t stream);
+// Over quantised rows, of which `args.cache` gives the extents alone.
+wb200_status launch_attention_quantized_general(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows, cudaStream_t stream);
 // Few rows per KV head (attention_paged_rows.cu): one launch where `clustered`, else two.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
 bool attention_paged_rows_clustered(const AttentionPagedArgs &args, int sm_count);

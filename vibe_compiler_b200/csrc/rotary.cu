@@ -1,6 +1,6 @@
 // Rotary positions: every pair of a head's elements is turned by the token's position times the pair's frequency, on rows
 // anywhere in memory (wb200_rope), or on the rows of a fused projection with the new K and V rows stored to the pages of a
-// KV cache on the way (wb200_rope_append).
+// KV cache on the way (wb200_rope_append), or quantised on the way (wb200_rope_append_quantized).
 //
 // The angle. A frequency is given in 2^-64 turns per position, so position * frequency in 64-bit integers IS the angle
 // modulo whole turns, for positions of either sign and any size; a product in f32 has lost the angle's fourth digit at
@@ -10,6 +10,7 @@
 //
 // Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below.
 #include "attention_paged.cuh"
+#include "quantized_rows.cuh"
 
 namespace wb200 {
 namespace {
@@ -113,44 +114,13 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   pdl_wait();
   pdl_launch_dependents();
   if constexpr (kAppend) {
-    // The tokens' sequences: every thread compares some sequences' token ranges with the block's tokens. A range that is not one of
-    // the rows' is reported whether or not a token of the block lies in it.
-    if (threadIdx.x < count) sequence_of[threadIdx.x] = -1;
-    __syncthreads();
-    for (int s = threadIdx.x; s < p.batch.sequences; s += kThreads) {
-      const int begin = p.batch.query_starts[s], end = p.batch.query_starts[s + 1];
-      if (begin < end && (begin < 0 || end > a.tokens)) {
-        raise_status(p.refused, kRefusedLength);
-        continue;
-      }
-      for (int t = max(begin, first); t < min(end, first + count); ++t) sequence_of[t - first] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x < count) {
-      const int s = sequence_of[threadIdx.x], token = first + static_cast<int>(threadIdx.x);
-      int state = 0;
-      // What attention would leave out as a whole is not written here in part: its positions mean nothing.
-      const PagedSequence sequence = s >= 0 ? paged_sequence(p.batch, p.cache, s, p.refused, true) : PagedSequence{0, 0, 0};
-      if (sequence.count > 0) {
-        const int position = sequence.keys - sequence.count + (token - sequence.begin);      // less than keys, which the table holds
-        if (position < 0) {
-          raise_status(p.refused, kRefusedLength);
-        } else {
-          const int slot = position / p.cache.page_size, row = position - slot * p.cache.page_size;
-          const int page = p.batch.page_table[s * p.batch.table_stride + slot];
-          if (page < 0 || page >= p.cache.pages) {
-            raise_status(p.refused, kRefusedPage);
-          } else {
-            state = 1;
-            k_row[threadIdx.x] = page * p.cache.k_page + row * p.cache.k_row;
-            v_row[threadIdx.x] = page * p.cache.v_page + row * p.cache.v_row;
-            position_of[threadIdx.x] = position;
-          }
-        }
-      }
-      state_of[threadIdx.x] = state;
-    }
-    __syncthreads();
+    if (threadIdx.x < count) state_of[threadIdx.x] = 0;
+    place_tokens(p.batch, p.cache, first, count, p.refused, sequence_of, [&](int t, int page, int row, int position) {
+      state_of[t] = 1;
+      k_row[t] = page * p.cache.k_page + row * p.cache.k_row;
+      v_row[t] = page * p.cache.v_page + row * p.cache.v_row;
+      position_of[t] = position;
+    });
   }
   for (int i = threadIdx.x; i < count * c.pairs; i += kThreads) {
     const int t = i / c.pairs, pair = i - t * c.pairs;
@@ -202,6 +172,144 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   }
 }
 
+__device__ __forceinline__ double2 sin_cos_of_turns_f64(unsigned long long phase) {
+  double s, c;
+  sincospi(static_cast<double>(static_cast<long long>(phase)) * 0x1p-63, &s, &c);
+  return make_double2(s, c);
+}
+
+// Rows of the fused projection with K and V quantised on the way to their pages. Q as above. Of a K or V row a lane takes eight
+// elements, an octet of lanes a group of 64, whose least and largest element it finds by three shuffles.
+// K is turned in f64 and rounded once to the type: a code is a decision next to a border, and so is a step's rounding, so the f32
+// rotation's last bit would give codes that differ between this kernel and the definition (and any other that follows it) in one
+// group of 30 thousand, by a whole step in an element of ten there. Each of a head's elements costs two f64 operations.
+constexpr int kMaxQuantizeAngles = 1024;
+template <int kFormat, bool kWide>
+__global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ QuantizedRowsArgs rows,
+                                                                   const __grid_constant__ RotaryConstants c) {
+  constexpr int kVec = kWide ? 8 : 1;
+  __shared__ float2 angles[kMaxQuantizeAngles];
+  __shared__ double2 fine_angles[kMaxQuantizeAngles];
+  __shared__ int page_of[kMaxTokensPerBlock], row_of[kMaxTokensPerBlock], position_of[kMaxTokensPerBlock];
+  __shared__ int sequence_of[kMaxTokensPerBlock];
+  const RopeArgs &a = p.a;
+  const int first = blockIdx.x * p.tokens_per_block;
+  const int count = min(p.tokens_per_block, a.tokens - first);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < count) page_of[threadIdx.x] = -1;
+  place_tokens(p.batch, p.cache, first, count, p.refused, sequence_of, [&](int t, int page, int row, int position) {
+    page_of[t] = page;
+    row_of[t] = row;
+    position_of[t] = position;
+  });
+  for (int i = threadIdx.x; i < count * c.pairs; i += kThreads) {
+    const int t = i / c.pairs, pair = i - t * c.pairs;
+    long long position;
+    if (!a.positions) position = page_of[t] >= 0 ? position_of[t] : 0;
+    else position = a.position_bytes == 8 ? static_cast<const long long *>(a.positions)[first + t] : static_cast<const int *>(a.positions)[first + t];
+    const unsigned long long phase = static_cast<unsigned long long>(position) * c.turns[pair];
+    const float2 sc = sin_cos_of_turns(phase);
+    angles[i] = make_float2(sc.x * c.magnitude, sc.y * c.magnitude);
+    const double2 fine = sin_cos_of_turns_f64(phase);
+    fine_angles[i] = make_double2(fine.x * c.magnitude, fine.y * c.magnitude);
+  }
+  __syncthreads();
+  const uint16_t *const x_rows = static_cast<const uint16_t *>(a.x);
+  // Q: a thread keeps to one item of the head and takes every groups-th head of the block's tokens.
+  const int lanes = min(p.items, kThreads), groups = kThreads / lanes, group = static_cast<int>(threadIdx.x) / lanes;
+  if (group < groups && p.q_heads > 0) {
+    for (int item = static_cast<int>(threadIdx.x) - group * lanes; item < p.items; item += lanes) {
+      int t = 0, head = group;
+      while (true) {
+        while (head >= p.q_heads) { head -= p.q_heads; ++t; }
+        if (t >= count) break;
+        if (page_of[t] >= 0) {
+          const bool rotates = item * kVec < c.pairs;
+          const int d0 = (rotates && !a.interleaved ? 1 : 2) * item * kVec, d1 = d0 + (rotates && !a.interleaved ? c.pairs : kVec);
+          const bool has1 = d1 + kVec <= a.head_dim;
+          const uint16_t *x = x_rows + (first + t) * a.x_token + head * a.x_head;
+          uint16_t *out = static_cast<uint16_t *>(a.out) + (first + t) * a.out_token + head * a.out_head;
+          Elements<kFormat, kVec> v0, v1;
+          v0.load(x + d0);
+          if (has1) v1.load(x + d1);
+          if (rotates) turn(v0, v1, angles + t * c.pairs + item * kVec, a.interleaved);
+          v0.store(out + d0);
+          if (has1) v1.store(out + d1);
+        }
+        head += groups;
+      }
+    }
+  }
+  // K and V: rows of 8, 16 or 32 lanes, eight elements a lane.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int shift = a.head_dim <= 64 ? 3 : a.head_dim <= 128 ? 4 : 5;
+  const int at_once = 32 >> shift, heads = 2 * p.cache.kv_heads, all = count * heads;
+  const int slot = lane & ((1 << shift) - 1), e0 = 8 * slot;
+#pragma unroll 1
+  for (int base = warp * at_once; base < all; base += (kThreads / 32) * at_once) {
+    const int row = base + (lane >> shift), t = min(row, all - 1) / heads;
+    const bool is_v = row - t * heads >= p.cache.kv_heads;
+    const int head = row - t * heads - (is_v ? p.cache.kv_heads : 0);
+    const bool live = row < all && e0 < a.head_dim && page_of[t] >= 0;
+    float v[8] = {};
+    if (live) {
+      const uint16_t *x = x_rows + (first + t) * a.x_token + (p.q_heads + (is_v ? p.cache.kv_heads : 0) + head) * a.x_head;
+      Elements<kFormat, kVec> own[8 / kVec];
+#pragma unroll
+      for (int i = 0; i < 8 / kVec; ++i) own[i].load(x + e0 + i * kVec);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = own[i / kVec].get(i % kVec);
+      const double2 *turns = fine_angles + t * c.pairs;
+      if (!is_v && e0 < 2 * c.pairs) {
+        if (a.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            if (!kWide && e0 + i >= 2 * c.pairs) break;
+            const double2 u = turns[(e0 + i) >> 1];
+            const double b = v[i], w = v[i + 1];
+            v[i] = widen_bits(narrow_bits(static_cast<float>(fma(b, u.y, -(w * u.x))), kFormat), kFormat);
+            v[i + 1] = widen_bits(narrow_bits(static_cast<float>(fma(w, u.y, b * u.x)), kFormat), kFormat);
+          }
+        } else {
+          Elements<kFormat, kVec> other[8 / kVec];
+#pragma unroll
+          for (int i = 0; i < 8 / kVec; ++i) {
+            const int e = e0 + i * kVec;
+            if (e < 2 * c.pairs) other[i].load(x + (e < c.pairs ? e + c.pairs : e - c.pairs));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int e = e0 + i;
+            if (!kWide && e >= 2 * c.pairs) break;
+            const double2 u = turns[e < c.pairs ? e : e - c.pairs];
+            const double crossed = static_cast<double>(other[i / kVec].get(i % kVec)) * u.x;
+            v[i] = widen_bits(narrow_bits(static_cast<float>(fma(static_cast<double>(v[i]), u.y, e < c.pairs ? -crossed : crossed)), kFormat), kFormat);
+          }
+        }
+      }
+    }
+    uint32_t pair;
+    const uint32_t word = quantize8<kFormat>(v, live, &pair);
+    if (live) {
+      const QuantizedRows &to = is_v ? rows.v : rows.k;
+      *reinterpret_cast<uint32_t *>(to.codes + page_of[t] * to.codes_page + row_of[t] * to.codes_row + head * to.codes_head + 4 * slot) = word;
+      if ((slot & 7) == 0) to.steps[page_of[t] * to.steps_page + row_of[t] * to.steps_row + head * to.steps_head + (slot >> 3)] = pair;
+    }
+  }
+}
+
+// A block's threads pass over its tokens' heads about twice, so that the blocks of an SM overlap one another's positions, angles,
+// loads and stores; few tokens get a block each.
+int tokens_per_block(const RopeArgs &a, const RotaryConstants &c, int items, int most_angles) {
+  const int groups = items < kThreads ? kThreads / items : 1;
+  int per_block = (2 * groups + a.heads - 1) / a.heads;
+  if (per_block > kMaxTokensPerBlock) per_block = kMaxTokensPerBlock;
+  if (c.pairs > 0 && per_block > most_angles / c.pairs) per_block = most_angles / c.pairs;
+  while (per_block > 1 && a.tokens / per_block < 148 * 8) --per_block;
+  return per_block;
+}
+
 template <bool kAppend>
 wb200_status launch(RotaryParams p, const RotaryConstants &c, bool aligned, cudaStream_t stream) {
   const RopeArgs &a = p.a;
@@ -210,15 +318,10 @@ wb200_status launch(RotaryParams p, const RotaryConstants &c, bool aligned, cuda
   const bool wide = aligned && c.pairs % vec == 0 && a.head_dim % vec == 0;
   const int step = 2 * (wide ? vec : 1);
   p.items = (a.head_dim + step - 1) / step;   // rotated pairs fill whole items
-  // A block's threads pass over its tokens' heads about twice, so that the eight blocks of an SM overlap one another's positions,
-  // angles, loads and stores; few tokens get a block each. Gradient of 16384 x 40 x 128 bf16 (336 MB, 51 us at the copy rate) and
-  // prompts of 13 thousand tokens x 48 heads: 60 / 73 us; four passes 61 / 74, eight 61 / 76, sixteen 72 / 88; two heads of a thread
-  // in flight 65 / 84 (58 registers, four blocks to an SM); blocks of 128 threads 67 / 84, of 512 70 / 78.
-  const int groups = p.items < kThreads ? kThreads / p.items : 1;
-  int per_block = (2 * groups + a.heads - 1) / a.heads;
-  if (per_block > kMaxTokensPerBlock) per_block = kMaxTokensPerBlock;
-  if (c.pairs > 0 && per_block > kMaxAnglesPerBlock / c.pairs) per_block = kMaxAnglesPerBlock / c.pairs;
-  while (per_block > 1 && a.tokens / per_block < 148 * 8) --per_block;
+  // Gradient of 16384 x 40 x 128 bf16 (336 MB, 51 us at the copy rate) and prompts of 13 thousand tokens x 48 heads: 60 / 73 us; four
+  // passes of a block 61 / 74, eight 61 / 76, sixteen 72 / 88; two heads of a thread in flight 65 / 84 (58 registers, four blocks to
+  // an SM); blocks of 128 threads 67 / 84, of 512 70 / 78.
+  const int per_block = tokens_per_block(a, c, p.items, kMaxAnglesPerBlock);
   p.tokens_per_block = per_block;
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + per_block - 1) / per_block);
   void (*kernel)(const RotaryParams, const RotaryConstants);
@@ -254,6 +357,27 @@ wb200_status launch_rope_append(const RopeArgs &a, const RotaryConstants &c, con
   const bool aligned = rows_aligned(a.x, a.x_token, a.x_head, 2) && rows_aligned(a.out, a.out_token, a.out_head, 2) &&
                        rows_aligned(cache.k, cache.k_page, cache.k_row, 2, cache.k_head) && rows_aligned(cache.v, cache.v_page, cache.v_row, 2, cache.v_head);
   return launch<true>(p, c, aligned, stream);
+}
+
+wb200_status launch_rope_append_quantized(const RopeArgs &a, const RotaryConstants &c, const PagedCacheArgs &cache, const QuantizedRowsArgs &rows,
+                                          const PagedBatchArgs &batch, int *refused, cudaStream_t stream) {
+  RotaryParams p{};
+  p.a = a;
+  p.cache = cache;
+  p.batch = batch;
+  p.q_heads = a.heads - 2 * cache.kv_heads;
+  p.refused = refused;
+  // head_dim is a multiple of 8
+  const bool wide = rows_aligned(a.x, a.x_token, a.x_head, 2) && rows_aligned(a.out, a.out_token, a.out_head, 2) && c.pairs % 8 == 0;
+  const int step = wide ? 16 : 2;
+  p.items = (a.head_dim + step - 1) / step;
+  p.tokens_per_block = tokens_per_block(a, c, p.items, kMaxQuantizeAngles);
+  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + p.tokens_per_block - 1) / p.tokens_per_block);
+  const bool bf16 = a.format == WB200_BF16;
+  const auto kernel = wide ? (bf16 ? rotary_quantize_kernel<WB200_BF16, true> : rotary_quantize_kernel<WB200_F16, true>)
+                           : (bf16 ? rotary_quantize_kernel<WB200_BF16, false> : rotary_quantize_kernel<WB200_F16, false>);
+  WB200_CUDA_CHECK(launch_dependent(kernel, blocks, kThreads, 0, stream, p, rows, c));
+  return WB200_OK;
 }
 
 }  // namespace wb200

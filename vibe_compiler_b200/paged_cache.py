@@ -1,9 +1,9 @@
 """Objects of serving from a paged KV cache, as the backend's paged operators take them.
 
-`PagedCache` is one layer's K and V cut into pages, `PagedBatch` the new tokens of one step and where their sequences' keys
+`PagedCache` is one layer's K and V cut into pages, `QuantizedCache` the same held in four bits, `PagedBatch` the new tokens of one step and where their sequences' keys
 lie, `RotaryTable` the constants of a rotation. `PageTables` keeps the page table, the lengths and the page counts of a set
 of sequences through the backend's book-keeping calls. Nothing is computed on the tensors here: every operator is a method
-of `B200TargetModelBackend` (`rope`, `rope_append`, `attention_paged`, `pages_*`) that launches library kernels.
+of `B200TargetModelBackend` (`rope`, `rope_append`, `cache_read`, `attention_paged`, `pages_*`) that launches library kernels.
 """
 from __future__ import annotations
 
@@ -18,7 +18,9 @@ from . import _abi as abi
 
 _FORMATS = {torch.bfloat16: abi.BF16, torch.float16: abi.F16, torch.float32: abi.F32}
 _CACHE_PACK = struct.Struct("=6I8q").pack
+_QUANTIZED_PACK = struct.Struct("=6I2Q6q2Q6q").pack
 _BATCH_PACK = struct.Struct("=4I4q").pack
+assert len(_QUANTIZED_PACK(*[0] * 22)) == C.sizeof(abi.QuantizedCacheDesc)
 assert len(_CACHE_PACK(*[0] * 14)) == C.sizeof(abi.PagedCacheDesc) and len(_BATCH_PACK(*[0] * 8)) == C.sizeof(abi.PagedBatchDesc)
 
 
@@ -102,7 +104,8 @@ class PagedCache:
     only). Any strides with the head dimension innermost: a cache laid out [pages, kv_heads, page_size, head_dim] is passed
     as its transposed view."""
 
-    __slots__ = ("_k", "_v", "_desc", "device_index")
+    __slots__ = ("_k", "_v", "_desc", "device_index", "shape", "dtype")
+    quantized = False
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _FORMATS:
@@ -111,7 +114,7 @@ class PagedCache:
             raise ValueError("k and v must be CUDA tensors of one device")
         if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
             raise ValueError("the head dimension of k and v must be contiguous")
-        self._k, self._v, self.device_index = k, v, k.device.index
+        self._k, self._v, self.device_index, self.shape, self.dtype = k, v, k.device.index, k.shape, k.dtype
         self._desc = abi.PagedCacheDesc.from_buffer_copy(_CACHE_PACK(
             k.shape[0], k.shape[1], k.shape[2], k.shape[3], _FORMATS[k.dtype], 0, k.data_ptr(), v.data_ptr(),
             k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2)))
@@ -130,6 +133,67 @@ class PagedCache:
     @property
     def page_size(self) -> int:
         return self._k.shape[1]
+
+
+class QuantizedCache:
+    """One layer's K and V held in four bits: codes, uint8 [pages, page_size, kv_heads, head_dim / 2], two to a byte, the even
+    element in the low half, and steps [pages, page_size, kv_heads, groups, 2] of bfloat16 or float16, the pair (step, low) of
+    every 64 elements (the last group of a head takes what is left): a code c stands for low + c * step. The calls that take a
+    PagedCache take one of these in its place; queries and projections are of the steps' type. head_dim is a multiple of 8 up to
+    256. Any strides that keep rows of codes and pairs of steps contiguous; `zeros` lays the rows of a head one behind the other
+    ([pages, kv_heads, page_size, ...] in memory), which the kernels read widest."""
+
+    __slots__ = ("_tensors", "_desc", "device_index", "shape", "dtype")
+    quantized = True
+    GROUP = 64
+
+    def __init__(self, k_codes: torch.Tensor, k_steps: torch.Tensor, v_codes: torch.Tensor, v_steps: torch.Tensor):
+        dtype, shape = k_steps.dtype, tuple(k_codes.shape)
+        if k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or len(shape) != 4 or v_codes.shape != shape:
+            raise ValueError("codes must be uint8 [pages, page_size, kv_heads, head_dim / 2] tensors")
+        head_dim = 2 * shape[3]
+        if dtype not in (torch.bfloat16, torch.float16) or v_steps.dtype != dtype or \
+                any(t.shape != (*shape[:3], -(-head_dim // self.GROUP), 2) for t in (k_steps, v_steps)):
+            raise ValueError("steps must be [pages, page_size, kv_heads, groups of 64 elements, 2] tensors of bfloat16 or float16")
+        device = k_codes.get_device()
+        if device < 0 or any(t.get_device() != device for t in (k_steps, v_codes, v_steps)):
+            raise ValueError("codes and steps must be CUDA tensors of one device")
+        if any(t.stride(3) != 1 and shape[3] > 1 for t in (k_codes, v_codes)):
+            raise ValueError("rows of codes must be contiguous")
+        if any(t.stride(4) != 1 or (t.stride(3) != 2 and t.shape[3] > 1) or any(t.stride(i) % 2 and t.shape[i] > 1 for i in range(3)) for t in (k_steps, v_steps)):
+            raise ValueError("steps must be contiguous pairs, one behind the other")
+        self._tensors, self.device_index, self.shape, self.dtype = (k_codes, k_steps, v_codes, v_steps), device, (*shape[:3], head_dim), dtype
+        rows = [x for codes, steps in ((k_codes, k_steps), (v_codes, v_steps))
+                for x in (codes.data_ptr(), steps.data_ptr(), *codes.stride()[:3], *(n // 2 for n in steps.stride()[:3]))]
+        self._desc = abi.QuantizedCacheDesc.from_buffer_copy(_QUANTIZED_PACK(*shape[:3], head_dim, _FORMATS[dtype], 4, *rows))
+
+    @classmethod
+    def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16, device="cuda") -> "QuantizedCache":
+        if head_dim % 2:
+            raise ValueError("head_dim must be even")
+        tensors = []
+        for _ in range(2):
+            tensors.append(torch.zeros(pages, kv_heads, page_size, head_dim // 2, dtype=torch.uint8, device=device).transpose(1, 2))
+            tensors.append(torch.zeros(pages, kv_heads, page_size, -(-head_dim // cls.GROUP), 2, dtype=dtype, device=device).transpose(1, 2))
+        return cls(*tensors)
+
+    # As for PagedCache: copies and assigned tensors are what the calls read.
+    def __reduce__(self):
+        return type(self), self._tensors
+
+    def _with(self, at: int, value) -> None:
+        tensors = list(self._tensors)
+        tensors[at] = value
+        self.__init__(*tensors)
+
+    k_codes = property(lambda self: self._tensors[0], lambda self, value: self._with(0, value))
+    k_steps = property(lambda self: self._tensors[1], lambda self, value: self._with(1, value))
+    v_codes = property(lambda self: self._tensors[2], lambda self, value: self._with(2, value))
+    v_steps = property(lambda self: self._tensors[3], lambda self, value: self._with(3, value))
+
+    @property
+    def page_size(self) -> int:
+        return self.shape[1]
 
 
 class PagedBatch:
@@ -180,7 +244,7 @@ class PagedBatch:
 class PageTables:
     """The page table, lengths and page counts of `sequences` sequences over a cache of `pages` pages, kept on the device and
     changed in place by the calls below (no host copy; each returns the call's device result). `caches` of the calls that
-    move pages are every layer's PagedCache."""
+    move pages are every layer's PagedCache, or every layer's QuantizedCache."""
 
     def __init__(self, backend, sequences: int, width: int, pages: int, page_size: int):
         device = torch.device("cuda", backend.device)
