@@ -167,6 +167,12 @@ PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
   if (longest > a.batch.tokens) longest = a.batch.tokens;
   return longest * (a.q_heads / a.cache.kv_heads) > kRowsAtMost && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
 }
+PagedKernel choose_attention_quantized(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows) {
+  return attention_quantized_rows_supports(a, rows) ? PagedKernel::rows : PagedKernel::general;
+}
+uint64_t attention_quantized_workspace(PagedKernel kernel, int sm_count) {
+  return kernel == PagedKernel::general ? 0 : attention_quantized_rows_workspace(sm_count);
+}
 uint64_t attention_paged_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;
   return kernel == PagedKernel::rows ? attention_paged_rows_workspace(sm_count) : attention_paged_chunk_workspace(sm_count);
@@ -361,8 +367,13 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
 
 uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
                                                    const wb200_attention_paged_params *p) {
-  if (!backend || ((cache || batch || p) && !(cache && batch && p))) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
-  return 0;
+  if (!backend) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
+  if (!cache && !batch && !p) return attention_quantized_workspace(PagedKernel::rows, backend->sm_count);
+  if (!cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
+  AttentionPagedArgs a{};
+  QuantizedRowsArgs rows;
+  if (make_attention_quantized(nullptr, cache, batch, p, &a, &rows) != WB200_OK) return 0;
+  return attention_quantized_workspace(choose_attention_quantized(a, rows), backend->sm_count);
 }
 
 wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
@@ -374,10 +385,14 @@ wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quant
   if (st != WB200_OK) return st;
   bool done;
   if ((st = check_attention_buffers(a, &done)) != WB200_OK || done) return st;
+  const PagedKernel kernel = choose_attention_quantized(a, rows);
+  if ((st = check_workspace(p, attention_quantized_workspace(kernel, backend->sm_count), "wb200_attention_quantized_workspace_bytes")) != WB200_OK) return st;
   DeviceGuard guard(backend->device);
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
-  st = launch_attention_quantized_general(a, rows, stream);
-  if (st == WB200_OK) backend->launches += 1;
+  if (kernel == PagedKernel::general) st = launch_attention_quantized_general(a, rows, stream);
+  else st = launch_attention_quantized_rows(a, rows, backend->sm_count, stream);
+  const bool one = kernel == PagedKernel::general || (kernel == PagedKernel::rows && attention_quantized_rows_clustered(a, backend->sm_count));
+  if (st == WB200_OK) backend->launches += one ? 1 : 2;
   return st;
 }
 

@@ -1,0 +1,608 @@
+// Attention of few new tokens over a paged KV cache held in four bits: decoding and drafted tokens (head_dim 64 and 128).
+//
+// How the work is dealt to the CTAs and folded is the 16-bit kernel's (attention_paged_walk.cuh). What differs is the arithmetic of a
+// tile of 16 keys. At 4.5 bits an element, an SM's share of HBM brings 16 keys of K and V (2304 bytes at head_dim 128) every 99
+// clocks, 396 issue slots of a scheduler for one warp's tile, so nothing may be widened element by element:
+//   codes    are the matrix operands as they are. A masked word of codes, w & 0x000f000f, read as two f16, is the codes of two
+//            elements times 2^-24 (subnormal numbers, which the tensor cores multiply exactly), w & 0x00f000f0 two others' times
+//            2^-20: five instructions for the eight elements of a word. The powers of two go into Q, and into the result.
+//   K        S^T = C Q^T, keys on the 16-wide side, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g.
+//            The sums over codes are exact up to f32's: Q is scaled to f16 by a power of two of its own a row.
+//   V        O^T = C P^T with step_g folded into the probabilities, p'_g = p step_g 2^e, rounded to f16 (11 bits, whatever the
+//            type), and sum_j p_j low_g,j beside it in f32. e follows the largest step so far, so p' stays below f16's largest.
+//            P, as S^T leaves it, becomes the other operand by movmatrix; rows of K or V are never transposed: two keys' words
+//            interleaved by halves (prmt) are the pairs that the instruction wants.
+//   maximum  The exponent's reference moves only when a score is beyond 2^8 times it: one vote a tile instead of shuffles.
+// A CTA is four warps; each streams every fourth 16-key tile of the share through a ring of its own (cp.async, rows XOR-swizzled).
+// Bound: HBM, then the warps' instructions.
+#include "attention_paged_walk.cuh"
+#include "quantized_rows.cuh"
+
+namespace wb200 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kTileKeys = 16;
+constexpr int kStepKeys = kWarps * kTileKeys;
+constexpr int kUnitSteps = 8;
+constexpr int kLeastSteps = 4;
+constexpr float kMovesBeyond = 8.f;             // log2
+constexpr float kScaledSteps = 255.f;           // p' = p step 2^e <= 2^8 * 255 < 65504
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;      // nibbles 0 and 4 of a word as f16: code * 2^-24; 1 and 5: code * 2^-20
+
+template <int kD>
+struct QuantShape {
+  static constexpr int kGroups = kD / kQuantGroup;
+  static constexpr int kRowBytes = kD / 2;
+  static constexpr int kCodeBytes = kTileKeys * kRowBytes;
+  static constexpr int kStepBytes = kTileKeys * kGroups * 4;
+  static constexpr int kStageBytes = 2 * (kCodeBytes + kStepBytes);     // K codes, V codes, K steps, V steps
+  static constexpr int kStages = kD == 128 ? 4 : 8;
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kRecord = kRowRecord<kD>;
+  static constexpr int kRecordsOff = kWarps * kRingBytes;
+  static constexpr int kSmemBytes = kRecordsOff + kWarps * 8 * kRecord * 4;
+  static_assert(kStageBytes % 128 == 0, "tiles begin on 128 bytes");
+};
+// CTAs to an SM: as many as the registers of a thread allow (tiles of 8 rows, of 16).
+constexpr int ctas_per_sm(bool narrow) { return narrow ? 4 : 2; }
+static_assert(4 * (QuantShape<128>::kSmemBytes + 512 + 1024) <= 228 * 1024, "four CTAs to an SM");
+
+struct QuantRowsParams : RowsFold {
+  QuantizedRowsArgs rows;
+  float scale_log2;
+  unsigned long long by_grid;       // as RowsWalk takes it
+};
+
+// Byte offset of 16-byte chunk c of row r in a tile of codes: lines of 128 bytes, the chunks of a line swizzled so that the words of
+// rows 2t, t = 0 .. 3, which a warp reads at once, lie in different banks.
+template <int kRowBytes>
+__device__ __forceinline__ uint32_t code_offset(int r, int c) {
+  if constexpr (kRowBytes == 64) return static_cast<uint32_t>((r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4));
+  else return static_cast<uint32_t>((r >> 2) * 128 + (((((r & 3) << 1) | c) ^ (((r >> 2) & 1) << 1)) << 4));
+}
+template <int kBytes>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, uint32_t src_bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t src) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_shared_u64(uint32_t src) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(src) : "memory");
+  return v;
+}
+// The steps of a row's groups.
+template <int kGroups>
+__device__ __forceinline__ void load_steps(uint32_t src, uint32_t (&v)[kGroups]) {
+  if constexpr (kGroups == 2) {
+    const uint2 w = ld_shared_u64(src);
+    v[0] = w.x;
+    v[1] = w.y;
+  } else {
+    v[0] = ld_shared_u32(src);
+  }
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+// 2^(exponent - that of x's leading bit) for x > 0 and finite, within the normal numbers.
+__device__ __forceinline__ float power_against(float x, int exponent) {
+  const int field = 254 + exponent - static_cast<int>(__float_as_uint(x) >> 23);
+  return __uint_as_float(static_cast<uint32_t>(min(max(field, 1), 254)) << 23);
+}
+
+// kTiles tiles of eight rows.
+template <bool kBf16, int kD, int kTiles, bool kAligned, bool kClustered>
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attention_quantized_rows_kernel(const __grid_constant__ QuantRowsParams p) {
+  using S = QuantShape<kD>;
+  constexpr int kFormat = kBf16 ? WB200_BF16 : WB200_F16;
+  constexpr int kRows = 8 * kTiles, kGroups = S::kGroups;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long warp_totals[kWarps], start_prefix;
+  __shared__ int start_sequence;
+  const AttentionPagedArgs &a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  RowsWalk<kRows, kStepKeys, kUnitSteps, kLeastSteps, kWarps, kClustered> walk(a, p.group, p.by_grid);
+  walk.find_share(warp_totals, &start_sequence, &start_prefix);
+  uint64_t policy = 0;
+  RowsSplit split = {};
+
+  const uint32_t ring_addr = smem_u32(smem + warp * S::kRingBytes);
+  float *records = reinterpret_cast<float *>(smem + S::kRecordsOff);   // [warp][8][kRecord]
+
+  // Of the walk's part this warp takes every fourth tile.
+  struct Part : RowsPart {
+    int first_key, key_end, tiles;
+  } part = {};
+  const int *pages = nullptr;
+  const uint8_t *k_base = nullptr, *v_base = nullptr;
+  const uint32_t *step_base = nullptr;                 // of K for lanes 0 to 15, of V for the others
+  const int64_t step_page = lane < 16 ? p.rows.k.steps_page : p.rows.v.steps_page, step_row = lane < 16 ? p.rows.k.steps_row : p.rows.v.steps_row;
+  auto next_part = [&]() {
+    if (!walk.next()) return false;
+    static_cast<RowsPart &>(part) = walk.part;
+    part.key_end = min(part.keys, part.step1 * kStepKeys);
+    part.first_key = part.step0 * kStepKeys + warp * kTileKeys;
+    part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
+    policy = l2_policy(static_cast<long long>(part.sequence.count) * p.group > kRows);
+    pages = a.batch.page_table + part.s * a.batch.table_stride;
+    k_base = p.rows.k.codes + part.kv_head * p.rows.k.codes_head;
+    v_base = p.rows.v.codes + part.kv_head * p.rows.v.codes_head;
+    step_base = lane < 16 ? p.rows.k.steps + part.kv_head * p.rows.k.steps_head : p.rows.v.steps + part.kv_head * p.rows.v.steps_head;
+    return true;
+  };
+  // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
+  auto look_up = [&](int tile) {
+    const int key = part.first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
+    return tile < part.tiles && key < part.key_end ? pages[key / a.cache.page_size] : -1;
+  };
+  auto issue_tile = [&](int tile, int slot, int page) {
+    if (tile < part.tiles) {
+      const int key0 = part.first_key + tile * kStepKeys;
+      const uint32_t k_dst = ring_addr + slot * S::kStageBytes, v_dst = k_dst + S::kCodeBytes;
+      const int own_key = key0 + (lane & 15);
+      const bool inside = page >= 0 && page < a.cache.pages;
+      if (!inside && own_key < part.key_end) raise_status(a.refused, kRefusedPage);
+      const bool mine = inside && own_key < part.key_end;        // other rows are zeros
+      const unsigned int seen = __ballot_sync(0xffffffffu, mine);
+      const int place = inside ? page : 0;
+      const int in_page = (kAligned ? key0 : own_key) % a.cache.page_size;
+      const int64_t k_row = place * p.rows.k.codes_page + in_page * p.rows.k.codes_row;
+      const int64_t v_row = place * p.rows.v.codes_page + in_page * p.rows.v.codes_row;
+      constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
+#pragma unroll
+      for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+        const int r = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
+        int64_t k_at, v_at;
+        if constexpr (kAligned) {
+          k_at = k_row + r * p.rows.k.codes_row;
+          v_at = v_row + r * p.rows.v.codes_row;
+        } else {
+          k_at = __shfl_sync(0xffffffffu, k_row, r);
+          v_at = __shfl_sync(0xffffffffu, v_row, r);
+        }
+        const bool reads = (seen >> r) & 1u;
+        cp_async16_hint(policy, k_dst + code_offset<S::kRowBytes>(r, c), k_base + (reads ? k_at + c * 16 : 0), reads ? 16u : 0u);
+        cp_async16_hint(policy, v_dst + code_offset<S::kRowBytes>(r, c), v_base + (reads ? v_at + c * 16 : 0), reads ? 16u : 0u);
+      }
+      const int64_t step_at = place * step_page + (kAligned ? in_page + (lane & 15) : in_page) * step_row;
+      cp_async_small<4 * kGroups>(v_dst + S::kCodeBytes + (lane >> 4) * S::kStepBytes + (lane & 15) * (4 * kGroups), step_base + (mine ? step_at : 0), mine ? 4u * kGroups : 0u);
+    }
+    cp_async_commit();
+  };
+  int page = -1;                                       // of the next tile to be issued
+  auto fill_ring = [&]() {
+    page = look_up(0);
+#pragma unroll 1
+    for (int i = 0; i < S::kStages; ++i) {
+      const int next = look_up(i + 1);
+      issue_tile(i, i, page);
+      page = next;
+    }
+  };
+
+  bool more = next_part();
+  if (more) fill_ring();
+  while (more) {
+    // A lane's rows are 2t and 2t + 1 of each tile, its elements 8g .. 8g + 7 of each group: acc[.][.][i] holds elements 2i (two rows)
+    // and 2i + 1.
+    float m_run[kTiles][2], l_run[kTiles][2], low_sum[kTiles][kGroups][2], acc[kTiles][kGroups][4][4];
+    float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of the sums over codes; of the lows
+    uint32_t q_frag[kTiles][kGroups][4][2];
+    int last_key[kTiles][2];                           // that the row sees
+    float v_scale = 1.f, step_limit = 0.f;             // 2^e; steps beyond the limit move it (no step yet: any)
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      // The row's elements 64 gr + 16 t + .. of this lane's row g of the tile, scaled by a power of two that brings the row's largest to
+      // 2^14, and those that meet codes times 2^-20 to a sixteenth of that.
+      const int packed = part.row0 + 8 * n + g, token = packed / p.group;
+      uint4 bits[kGroups][2];
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        bits[gr][0] = bits[gr][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (8 * n + g < part.rows) {
+          const uint4 *row = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + static_cast<int64_t>(part.sequence.begin + token) * a.q_token +
+                                                             (part.kv_head * p.group + packed - token * p.group) * a.q_head + gr * kQuantGroup + 16 * t);
+          bits[gr][0] = row[0];
+          bits[gr][1] = row[1];
+        }
+      }
+      auto element = [&](int gr, int e) {
+        const uint4 w = bits[gr][e >> 3];
+        const uint32_t pair = (e & 4) ? ((e & 2) ? w.w : w.z) : ((e & 2) ? w.y : w.x);
+        return widen_bits(e & 1 ? pair >> 16 : pair & 0xffffu, kFormat);
+      };
+      float largest = 0.f, sums[kGroups];
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        sums[gr] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = element(gr, e);
+          largest = fmaxf(largest, fabsf(x));
+          sums[gr] += x;
+        }
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], off);
+      }
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+      const float power = largest > 0.f && largest < INFINITY ? power_against(largest, 14) : 1.f;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int e = 8 * w + 2 * h;
+            const __half2 even = __floats2half2_rn(element(gr, e) * power, element(gr, e + 4) * power);
+            const __half2 odd = __floats2half2_rn(element(gr, e + 1) * (power * 0.0625f), element(gr, e + 5) * (power * 0.0625f));
+            q_frag[n][gr][2 * w + h][0] = *reinterpret_cast<const uint32_t *>(&even);
+            q_frag[n][gr][2 * w + h][1] = *reinterpret_cast<const uint32_t *>(&odd);
+          }
+      const float scale = p.scale_log2 * (0x1p24f / power);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row_scale[n][i] = __shfl_sync(0xffffffffu, scale, 4 * (2 * t + i));
+        m_run[n][i] = -INFINITY;
+        l_run[n][i] = 0.f;
+        last_key[n][i] = paged_visible(part.sequence, (part.row0 + 8 * n + 2 * t + i) / p.group, a.causal) - 1;
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          q_sum[n][gr][i] = __shfl_sync(0xffffffffu, sums[gr], 4 * (2 * t + i)) * p.scale_log2;
+          low_sum[n][gr][i] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[n][gr][j][0] = acc[n][gr][j][1] = acc[n][gr][j][2] = acc[n][gr][j][3] = 0.f;
+    }
+    const int masked_from = min(part.key_end, paged_visible(part.sequence, part.row0 / p.group, a.causal));   // hidden from some row from here on
+
+    int slot = 0;
+#pragma unroll 1
+    for (int tile = 0; tile < part.tiles; ++tile) {
+      const int next = look_up(tile + S::kStages + 1);
+      cp_async_wait<S::kStages - 1>();
+      __syncwarp();
+      const uint32_t k_src = ring_addr + slot * S::kStageBytes, v_src = k_src + S::kCodeBytes, step_src = v_src + S::kCodeBytes;
+      // S^T: keys g and g + 8, rows 2t and 2t + 1
+      float score[kTiles][2][2];                       // [tile][key][row]
+      {
+        uint32_t k_steps[2][kGroups];
+        float dot[kTiles][kGroups][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_steps<kGroups>(step_src + (g + 8 * h) * (4 * kGroups), k_steps[h]);
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          const uint2 w0 = ld_shared_u64(k_src + code_offset<S::kRowBytes>(g, 2 * gr + (t >> 1)) + 8 * (t & 1));
+          const uint2 w1 = ld_shared_u64(k_src + code_offset<S::kRowBytes>(g + 8, 2 * gr + (t >> 1)) + 8 * (t & 1));
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) dot[n][gr][0] = dot[n][gr][1] = dot[n][gr][2] = dot[n][gr][3] = 0.f;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t x = w ? w0.y : w0.x, y = w ? w1.y : w1.x;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t xs = x >> (8 * h), ys = y >> (8 * h);
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n)
+                mma_f16(dot[n][gr], xs & kEven, ys & kEven, xs & kOdd, ys & kOdd, q_frag[n][gr][2 * w + h][0], q_frag[n][gr][2 * w + h][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float step[kGroups], low[kGroups];
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            step[gr] = quant_step(k_steps[h][gr], kFormat);
+            low[gr] = quant_low(k_steps[h][gr], kFormat);
+          }
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float x = step[0] * dot[n][0][2 * h + i], y = low[0] * q_sum[n][0][i];
+#pragma unroll
+              for (int gr = 1; gr < kGroups; ++gr) {
+                x = fmaf(step[gr], dot[n][gr][2 * h + i], x);
+                y = fmaf(low[gr], q_sum[n][gr][i], y);
+              }
+              score[n][h][i] = fmaf(x, row_scale[n][i], y);
+            }
+        }
+      }
+      const int key0 = part.first_key + tile * kStepKeys;
+      if (key0 + kTileKeys > masked_from) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (key0 + g + 8 * h >= part.key_end || key0 + g + 8 * h > last_key[n][i]) score[n][h][i] = -INFINITY;
+      }
+      float v_step[2][kGroups], v_low[2][kGroups];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pairs[kGroups];
+        load_steps<kGroups>(step_src + S::kStepBytes + (g + 8 * h) * (4 * kGroups), pairs);
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          v_step[h][gr] = quant_step(pairs[gr], kFormat);
+          v_low[h][gr] = quant_low(pairs[gr], kFormat);
+        }
+      }
+      float largest_step = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) largest_step = fmaxf(largest_step, fmaxf(v_step[0][gr], v_step[1][gr]));
+      bool moves = largest_step > step_limit;
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) moves = moves || fmaxf(score[n][0][i], score[n][1][i]) > m_run[n][i] + kMovesBeyond;
+      if (__any_sync(0xffffffffu, moves)) {
+        float factor = 1.f;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) largest_step = fmaxf(largest_step, __shfl_xor_sync(0xffffffffu, largest_step, off));
+        if (largest_step > step_limit) {
+          const float power = power_against(largest_step, 6);
+          if (step_limit > 0.f) factor = power / v_scale;
+          v_scale = power;
+          step_limit = kScaledSteps / power;
+        }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(score[n][0][i], score[n][1][i]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            float alpha = 1.f;
+            if (top > m_run[n][i] + kMovesBeyond) {
+              alpha = exp2_fast(m_run[n][i] - top);
+              m_run[n][i] = top;
+            }
+            l_run[n][i] *= alpha;
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              low_sum[n][gr][i] *= alpha;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                acc[n][gr][j][i] *= alpha * factor;
+                acc[n][gr][j][2 + i] *= alpha * factor;
+              }
+            }
+          }
+      }
+      uint32_t p_frag[kTiles][kGroups][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        float pr[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float m_exp = m_run[n][i] == -INFINITY ? 0.f : m_run[n][i];
+          pr[0][i] = exp2_fast(score[n][0][i] - m_exp);
+          pr[1][i] = exp2_fast(score[n][1][i] - m_exp);
+          l_run[n][i] += pr[0][i] + pr[1][i];
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) low_sum[n][gr][i] = fmaf(pr[0][i], v_low[0][gr], fmaf(pr[1][i], v_low[1][gr], low_sum[n][gr][i]));
+        }
+        // p' is rounded to f16, as the product's operands are; p itself, in the sum and beside the lows, is not.
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float weight = v_step[h][gr] * v_scale;
+            const __half2 both = __floats2half2_rn(pr[h][0] * weight, pr[h][1] * weight);
+            p_frag[n][gr][h] = transposed(*reinterpret_cast<const uint32_t *>(&both));
+          }
+      }
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        uint32_t x[2][2];                              // keys 2t and 2t + 1 (+ 8): elements 8g .. + 3, .. + 7
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = ld_shared_u32(v_src + code_offset<S::kRowBytes>(2 * t + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
+          const uint32_t w1 = ld_shared_u32(v_src + code_offset<S::kRowBytes>(2 * t + 1 + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
+          x[h][0] = __byte_perm(w0, w1, 0x5410);
+          x[h][1] = __byte_perm(w0, w1, 0x7632);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t u = x[0][j >> 1] >> (8 * (j & 1)), w = x[1][j >> 1] >> (8 * (j & 1));
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u & kEven, u & kOdd, w & kEven, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
+        }
+      }
+      __syncwarp();   // every lane has read the slot
+      issue_tile(tile + S::kStages, slot, page);
+      page = next;
+      if (++slot == S::kStages) slot = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l_run[n][i] += __shfl_xor_sync(0xffffffffu, l_run[n][i], off);
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) low_sum[n][gr][i] += __shfl_xor_sync(0xffffffffu, low_sum[n][gr][i], off);
+        }
+    // The next part's first tiles are on their way while this one's state is put together. (The ring's groups of copies have all
+    // been waited for but the empty ones behind the last tile.)
+    const Part done = part;
+    more = next_part();
+    if (more) fill_ring();
+    const bool whole = done.whole();
+    const float unscale = 1.f / v_scale;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {                 // eight rows at a time
+      __syncthreads();                                 // the records of the rows before have been read
+      float *mine_records = records + warp * (8 * S::kRecord);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[2 * j] = fmaf(acc[n][gr][j][i] * 0x1p24f, unscale, low_sum[n][gr][i]);
+            v[2 * j + 1] = fmaf(acc[n][gr][j][2 + i] * 0x1p20f, unscale, low_sum[n][gr][i]);
+          }
+          float4 *to = reinterpret_cast<float4 *>(mine_records + (2 * t + i) * S::kRecord + gr * kQuantGroup + 8 * g);
+          to[0] = make_float4(v[0], v[1], v[2], v[3]);
+          to[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+        if (g == 0) *reinterpret_cast<float2 *>(mine_records + (2 * t + i) * S::kRecord + kD) = make_float2(m_run[n][i], l_run[n][i]);
+      }
+      __syncthreads();
+      for (int r = warp; r < 8 && r + 8 * n < done.rows; r += kWarps) {      // a warp per row
+        float top, l;
+        Slice<kD> sum;
+        fold_warps<kD, kWarps>(records, r, lane, top, l, sum);
+        const int row = r + 8 * n;
+        if constexpr (kClustered) {                    // over the first warp's record, which this warp has read
+          sum.store(records + r * S::kRecord, lane);
+          if (lane == 0) *reinterpret_cast<float2 *>(records + r * S::kRecord + kD) = make_float2(top, l);
+        } else if (whole) {
+          const int packed = done.row0 + row, token = packed / p.group;
+          write_row<kBf16, kD>(a, done.sequence.begin + token, done.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+        } else {
+          float *record = p.records + ((static_cast<int64_t>(blockIdx.x) * 2 + (done.step0 == 0 ? 1 : 0)) * kRows + row) * S::kRecord;
+          sum.store(record, lane);
+          if (lane == 0) *reinterpret_cast<float2 *>(record + kD) = make_float2(top, l);
+        }
+      }
+      if constexpr (kClustered) {
+        cluster_sync_all();                            // the CTAs' states are in their shared memory
+        if (blockIdx.x == 0) {
+          for (int r = warp; r < 8 && r + 8 * n < done.rows; r += kWarps) {
+            float top, l;
+            Slice<kD> sum;
+            fold_cluster<kD>(records + r * S::kRecord, lane, top, l, sum);
+            const int packed = done.row0 + r + 8 * n, token = packed / p.group;
+            write_row<kBf16, kD>(a, done.sequence.begin + token, done.kv_head * p.group + packed - token * p.group, lane, top, l, sum);
+          }
+        }
+        cluster_sync_all();                            // and are kept until they have been read
+      }
+    }
+    if (!kClustered && done.step0 == 0 && !whole) split = walk.split_of(done);
+  }
+  cp_async_wait<0>();
+  if (!kClustered && threadIdx.x == 0) p.splits[blockIdx.x] = split;
+}
+
+using QuantRowsKernel = void (*)(const QuantRowsParams);
+#define WB200_QUANT_ROWS_KERNELS(D, TILES, CLUSTERED)                                                                                   \
+  {{attention_quantized_rows_kernel<false, D, TILES, false, CLUSTERED>, attention_quantized_rows_kernel<false, D, TILES, true, CLUSTERED>}, \
+   {attention_quantized_rows_kernel<true, D, TILES, false, CLUSTERED>, attention_quantized_rows_kernel<true, D, TILES, true, CLUSTERED>}}
+const QuantRowsKernel kKernels[2][2][2][2][2] = {      // [clustered][head_dim 128][narrow][bf16][aligned]
+    {{WB200_QUANT_ROWS_KERNELS(64, 2, false), WB200_QUANT_ROWS_KERNELS(64, 1, false)},
+     {WB200_QUANT_ROWS_KERNELS(128, 2, false), WB200_QUANT_ROWS_KERNELS(128, 1, false)}},
+    {{WB200_QUANT_ROWS_KERNELS(64, 2, true), WB200_QUANT_ROWS_KERNELS(64, 1, true)},
+     {WB200_QUANT_ROWS_KERNELS(128, 2, true), WB200_QUANT_ROWS_KERNELS(128, 1, true)}}};
+void (*const kFoldKernels[2][2][2])(const RowsFold) = {      // [head_dim 128][narrow][bf16]
+    {{attention_paged_fold_kernel<false, 64, 16>, attention_paged_fold_kernel<true, 64, 16>},
+     {attention_paged_fold_kernel<false, 64, 8>, attention_paged_fold_kernel<true, 64, 8>}},
+    {{attention_paged_fold_kernel<false, 128, 16>, attention_paged_fold_kernel<true, 128, 16>},
+     {attention_paged_fold_kernel<false, 128, 8>, attention_paged_fold_kernel<true, 128, 8>}}};
+
+constexpr int kMostCtas = ctas_per_sm(true);
+size_t rows_record_bytes(int sm_count) { return static_cast<size_t>(sm_count) * kMostCtas * 2 * 16 * kRowRecord<128> * sizeof(float); }
+// Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
+bool is_narrow(const AttentionPagedArgs &a) { return static_cast<int64_t>(a.q_heads / a.cache.kv_heads) * (a.batch.max_query > 0 ? a.batch.max_query : 1) <= 8; }
+
+}  // namespace
+
+bool attention_quantized_rows_supports(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows) {
+  if (a.cache.head_dim != 64 && a.cache.head_dim != 128) return false;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) |
+                        static_cast<uint64_t>((a.q_token | a.q_head | a.out_token | a.out_head) * 2) | reinterpret_cast<uintptr_t>(rows.k.codes) |
+                        reinterpret_cast<uintptr_t>(rows.v.codes) |
+                        static_cast<uint64_t>(rows.k.codes_page | rows.k.codes_row | rows.k.codes_head | rows.v.codes_page | rows.v.codes_row | rows.v.codes_head);
+  const uint64_t steps = reinterpret_cast<uintptr_t>(rows.k.steps) | reinterpret_cast<uintptr_t>(rows.v.steps) |
+                         static_cast<uint64_t>((rows.k.steps_page | rows.k.steps_row | rows.k.steps_head | rows.v.steps_page | rows.v.steps_row | rows.v.steps_head) * 4);
+  const uint64_t step_bytes = a.cache.head_dim / kQuantGroup * 4;
+  return (bits & 15u) == 0 && (steps & (step_bytes - 1)) == 0;     // rows begin on 16 bytes, a row's steps on their size
+}
+
+// Clusters where all units' are resident at once and, at the longest the page table can hold, an eighth of a unit's keys through one CTA
+// does not take longer than all keys through the whole GPU and the second launch.
+bool attention_quantized_rows_clustered(const AttentionPagedArgs &a, int sm_count) {
+  const int64_t units = static_cast<int64_t>(a.batch.sequences) * a.cache.kv_heads;
+  if (units * kRowsCluster > sm_count * 2 * 7 / 8) return false;
+  const double unit_bytes = (a.cache.head_dim + 8.0 * (a.cache.head_dim / kQuantGroup)) * a.cache.page_size * a.batch.table_width;
+  return unit_bytes / kRowsCluster / 20.0 <= static_cast<double>(units) * unit_bytes / 5500.0 + 4000.0;
+}
+
+size_t attention_quantized_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kMostCtas * sizeof(RowsSplit); }
+
+wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream) {
+  const bool narrow = is_narrow(a);
+  const unsigned grid = static_cast<unsigned>(sm_count * ctas_per_sm(narrow));
+  QuantRowsParams p{};
+  p.a = a;
+  p.rows = rows;
+  p.group = a.q_heads / a.cache.kv_heads;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.by_grid = ~0ull / grid + 1;
+  p.records = static_cast<float *>(a.workspace);
+  p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
+  const int wide = a.cache.head_dim == 128 ? 1 : 0, bf16 = a.cache.format == WB200_BF16 ? 1 : 0;
+  static PerDeviceOnce attributes;
+  const wb200_status st = attributes.run([]() -> wb200_status {
+    for (int d = 0; d < 2; ++d)
+      for (int n = 0; n < 2; ++n)
+        for (int b = 0; b < 2; ++b)
+          for (int al = 0; al < 2; ++al)
+            for (int c = 0; c < 2; ++c)
+              WB200_CUDA_CHECK(cudaFuncSetAttribute(kKernels[c][d][n][b][al], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                    d ? QuantShape<128>::kSmemBytes : QuantShape<64>::kSmemBytes));
+    return WB200_OK;
+  });
+  if (st != WB200_OK) return st;
+  const size_t smem = wide ? QuantShape<128>::kSmemBytes : QuantShape<64>::kSmemBytes;
+  const bool aligned = a.cache.page_size % kTileKeys == 0;
+  if (attention_quantized_rows_clustered(a, sm_count)) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(kRowsCluster, static_cast<unsigned>(a.batch.sequences) * a.cache.kv_heads);
+    config.blockDim = dim3(kWarps * 32);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes_of[2];
+    attributes_of[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes_of[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes_of[1].id = cudaLaunchAttributeClusterDimension;
+    attributes_of[1].val.clusterDim.x = kRowsCluster; attributes_of[1].val.clusterDim.y = 1; attributes_of[1].val.clusterDim.z = 1;
+    config.attrs = attributes_of;
+    config.numAttrs = 2;
+    WB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kKernels[1][wide][narrow][bf16][aligned], p));
+    return WB200_OK;
+  }
+  WB200_CUDA_CHECK(launch_dependent(kKernels[0][wide][narrow][bf16][aligned], grid, kWarps * 32, smem, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], dim3(grid, narrow ? 8 : 16), a.cache.head_dim, 0, stream, static_cast<const RowsFold &>(p)));
+  return WB200_OK;
+}
+
+}  // namespace wb200

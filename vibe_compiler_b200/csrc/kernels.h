@@ -360,6 +360,11 @@ struct AttentionPagedArgs {
 wb200_status launch_attention_paged_general(const AttentionPagedArgs &args, cudaStream_t stream);
 // Over quantised rows, of which `args.cache` gives the extents alone.
 wb200_status launch_attention_quantized_general(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows, cudaStream_t stream);
+// Few rows per KV head (attention_quantized_rows.cu): one launch where `clustered`, else two.
+bool attention_quantized_rows_supports(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows);
+bool attention_quantized_rows_clustered(const AttentionPagedArgs &args, int sm_count);
+size_t attention_quantized_rows_workspace(int sm_count);
+wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream);
 // Few rows per KV head (attention_paged_rows.cu): one launch where `clustered`, else two.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
 bool attention_paged_rows_clustered(const AttentionPagedArgs &args, int sm_count);
