@@ -3,15 +3,17 @@
 // How the work is dealt to the CTAs and folded is the 16-bit kernel's (attention_paged_walk.cuh). What differs is the arithmetic of a
 // tile of 16 keys. At 4.5 bits an element, an SM's share of HBM brings 16 keys of K and V (2304 bytes at head_dim 128) every 99
 // clocks, 396 issue slots of a scheduler for one warp's tile, so nothing may be widened element by element:
-//   codes    are the matrix operands as they are. A masked word of codes, w & 0x000f000f, read as two f16, is the codes of two
-//            elements times 2^-24 (subnormal numbers, which the tensor cores multiply exactly), w & 0x00f000f0 two others' times
-//            2^-20: five instructions for the eight elements of a word. The powers of two go into Q, and into the result.
+//   codes    are the matrix operands as they are. Bits 0 to 7 of two f16, w & 0x00ff00ff, are (even code + 16 odd code) 2^-24 of two
+//            pairs of elements, w & 0x00f000f0 the odd codes' part (subnormal numbers, which the tensor cores multiply exactly). The
+//            powers of two go into Q, and into the result.
 //   K        S^T = C Q^T, keys on the 16-wide side, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g.
+//            Even codes are the difference of the two (an f16 subtraction: the unit that masks is the one in demand).
 //            The sums over codes are exact up to f32's: Q is scaled to f16 by a power of two of its own a row.
 //   V        O^T = C P^T with step_g folded into the probabilities, p'_g = p step_g 2^e, rounded to f16 (11 bits, whatever the
 //            type), and sum_j p_j low_g,j beside it in f32. e follows the largest step so far, so p' stays below f16's largest.
 //            P, as S^T leaves it, becomes the other operand by movmatrix; rows of K or V are never transposed: two keys' words
-//            interleaved by halves (prmt) are the pairs that the instruction wants.
+//            interleaved by halves (prmt) are the pairs that the instruction wants. Sums with the odd codes in them and sums of
+//            those alone are rows of one product, subtracted at the end.
 //   maximum  The exponent's reference moves only when a score is beyond 2^8 times it: one vote a tile instead of shuffles.
 // A CTA is four warps; each streams every fourth 16-key tile of the share through a ring of its own (cp.async, rows XOR-swizzled).
 // Bound: HBM, then the warps' instructions.
@@ -28,7 +30,7 @@ constexpr int kUnitSteps = 8;
 constexpr int kLeastSteps = 4;
 constexpr float kMovesBeyond = 8.f;             // log2
 constexpr float kScaledSteps = 255.f;           // p' = p step 2^e <= 2^8 * 255 < 65504
-constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;      // nibbles 0 and 4 of a word as f16: code * 2^-24; 1 and 5: code * 2^-20
+constexpr uint32_t kBoth = 0x00ff00ffu, kOdd = 0x00f000f0u;
 
 template <int kD>
 struct QuantShape {
@@ -48,8 +50,14 @@ struct QuantShape {
 constexpr int ctas_per_sm(bool narrow) { return narrow ? 4 : 2; }
 static_assert(4 * (QuantShape<128>::kSmemBytes + 512 + 1024) <= 228 * 1024, "four CTAs to an SM");
 
+// Strides small enough for one 32-bit product: codes in 16 bytes, steps in a row's steps.
+struct ShortStrides {
+  uint32_t page, row;
+};
 struct QuantRowsParams : RowsFold {
   QuantizedRowsArgs rows;
+  ShortStrides k_codes, v_codes, k_steps, v_steps;
+  int step_slots, step_rows;        // a step of keys in pages and rows of the next one
   float scale_log2;
   unsigned long long by_grid;       // as RowsWalk takes it
 };
@@ -65,32 +73,27 @@ template <int kBytes>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, uint32_t src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t src) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 ld_shared_u64(uint32_t src) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(src) : "memory");
-  return v;
-}
 // The steps of a row's groups.
 template <int kGroups>
-__device__ __forceinline__ void load_steps(uint32_t src, uint32_t (&v)[kGroups]) {
+__device__ __forceinline__ void load_steps(const uint8_t *src, uint32_t (&v)[kGroups]) {
   if constexpr (kGroups == 2) {
-    const uint2 w = ld_shared_u64(src);
+    const uint2 w = *reinterpret_cast<const uint2 *>(src);
     v[0] = w.x;
     v[1] = w.y;
   } else {
-    v[0] = ld_shared_u32(src);
+    v[0] = *reinterpret_cast<const uint32_t *>(src);
   }
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Bytes 1 and 3 as bytes 0 and 2.
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t v) { return __byte_perm(v, 0u, 0x4341); }
+__device__ __forceinline__ uint32_t subtract_f16x2(uint32_t a, uint32_t b) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&d);
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t d;
@@ -123,7 +126,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
   uint64_t policy = 0;
   RowsSplit split = {};
 
-  const uint32_t ring_addr = smem_u32(smem + warp * S::kRingBytes);
+  uint8_t *const ring = smem + warp * S::kRingBytes;
+  const uint32_t ring_addr = smem_u32(ring);
   float *records = reinterpret_cast<float *>(smem + S::kRecordsOff);   // [warp][8][kRecord]
 
   // Of the walk's part this warp takes every fourth tile.
@@ -131,9 +135,17 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
     int first_key, key_end, tiles;
   } part = {};
   const int *pages = nullptr;
+  // Where this lane's chunk of a tile's first row lies in a page, of K and of V, and its steps (of K for lanes 0 to 15, of V for the
+  // others): a row per kChunks lanes, or the row of the lane's own key where tiles span pages.
+  constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
+  const int chunk_row = lane / kChunks, chunk = lane % kChunks;
   const uint8_t *k_base = nullptr, *v_base = nullptr;
-  const uint32_t *step_base = nullptr;                 // of K for lanes 0 to 15, of V for the others
-  const int64_t step_page = lane < 16 ? p.rows.k.steps_page : p.rows.v.steps_page, step_row = lane < 16 ? p.rows.k.steps_row : p.rows.v.steps_row;
+  const uint8_t *step_base = nullptr;
+  const ShortStrides step_strides = lane < 16 ? p.k_steps : p.v_steps;
+  const uint32_t code_dst = code_offset<S::kRowBytes>(chunk_row, chunk);
+  const uint32_t step_dst = 2 * S::kCodeBytes + (lane >> 4) * S::kStepBytes + (lane & 15) * (4 * kGroups);
+  // The next tile to be issued: its first key, and the place of that key (kAligned: pages are whole tiles) or of the lane's key of it.
+  int issue_key = 0, issue_slot = 0, issue_row = 0, page = -1, page_row = 0;
   auto next_part = [&]() {
     if (!walk.next()) return false;
     static_cast<RowsPart &>(part) = walk.part;
@@ -142,67 +154,84 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
     part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
     policy = l2_policy(static_cast<long long>(part.sequence.count) * p.group > kRows);
     pages = a.batch.page_table + part.s * a.batch.table_stride;
-    k_base = p.rows.k.codes + part.kv_head * p.rows.k.codes_head;
-    v_base = p.rows.v.codes + part.kv_head * p.rows.v.codes_head;
-    step_base = lane < 16 ? p.rows.k.steps + part.kv_head * p.rows.k.steps_head : p.rows.v.steps + part.kv_head * p.rows.v.steps_head;
+    const int row = kAligned ? chunk_row : 0, step_row = kAligned ? lane & 15 : 0;
+    k_base = p.rows.k.codes + part.kv_head * p.rows.k.codes_head + row * p.rows.k.codes_row + chunk * 16;
+    v_base = p.rows.v.codes + part.kv_head * p.rows.v.codes_head + row * p.rows.v.codes_row + chunk * 16;
+    const QuantizedRows &own = lane < 16 ? p.rows.k : p.rows.v;
+    step_base = reinterpret_cast<const uint8_t *>(own.steps + part.kv_head * own.steps_head + step_row * own.steps_row);
+    issue_key = part.first_key;
+    const int key = issue_key + (kAligned ? 0 : lane & 15);
+    issue_slot = key / a.cache.page_size;
+    issue_row = key - issue_slot * a.cache.page_size;
     return true;
   };
-  // The page of a tile (kAligned: pages are whole tiles) or of the lane's key of it, looked up one tile ahead of its copies.
-  auto look_up = [&](int tile) {
-    const int key = part.first_key + tile * kStepKeys + (kAligned ? 0 : lane & 15);
-    return tile < part.tiles && key < part.key_end ? pages[key / a.cache.page_size] : -1;
+  // The page of the next tile, looked up one tile ahead of its copies.
+  auto look_up = [&]() {
+    page_row = issue_row;
+    page = issue_key + (kAligned ? 0 : lane & 15) < part.key_end ? pages[issue_slot] : -1;
+    issue_slot += p.step_slots;
+    issue_row += p.step_rows;
+    if (issue_row >= a.cache.page_size) { issue_row -= a.cache.page_size; ++issue_slot; }
   };
-  auto issue_tile = [&](int tile, int slot, int page) {
-    if (tile < part.tiles) {
-      const int key0 = part.first_key + tile * kStepKeys;
-      const uint32_t k_dst = ring_addr + slot * S::kStageBytes, v_dst = k_dst + S::kCodeBytes;
-      const int own_key = key0 + (lane & 15);
+  auto issue_tile = [&](uint32_t stage) {
+    if (issue_key < part.key_end) {
+      const uint32_t code_to = stage + code_dst;
+      const int own_key = issue_key + (lane & 15);
       const bool inside = page >= 0 && page < a.cache.pages;
-      if (!inside && own_key < part.key_end) raise_status(a.refused, kRefusedPage);
-      const bool mine = inside && own_key < part.key_end;        // other rows are zeros
-      const unsigned int seen = __ballot_sync(0xffffffffu, mine);
-      const int place = inside ? page : 0;
-      const int in_page = (kAligned ? key0 : own_key) % a.cache.page_size;
-      const int64_t k_row = place * p.rows.k.codes_page + in_page * p.rows.k.codes_row;
-      const int64_t v_row = place * p.rows.v.codes_page + in_page * p.rows.v.codes_row;
-      constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
+      const uint32_t place = inside ? page : 0;
+      const uint64_t k_at = static_cast<uint64_t>(place) * p.k_codes.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.k_codes.row;
+      const uint64_t v_at = static_cast<uint64_t>(place) * p.v_codes.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.v_codes.row;
+      const uint64_t step_at = static_cast<uint64_t>(place) * step_strides.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * step_strides.row;
+      if (kAligned && inside && issue_key + kTileKeys <= part.key_end) {
+        const uint8_t *const k_from = k_base + k_at * 16, *const v_from = v_base + v_at * 16;
 #pragma unroll
-      for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
-        const int r = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
-        int64_t k_at, v_at;
-        if constexpr (kAligned) {
-          k_at = k_row + r * p.rows.k.codes_row;
-          v_at = v_row + r * p.rows.v.codes_row;
-        } else {
-          k_at = __shfl_sync(0xffffffffu, k_row, r);
-          v_at = __shfl_sync(0xffffffffu, v_row, r);
+        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+          cp_async16_hint(policy, code_to + i * (kRowsAtOnce * S::kRowBytes), k_from + i * kRowsAtOnce * p.rows.k.codes_row, 16u);
+          cp_async16_hint(policy, code_to + S::kCodeBytes + i * (kRowsAtOnce * S::kRowBytes), v_from + i * kRowsAtOnce * p.rows.v.codes_row, 16u);
         }
-        const bool reads = (seen >> r) & 1u;
-        cp_async16_hint(policy, k_dst + code_offset<S::kRowBytes>(r, c), k_base + (reads ? k_at + c * 16 : 0), reads ? 16u : 0u);
-        cp_async16_hint(policy, v_dst + code_offset<S::kRowBytes>(r, c), v_base + (reads ? v_at + c * 16 : 0), reads ? 16u : 0u);
+        cp_async_small<4 * kGroups>(stage + step_dst, step_base + step_at * (4 * kGroups), 4u * kGroups);
+      } else {
+        if (!inside && own_key < part.key_end) raise_status(a.refused, kRefusedPage);
+        const bool mine = inside && own_key < part.key_end;      // other rows are zeros
+        const unsigned int seen = __ballot_sync(0xffffffffu, mine);
+#pragma unroll
+        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+          const int r = i * kRowsAtOnce + chunk_row;
+          const bool reads = (seen >> r) & 1u;
+          int64_t k_from, v_from;
+          if constexpr (kAligned) {
+            k_from = k_at * 16 + i * kRowsAtOnce * p.rows.k.codes_row;
+            v_from = v_at * 16 + i * kRowsAtOnce * p.rows.v.codes_row;
+          } else {
+            k_from = __shfl_sync(0xffffffffu, k_at, r) * 16;
+            v_from = __shfl_sync(0xffffffffu, v_at, r) * 16;
+          }
+          cp_async16_hint(policy, code_to + i * (kRowsAtOnce * S::kRowBytes), reads ? k_base + k_from : p.rows.k.codes, reads ? 16u : 0u);
+          cp_async16_hint(policy, code_to + S::kCodeBytes + i * (kRowsAtOnce * S::kRowBytes), reads ? v_base + v_from : p.rows.v.codes, reads ? 16u : 0u);
+        }
+        cp_async_small<4 * kGroups>(stage + step_dst, mine ? step_base + step_at * (4 * kGroups) : reinterpret_cast<const uint8_t *>(p.rows.k.steps),
+                                    mine ? 4u * kGroups : 0u);
       }
-      const int64_t step_at = place * step_page + (kAligned ? in_page + (lane & 15) : in_page) * step_row;
-      cp_async_small<4 * kGroups>(v_dst + S::kCodeBytes + (lane >> 4) * S::kStepBytes + (lane & 15) * (4 * kGroups), step_base + (mine ? step_at : 0), mine ? 4u * kGroups : 0u);
     }
     cp_async_commit();
+    issue_key += kStepKeys;
   };
-  int page = -1;                                       // of the next tile to be issued
   auto fill_ring = [&]() {
-    page = look_up(0);
 #pragma unroll 1
     for (int i = 0; i < S::kStages; ++i) {
-      const int next = look_up(i + 1);
-      issue_tile(i, i, page);
-      page = next;
+      look_up();
+      issue_tile(ring_addr + i * S::kStageBytes);
     }
+    look_up();
   };
 
   bool more = next_part();
   if (more) fill_ring();
   while (more) {
-    // A lane's rows are 2t and 2t + 1 of each tile, its elements 8g .. 8g + 7 of each group: acc[.][.][i] holds elements 2i (two rows)
-    // and 2i + 1.
-    float m_run[kTiles][2], l_run[kTiles][2], low_sum[kTiles][kGroups][2], acc[kTiles][kGroups][4][4];
+    // A lane's rows are 2t and 2t + 1 of each tile, its elements 8g .. 8g + 7 of each group: acc[.][.][i] holds the sums over both codes of
+    // elements 2i and 2i + 1 (two rows), and over the odd ones (two rows).
+    float m_exp[kTiles][2], bound[kTiles][2];          // the reference, 0 as long as there is none; scores beyond the bound move it
+    float l_run[kTiles][2], low_sum[kTiles][kGroups][2], acc[kTiles][kGroups][4][4];
     float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of the sums over codes; of the lows
     uint32_t q_frag[kTiles][kGroups][4][2];
     int last_key[kTiles][2];                           // that the row sees
@@ -260,7 +289,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         row_scale[n][i] = __shfl_sync(0xffffffffu, scale, 4 * (2 * t + i));
-        m_run[n][i] = -INFINITY;
+        bound[n][i] = -INFINITY;
+        m_exp[n][i] = 0.f;
         l_run[n][i] = 0.f;
         last_key[n][i] = paged_visible(part.sequence, (part.row0 + 8 * n + 2 * t + i) / p.group, a.causal) - 1;
 #pragma unroll
@@ -276,13 +306,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
     }
     const int masked_from = min(part.key_end, paged_visible(part.sequence, part.row0 / p.group, a.causal));   // hidden from some row from here on
 
-    int slot = 0;
+    int stage = 0;                                     // byte offset in the ring
+    int key0 = part.first_key;
 #pragma unroll 1
-    for (int tile = 0; tile < part.tiles; ++tile) {
-      const int next = look_up(tile + S::kStages + 1);
+    for (int tile = part.tiles; tile > 0; --tile, key0 += kStepKeys) {
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
-      const uint32_t k_src = ring_addr + slot * S::kStageBytes, v_src = k_src + S::kCodeBytes, step_src = v_src + S::kCodeBytes;
+      const uint8_t *const k_src = ring + stage, *const v_src = k_src + S::kCodeBytes, *const step_src = v_src + S::kCodeBytes;
       // S^T: keys g and g + 8, rows 2t and 2t + 1
       float score[kTiles][2][2];                       // [tile][key][row]
       {
@@ -292,8 +322,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
         for (int h = 0; h < 2; ++h) load_steps<kGroups>(step_src + (g + 8 * h) * (4 * kGroups), k_steps[h]);
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
-          const uint2 w0 = ld_shared_u64(k_src + code_offset<S::kRowBytes>(g, 2 * gr + (t >> 1)) + 8 * (t & 1));
-          const uint2 w1 = ld_shared_u64(k_src + code_offset<S::kRowBytes>(g + 8, 2 * gr + (t >> 1)) + 8 * (t & 1));
+          const uint2 w0 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(g, 2 * gr + (t >> 1)) + 8 * (t & 1));
+          const uint2 w1 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(g + 8, 2 * gr + (t >> 1)) + 8 * (t & 1));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) dot[n][gr][0] = dot[n][gr][1] = dot[n][gr][2] = dot[n][gr][3] = 0.f;
 #pragma unroll
@@ -301,10 +331,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
             const uint32_t x = w ? w0.y : w0.x, y = w ? w1.y : w1.x;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t xs = x >> (8 * h), ys = y >> (8 * h);
+              const uint32_t xs = h ? upper_bytes(x) : x & kBoth, ys = h ? upper_bytes(y) : y & kBoth;
+              const uint32_t x_odd = xs & kOdd, y_odd = ys & kOdd, x_even = subtract_f16x2(xs, x_odd), y_even = subtract_f16x2(ys, y_odd);
 #pragma unroll
               for (int n = 0; n < kTiles; ++n)
-                mma_f16(dot[n][gr], xs & kEven, ys & kEven, xs & kOdd, ys & kOdd, q_frag[n][gr][2 * w + h][0], q_frag[n][gr][2 * w + h][1]);
+                mma_f16(dot[n][gr], x_even, y_even, x_odd, y_odd, q_frag[n][gr][2 * w + h][0], q_frag[n][gr][2 * w + h][1]);
             }
           }
         }
@@ -330,7 +361,6 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
             }
         }
       }
-      const int key0 = part.first_key + tile * kStepKeys;
       if (key0 + kTileKeys > masked_from) {
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
@@ -358,7 +388,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) moves = moves || fmaxf(score[n][0][i], score[n][1][i]) > m_run[n][i] + kMovesBeyond;
+        for (int i = 0; i < 2; ++i) moves = moves || fmaxf(score[n][0][i], score[n][1][i]) > bound[n][i];
       if (__any_sync(0xffffffffu, moves)) {
         float factor = 1.f;
 #pragma unroll
@@ -377,9 +407,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
             float alpha = 1.f;
-            if (top > m_run[n][i] + kMovesBeyond) {
-              alpha = exp2_fast(m_run[n][i] - top);
-              m_run[n][i] = top;
+            if (top > bound[n][i]) {
+              alpha = exp2_fast(bound[n][i] - kMovesBeyond - top);   // 0 at first
+              m_exp[n][i] = top;
+              bound[n][i] = top + kMovesBeyond;
             }
             l_run[n][i] *= alpha;
 #pragma unroll
@@ -399,9 +430,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
         float pr[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float m_exp = m_run[n][i] == -INFINITY ? 0.f : m_run[n][i];
-          pr[0][i] = exp2_fast(score[n][0][i] - m_exp);
-          pr[1][i] = exp2_fast(score[n][1][i] - m_exp);
+          pr[0][i] = exp2_fast(score[n][0][i] - m_exp[n][i]);
+          pr[1][i] = exp2_fast(score[n][1][i] - m_exp[n][i]);
           l_run[n][i] += pr[0][i] + pr[1][i];
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) low_sum[n][gr][i] = fmaf(pr[0][i], v_low[0][gr], fmaf(pr[1][i], v_low[1][gr], low_sum[n][gr][i]));
@@ -421,22 +451,23 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
         uint32_t x[2][2];                              // keys 2t and 2t + 1 (+ 8): elements 8g .. + 3, .. + 7
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = ld_shared_u32(v_src + code_offset<S::kRowBytes>(2 * t + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
-          const uint32_t w1 = ld_shared_u32(v_src + code_offset<S::kRowBytes>(2 * t + 1 + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
+          const uint32_t w0 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(2 * t + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
+          const uint32_t w1 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(2 * t + 1 + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
           x[h][0] = __byte_perm(w0, w1, 0x5410);
           x[h][1] = __byte_perm(w0, w1, 0x7632);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t u = x[0][j >> 1] >> (8 * (j & 1)), w = x[1][j >> 1] >> (8 * (j & 1));
+          const uint32_t u = (j & 1) ? upper_bytes(x[0][j >> 1]) : x[0][j >> 1] & kBoth, w = (j & 1) ? upper_bytes(x[1][j >> 1]) : x[1][j >> 1] & kBoth;
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u & kEven, u & kOdd, w & kEven, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
+          for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u, u & kOdd, w, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
         }
       }
       __syncwarp();   // every lane has read the slot
-      issue_tile(tile + S::kStages, slot, page);
-      page = next;
-      if (++slot == S::kStages) slot = 0;
+      issue_tile(ring_addr + stage);
+      look_up();
+      stage += S::kStageBytes;
+      if (stage == S::kRingBytes) stage = 0;
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
@@ -466,14 +497,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           float v[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[2 * j] = fmaf(acc[n][gr][j][i] * 0x1p24f, unscale, low_sum[n][gr][i]);
+            v[2 * j] = fmaf((acc[n][gr][j][i] - acc[n][gr][j][2 + i]) * 0x1p24f, unscale, low_sum[n][gr][i]);
             v[2 * j + 1] = fmaf(acc[n][gr][j][2 + i] * 0x1p20f, unscale, low_sum[n][gr][i]);
           }
           float4 *to = reinterpret_cast<float4 *>(mine_records + (2 * t + i) * S::kRecord + gr * kQuantGroup + 8 * g);
           to[0] = make_float4(v[0], v[1], v[2], v[3]);
           to[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
-        if (g == 0) *reinterpret_cast<float2 *>(mine_records + (2 * t + i) * S::kRecord + kD) = make_float2(m_run[n][i], l_run[n][i]);
+        if (g == 0) *reinterpret_cast<float2 *>(mine_records + (2 * t + i) * S::kRecord + kD) = make_float2(bound[n][i] == -INFINITY ? -INFINITY : m_exp[n][i], l_run[n][i]);
       }
       __syncthreads();
       for (int r = warp; r < 8 && r + 8 * n < done.rows; r += kWarps) {      // a warp per row
@@ -544,6 +575,11 @@ bool attention_quantized_rows_supports(const AttentionPagedArgs &a, const Quanti
   const uint64_t steps = reinterpret_cast<uintptr_t>(rows.k.steps) | reinterpret_cast<uintptr_t>(rows.v.steps) |
                          static_cast<uint64_t>((rows.k.steps_page | rows.k.steps_row | rows.k.steps_head | rows.v.steps_page | rows.v.steps_row | rows.v.steps_head) * 4);
   const uint64_t step_bytes = a.cache.head_dim / kQuantGroup * 4;
+  // Strides of pages and rows fit 32 bits in units of what they are aligned to.
+  const QuantizedRows *both[2] = {&rows.k, &rows.v};
+  for (const QuantizedRows *r : both)
+    for (const int64_t stride : {r->codes_page / 16, r->codes_row / 16, r->steps_page, r->steps_row})
+      if (stride < 0 || stride > 0x7fffffffll) return false;
   return (bits & 15u) == 0 && (steps & (step_bytes - 1)) == 0;     // rows begin on 16 bytes, a row's steps on their size
 }
 
@@ -567,6 +603,14 @@ wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &a, const 
   p.group = a.q_heads / a.cache.kv_heads;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.by_grid = ~0ull / grid + 1;
+  const int64_t groups = a.cache.head_dim / kQuantGroup;
+  auto shorten = [](int64_t page, int64_t row, int64_t unit) { return ShortStrides{static_cast<uint32_t>(page / unit), static_cast<uint32_t>(row / unit)}; };
+  p.k_codes = shorten(rows.k.codes_page, rows.k.codes_row, 16);
+  p.v_codes = shorten(rows.v.codes_page, rows.v.codes_row, 16);
+  p.k_steps = shorten(rows.k.steps_page, rows.k.steps_row, groups);
+  p.v_steps = shorten(rows.v.steps_page, rows.v.steps_row, groups);
+  p.step_slots = kStepKeys / a.cache.page_size;
+  p.step_rows = kStepKeys % a.cache.page_size;
   p.records = static_cast<float *>(a.workspace);
   p.splits = reinterpret_cast<RowsSplit *>(static_cast<uint8_t *>(a.workspace) + rows_record_bytes(sm_count));
   const int wide = a.cache.head_dim == 128 ? 1 : 0, bf16 = a.cache.format == WB200_BF16 ? 1 : 0;
