@@ -1,7 +1,7 @@
 // Attention of few new tokens over a paged KV cache held in four bits: decoding and drafted tokens (head_dim 64 and 128).
 //
 // How the work is dealt to the CTAs and folded is the 16-bit kernel's (attention_paged_walk.cuh). What differs is the arithmetic of a
-// tile of 16 keys. At 4.5 bits an element, an SM's share of HBM brings 16 keys of K and V (2304 bytes at head_dim 128) every 99
+// tile of 32 keys. At 4.5 bits an element, an SM's share of HBM brings 16 keys of K and V (2304 bytes at head_dim 128) every 99
 // clocks, 396 issue slots of a scheduler for one warp's tile, so nothing may be widened element by element:
 //   codes    are the matrix operands as they are. Bits 0 to 7 of two f16, w & 0x00ff00ff, are (even code + 16 odd code) 2^-24 of two
 //            pairs of elements, w & 0x00f000f0 the odd codes' part (subnormal numbers, which the tensor cores multiply exactly). The
@@ -24,10 +24,11 @@ namespace wb200 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kTileKeys = 16;
+constexpr int kBlocks = 2;                      // of 16 keys, a side of the matrix instruction, in a warp's tile
+constexpr int kTileKeys = 16 * kBlocks;
 constexpr int kStepKeys = kWarps * kTileKeys;
-constexpr int kUnitSteps = 8;
-constexpr int kLeastSteps = 4;
+constexpr int kUnitSteps = 5;
+constexpr int kLeastSteps = 2;
 constexpr float kMovesBeyond = 8.f;             // log2
 constexpr float kScaledSteps = 255.f;           // p' = p step 2^e <= 2^8 * 255 < 65504
 constexpr uint32_t kBoth = 0x00ff00ffu, kOdd = 0x00f000f0u;
@@ -39,7 +40,7 @@ struct QuantShape {
   static constexpr int kCodeBytes = kTileKeys * kRowBytes;
   static constexpr int kStepBytes = kTileKeys * kGroups * 4;
   static constexpr int kStageBytes = 2 * (kCodeBytes + kStepBytes);     // K codes, V codes, K steps, V steps
-  static constexpr int kStages = kD == 128 ? 4 : 8;
+  static constexpr int kStages = kD == 128 ? 3 : 6;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kRecord = kRowRecord<kD>;
   static constexpr int kRecordsOff = kWarps * kRingBytes;
@@ -47,8 +48,8 @@ struct QuantShape {
   static_assert(kStageBytes % 128 == 0, "tiles begin on 128 bytes");
 };
 // CTAs to an SM: as many as the registers of a thread allow (tiles of 8 rows, of 16).
-constexpr int ctas_per_sm(bool narrow) { return narrow ? 4 : 2; }
-static_assert(4 * (QuantShape<128>::kSmemBytes + 512 + 1024) <= 228 * 1024, "four CTAs to an SM");
+constexpr int ctas_per_sm(bool narrow) { return narrow ? 3 : 2; }
+static_assert(3 * (QuantShape<128>::kSmemBytes + 512 + 1024) <= 228 * 1024, "three CTAs to an SM");
 
 // Strides small enough for one 32-bit product: codes in 16 bytes, steps in a row's steps.
 struct ShortStrides {
@@ -135,15 +136,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
     int first_key, key_end, tiles;
   } part = {};
   const int *pages = nullptr;
-  // Where this lane's chunk of a tile's first row lies in a page, of K and of V, and its steps (of K for lanes 0 to 15, of V for the
-  // others): a row per kChunks lanes, or the row of the lane's own key where tiles span pages.
+  // Where this lane's chunk of a tile's first row lies in a page, of K and of V, and the steps of its key (a lane has one key of a
+  // tile): a row per kChunks lanes, or the row of the lane's own key where tiles span pages.
   constexpr int kChunks = S::kRowBytes / 16, kRowsAtOnce = 32 / kChunks;
   const int chunk_row = lane / kChunks, chunk = lane % kChunks;
   const uint8_t *k_base = nullptr, *v_base = nullptr;
-  const uint8_t *step_base = nullptr;
-  const ShortStrides step_strides = lane < 16 ? p.k_steps : p.v_steps;
+  const uint8_t *k_step_base = nullptr, *v_step_base = nullptr;
   const uint32_t code_dst = code_offset<S::kRowBytes>(chunk_row, chunk);
-  const uint32_t step_dst = 2 * S::kCodeBytes + (lane >> 4) * S::kStepBytes + (lane & 15) * (4 * kGroups);
+  const uint32_t step_dst = 2 * S::kCodeBytes + lane * (4 * kGroups);
   // The next tile to be issued: its first key, and the place of that key (kAligned: pages are whole tiles) or of the lane's key of it.
   int issue_key = 0, issue_slot = 0, issue_row = 0, page = -1, page_row = 0;
   auto next_part = [&]() {
@@ -154,13 +154,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
     part.tiles = part.key_end > part.first_key ? (part.key_end - part.first_key + kStepKeys - 1) / kStepKeys : 0;
     policy = l2_policy(static_cast<long long>(part.sequence.count) * p.group > kRows);
     pages = a.batch.page_table + part.s * a.batch.table_stride;
-    const int row = kAligned ? chunk_row : 0, step_row = kAligned ? lane & 15 : 0;
+    const int row = kAligned ? chunk_row : 0, step_row = kAligned ? lane : 0;
     k_base = p.rows.k.codes + part.kv_head * p.rows.k.codes_head + row * p.rows.k.codes_row + chunk * 16;
     v_base = p.rows.v.codes + part.kv_head * p.rows.v.codes_head + row * p.rows.v.codes_row + chunk * 16;
-    const QuantizedRows &own = lane < 16 ? p.rows.k : p.rows.v;
-    step_base = reinterpret_cast<const uint8_t *>(own.steps + part.kv_head * own.steps_head + step_row * own.steps_row);
+    k_step_base = reinterpret_cast<const uint8_t *>(p.rows.k.steps + part.kv_head * p.rows.k.steps_head + step_row * p.rows.k.steps_row);
+    v_step_base = reinterpret_cast<const uint8_t *>(p.rows.v.steps + part.kv_head * p.rows.v.steps_head + step_row * p.rows.v.steps_row);
     issue_key = part.first_key;
-    const int key = issue_key + (kAligned ? 0 : lane & 15);
+    const int key = issue_key + (kAligned ? 0 : lane);
     issue_slot = key / a.cache.page_size;
     issue_row = key - issue_slot * a.cache.page_size;
     return true;
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
   // The page of the next tile, looked up one tile ahead of its copies.
   auto look_up = [&]() {
     page_row = issue_row;
-    page = issue_key + (kAligned ? 0 : lane & 15) < part.key_end ? pages[issue_slot] : -1;
+    page = issue_key + (kAligned ? 0 : lane) < part.key_end ? pages[issue_slot] : -1;
     issue_slot += p.step_slots;
     issue_row += p.step_rows;
     if (issue_row >= a.cache.page_size) { issue_row -= a.cache.page_size; ++issue_slot; }
@@ -176,12 +176,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
   auto issue_tile = [&](uint32_t stage) {
     if (issue_key < part.key_end) {
       const uint32_t code_to = stage + code_dst;
-      const int own_key = issue_key + (lane & 15);
+      const int own_key = issue_key + lane;
       const bool inside = page >= 0 && page < a.cache.pages;
       const uint32_t place = inside ? page : 0;
       const uint64_t k_at = static_cast<uint64_t>(place) * p.k_codes.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.k_codes.row;
       const uint64_t v_at = static_cast<uint64_t>(place) * p.v_codes.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.v_codes.row;
-      const uint64_t step_at = static_cast<uint64_t>(place) * step_strides.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * step_strides.row;
+      const uint64_t k_step_at = static_cast<uint64_t>(place) * p.k_steps.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.k_steps.row;
+      const uint64_t v_step_at = static_cast<uint64_t>(place) * p.v_steps.page + static_cast<uint64_t>(static_cast<uint32_t>(page_row)) * p.v_steps.row;
       if (kAligned && inside && issue_key + kTileKeys <= part.key_end) {
         const uint8_t *const k_from = k_base + k_at * 16, *const v_from = v_base + v_at * 16;
 #pragma unroll
@@ -189,7 +190,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           cp_async16_hint(policy, code_to + i * (kRowsAtOnce * S::kRowBytes), k_from + i * kRowsAtOnce * p.rows.k.codes_row, 16u);
           cp_async16_hint(policy, code_to + S::kCodeBytes + i * (kRowsAtOnce * S::kRowBytes), v_from + i * kRowsAtOnce * p.rows.v.codes_row, 16u);
         }
-        cp_async_small<4 * kGroups>(stage + step_dst, step_base + step_at * (4 * kGroups), 4u * kGroups);
+        cp_async_small<4 * kGroups>(stage + step_dst, k_step_base + k_step_at * (4 * kGroups), 4u * kGroups);
+        cp_async_small<4 * kGroups>(stage + step_dst + S::kStepBytes, v_step_base + v_step_at * (4 * kGroups), 4u * kGroups);
       } else {
         if (!inside && own_key < part.key_end) raise_status(a.refused, kRefusedPage);
         const bool mine = inside && own_key < part.key_end;      // other rows are zeros
@@ -209,8 +211,9 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           cp_async16_hint(policy, code_to + i * (kRowsAtOnce * S::kRowBytes), reads ? k_base + k_from : p.rows.k.codes, reads ? 16u : 0u);
           cp_async16_hint(policy, code_to + S::kCodeBytes + i * (kRowsAtOnce * S::kRowBytes), reads ? v_base + v_from : p.rows.v.codes, reads ? 16u : 0u);
         }
-        cp_async_small<4 * kGroups>(stage + step_dst, mine ? step_base + step_at * (4 * kGroups) : reinterpret_cast<const uint8_t *>(p.rows.k.steps),
-                                    mine ? 4u * kGroups : 0u);
+        const uint8_t *const some = reinterpret_cast<const uint8_t *>(p.rows.k.steps);
+        cp_async_small<4 * kGroups>(stage + step_dst, mine ? k_step_base + k_step_at * (4 * kGroups) : some, mine ? 4u * kGroups : 0u);
+        cp_async_small<4 * kGroups>(stage + step_dst + S::kStepBytes, mine ? v_step_base + v_step_at * (4 * kGroups) : some, mine ? 4u * kGroups : 0u);
       }
     }
     cp_async_commit();
@@ -313,17 +316,15 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint8_t *const k_src = ring + stage, *const v_src = k_src + S::kCodeBytes, *const step_src = v_src + S::kCodeBytes;
-      // S^T: keys g and g + 8, rows 2t and 2t + 1
-      float score[kTiles][2][2];                       // [tile][key][row]
-      {
-        uint32_t k_steps[2][kGroups];
+      // S^T: keys g and g + 8 of each block, rows 2t and 2t + 1
+      float score[kTiles][2 * kBlocks][2];             // [tile][key][row]
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
         float dot[kTiles][kGroups][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) load_steps<kGroups>(step_src + (g + 8 * h) * (4 * kGroups), k_steps[h]);
-#pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
-          const uint2 w0 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(g, 2 * gr + (t >> 1)) + 8 * (t & 1));
-          const uint2 w1 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(g + 8, 2 * gr + (t >> 1)) + 8 * (t & 1));
+          const uint2 w0 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(16 * b + g, 2 * gr + (t >> 1)) + 8 * (t & 1));
+          const uint2 w1 = *reinterpret_cast<const uint2 *>(k_src + code_offset<S::kRowBytes>(16 * b + g + 8, 2 * gr + (t >> 1)) + 8 * (t & 1));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) dot[n][gr][0] = dot[n][gr][1] = dot[n][gr][2] = dot[n][gr][3] = 0.f;
 #pragma unroll
@@ -341,23 +342,19 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float step[kGroups], low[kGroups];
-#pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr) {
-            step[gr] = quant_step(k_steps[h][gr], kFormat);
-            low[gr] = quant_low(k_steps[h][gr], kFormat);
-          }
+          uint32_t pairs[kGroups];
+          load_steps<kGroups>(step_src + (16 * b + g + 8 * h) * (4 * kGroups), pairs);
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float x = step[0] * dot[n][0][2 * h + i], y = low[0] * q_sum[n][0][i];
+              float x = quant_step(pairs[0], kFormat) * dot[n][0][2 * h + i], y = quant_low(pairs[0], kFormat) * q_sum[n][0][i];
 #pragma unroll
               for (int gr = 1; gr < kGroups; ++gr) {
-                x = fmaf(step[gr], dot[n][gr][2 * h + i], x);
-                y = fmaf(low[gr], q_sum[n][gr][i], y);
+                x = fmaf(quant_step(pairs[gr], kFormat), dot[n][gr][2 * h + i], x);
+                y = fmaf(quant_low(pairs[gr], kFormat), q_sum[n][gr][i], y);
               }
-              score[n][h][i] = fmaf(x, row_scale[n][i], y);
+              score[n][2 * b + h][i] = fmaf(x, row_scale[n][i], y);
             }
         }
       }
@@ -365,30 +362,35 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int k = 0; k < 2 * kBlocks; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (key0 + g + 8 * h >= part.key_end || key0 + g + 8 * h > last_key[n][i]) score[n][h][i] = -INFINITY;
+              if (key0 + g + 8 * k >= part.key_end || key0 + g + 8 * k > last_key[n][i]) score[n][k][i] = -INFINITY;
       }
-      float v_step[2][kGroups], v_low[2][kGroups];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pairs[kGroups];
-        load_steps<kGroups>(step_src + S::kStepBytes + (g + 8 * h) * (4 * kGroups), pairs);
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          v_step[h][gr] = quant_step(pairs[gr], kFormat);
-          v_low[h][gr] = quant_low(pairs[gr], kFormat);
-        }
-      }
+      float v_step[2 * kBlocks][kGroups], v_low[2 * kBlocks][kGroups];
       float largest_step = 0.f;
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) largest_step = fmaxf(largest_step, fmaxf(v_step[0][gr], v_step[1][gr]));
+      for (int k = 0; k < 2 * kBlocks; ++k) {
+        uint32_t pairs[kGroups];
+        load_steps<kGroups>(step_src + S::kStepBytes + (g + 8 * k) * (4 * kGroups), pairs);
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          v_step[k][gr] = quant_step(pairs[gr], kFormat);
+          v_low[k][gr] = quant_low(pairs[gr], kFormat);
+          largest_step = fmaxf(largest_step, v_step[k][gr]);
+        }
+      }
       bool moves = largest_step > step_limit;
+      float row_top[kTiles][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) moves = moves || fmaxf(score[n][0][i], score[n][1][i]) > bound[n][i];
+        for (int i = 0; i < 2; ++i) {
+          row_top[n][i] = score[n][0][i];
+#pragma unroll
+          for (int k = 1; k < 2 * kBlocks; ++k) row_top[n][i] = fmaxf(row_top[n][i], score[n][k][i]);
+          moves = moves || row_top[n][i] > bound[n][i];
+        }
       if (__any_sync(0xffffffffu, moves)) {
         float factor = 1.f;
 #pragma unroll
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(score[n][0][i], score[n][1][i]);
+            float top = row_top[n][i];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
             float alpha = 1.f;
@@ -424,43 +426,48 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
             }
           }
       }
-      uint32_t p_frag[kTiles][kGroups][2];
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        float pr[2][2];
+      for (int b = 0; b < kBlocks; ++b) {
+        uint32_t p_frag[kTiles][kGroups][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          pr[0][i] = exp2_fast(score[n][0][i] - m_exp[n][i]);
-          pr[1][i] = exp2_fast(score[n][1][i] - m_exp[n][i]);
-          l_run[n][i] += pr[0][i] + pr[1][i];
+        for (int n = 0; n < kTiles; ++n) {
+          float pr[2][2];
 #pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr) low_sum[n][gr][i] = fmaf(pr[0][i], v_low[0][gr], fmaf(pr[1][i], v_low[1][gr], low_sum[n][gr][i]));
+          for (int i = 0; i < 2; ++i) {
+            pr[0][i] = exp2_fast(score[n][2 * b][i] - m_exp[n][i]);
+            pr[1][i] = exp2_fast(score[n][2 * b + 1][i] - m_exp[n][i]);
+            l_run[n][i] += pr[0][i] + pr[1][i];
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr)
+              low_sum[n][gr][i] = fmaf(pr[0][i], v_low[2 * b][gr], fmaf(pr[1][i], v_low[2 * b + 1][gr], low_sum[n][gr][i]));
+          }
+          // p' is rounded to f16, as the product's operands are; p itself, in the sum and beside the lows, is not.
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float weight = v_step[2 * b + h][gr] * v_scale;
+              const __half2 both = __floats2half2_rn(pr[h][0] * weight, pr[h][1] * weight);
+              p_frag[n][gr][h] = transposed(*reinterpret_cast<const uint32_t *>(&both));
+            }
         }
-        // p' is rounded to f16, as the product's operands are; p itself, in the sum and beside the lows, is not.
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr)
+        for (int gr = 0; gr < kGroups; ++gr) {
+          uint32_t x[2][2];                            // keys 2t and 2t + 1 (+ 8): elements 8g .. + 3, .. + 7
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float weight = v_step[h][gr] * v_scale;
-            const __half2 both = __floats2half2_rn(pr[h][0] * weight, pr[h][1] * weight);
-            p_frag[n][gr][h] = transposed(*reinterpret_cast<const uint32_t *>(&both));
+            const int row = 16 * b + 2 * t + 8 * h;
+            const uint32_t w0 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(row, 2 * gr + (g >> 2)) + 4 * (g & 3));
+            const uint32_t w1 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(row + 1, 2 * gr + (g >> 2)) + 4 * (g & 3));
+            x[h][0] = __byte_perm(w0, w1, 0x5410);
+            x[h][1] = __byte_perm(w0, w1, 0x7632);
           }
-      }
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        uint32_t x[2][2];                              // keys 2t and 2t + 1 (+ 8): elements 8g .. + 3, .. + 7
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t u = (j & 1) ? upper_bytes(x[0][j >> 1]) : x[0][j >> 1] & kBoth, w = (j & 1) ? upper_bytes(x[1][j >> 1]) : x[1][j >> 1] & kBoth;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(2 * t + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
-          const uint32_t w1 = *reinterpret_cast<const uint32_t *>(v_src + code_offset<S::kRowBytes>(2 * t + 1 + 8 * h, 2 * gr + (g >> 2)) + 4 * (g & 3));
-          x[h][0] = __byte_perm(w0, w1, 0x5410);
-          x[h][1] = __byte_perm(w0, w1, 0x7632);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t u = (j & 1) ? upper_bytes(x[0][j >> 1]) : x[0][j >> 1] & kBoth, w = (j & 1) ? upper_bytes(x[1][j >> 1]) : x[1][j >> 1] & kBoth;
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u, u & kOdd, w, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
+            for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u, u & kOdd, w, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
+          }
         }
       }
       __syncwarp();   // every lane has read the slot
