@@ -4,16 +4,18 @@
 // tile of 32 keys. At 4.5 bits an element, an SM's share of HBM brings 16 keys of K and V (2304 bytes at head_dim 128) every 99
 // clocks, 396 issue slots of a scheduler for one warp's tile, so nothing may be widened element by element:
 //   codes    are the matrix operands as they are. Bits 0 to 7 of two f16, w & 0x00ff00ff, are (even code + 16 odd code) 2^-24 of two
-//            pairs of elements, w & 0x00f000f0 the odd codes' part (subnormal numbers, which the tensor cores multiply exactly). The
-//            powers of two go into Q, and into the result.
-//   K        S^T = C Q^T, keys on the 16-wide side, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g.
-//            Even codes are the difference of the two (an f16 subtraction: the unit that masks is the one in demand).
-//            The sums over codes are exact up to f32's: Q is scaled to f16 by a power of two of its own a row.
-//   V        O^T = C P^T with step_g folded into the probabilities, p'_g = p step_g 2^e, rounded to f16 (11 bits, whatever the
-//            type), and sum_j p_j low_g,j beside it in f32. e follows the largest step so far, so p' stays below f16's largest.
+//            pairs of elements, w & 0x00f000f0 the odd codes' part (subnormal numbers, which the tensor cores multiply exactly): four
+//            instructions for the eight elements of a word. The powers of two go into Q, and into the result.
+//   K        S^T = C Q^T, keys on the 16-wide side, with the odd codes' share of the even elements' sums taken off by a product with
+//            -Q, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g. The products are exact: Q is scaled
+//            to f16 by a power of two of its own a row.
+//   V        O^T = C P^T, sums with the odd codes in them and sums of those alone as rows of one product, subtracted at the end.
+//            step_g is folded into the probabilities, p'_g = p step_g 2^e, rounded to f16 (11 bits, whatever the type), and
+//            sum_j p_j low_g,j runs beside it in f32. e follows the largest step so far, so p' stays below f16's largest.
 //            P, as S^T leaves it, becomes the other operand by movmatrix; rows of K or V are never transposed: two keys' words
-//            interleaved by halves (prmt) are the pairs that the instruction wants. Sums with the odd codes in them and sums of
-//            those alone are rows of one product, subtracted at the end.
+//            interleaved by halves (prmt) are the pairs that the instruction wants.
+//   four rows  of a sequence or fewer, head_dim 128: Q stands in the columns twice, and P^T in the second four carries the second
+//            group's steps, so a lane weighs its probabilities for one group.
 //   maximum  The exponent's reference moves only when a score is beyond 2^8 times it: one vote a tile instead of shuffles.
 // A CTA is four warps; each streams every fourth 16-key tile of the share through a ring of its own (cp.async, rows XOR-swizzled).
 // Bound: HBM, then the warps' instructions.
@@ -30,7 +32,8 @@ constexpr int kStepKeys = kWarps * kTileKeys;
 constexpr int kUnitSteps = 5;
 constexpr int kLeastSteps = 2;
 constexpr float kMovesBeyond = 8.f;             // log2
-constexpr float kScaledSteps = 255.f;           // p' = p step 2^e <= 2^8 * 255 < 65504
+constexpr int kStepExponent = 5;                // of step 2^e when e is chosen; steps of twice that do not move it, so p' < 2^8 2^7
+constexpr int kLeastExponent = -120, kMostExponent = 60;         // of 2^e, so that sums with it stay in f32
 constexpr uint32_t kBoth = 0x00ff00ffu, kOdd = 0x00f000f0u;
 
 template <int kD>
@@ -44,12 +47,13 @@ struct QuantShape {
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kRecord = kRowRecord<kD>;
   static constexpr int kRecordsOff = kWarps * kRingBytes;
-  static constexpr int kSmemBytes = kRecordsOff + kWarps * 8 * kRecord * 4;
+  static constexpr int kQueryOff = kRecordsOff + kWarps * 8 * kRecord * 4;
+  static constexpr int smem_bytes(int rows) { return kQueryOff + (rows > 8 ? 2 : 1) * kGroups * 8 * 128; }   // operands of Q
   static_assert(kStageBytes % 128 == 0, "tiles begin on 128 bytes");
 };
-// CTAs to an SM: as many as the registers of a thread allow (tiles of 8 rows, of 16).
-constexpr int ctas_per_sm(bool narrow) { return narrow ? 3 : 2; }
-static_assert(3 * (QuantShape<128>::kSmemBytes + 512 + 1024) <= 228 * 1024, "three CTAs to an SM");
+// CTAs to an SM: as many as the registers of a thread allow.
+constexpr int ctas_per_sm(int rows) { return rows <= 8 ? 3 : 2; }
+static_assert(3 * (QuantShape<128>::smem_bytes(8) + 256 + 1024) <= 228 * 1024, "three CTAs to an SM");
 
 // Strides small enough for one 32-bit product: codes in 16 bytes, steps in a row's steps.
 struct ShortStrides {
@@ -92,10 +96,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 // Bytes 1 and 3 as bytes 0 and 2.
 __device__ __forceinline__ uint32_t upper_bytes(uint32_t v) { return __byte_perm(v, 0u, 0x4341); }
-__device__ __forceinline__ uint32_t subtract_f16x2(uint32_t a, uint32_t b) {
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-  return *reinterpret_cast<const uint32_t *>(&d);
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
@@ -107,12 +107,16 @@ __device__ __forceinline__ float power_against(float x, int exponent) {
   return __uint_as_float(static_cast<uint32_t>(min(max(field, 1), 254)) << 23);
 }
 
-// kTiles tiles of eight rows.
-template <bool kBf16, int kD, int kTiles, bool kAligned, bool kClustered>
-__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attention_quantized_rows_kernel(const __grid_constant__ QuantRowsParams p) {
+// Tiles of kRows rows: 4, 8 or 16.
+template <bool kBf16, int kD, int kRows, bool kAligned, bool kClustered>
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_quantized_rows_kernel(const __grid_constant__ QuantRowsParams p) {
   using S = QuantShape<kD>;
   constexpr int kFormat = kBf16 ? WB200_BF16 : WB200_F16;
-  constexpr int kRows = 8 * kTiles, kGroups = S::kGroups;
+  constexpr int kMantissa = kBf16 ? 7 : 10, kExponentBias = kBf16 ? 127 : 15;
+  constexpr int kGroups = S::kGroups, kTiles = kRows == 16 ? 2 : 1;          // eight columns of the products each
+  constexpr bool kTwice = kRows == 4;                  // columns 4 to 7 are the same rows, for the second group of V
+  constexpr int kWeighed = kTwice ? 1 : kGroups;       // groups that a lane weighs its probabilities for
+  static_assert(!kTwice || kGroups == 2, "two groups share the columns");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long warp_totals[kWarps], start_prefix;
   __shared__ int start_sequence;
@@ -130,6 +134,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
   uint8_t *const ring = smem + warp * S::kRingBytes;
   const uint32_t ring_addr = smem_u32(ring);
   float *records = reinterpret_cast<float *>(smem + S::kRecordsOff);   // [warp][8][kRecord]
+  uint32_t *operands = reinterpret_cast<uint32_t *>(smem + S::kQueryOff);
 
   // Of the walk's part this warp takes every fourth tile.
   struct Part : RowsPart {
@@ -231,24 +236,26 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
   bool more = next_part();
   if (more) fill_ring();
   while (more) {
-    // A lane's rows are 2t and 2t + 1 of each tile, its elements 8g .. 8g + 7 of each group: acc[.][.][i] holds the sums over both codes of
-    // elements 2i and 2i + 1 (two rows), and over the odd ones (two rows).
-    float m_exp[kTiles][2], bound[kTiles][2];          // the reference, 0 as long as there is none; scores beyond the bound move it
-    float l_run[kTiles][2], low_sum[kTiles][kGroups][2], acc[kTiles][kGroups][4][4];
+    // A lane's columns are 2t and 2t + 1 of each eight, its elements 8g .. 8g + 7 of each group: acc[.][.][i] holds the sums over both
+    // codes of elements 2i and 2i + 1 (two columns), and over the odd ones (two columns). A column's row: column_row().
+    auto column_row = [](int column) { return kTwice ? column & 3 : column; };
+    const int own_group = kTwice ? t >> 1 : 0;         // the first that this lane weighs for
+    float minus_reference[kTiles][2], bound[kTiles][2];          // of the exponent, e in it; relative scores beyond the bound move it
+    float l_run[kTiles][2], low_sum[kTiles][kWeighed][2], acc[kTiles][kGroups][4][4];
     float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of the sums over codes; of the lows
-    uint32_t q_frag[kTiles][kGroups][4][2];
+    uint32_t q_frag[kTiles][kGroups][2][2][2], q_fix[kTiles][kGroups][2][2];
     int last_key[kTiles][2];                           // that the row sees
-    float v_scale = 1.f, step_limit = 0.f;             // 2^e; steps beyond the limit move it (no step yet: any)
+    int exponent = 0;                                  // e
+    uint32_t step_limit = 0;                           // bits of a step; greater ones move e
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      // The row's elements 64 gr + 16 t + .. of this lane's row g of the tile, scaled by a power of two that brings the row's largest to
-      // 2^14, and those that meet codes times 2^-20 to a sixteenth of that.
-      const int packed = part.row0 + 8 * n + g, token = packed / p.group;
+      // The row's elements 64 gr + 16 t + .. of this lane's column g.
+      const int packed = part.row0 + 8 * n + column_row(g), token = packed / p.group;
       uint4 bits[kGroups][2];
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
         bits[gr][0] = bits[gr][1] = make_uint4(0u, 0u, 0u, 0u);
-        if (8 * n + g < part.rows) {
+        if (8 * n + column_row(g) < part.rows) {
           const uint4 *row = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + static_cast<int64_t>(part.sequence.begin + token) * a.q_token +
                                                              (part.kv_head * p.group + packed - token * p.group) * a.q_head + gr * kQuantGroup + 16 * t);
           bits[gr][0] = row[0];
@@ -275,38 +282,54 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
       }
 #pragma unroll
       for (int off = 1; off < 4; off <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+      // Scaled by a power of two that brings the row's largest to 2^14, and those that meet odd codes, 16 times as large, to a sixteenth.
+      // The operands are the same for all warps, who make a part of them each.
       const float power = largest > 0.f && largest < INFINITY ? power_against(largest, 14) : 1.f;
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < 2; ++w) {
+          if (((n * kGroups + gr) * 2 + w) % kWarps != warp) continue;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int e = 8 * w + 2 * h;
             const __half2 even = __floats2half2_rn(element(gr, e) * power, element(gr, e + 4) * power);
             const __half2 odd = __floats2half2_rn(element(gr, e + 1) * (power * 0.0625f), element(gr, e + 5) * (power * 0.0625f));
-            q_frag[n][gr][2 * w + h][0] = *reinterpret_cast<const uint32_t *>(&even);
-            q_frag[n][gr][2 * w + h][1] = *reinterpret_cast<const uint32_t *>(&odd);
+            operands[((((n * kGroups + gr) * 2 + w) * 2 + h) * 2 + 0) * 32 + lane] = *reinterpret_cast<const uint32_t *>(&even);
+            operands[((((n * kGroups + gr) * 2 + w) * 2 + h) * 2 + 1) * 32 + lane] = *reinterpret_cast<const uint32_t *>(&odd);
           }
+        }
       const float scale = p.scale_log2 * (0x1p24f / power);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         row_scale[n][i] = __shfl_sync(0xffffffffu, scale, 4 * (2 * t + i));
         bound[n][i] = -INFINITY;
-        m_exp[n][i] = 0.f;
+        minus_reference[n][i] = 0.f;
         l_run[n][i] = 0.f;
-        last_key[n][i] = paged_visible(part.sequence, (part.row0 + 8 * n + 2 * t + i) / p.group, a.causal) - 1;
+        last_key[n][i] = paged_visible(part.sequence, (part.row0 + 8 * n + column_row(2 * t + i)) / p.group, a.causal) - 1;
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          q_sum[n][gr][i] = __shfl_sync(0xffffffffu, sums[gr], 4 * (2 * t + i)) * p.scale_log2;
-          low_sum[n][gr][i] = 0.f;
-        }
+        for (int gr = 0; gr < kGroups; ++gr) q_sum[n][gr][i] = __shfl_sync(0xffffffffu, sums[gr], 4 * (2 * t + i)) * p.scale_log2;
+#pragma unroll
+        for (int gr = 0; gr < kWeighed; ++gr) low_sum[n][gr][i] = 0.f;
       }
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][gr][j][0] = acc[n][gr][j][1] = acc[n][gr][j][2] = acc[n][gr][j][3] = 0.f;
     }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) q_frag[n][gr][w][h][odd] = operands[((((n * kGroups + gr) * 2 + w) * 2 + h) * 2 + odd) * 32 + lane];
+            q_fix[n][gr][w][h] = q_frag[n][gr][w][h][0] ^ 0x80008000u;
+          }
     const int masked_from = min(part.key_end, paged_visible(part.sequence, part.row0 / p.group, a.causal));   // hidden from some row from here on
 
     int stage = 0;                                     // byte offset in the ring
@@ -316,8 +339,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint8_t *const k_src = ring + stage, *const v_src = k_src + S::kCodeBytes, *const step_src = v_src + S::kCodeBytes;
-      // S^T: keys g and g + 8 of each block, rows 2t and 2t + 1
-      float score[kTiles][2 * kBlocks][2];             // [tile][key][row]
+      // S^T: keys g and g + 8 of each block, relative to the reference
+      float score[kTiles][2 * kBlocks][2];             // [tile][key][column]
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         float dot[kTiles][kGroups][4];
@@ -330,13 +353,12 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint32_t x = w ? w0.y : w0.x, y = w ? w1.y : w1.x;
+            const uint32_t x0 = x & kBoth, x1 = upper_bytes(x), y0 = y & kBoth, y1 = upper_bytes(y);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t xs = h ? upper_bytes(x) : x & kBoth, ys = h ? upper_bytes(y) : y & kBoth;
-              const uint32_t x_odd = xs & kOdd, y_odd = ys & kOdd, x_even = subtract_f16x2(xs, x_odd), y_even = subtract_f16x2(ys, y_odd);
-#pragma unroll
-              for (int n = 0; n < kTiles; ++n)
-                mma_f16(dot[n][gr], x_even, y_even, x_odd, y_odd, q_frag[n][gr][2 * w + h][0], q_frag[n][gr][2 * w + h][1]);
+            for (int n = 0; n < kTiles; ++n) {
+              mma_f16(dot[n][gr], x0, y0, x0 & kOdd, y0 & kOdd, q_frag[n][gr][w][0][0], q_frag[n][gr][w][0][1]);
+              mma_f16(dot[n][gr], x1, y1, x1 & kOdd, y1 & kOdd, q_frag[n][gr][w][1][0], q_frag[n][gr][w][1][1]);
+              mma_f16(dot[n][gr], x0 & kOdd, y0 & kOdd, x1 & kOdd, y1 & kOdd, q_fix[n][gr][w][0], q_fix[n][gr][w][1]);
             }
           }
         }
@@ -348,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float x = quant_step(pairs[0], kFormat) * dot[n][0][2 * h + i], y = quant_low(pairs[0], kFormat) * q_sum[n][0][i];
+              float x = quant_step(pairs[0], kFormat) * dot[n][0][2 * h + i], y = fmaf(quant_low(pairs[0], kFormat), q_sum[n][0][i], minus_reference[n][i]);
 #pragma unroll
               for (int gr = 1; gr < kGroups; ++gr) {
                 x = fmaf(quant_step(pairs[gr], kFormat), dot[n][gr][2 * h + i], x);
@@ -367,20 +389,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
             for (int i = 0; i < 2; ++i)
               if (key0 + g + 8 * k >= part.key_end || key0 + g + 8 * k > last_key[n][i]) score[n][k][i] = -INFINITY;
       }
-      float v_step[2 * kBlocks][kGroups], v_low[2 * kBlocks][kGroups];
-      float largest_step = 0.f;
+      uint32_t v_steps[2 * kBlocks][kWeighed], largest_step = 0;
 #pragma unroll
       for (int k = 0; k < 2 * kBlocks; ++k) {
-        uint32_t pairs[kGroups];
-        load_steps<kGroups>(step_src + S::kStepBytes + (g + 8 * k) * (4 * kGroups), pairs);
+        load_steps<kWeighed>(step_src + S::kStepBytes + (g + 8 * k) * (4 * kGroups) + 4 * own_group, v_steps[k]);
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          v_step[k][gr] = quant_step(pairs[gr], kFormat);
-          v_low[k][gr] = quant_low(pairs[gr], kFormat);
-          largest_step = fmaxf(largest_step, v_step[k][gr]);
-        }
+        for (int gr = 0; gr < kWeighed; ++gr) largest_step = __vmaxu2(largest_step, v_steps[k][gr]);     // steps are not negative: their bits are in order
       }
-      bool moves = largest_step > step_limit;
+      bool moves = (largest_step & 0xffffu) > step_limit;
       float row_top[kTiles][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
@@ -392,14 +408,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           moves = moves || row_top[n][i] > bound[n][i];
         }
       if (__any_sync(0xffffffffu, moves)) {
-        float factor = 1.f;
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) largest_step = fmaxf(largest_step, __shfl_xor_sync(0xffffffffu, largest_step, off));
+        // The references move: to the rows' largest scores where those are beyond the bound, all by the change of e.
+        const int before = exponent;
+        largest_step = __reduce_max_sync(0xffffffffu, largest_step & 0xffffu);
         if (largest_step > step_limit) {
-          const float power = power_against(largest_step, 6);
-          if (step_limit > 0.f) factor = power / v_scale;
-          v_scale = power;
-          step_limit = kScaledSteps / power;
+          const int field = static_cast<int>(largest_step >> kMantissa);
+          exponent = min(max(kStepExponent + kExponentBias - max(field, 1), kLeastExponent), kMostExponent);
+          step_limit = (static_cast<uint32_t>(field + 2) << kMantissa) - 1;
         }
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
@@ -408,46 +423,50 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
             float top = row_top[n][i];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            float alpha = 1.f;
+            float shift = bound[n][i] == -INFINITY ? 0.f : static_cast<float>(before - exponent), alpha = exp2_fast(-shift);
             if (top > bound[n][i]) {
-              alpha = exp2_fast(bound[n][i] - kMovesBeyond - top);   // 0 at first
-              m_exp[n][i] = top;
-              bound[n][i] = top + kMovesBeyond;
+              shift = top - static_cast<float>(exponent);
+              alpha = bound[n][i] == -INFINITY ? 0.f : exp2_fast(-shift);
+              bound[n][i] = 0.f;
             }
+            if (bound[n][i] != -INFINITY) bound[n][i] = kMovesBeyond + static_cast<float>(exponent);
+            minus_reference[n][i] -= shift;
+#pragma unroll
+            for (int k = 0; k < 2 * kBlocks; ++k) score[n][k][i] -= shift;
             l_run[n][i] *= alpha;
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr) {
-              low_sum[n][gr][i] *= alpha;
+            for (int gr = 0; gr < kWeighed; ++gr) low_sum[n][gr][i] *= alpha;
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                acc[n][gr][j][i] *= alpha * factor;
-                acc[n][gr][j][2 + i] *= alpha * factor;
+                acc[n][gr][j][i] *= alpha;
+                acc[n][gr][j][2 + i] *= alpha;
               }
-            }
           }
       }
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        uint32_t p_frag[kTiles][kGroups][2];
+        uint32_t p_frag[kTiles][kWeighed][2];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
           float pr[2][2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            pr[0][i] = exp2_fast(score[n][2 * b][i] - m_exp[n][i]);
-            pr[1][i] = exp2_fast(score[n][2 * b + 1][i] - m_exp[n][i]);
+            pr[0][i] = exp2_fast(score[n][2 * b][i]);
+            pr[1][i] = exp2_fast(score[n][2 * b + 1][i]);
             l_run[n][i] += pr[0][i] + pr[1][i];
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr)
-              low_sum[n][gr][i] = fmaf(pr[0][i], v_low[2 * b][gr], fmaf(pr[1][i], v_low[2 * b + 1][gr], low_sum[n][gr][i]));
+            for (int gr = 0; gr < kWeighed; ++gr)
+              low_sum[n][gr][i] = fmaf(pr[0][i], quant_low(v_steps[2 * b][gr], kFormat), fmaf(pr[1][i], quant_low(v_steps[2 * b + 1][gr], kFormat), low_sum[n][gr][i]));
           }
           // p' is rounded to f16, as the product's operands are; p itself, in the sum and beside the lows, is not.
 #pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr)
+          for (int gr = 0; gr < kWeighed; ++gr)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float weight = v_step[2 * b + h][gr] * v_scale;
-              const __half2 both = __floats2half2_rn(pr[h][0] * weight, pr[h][1] * weight);
+              const float step = quant_step(v_steps[2 * b + h][gr], kFormat);
+              const __half2 both = __floats2half2_rn(pr[h][0] * step, pr[h][1] * step);
               p_frag[n][gr][h] = transposed(*reinterpret_cast<const uint32_t *>(&both));
             }
         }
@@ -466,7 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
           for (int j = 0; j < 4; ++j) {
             const uint32_t u = (j & 1) ? upper_bytes(x[0][j >> 1]) : x[0][j >> 1] & kBoth, w = (j & 1) ? upper_bytes(x[1][j >> 1]) : x[1][j >> 1] & kBoth;
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u, u & kOdd, w, w & kOdd, p_frag[n][gr][0], p_frag[n][gr][1]);
+            for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][gr][j], u, u & kOdd, w, w & kOdd, p_frag[n][kTwice ? 0 : gr][0], p_frag[n][kTwice ? 0 : gr][1]);
           }
         }
       }
@@ -476,42 +495,49 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
       stage += S::kStageBytes;
       if (stage == S::kRingBytes) stage = 0;
     }
+    // The state without e.
+    const float unscale = exp2_fast(static_cast<float>(-exponent));
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           l_run[n][i] += __shfl_xor_sync(0xffffffffu, l_run[n][i], off);
 #pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr) low_sum[n][gr][i] += __shfl_xor_sync(0xffffffffu, low_sum[n][gr][i], off);
+          for (int gr = 0; gr < kWeighed; ++gr) low_sum[n][gr][i] += __shfl_xor_sync(0xffffffffu, low_sum[n][gr][i], off);
         }
+        l_run[n][i] *= unscale;
+        minus_reference[n][i] = bound[n][i] == -INFINITY ? INFINITY : minus_reference[n][i] - static_cast<float>(exponent);
+      }
     // The next part's first tiles are on their way while this one's state is put together. (The ring's groups of copies have all
     // been waited for but the empty ones behind the last tile.)
     const Part done = part;
     more = next_part();
     if (more) fill_ring();
     const bool whole = done.whole();
-    const float unscale = 1.f / v_scale;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {                 // eight rows at a time
       __syncthreads();                                 // the records of the rows before have been read
       float *mine_records = records + warp * (8 * S::kRecord);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        const int row = column_row(2 * t + i);
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
+        for (int gr = 0; gr < kWeighed; ++gr) {
           float v[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[2 * j] = fmaf((acc[n][gr][j][i] - acc[n][gr][j][2 + i]) * 0x1p24f, unscale, low_sum[n][gr][i]);
-            v[2 * j + 1] = fmaf(acc[n][gr][j][2 + i] * 0x1p20f, unscale, low_sum[n][gr][i]);
+            const float both = kTwice && own_group ? acc[n][kGroups - 1][j][i] : acc[n][gr][j][i];
+            const float odd = kTwice && own_group ? acc[n][kGroups - 1][j][2 + i] : acc[n][gr][j][2 + i];
+            v[2 * j] = ((both - odd) * 0x1p24f + low_sum[n][gr][i]) * unscale;
+            v[2 * j + 1] = (odd * 0x1p20f + low_sum[n][gr][i]) * unscale;
           }
-          float4 *to = reinterpret_cast<float4 *>(mine_records + (2 * t + i) * S::kRecord + gr * kQuantGroup + 8 * g);
+          float4 *to = reinterpret_cast<float4 *>(mine_records + row * S::kRecord + (gr + own_group) * kQuantGroup + 8 * g);
           to[0] = make_float4(v[0], v[1], v[2], v[3]);
           to[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
-        if (g == 0) *reinterpret_cast<float2 *>(mine_records + (2 * t + i) * S::kRecord + kD) = make_float2(bound[n][i] == -INFINITY ? -INFINITY : m_exp[n][i], l_run[n][i]);
+        if (g == 0 && own_group == 0) *reinterpret_cast<float2 *>(mine_records + row * S::kRecord + kD) = make_float2(-minus_reference[n][i], l_run[n][i]);
       }
       __syncthreads();
       for (int r = warp; r < 8 && r + 8 * n < done.rows; r += kWarps) {      // a warp per row
@@ -552,24 +578,30 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kTiles == 1)) attenti
 }
 
 using QuantRowsKernel = void (*)(const QuantRowsParams);
-#define WB200_QUANT_ROWS_KERNELS(D, TILES, CLUSTERED)                                                                                   \
-  {{attention_quantized_rows_kernel<false, D, TILES, false, CLUSTERED>, attention_quantized_rows_kernel<false, D, TILES, true, CLUSTERED>}, \
-   {attention_quantized_rows_kernel<true, D, TILES, false, CLUSTERED>, attention_quantized_rows_kernel<true, D, TILES, true, CLUSTERED>}}
-const QuantRowsKernel kKernels[2][2][2][2][2] = {      // [clustered][head_dim 128][narrow][bf16][aligned]
-    {{WB200_QUANT_ROWS_KERNELS(64, 2, false), WB200_QUANT_ROWS_KERNELS(64, 1, false)},
-     {WB200_QUANT_ROWS_KERNELS(128, 2, false), WB200_QUANT_ROWS_KERNELS(128, 1, false)}},
-    {{WB200_QUANT_ROWS_KERNELS(64, 2, true), WB200_QUANT_ROWS_KERNELS(64, 1, true)},
-     {WB200_QUANT_ROWS_KERNELS(128, 2, true), WB200_QUANT_ROWS_KERNELS(128, 1, true)}}};
-void (*const kFoldKernels[2][2][2])(const RowsFold) = {      // [head_dim 128][narrow][bf16]
-    {{attention_paged_fold_kernel<false, 64, 16>, attention_paged_fold_kernel<true, 64, 16>},
-     {attention_paged_fold_kernel<false, 64, 8>, attention_paged_fold_kernel<true, 64, 8>}},
-    {{attention_paged_fold_kernel<false, 128, 16>, attention_paged_fold_kernel<true, 128, 16>},
-     {attention_paged_fold_kernel<false, 128, 8>, attention_paged_fold_kernel<true, 128, 8>}}};
+// Tiles of 4, 8 or 16 rows (index 0, 1, 2), the narrowest that a sequence's rows fit, as far as the caller says. Four rows share their
+// columns with a second group, which head_dim 64 has not.
+constexpr int kSizes = 3;
+constexpr int size_rows(int size, int head_dim) { return size == 0 ? (head_dim == 128 ? 4 : 8) : 8 * size; }
+template <bool kBf16, int kD, int kSize, bool kAligned, bool kClustered>
+constexpr QuantRowsKernel rows_kernel() { return attention_quantized_rows_kernel<kBf16, kD, size_rows(kSize, kD), kAligned, kClustered>; }
+#define WB200_QUANT_ROWS_KERNELS(D, SIZE, CLUSTERED)                                                     \
+  {{rows_kernel<false, D, SIZE, false, CLUSTERED>(), rows_kernel<false, D, SIZE, true, CLUSTERED>()},    \
+   {rows_kernel<true, D, SIZE, false, CLUSTERED>(), rows_kernel<true, D, SIZE, true, CLUSTERED>()}}
+#define WB200_QUANT_ROWS_SIZES(D, CLUSTERED) \
+  {WB200_QUANT_ROWS_KERNELS(D, 0, CLUSTERED), WB200_QUANT_ROWS_KERNELS(D, 1, CLUSTERED), WB200_QUANT_ROWS_KERNELS(D, 2, CLUSTERED)}
+const QuantRowsKernel kKernels[2][2][kSizes][2][2] = {      // [clustered][head_dim 128][size][bf16][aligned]
+    {WB200_QUANT_ROWS_SIZES(64, false), WB200_QUANT_ROWS_SIZES(128, false)}, {WB200_QUANT_ROWS_SIZES(64, true), WB200_QUANT_ROWS_SIZES(128, true)}};
+#define WB200_QUANT_FOLDS(D, SIZE) {attention_paged_fold_kernel<false, D, size_rows(SIZE, D)>, attention_paged_fold_kernel<true, D, size_rows(SIZE, D)>}
+void (*const kFoldKernels[2][kSizes][2])(const RowsFold) = {      // [head_dim 128][size][bf16]
+    {WB200_QUANT_FOLDS(64, 0), WB200_QUANT_FOLDS(64, 1), WB200_QUANT_FOLDS(64, 2)},
+    {WB200_QUANT_FOLDS(128, 0), WB200_QUANT_FOLDS(128, 1), WB200_QUANT_FOLDS(128, 2)}};
 
-constexpr int kMostCtas = ctas_per_sm(true);
+constexpr int kMostCtas = ctas_per_sm(8);
 size_t rows_record_bytes(int sm_count) { return static_cast<size_t>(sm_count) * kMostCtas * 2 * 16 * kRowRecord<128> * sizeof(float); }
-// Tiles of 8 rows where a sequence's rows fit one, as far as the caller says.
-bool is_narrow(const AttentionPagedArgs &a) { return static_cast<int64_t>(a.q_heads / a.cache.kv_heads) * (a.batch.max_query > 0 ? a.batch.max_query : 1) <= 8; }
+int size_of(const AttentionPagedArgs &a) {
+  const int64_t rows = static_cast<int64_t>(a.q_heads / a.cache.kv_heads) * (a.batch.max_query > 0 ? a.batch.max_query : 1);
+  return rows <= 4 ? 0 : rows <= 8 ? 1 : 2;
+}
 
 }  // namespace
 
@@ -602,8 +634,8 @@ bool attention_quantized_rows_clustered(const AttentionPagedArgs &a, int sm_coun
 size_t attention_quantized_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kMostCtas * sizeof(RowsSplit); }
 
 wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream) {
-  const bool narrow = is_narrow(a);
-  const unsigned grid = static_cast<unsigned>(sm_count * ctas_per_sm(narrow));
+  const int size = size_of(a), size_row_count = size_rows(size, a.cache.head_dim);
+  const unsigned grid = static_cast<unsigned>(sm_count * ctas_per_sm(size_row_count));
   QuantRowsParams p{};
   p.a = a;
   p.rows = rows;
@@ -624,16 +656,16 @@ wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &a, const 
   static PerDeviceOnce attributes;
   const wb200_status st = attributes.run([]() -> wb200_status {
     for (int d = 0; d < 2; ++d)
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kSizes; ++n)
         for (int b = 0; b < 2; ++b)
           for (int al = 0; al < 2; ++al)
             for (int c = 0; c < 2; ++c)
               WB200_CUDA_CHECK(cudaFuncSetAttribute(kKernels[c][d][n][b][al], cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                    d ? QuantShape<128>::kSmemBytes : QuantShape<64>::kSmemBytes));
+                                                    d ? QuantShape<128>::smem_bytes(size_rows(n, 128)) : QuantShape<64>::smem_bytes(size_rows(n, 64))));
     return WB200_OK;
   });
   if (st != WB200_OK) return st;
-  const size_t smem = wide ? QuantShape<128>::kSmemBytes : QuantShape<64>::kSmemBytes;
+  const size_t smem = wide ? QuantShape<128>::smem_bytes(size_row_count) : QuantShape<64>::smem_bytes(size_row_count);
   const bool aligned = a.cache.page_size % kTileKeys == 0;
   if (attention_quantized_rows_clustered(a, sm_count)) {
     cudaLaunchConfig_t config = {};
@@ -648,11 +680,11 @@ wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &a, const 
     attributes_of[1].val.clusterDim.x = kRowsCluster; attributes_of[1].val.clusterDim.y = 1; attributes_of[1].val.clusterDim.z = 1;
     config.attrs = attributes_of;
     config.numAttrs = 2;
-    WB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kKernels[1][wide][narrow][bf16][aligned], p));
+    WB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kKernels[1][wide][size][bf16][aligned], p));
     return WB200_OK;
   }
-  WB200_CUDA_CHECK(launch_dependent(kKernels[0][wide][narrow][bf16][aligned], grid, kWarps * 32, smem, stream, p));
-  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][narrow][bf16], dim3(grid, narrow ? 8 : 16), a.cache.head_dim, 0, stream, static_cast<const RowsFold &>(p)));
+  WB200_CUDA_CHECK(launch_dependent(kKernels[0][wide][size][bf16][aligned], grid, kWarps * 32, smem, stream, p));
+  WB200_CUDA_CHECK(launch_dependent(kFoldKernels[wide][size][bf16], dim3(grid, size_row_count), a.cache.head_dim, 0, stream, static_cast<const RowsFold &>(p)));
   return WB200_OK;
 }
 
