@@ -161,17 +161,23 @@ wb200_status make_attention_quantized(wb200_backend *backend, const wb200_quanti
 // the keys, which HBM bounds; a row tile of the chunk kernel takes as long for one row as for 128.
 constexpr int kRowsAtMost = 16;
 enum class PagedKernel { general, rows, chunk };
-PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
-  if (!attention_paged_rows_supports(a)) return PagedKernel::general;
+// The most packed rows of one sequence.
+int64_t most_rows(const AttentionPagedArgs &a) {
   int64_t longest = a.batch.max_query > 0 ? a.batch.max_query : (a.batch.tokens <= a.batch.sequences ? 1 : a.batch.tokens);
   if (longest > a.batch.tokens) longest = a.batch.tokens;
-  return longest * (a.q_heads / a.cache.kv_heads) > kRowsAtMost && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
+  return longest * (a.q_heads / a.cache.kv_heads);
+}
+PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
+  if (!attention_paged_rows_supports(a)) return PagedKernel::general;
+  return most_rows(a) > kRowsAtMost && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
 }
 PagedKernel choose_attention_quantized(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows) {
-  return attention_quantized_rows_supports(a, rows) ? PagedKernel::rows : PagedKernel::general;
+  if (!attention_quantized_rows_supports(a, rows)) return PagedKernel::general;
+  return most_rows(a) > kRowsAtMost && attention_quantized_chunk_supports(a, rows) ? PagedKernel::chunk : PagedKernel::rows;
 }
 uint64_t attention_quantized_workspace(PagedKernel kernel, int sm_count) {
-  return kernel == PagedKernel::general ? 0 : attention_quantized_rows_workspace(sm_count);
+  if (kernel == PagedKernel::general) return 0;
+  return kernel == PagedKernel::rows ? attention_quantized_rows_workspace(sm_count) : attention_quantized_chunk_workspace(sm_count);
 }
 uint64_t attention_paged_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;
@@ -368,7 +374,10 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
 uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
                                                    const wb200_attention_paged_params *p) {
   if (!backend) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
-  if (!cache && !batch && !p) return attention_quantized_workspace(PagedKernel::rows, backend->sm_count);
+  if (!cache && !batch && !p) {
+    const uint64_t rows = attention_quantized_rows_workspace(backend->sm_count), chunk = attention_quantized_chunk_workspace(backend->sm_count);
+    return rows > chunk ? rows : chunk;
+  }
   if (!cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
   AttentionPagedArgs a{};
   QuantizedRowsArgs rows;
@@ -390,7 +399,8 @@ wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quant
   DeviceGuard guard(backend->device);
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   if (kernel == PagedKernel::general) st = launch_attention_quantized_general(a, rows, stream);
-  else st = launch_attention_quantized_rows(a, rows, backend->sm_count, stream);
+  else if (kernel == PagedKernel::rows) st = launch_attention_quantized_rows(a, rows, backend->sm_count, stream);
+  else st = launch_attention_quantized_chunk(a, rows, backend->sm_count, stream);
   const bool one = kernel == PagedKernel::general || (kernel == PagedKernel::rows && attention_quantized_rows_clustered(a, backend->sm_count));
   if (st == WB200_OK) backend->launches += one ? 1 : 2;
   return st;

@@ -365,6 +365,10 @@ bool attention_quantized_rows_supports(const AttentionPagedArgs &args, const Qua
 bool attention_quantized_rows_clustered(const AttentionPagedArgs &args, int sm_count);
 size_t attention_quantized_rows_workspace(int sm_count);
 wb200_status launch_attention_quantized_rows(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream);
+// Chunks of tokens on tcgen05 tensor cores (attention_quantized_chunk.cu): two launches.
+bool attention_quantized_chunk_supports(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows);
+size_t attention_quantized_chunk_workspace(int sm_count);
+wb200_status launch_attention_quantized_chunk(const AttentionPagedArgs &args, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream);
 // Few rows per KV head (attention_paged_rows.cu): one launch where `clustered`, else two.
 bool attention_paged_rows_supports(const AttentionPagedArgs &args);
 bool attention_paged_rows_clustered(const AttentionPagedArgs &args, int sm_count);
