@@ -15,8 +15,8 @@
 //            Where the sequence has rows for one tile only, its odd key tiles take the second tile's place, and the two halves
 //            of the state are joined at the end, by both tiles' warps, half of the columns each: a step of one row tile takes
 //            1820 clocks instead of nearly the 3250 of two.
-//   codes    Of a cache held in four bits (kQuantized) four decoder warps, two for K and two for V, take the loaders' place: they read
-//            codes, and write their values, rounded to the type as the products want them, where TMA would write the rows.
+//   codes    Of a cache held in four bits (kQuantized) eight decoder warps, four for K and four for V, take the loaders' place: they
+//            read codes, and write their values, rounded to the type as the products want them, where TMA would write the rows.
 //   shares   All items lie one behind the other on one axis of work, cut into equal shares for the CTAs, so ragged batches and
 //            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A cut near the end of
 //            an item moves to it; others leave f32 records of the item's parts, folded by a second kernel.
@@ -39,10 +39,10 @@ constexpr int kTileM = 128;                     // packed rows per Q tile (TMEM 
 constexpr int kTileN = 128;                     // keys per tile
 constexpr int kBlockBytes = 128 * 128;          // [128 rows][128 B], swizzled
 constexpr int kOutStageBytes = 32 * 128;        // a softmax warp's 32 rows x 64 columns of output
-// Warps: Q and K loader, MMA, V loader, scheduler, 2 x 4 softmax; behind them, for codes, two decoders of K and two of V.
+// Warps: Q and K loader, MMA, V loader, scheduler, 2 x 4 softmax; behind them, for codes, four decoders of K and four of V.
 template <bool kQuantized>
-constexpr int kChunkThreads = kQuantized ? 512 : 384;
-constexpr int kDecoders = 2;                    // warps to an operand
+constexpr int kChunkThreads = kQuantized ? 640 : 384;
+constexpr int kDecoders = 4;                    // warps to an operand
 constexpr int kSegments = 4;                    // segments handed out and not yet taken in by every warp
 template <bool kQuantized>
 constexpr int kReaders = kQuantized ? 10 + 2 * kDecoders : 11;   // warps that take them
@@ -553,8 +553,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   };
 
   // setmaxnreg.inc waits until the CTA's own register pool can supply the request: the totals must fit the launch's.
-  constexpr int kBaseRegs = kQuantized ? 64 : 104, kSoftmaxRegs = kQuantized ? 176 : 200, kDecoderRegs = 96;
-  static_assert(128 * kBaseRegs + 256 * kSoftmaxRegs + (kQuantized ? 128 * kDecoderRegs : 0) <= kThreads * (kQuantized ? 128 : 168),
+  constexpr int kBaseRegs = kQuantized ? 80 : 104, kSoftmaxRegs = kQuantized ? 104 : 200, kDecoderRegs = 96;
+  static_assert(128 * kBaseRegs + 256 * kSoftmaxRegs + (kQuantized ? 256 * kDecoderRegs : 0) <= kThreads * (kQuantized ? 96 : 168),
                 "setmaxnreg totals exceed the launch allocation");
   if (warp < 4) {
   setmaxnreg_dec<kBaseRegs>();
@@ -826,20 +826,21 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
   } else if (kQuantized && warp >= 12) {
     setmaxnreg_dec<kDecoderRegs>();
     if constexpr (kQuantized) {
-      // ------------------------------------------------------------ decoders: K by the first kDecoders warps, V by the others, a part of
-      // a tile's rows each. A lane takes 16 bytes of codes, 32 elements of a row, at a time; the next kAtOnce rows' codes are on
-      // their way while this one's are decoded.
-      constexpr int kLanes = kHd / 32, kRowsAtOnce = 32 / kLanes, kAtOnce = 32 / kRowsAtOnce;       // lanes to a row; a batch is 32 rows
-      constexpr int kMyRows = kTileN / kDecoders, kBatches = kMyRows / 32;
+      // ------------------------------------------------------------ decoders: K by the first kDecoders warps, V by the others, 32 rows of
+      // a tile each. A lane takes 16 bytes of codes, 32 elements of a row, of every kRowsAtOnce-th row. The next tile's codes are on
+      // their way while this one's are decoded, and its pages while those are asked for. The code is the same for K and V, and in one
+      // loop, as all warps' loops together have to stay in the instruction cache.
+      constexpr int kLanes = kHd / 32, kRowsAtOnce = 32 / kLanes, kAtOnce = 32 / kRowsAtOnce;       // lanes to a row
+      static_assert(kDecoders * 32 == kTileN, "32 rows to a decoder");
       const bool is_v = warp >= 12 + kDecoders;
-      const int row0 = ((warp - 12) & (kDecoders - 1)) * kMyRows;
-      const int chunk = lane % kLanes, lane_row = lane / kLanes;
+      const int row0 = ((warp - 12) & (kDecoders - 1)) * 32, chunk = lane % kLanes, lane_row = lane / kLanes;
       const QuantizedRows &rows = is_v ? p.rows.v : p.rows.k;
-      const int page_size = p.a.cache.page_size;
-      // Where the lane's 16-byte chunks go in a row of its batch: 64-column block, and chunks of it. Lanes of the two blocks take their
-      // words in another order, so that eight lanes' stores fall into different banks.
-      const uint32_t dst_block = kHd == 128 ? (chunk >> 1) * kBlockBytes : 0;
-      const int dst_chunk = (chunk & 1) * 4, turned = kHd == 128 ? (chunk >> 1) * 2 : 0;
+      const int page_size = p.a.cache.page_size, tile_slots = kTileN / page_size, tile_rows = kTileN % page_size;
+      // Where the lane's 16 bytes go in a row: 64-column block, and chunks of it. Lanes of the two blocks take their words in another
+      // order, so that eight lanes' stores fall into different banks.
+      const int turned = kHd == 128 ? (chunk >> 1) * 2 : 0;
+      const uint32_t dst = smem_base + L::kRingOff + (kHd == 128 ? (chunk >> 1) * kBlockBytes : 0) + (row0 + lane_row) * 128;
+      const uint32_t dst_chunk = (((chunk & 1) * 4 + turned) ^ (lane_row & 7)) << 4;                // of the first word; rows 8 apart are swizzled alike
       uint32_t position = 0;
       bool ok = true;
       Segment seg;
@@ -848,23 +849,31 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const int *pages = p.a.batch.page_table + seg.sequence * p.a.batch.table_stride;
         const uint8_t *codes = rows.codes + seg.kv_head * rows.codes_head + chunk * 16;
         const uint32_t *steps = rows.steps + seg.kv_head * rows.steps_head + (kHd == 128 ? chunk >> 1 : 0);
-        // The lane's key of a batch, and where it lies; batch n is the n-th of this warp's in the segment.
-        auto batch_key = [&](int n) { return (seg.t0 + n / kBatches) * kTileN + row0 + (n % kBatches) * 32; };
-        auto look_up = [&](int n, int *in_page) {
-          const int key = batch_key(n) + lane, slot = key / page_size;
-          *in_page = key - slot * page_size;
-          return n < tiles * kBatches && key < seg.keys ? pages[slot] : -1;
+        // The lane's key of the tile that is looked up next, and its place.
+        int key = seg.t0 * kTileN + row0 + lane, left = tiles;
+        int slot_of = key / page_size, row_of = key - slot_of * page_size;
+        int page = -1, in_page = 0;
+        bool wanted = false;
+        auto look_up = [&]() {
+          wanted = left > 0 && key < seg.keys;
+          page = wanted ? pages[slot_of] : -1;
+          in_page = row_of;
+          --left;
+          key += kTileN;
+          slot_of += tile_slots;
+          row_of += tile_rows;
+          if (row_of >= page_size) { row_of -= page_size; ++slot_of; }
         };
         uint4 word[kAtOnce];
         uint32_t pair[kAtOnce];
-        auto load = [&](int n, int page, int in_page) {
+        auto load = [&]() {                              // of what was looked up
           const bool inside = page >= 0 && page < p.a.cache.pages;
-          if (!inside && n < tiles * kBatches && batch_key(n) + lane < seg.keys) raise_status(p.a.refused, kRefusedPage);
+          if (wanted && !inside) raise_status(p.a.refused, kRefusedPage);
           const int place = inside ? page : -1;
 #pragma unroll
           for (int u = 0; u < kAtOnce; ++u) {
             const int from = u * kRowsAtOnce + lane_row, row_page = __shfl_sync(0xffffffffu, place, from), row = __shfl_sync(0xffffffffu, in_page, from);
-            word[u] = make_uint4(0u, 0u, 0u, 0u);      // rows without a key, or without a page, are zeros
+            word[u] = make_uint4(0u, 0u, 0u, 0u);        // rows without a key, or without a page, are zeros
             pair[u] = 0u;
             if (row_page >= 0) {
               word[u] = *reinterpret_cast<const uint4 *>(codes + row_page * rows.codes_page + row * rows.codes_row);
@@ -872,25 +881,23 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             }
           }
         };
-        int in_page, page = look_up(0, &in_page);
-        load(0, page, in_page);
-        page = look_up(1, &in_page);
+        look_up();
+        load();
+        look_up();
 #pragma unroll 1
-        for (int n = 0; ok && n < tiles * kBatches; ++n) {
-          const int j = n / kBatches;
+        for (int j = 0; ok && j < tiles; ++j) {
           const uint32_t at = position + ring_place(seg, j, tiles, is_v);
           const int slot = at % L::kSlots;
           uint4 word_now[kAtOnce];
           uint32_t pair_now[kAtOnce];
 #pragma unroll
           for (int u = 0; u < kAtOnce; ++u) { word_now[u] = word[u]; pair_now[u] = pair[u]; }
-          load(n + 1, page, in_page);
-          page = look_up(n + 2, &in_page);
-          if (n % kBatches == 0 && !__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), ((at / L::kSlots) & 1u) ^ 1u, abort_word, 102))) { ok = false; break; }
-          const uint32_t tile = smem_base + L::kRingOff + slot * L::kTileBytes + dst_block;
+          load();
+          look_up();
+          if (!__all_sync(0xffffffffu, mbar_wait(kv_empty(slot), ((at / L::kSlots) & 1u) ^ 1u, abort_word, 102))) { ok = false; break; }
+          const uint32_t tile = dst + slot * L::kTileBytes;
 #pragma unroll
           for (int u = 0; u < kAtOnce; ++u) {
-            const int row = row0 + (n % kBatches) * 32 + u * kRowsAtOnce + lane_row;
             const uint32_t step2 = __byte_perm(pair_now[u], 0u, 0x1010), low2 = __byte_perm(pair_now[u], 0u, 0x3232);
             const uint4 w = word_now[u];
             const uint32_t words[4] = {turned ? w.z : w.x, turned ? w.w : w.y, turned ? w.x : w.z, turned ? w.y : w.w};
@@ -898,14 +905,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             for (int c = 0; c < 4; ++c) {
               uint32_t v[4];
               decode_word<kBf16>(words[c], step2, low2, v);
-              st_shared_v4(tile + row * 128 + (((dst_chunk + (c ^ turned)) ^ (row & 7)) << 4), v);
+              st_shared_v4(tile + u * (kRowsAtOnce * 128) + (dst_chunk ^ (c << 4)), v);
             }
           }
-          if (n % kBatches == kBatches - 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(kv_full(slot));
-          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv_full(slot));
         }
         position += 2 * tiles;
       }
@@ -945,27 +950,47 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         if (!mbar_wait(s_full(t), tiles_done & 1u, abort_word, 110 + t)) { ok = false; break; }
         tc_fence_after();
         const int key0 = key_base + j * key_step;
-        uint32_t r[128];
+        // With eight more warps a thread has no room for its row's 128 scores: it reads them a second time, 32 at a time.
+        uint32_t r[kQuantized ? 32 : 128];
+        const bool masked = key0 + kTileN > masked_from;
+        const int visible_in_tile = row_limit - key0;
+        float raw_max;
+        if constexpr (kQuantized) {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
-        tmem_wait_ld();
-        if (key0 + kTileN > masked_from) {
-          const int visible_in_tile = row_limit - key0;
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_32x32(s_addr + c * 32, r);
+            tmem_wait_ld();
+            if (masked) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > visible_in_tile) r[i] = 0xff800000u;   // -inf
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i > visible_in_tile) r[i] = 0xff800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          }
+          raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i > visible_in_tile) r[i] = 0xff800000u;   // -inf
+          }
+          float mx[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) mx[a] = fmax3(__uint_as_float(r[32 * a]), __uint_as_float(r[32 * a + 1]), __uint_as_float(r[32 * a + 2]));
+#pragma unroll
+          for (int i = 3; i + 1 < 32; i += 2) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) mx[a] = fmax3(mx[a], __uint_as_float(r[32 * a + i]), __uint_as_float(r[32 * a + i + 1]));
+          }
+#pragma unroll
+          for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], __uint_as_float(r[32 * a + 31]));
+          raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         }
-        float mx[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) mx[a] = fmax3(__uint_as_float(r[32 * a]), __uint_as_float(r[32 * a + 1]), __uint_as_float(r[32 * a + 2]));
-#pragma unroll
-        for (int i = 3; i + 1 < 32; i += 2) {
-#pragma unroll
-          for (int a = 0; a < 4; ++a) mx[a] = fmax3(mx[a], __uint_as_float(r[32 * a + i]), __uint_as_float(r[32 * a + i + 1]));
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], __uint_as_float(r[32 * a + 31]));
-        const float raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         m_true = fmaxf(m_true, raw_max * p.scale_log2);
         float alpha = 1.0f;
         const bool moves = m_true - m_ref > kRescaleThreshold, any_moves = __any_sync(0xffffffffu, moves);
@@ -979,9 +1004,19 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t packed[16];
+          const int base = kQuantized ? 0 : 32 * c;
+          if constexpr (kQuantized) {
+            tmem_ld_32x32(s_addr + c * 32, r);
+            tmem_wait_ld();
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i > visible_in_tile) r[i] = 0xff800000u;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const unsigned long long x2 = fma_f32x2(pack_f32x2(__uint_as_float(r[32 * c + i]), __uint_as_float(r[32 * c + i + 1])), scale2, neg_m2);
+            const unsigned long long x2 = fma_f32x2(pack_f32x2(__uint_as_float(r[base + i]), __uint_as_float(r[base + i + 1])), scale2, neg_m2);
             float x0, x1;
             unpack_f32x2(x2, x0, x1);
             const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
