@@ -950,24 +950,29 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         if (!mbar_wait(s_full(t), tiles_done & 1u, abort_word, 110 + t)) { ok = false; break; }
         tc_fence_after();
         const int key0 = key_base + j * key_step;
-        // With eight more warps a thread has no room for its row's 128 scores: it reads them a second time, 32 at a time.
-        uint32_t r[kQuantized ? 32 : 128];
+        // With eight more warps a thread has no room for its row's 128 scores: the last 64 are read for the maximum, and again once the
+        // first 64 have given way to P.
+        uint32_t r[kQuantized ? 64 : 128];
         const bool masked = key0 + kTileN > masked_from;
         const int visible_in_tile = row_limit - key0;
+        auto read_half = [&](int half) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_addr + (2 * half + c) * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (64 * half + i > visible_in_tile) r[i] = 0xff800000u;
+          }
+        };
         float raw_max;
         if constexpr (kQuantized) {
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_32x32(s_addr + c * 32, r);
-            tmem_wait_ld();
-            if (masked) {
+          for (int half = 1; half >= 0; --half) {
+            read_half(half);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * c + i > visible_in_tile) r[i] = 0xff800000u;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+            for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
           }
           raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         } else {
@@ -1004,16 +1009,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t packed[16];
-          const int base = kQuantized ? 0 : 32 * c;
-          if constexpr (kQuantized) {
-            tmem_ld_32x32(s_addr + c * 32, r);
-            tmem_wait_ld();
-            if (masked) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * c + i > visible_in_tile) r[i] = 0xff800000u;
-            }
-          }
+          const int base = kQuantized ? 32 * (c & 1) : 32 * c;
+          if (kQuantized && c == 2) read_half(1);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const unsigned long long x2 = fma_f32x2(pack_f32x2(__uint_as_float(r[base + i]), __uint_as_float(r[base + i + 1])), scale2, neg_m2);
