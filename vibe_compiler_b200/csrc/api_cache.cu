@@ -173,7 +173,10 @@ PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
 }
 PagedKernel choose_attention_quantized(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows) {
   if (!attention_quantized_rows_supports(a, rows)) return PagedKernel::general;
-  return most_rows(a) > kRowsAtMost && attention_quantized_chunk_supports(a, rows) ? PagedKernel::chunk : PagedKernel::rows;
+  // Two tiles of 16 rows a sequence, which read its keys twice, still are the shorter at head_dim 64: 17 sequences of 5000 keys, 4 KV
+  // heads, 32 rows 32 us and 36 us, 48 rows 41 and 36; at head_dim 128, 8 KV heads, 20 rows 81 and 81.
+  const int64_t at_most = a.cache.head_dim == 64 ? 2 * kRowsAtMost : kRowsAtMost;
+  return most_rows(a) > at_most && attention_quantized_chunk_supports(a, rows) ? PagedKernel::chunk : PagedKernel::rows;
 }
 uint64_t attention_quantized_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;

@@ -50,14 +50,18 @@ constexpr int kPParts = 2;
 constexpr int kFirstChunks = 3;                 // 32-key chunks of the first part of P, of 4
 constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
 constexpr int kMaxSequences = 4096;             // staged in shared memory
-// Work, in twelfths of a step of two row tiles (3250 clocks): a key tile of two row tiles, of one (1820 clocks), and what an item
-// costs by itself (its Q, the first scores, the write-out: 4700).
-constexpr int kPairWork = 12, kSingleWork = 7, kItemWork = 18;
+// Work, in twelfths of a step of two row tiles (3250 clocks; 4500 with codes to decode): a key tile of two row tiles, of one (1820
+// clocks; 3050), and what an item costs by itself (its Q, the first scores, the write-out: 4700). With codes, of weights 6 to 9 and 14 to
+// 32 these were the shortest over seven mixed batches (40 decoding sequences beside 8 chunks: 8 and 14 438 us, 7 and 24 425).
+constexpr int kPairWork = 12, kSingleWork = 7;
+template <bool kQuantized>
+constexpr int kItemWork = kQuantized ? 24 : 18;
 constexpr int kLeastWork = 24;                  // no share is made smaller
 constexpr int kLeastCut = 12;                   // a cut this near to an end of an item moves there
 // What cutting items costs a launch: the records' write-out, one more item to begin in each CTA, and the fold behind the last
-// CTA, about 11 us or six steps of two tiles.
-constexpr int kCutWork = 72;
+// CTA, about 11 us or six steps of two tiles (four and a half of the longer ones).
+template <bool kQuantized>
+constexpr int kCutWork = kQuantized ? 54 : 72;
 
 template <int kHd>
 struct Shape {
@@ -220,13 +224,17 @@ __device__ __forceinline__ Item make_item(const ChunkParams &p, int count, int k
   item.steps = max(1, max(item.n0, item.n1));
   return item;
 }
-__device__ __forceinline__ int item_work(const Item &item) { return kItemWork + item.steps * (item.halved ? kSingleWork : kPairWork); }
+template <bool kQuantized>
+__device__ __forceinline__ int item_work(const Item &item) {
+  return kItemWork<kQuantized> + item.steps * (item.halved ? kSingleWork : kPairWork);
+}
 // The key tile that a cut at work `x` of an item falls on; 0 and `steps` are the item's ends.
+template <bool kQuantized>
 __device__ __forceinline__ int cut_tile(const Item &item, int x, int least_cut) {
-  const int all = item_work(item), each = item.halved ? kSingleWork : kPairWork;
-  if (x < kItemWork + least_cut) return 0;
+  const int all = item_work<kQuantized>(item), each = item.halved ? kSingleWork : kPairWork;
+  if (x < kItemWork<kQuantized> + least_cut) return 0;
   if (x + least_cut > all) return item.steps;
-  return min(max((x - kItemWork + each / 2) / each, 1), item.steps - 1);
+  return min(max((x - kItemWork<kQuantized> + each / 2) / each, 1), item.steps - 1);
 }
 
 // A place between two key tiles: in front of tile `tile` of the item.
@@ -364,7 +372,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     if (threadIdx.x == 0) item_count = most_work = 0;
     __syncthreads();
     auto pairs_of = [&](int count) { return (count + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); };
-    auto pair_work = [&](int count, int keys, int pair) { return item_work(make_item(p, count, keys, pair)); };
+    auto pair_work = [&](int count, int keys, int pair) { return item_work<kQuantized>(make_item(p, count, keys, pair)); };
     // A lane per sequence; those of more than four items by the whole warp.
 #pragma unroll 1
     for (int start = warp * 32; start < sequences; start += kThreads) {
@@ -440,7 +448,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
       // much alike by counting, others by what a share can grow by.
       const long long counted = static_cast<long long>(__umul64hi(item_count + grid - 1, p.by_grid)) * most_work;
       const bool alike = 10ll * most_work * item_count <= 13ll * total;
-      const bool whole = alike ? (counted - kCutWork) * shares <= total : most_work <= kCutWork;
+      const bool whole = alike ? (counted - kCutWork<kQuantized>) * shares <= total : most_work <= kCutWork<kQuantized>;
       const int least_cut = static_cast<int>(max(static_cast<long long>(kLeastCut), min(cut_at(1) >> 6, 1ll << 20)));
       const int index = static_cast<int>(blockIdx.x) + warp;
       const long long x = cut_at(index);
@@ -487,8 +495,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
           rest -= __shfl_sync(0xffffffffu, sum, 31);
         }
         const Item item = make_item(p, q.y, q.z, place.pair);
-        const int all = item_work(item);
-        place.tile = whole ? (2 * rest < all ? 0 : item.steps) : cut_tile(item, static_cast<int>(rest), least_cut);
+        const int all = item_work<kQuantized>(item);
+        place.tile = whole ? (2 * rest < all ? 0 : item.steps) : cut_tile<kQuantized>(item, static_cast<int>(rest), least_cut);
         if (warp == 0) {
           if (lane == 0) first_staged = q;
         } else if (place.tile > 0 && place.tile < item.steps) {
@@ -876,8 +884,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             word[u] = make_uint4(0u, 0u, 0u, 0u);        // rows without a key, or without a page, are zeros
             pair[u] = 0u;
             if (row_page >= 0) {
-              word[u] = *reinterpret_cast<const uint4 *>(codes + row_page * rows.codes_page + row * rows.codes_row);
-              pair[u] = steps[row_page * rows.steps_page + row * rows.steps_row];
+              word[u] = __ldcg(reinterpret_cast<const uint4 *>(codes + row_page * rows.codes_page + row * rows.codes_row));
+              pair[u] = __ldcg(steps + row_page * rows.steps_page + row * rows.steps_row);
             }
           }
         };
