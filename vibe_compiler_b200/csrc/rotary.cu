@@ -252,24 +252,25 @@ __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_
     const bool is_v = row - t * heads >= p.cache.kv_heads;
     const int head = row - t * heads - (is_v ? p.cache.kv_heads : 0);
     const bool live = row < all && e0 < a.head_dim && page_of[t] >= 0;
-    float v[8] = {};
+    uint32_t v[4] = {};                                // as it is quantised: two elements to a word
     if (live) {
       const uint16_t *x = x_rows + (first + t) * a.x_token + (p.q_heads + (is_v ? p.cache.kv_heads : 0) + head) * a.x_head;
       Elements<kFormat, kVec> own[8 / kVec];
 #pragma unroll
       for (int i = 0; i < 8 / kVec; ++i) own[i].load(x + e0 + i * kVec);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = own[i / kVec].get(i % kVec);
+      for (int i = 0; i < 4; ++i) v[i] = kWide ? own[0].w[i & (Elements<kFormat, kVec>::kWords - 1)] : own[2 * i / kVec].w[0] | (own[(2 * i + 1) / kVec].w[0] << 16);
       const double2 *turns = fine_angles + t * c.pairs;
       if (!is_v && e0 < 2 * c.pairs) {
+        auto element = [&](int i) { return static_cast<double>(own[i / kVec].get(i % kVec)); };
+        auto rounded = [](double y) { return narrow_bits(static_cast<float>(y), kFormat); };
         if (a.interleaved) {
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
             if (!kWide && e0 + i >= 2 * c.pairs) break;
             const double2 u = turns[(e0 + i) >> 1];
-            const double b = v[i], w = v[i + 1];
-            v[i] = widen_bits(narrow_bits(static_cast<float>(fma(b, u.y, -(w * u.x))), kFormat), kFormat);
-            v[i + 1] = widen_bits(narrow_bits(static_cast<float>(fma(w, u.y, b * u.x)), kFormat), kFormat);
+            const double b = element(i), w = element(i + 1);
+            v[i >> 1] = rounded(fma(b, u.y, -(w * u.x))) | (rounded(fma(w, u.y, b * u.x)) << 16);
           }
         } else {
           Elements<kFormat, kVec> other[8 / kVec];
@@ -284,7 +285,8 @@ __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_
             if (!kWide && e >= 2 * c.pairs) break;
             const double2 u = turns[e < c.pairs ? e : e - c.pairs];
             const double crossed = static_cast<double>(other[i / kVec].get(i % kVec)) * u.x;
-            v[i] = widen_bits(narrow_bits(static_cast<float>(fma(static_cast<double>(v[i]), u.y, e < c.pairs ? -crossed : crossed)), kFormat), kFormat);
+            const uint32_t y = rounded(fma(element(i), u.y, e < c.pairs ? -crossed : crossed));
+            v[i >> 1] = i & 1 ? (v[i >> 1] & 0xffffu) | (y << 16) : (v[i >> 1] & 0xffff0000u) | y;
           }
         }
       }
@@ -299,11 +301,11 @@ __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_
   }
 }
 
-// A block's threads pass over its tokens' heads about twice, so that the blocks of an SM overlap one another's positions, angles,
-// loads and stores; few tokens get a block each.
-int tokens_per_block(const RopeArgs &a, const RotaryConstants &c, int items, int most_angles) {
+// A block's threads pass over its tokens' heads about `passes` times, so that the blocks of an SM overlap one another's positions,
+// angles, loads and stores; few tokens get a block each.
+int tokens_per_block(const RopeArgs &a, const RotaryConstants &c, int items, int passes, int most_angles) {
   const int groups = items < kThreads ? kThreads / items : 1;
-  int per_block = (2 * groups + a.heads - 1) / a.heads;
+  int per_block = (passes * groups + a.heads - 1) / a.heads;
   if (per_block > kMaxTokensPerBlock) per_block = kMaxTokensPerBlock;
   if (c.pairs > 0 && per_block > most_angles / c.pairs) per_block = most_angles / c.pairs;
   while (per_block > 1 && a.tokens / per_block < 148 * 8) --per_block;
@@ -321,7 +323,7 @@ wb200_status launch(RotaryParams p, const RotaryConstants &c, bool aligned, cuda
   // Gradient of 16384 x 40 x 128 bf16 (336 MB, 51 us at the copy rate) and prompts of 13 thousand tokens x 48 heads: 60 / 73 us; four
   // passes of a block 61 / 74, eight 61 / 76, sixteen 72 / 88; two heads of a thread in flight 65 / 84 (58 registers, four blocks to
   // an SM); blocks of 128 threads 67 / 84, of 512 70 / 78.
-  const int per_block = tokens_per_block(a, c, p.items, kMaxAnglesPerBlock);
+  const int per_block = tokens_per_block(a, c, p.items, 2, kMaxAnglesPerBlock);
   p.tokens_per_block = per_block;
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + per_block - 1) / per_block);
   void (*kernel)(const RotaryParams, const RotaryConstants);
@@ -371,7 +373,7 @@ wb200_status launch_rope_append_quantized(const RopeArgs &a, const RotaryConstan
   const bool wide = rows_aligned(a.x, a.x_token, a.x_head, 2) && rows_aligned(a.out, a.out_token, a.out_head, 2) && c.pairs % 8 == 0;
   const int step = wide ? 16 : 2;
   p.items = (a.head_dim + step - 1) / step;
-  p.tokens_per_block = tokens_per_block(a, c, p.items, kMaxQuantizeAngles);
+  p.tokens_per_block = tokens_per_block(a, c, p.items, 4, kMaxQuantizeAngles);
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + p.tokens_per_block - 1) / p.tokens_per_block);
   const bool bf16 = a.format == WB200_BF16;
   const auto kernel = wide ? (bf16 ? rotary_quantize_kernel<WB200_BF16, true> : rotary_quantize_kernel<WB200_F16, true>)
