@@ -582,7 +582,8 @@ wb200_status wb200_cache_read(wb200_backend *backend, const wb200_paged_cache *c
  * group stand
  *   low   its least element,  step  (its largest - low) / 15 in f32, rounded up,      both in `format`, and
  *   codes (x - low) / step in f32, to the nearest of 0 .. 15 (ties to even),
- * for the values low + code * step, each within half a step of its element. A group that holds an infinity or a NaN (or spans
+ * for the values low + code * step, each within half a step of its element (where low + 15 step would be beyond the format's
+ * largest number, step is rounded down). A group that holds an infinity or a NaN (or spans
  * more than f32 does) is NaN as a whole. Element e of a row lies in byte e / 2 of its codes, an even one in the low half;
  * group g's pair is word g of its steps, step in the low half. head_dim is a multiple of 8 up to 256. Attention and pages_copy
  * read these and nothing else, so a cache may be filled by other means too. Rows of codes begin on 4 bytes; on 16, with
@@ -599,8 +600,8 @@ typedef struct wb200_quantized_cache {
   uint32_t bits;            /* 4 */
   wb200_quantized_rows k, v;
 } wb200_quantized_cache;
-/* wb200_rope_append with the K and V rows quantised as they are written. K is turned in f64 and rounded to f32 and to `format`,
- * so that its codes are those of the definition but for angles' last bits. */
+/* wb200_rope_append with the K and V rows quantised as they are written. K is turned to more than f32 (about 46 bits) and rounded to
+ * f32 and to `format`, so that its codes are those that the definition gives an exact rotation. */
 wb200_status wb200_rope_append_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
                                          const wb200_rope_append_params *params);
 /* wb200_cache_read: the values low + code * step, rounded to `format`. */

@@ -22,6 +22,8 @@ def quantized(x):
         wanted = torch.where(whole, span, torch.zeros_like(span)) / torch.full_like(span, 15.0)
         step = wanted.to(dtype)
         step = (step.view(torch.int16) + (step.float() < wanted).to(torch.int16)).view(dtype)
+        beyond = low.double() + 15 * step.double() > torch.finfo(dtype).max                # rounded down where the type ends
+        step = (step.view(torch.int16) - beyond.to(torch.int16)).view(dtype)
         ratio = (part - low[..., None]) / step.float()[..., None]
         code = torch.where((step.float() > 0)[..., None] & whole[..., None], ratio, torch.zeros_like(part)).round().clamp(0, 15)
         codes[..., at] = code.to(torch.uint8)

@@ -146,6 +146,27 @@ def test_elements_are_within_half_a_step(backend, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_at_the_ends_of_the_type_stay_in_it(backend, dtype):
+    """Fifteen steps, rounded up, would lead beyond the type's largest number: the step is rounded down."""
+    largest = torch.finfo(dtype).max
+    low = 0.0 if dtype == torch.bfloat16 else -largest                          # bf16: a wider range leaves f32
+    rows = torch.stack([low * scale + (largest - low) * scale * torch.rand(128, generator=torch.Generator().manual_seed(i)) for i, scale in enumerate([1.0] * 6 + [0.99, 0.5])])
+    rows[:, 3], rows[:, 5] = torch.tensor([low] * 6 + [low * 0.99, low * 0.5]), torch.tensor([largest] * 6 + [largest * 0.99, largest * 0.5])
+    rows[:, 64], rows[:, 127] = rows[:, 3], rows[:, 5]
+    qkv = torch.stack((rows, rows.flip(0), rows), 1).to(dtype).cuda()
+    cache, batch = QuantizedCache.zeros(2, 16, 1, 128, dtype), make_batch([8], [8], 16, 2, 2)[0]
+    backend.rope_append(qkv.view(8, -1), cache, batch, None, q_heads=1)
+    for got, x in zip(backend.cache_read(cache, batch, 8), (qkv[:, 1:2], qkv[:, 2:])):
+        codes, steps = quant.quantized(x)
+        assert torch.equal(got.cpu(), quant.values(codes, steps).float().to(dtype)) and bool(got.isfinite().all())
+        step = steps.double()[..., 0].repeat_interleave(64, -1)
+        # half a step, 15 units in the step's last place where it was rounded down, and the result's rounding
+        eps = torch.finfo(dtype).eps
+        assert bool(((got.cpu().double() - x.cpu().double()).abs() <= step * (0.5 + 15 * eps + 2.0 ** -19) + x.cpu().double().abs() * eps).all())
+    backend.poll()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_groups_without_a_range_and_with_odd_values(backend, dtype):
     """Equal elements, zeros of both signs, the type's largest values, infinities and NaN: what they read back as."""
     largest, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal / 2 ** (7 if dtype == torch.bfloat16 else 10)

@@ -179,29 +179,6 @@ __device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&v)[4]) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
 }
 
-// The eight elements of a word of codes in order: low + code * step in the type, rounded once. A nibble behind the bits of 128 (bf16)
-// or 1024 (f16) is that number and the code.
-template <bool kBf16>
-__device__ __forceinline__ void decode_word(uint32_t word, uint32_t step2, uint32_t low2, uint32_t (&out)[4]) {
-  constexpr uint32_t kMagic = kBf16 ? 0x43004300u : 0x64006400u;
-  const uint32_t upper = word >> 4;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const uint32_t pair = (__byte_perm(word, upper, b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12)) & 0x000f000fu) | kMagic;
-    if constexpr (kBf16) {
-      const uint32_t magic = kMagic;
-      const __nv_bfloat162 code = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&pair), *reinterpret_cast<const __nv_bfloat162 *>(&magic));
-      const __nv_bfloat162 v = __hfma2(code, *reinterpret_cast<const __nv_bfloat162 *>(&step2), *reinterpret_cast<const __nv_bfloat162 *>(&low2));
-      out[b] = *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-      const uint32_t magic = kMagic;
-      const __half2 code = __hsub2(*reinterpret_cast<const __half2 *>(&pair), *reinterpret_cast<const __half2 *>(&magic));
-      const __half2 v = __hfma2(code, *reinterpret_cast<const __half2 *>(&step2), *reinterpret_cast<const __half2 *>(&low2));
-      out[b] = *reinterpret_cast<const uint32_t *>(&v);
-    }
-  }
-}
-
 // Token of a packed row, within its tile.
 __device__ __forceinline__ int token_of(const ChunkParams &p, int row) { return static_cast<int>(row * p.by_group >> 32); }
 // 128-key tiles that Q tile (or pair) whose last token is `last` visits.

@@ -1,7 +1,8 @@
 // K and V rows of a batch's tokens out of the pages of a cache, as they stand there (wb200_cache_read*): the inverse of the append.
 // A row held in four bits is widened and rounded once to the cache's type.
 //
-// A thread keeps to its eight elements of the token's K and V heads and walks the block's tokens, four loads on their way together.
+// A thread keeps to its elements of the token's K and V heads, sixteen where they are codes, eight of 16 bits, and walks the block's
+// tokens, four loads on their way together.
 // Bound: HBM, the rows read and the rows written.
 #include "attention_paged.cuh"
 #include "quantized_rows.cuh"
@@ -25,40 +26,54 @@ struct ReadParams {
 // kWide: 16-byte accesses to every 16-bit row.
 template <int kFormat, bool kQuantized, bool kWide>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
-  __shared__ int page_of[kMaxTokens], row_of[kMaxTokens], sequence_of[kMaxTokens];
+  __shared__ int state_of[kMaxTokens], sequence_of[kMaxTokens];
+  __shared__ int64_t rows_at[2][kMaxTokens], steps_at[2][kMaxTokens];        // of the token's row, of K and of V
   const int first = blockIdx.x * p.tokens_per_block, count = min(p.tokens_per_block, p.batch.tokens - first);
   pdl_wait();
   pdl_launch_dependents();
-  if (threadIdx.x < kMaxTokens) page_of[threadIdx.x] = -1;
+  if (threadIdx.x < kMaxTokens) state_of[threadIdx.x] = 0;
   place_tokens(p.batch, p.cache, first, count, p.refused, sequence_of, [&](int t, int page, int row, int) {
-    page_of[t] = page;
-    row_of[t] = row;
+    state_of[t] = 1;
+    if constexpr (kQuantized) {
+      rows_at[0][t] = page * p.rows.k.codes_page + row * p.rows.k.codes_row;
+      rows_at[1][t] = page * p.rows.v.codes_page + row * p.rows.v.codes_row;
+      steps_at[0][t] = page * p.rows.k.steps_page + row * p.rows.k.steps_row;
+      steps_at[1][t] = page * p.rows.v.steps_page + row * p.rows.v.steps_row;
+    } else {
+      rows_at[0][t] = page * p.cache.k_page + row * p.cache.k_row;
+      rows_at[1][t] = page * p.cache.v_page + row * p.cache.v_row;
+    }
   });
-  const int chunks = (p.cache.head_dim + 7) / 8, items = 2 * p.cache.kv_heads * chunks;
+  constexpr int kOctets = kQuantized ? 2 : 1;          // of elements to an item
+  const int chunks = (p.cache.head_dim + 8 * kOctets - 1) / (8 * kOctets), items = 2 * p.cache.kv_heads * chunks;
 #pragma unroll 1
   for (int item = threadIdx.x; item < items; item += kThreads) {
-    const int row_head = item / chunks, e0 = 8 * (item - row_head * chunks);
+    const int row_head = item / chunks, e0 = 8 * kOctets * (item - row_head * chunks);
     const bool is_v = row_head >= p.cache.kv_heads;
     const int head = row_head - (is_v ? p.cache.kv_heads : 0);
-    uint16_t *const to = static_cast<uint16_t *>(is_v ? p.a.v : p.a.k) + head * (is_v ? p.a.v_head : p.a.k_head) + e0;
     const int64_t to_token = is_v ? p.a.v_token : p.a.k_token;
-    const int width = min(8, p.cache.head_dim - e0);
+    uint16_t *to = static_cast<uint16_t *>(is_v ? p.a.v : p.a.k) + head * (is_v ? p.a.v_head : p.a.k_head) + e0 + first * to_token;
+    const int width = min(8 * kOctets, p.cache.head_dim - e0);
+    const QuantizedRows &r = is_v ? p.rows.v : p.rows.k;
+    const uint8_t *const codes = kQuantized ? r.codes + head * r.codes_head + e0 / 2 : nullptr;
+    const uint32_t *const steps = kQuantized ? r.steps + head * r.steps_head + e0 / kQuantGroup : nullptr;
+    const uint16_t *const plain = static_cast<const uint16_t *>(is_v ? p.cache.v : p.cache.k) + head * (is_v ? p.cache.v_head : p.cache.k_head) + e0;
 #pragma unroll 1
     for (int t0 = 0; t0 < count; t0 += kAtOnce) {
-      uint32_t w[kAtOnce][kQuantized ? 2 : 4];
+      uint32_t w[kAtOnce][kQuantized ? 3 : 4];
       bool live[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         const int t = t0 + u;
-        live[u] = t < count && page_of[t] >= 0;
+        live[u] = t < count && state_of[t];
         if (!live[u]) continue;
         if constexpr (kQuantized) {
-          const QuantizedRows &r = is_v ? p.rows.v : p.rows.k;
-          w[u][0] = *reinterpret_cast<const uint32_t *>(r.codes + page_of[t] * r.codes_page + row_of[t] * r.codes_row + head * r.codes_head + e0 / 2);
-          w[u][1] = r.steps[page_of[t] * r.steps_page + row_of[t] * r.steps_row + head * r.steps_head + e0 / kQuantGroup];
+          const uint32_t *const from = reinterpret_cast<const uint32_t *>(codes + rows_at[is_v][t]);
+          w[u][0] = from[0];
+          w[u][1] = width > 8 ? from[1] : 0u;
+          w[u][2] = steps[steps_at[is_v][t]];
         } else {
-          const uint16_t *from = static_cast<const uint16_t *>(is_v ? p.cache.v : p.cache.k) + page_of[t] * (is_v ? p.cache.v_page : p.cache.k_page) +
-                                 row_of[t] * (is_v ? p.cache.v_row : p.cache.k_row) + head * (is_v ? p.cache.v_head : p.cache.k_head) + e0;
+          const uint16_t *const from = plain + rows_at[is_v][t];
           if constexpr (kWide) {
             *reinterpret_cast<uint4 *>(w[u]) = *reinterpret_cast<const uint4 *>(from);
           } else {
@@ -69,25 +84,26 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
         }
       }
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
+      for (int u = 0; u < kAtOnce; ++u, to += to_token) {
         if (!live[u]) continue;
-        uint32_t out[4];
-        if constexpr (kQuantized) {
-          const float step = quant_step(w[u][1], kFormat), low = quant_low(w[u][1], kFormat);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            out[i] = narrow_bits(quant_value(w[u][0], 2 * i, step, low), kFormat) | (narrow_bits(quant_value(w[u][0], 2 * i + 1, step, low), kFormat) << 16);
-        } else {
+        for (int o = 0; o < kOctets; ++o) {
+          if (8 * o >= width) continue;
+          uint32_t out[4];
+          if constexpr (kQuantized) {
+            decode_word<kFormat == WB200_BF16>(w[u][o], __byte_perm(w[u][2], 0u, 0x1010), __byte_perm(w[u][2], 0u, 0x3232), out);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) out[i] = w[u][i];
-        }
-        uint16_t *const dst = to + (first + t0 + u) * to_token;
-        if constexpr (kWide) {
-          *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-        } else {
+            for (int i = 0; i < 4; ++i) out[i] = w[u][i];
+          }
+          uint16_t *const dst = to + 8 * o;
+          if constexpr (kWide) {
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < width) dst[i] = static_cast<uint16_t>(out[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 8; ++i)
+              if (8 * o + i < width) dst[i] = static_cast<uint16_t>(out[i >> 1] >> (16 * (i & 1)));
+          }
         }
       }
     }

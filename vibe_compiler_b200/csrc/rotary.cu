@@ -172,47 +172,62 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   }
 }
 
-__device__ __forceinline__ double2 sin_cos_of_turns_f64(unsigned long long phase) {
+// Sine and cosine as sums of two f32: (sine, its rest, cosine, its rest).
+__device__ __forceinline__ float4 fine_sin_cos_of_turns(unsigned long long phase, float magnitude) {
   double s, c;
   sincospi(static_cast<double>(static_cast<long long>(phase)) * 0x1p-63, &s, &c);
-  return make_double2(s, c);
+  s *= magnitude;
+  c *= magnitude;
+  const float sine = static_cast<float>(s), cosine = static_cast<float>(c);
+  return make_float4(sine, static_cast<float>(s - sine), cosine, static_cast<float>(c - cosine));
+}
+// a * (x + xr) + b * (y + yr), rounded once to f32: the products and their sum with what they leave (an FMA gives a product's rounding
+// error, Knuth's two-sum a sum's), good to about 2^-46 of the larger product.
+__device__ __forceinline__ float fine_sum(float a, float x, float xr, float b, float y, float yr) {
+  const float p = __fmul_rn(a, x), q = __fmul_rn(b, y), sum = __fadd_rn(p, q), q_part = __fsub_rn(sum, p);
+  const float left = __fadd_rn(__fsub_rn(p, __fsub_rn(sum, q_part)), __fsub_rn(q, q_part));
+  const float products = __fadd_rn(__fmaf_rn(a, x, -p), __fmaf_rn(b, y, -q));
+  return __fadd_rn(sum, __fadd_rn(left, __fmaf_rn(a, xr, __fmaf_rn(b, yr, products))));
 }
 
-// Rows of the fused projection with K and V quantised on the way to their pages. Q as above. Of a K or V row a lane takes eight
-// elements, an octet of lanes a group of 64, whose least and largest element it finds by three shuffles.
-// K is turned in f64 and rounded once to the type: a code is a decision next to a border, and so is a step's rounding, so the f32
-// rotation's last bit would give codes that differ between this kernel and the definition (and any other that follows it) in one
-// group of 30 thousand, by a whole step in an element of ten there. Each of a head's elements costs two f64 operations.
+// Rows of the fused projection with K and V quantised on the way to their pages. Q as above. Of a K or V row a lane takes sixteen
+// elements, a quad of lanes a group of 64, whose least and largest element it finds by two shuffles.
+// K is turned as if in more than f32 and rounded once to f32 and to the type: a code is a decision next to a border, and so is a step's
+// rounding, so the f32 rotation's last bit would give codes that differ between this kernel and the definition (and any other that
+// follows it) in one group of 30 thousand, by a whole step in an element of ten there. It takes fifteen f32 operations an element.
 constexpr int kMaxQuantizeAngles = 1024;
 template <int kFormat, bool kWide>
 __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ QuantizedRowsArgs rows,
                                                                    const __grid_constant__ RotaryConstants c) {
   constexpr int kVec = kWide ? 8 : 1;
   __shared__ float2 angles[kMaxQuantizeAngles];
-  __shared__ double2 fine_angles[kMaxQuantizeAngles];
-  __shared__ int page_of[kMaxTokensPerBlock], row_of[kMaxTokensPerBlock], position_of[kMaxTokensPerBlock];
+  __shared__ float4 fine_angles[kMaxQuantizeAngles];
+  __shared__ int64_t codes_at[2][kMaxTokensPerBlock], steps_at[2][kMaxTokensPerBlock];    // of the token's row, of K and of V
+  __shared__ int state_of[kMaxTokensPerBlock], position_of[kMaxTokensPerBlock];
   __shared__ int sequence_of[kMaxTokensPerBlock];
   const RopeArgs &a = p.a;
   const int first = blockIdx.x * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
   pdl_wait();
   pdl_launch_dependents();
-  if (threadIdx.x < count) page_of[threadIdx.x] = -1;
+  if (threadIdx.x < count) state_of[threadIdx.x] = 0;
   place_tokens(p.batch, p.cache, first, count, p.refused, sequence_of, [&](int t, int page, int row, int position) {
-    page_of[t] = page;
-    row_of[t] = row;
+    state_of[t] = 1;
     position_of[t] = position;
+    codes_at[0][t] = page * rows.k.codes_page + row * rows.k.codes_row;
+    codes_at[1][t] = page * rows.v.codes_page + row * rows.v.codes_row;
+    steps_at[0][t] = page * rows.k.steps_page + row * rows.k.steps_row;
+    steps_at[1][t] = page * rows.v.steps_page + row * rows.v.steps_row;
   });
   for (int i = threadIdx.x; i < count * c.pairs; i += kThreads) {
     const int t = i / c.pairs, pair = i - t * c.pairs;
     long long position;
-    if (!a.positions) position = page_of[t] >= 0 ? position_of[t] : 0;
+    if (!a.positions) position = state_of[t] ? position_of[t] : 0;
     else position = a.position_bytes == 8 ? static_cast<const long long *>(a.positions)[first + t] : static_cast<const int *>(a.positions)[first + t];
     const unsigned long long phase = static_cast<unsigned long long>(position) * c.turns[pair];
     const float2 sc = sin_cos_of_turns(phase);
     angles[i] = make_float2(sc.x * c.magnitude, sc.y * c.magnitude);
-    const double2 fine = sin_cos_of_turns_f64(phase);
-    fine_angles[i] = make_double2(fine.x * c.magnitude, fine.y * c.magnitude);
+    fine_angles[i] = fine_sin_cos_of_turns(phase, c.magnitude);
   }
   __syncthreads();
   const uint16_t *const x_rows = static_cast<const uint16_t *>(a.x);
@@ -224,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_
       while (true) {
         while (head >= p.q_heads) { head -= p.q_heads; ++t; }
         if (t >= count) break;
-        if (page_of[t] >= 0) {
+        if (state_of[t]) {
           const bool rotates = item * kVec < c.pairs;
           const int d0 = (rotates && !a.interleaved ? 1 : 2) * item * kVec, d1 = d0 + (rotates && !a.interleaved ? c.pairs : kVec);
           const bool has1 = d1 + kVec <= a.head_dim;
@@ -241,62 +256,67 @@ __global__ void __launch_bounds__(kThreads) rotary_quantize_kernel(const __grid_
       }
     }
   }
-  // K and V: rows of 8, 16 or 32 lanes, eight elements a lane.
+  // K and V: rows of 4, 8 or 16 lanes, sixteen elements a lane.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int shift = a.head_dim <= 64 ? 3 : a.head_dim <= 128 ? 4 : 5;
+  const int shift = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 3 : 4;
   const int at_once = 32 >> shift, heads = 2 * p.cache.kv_heads, all = count * heads;
-  const int slot = lane & ((1 << shift) - 1), e0 = 8 * slot;
+  const int slot = lane & ((1 << shift) - 1), e0 = 16 * slot, octets = max(0, min(2, (a.head_dim - e0) >> 3));
+  int t = (warp * at_once + (lane >> shift)) / heads, row_head = warp * at_once + (lane >> shift) - t * heads;
 #pragma unroll 1
-  for (int base = warp * at_once; base < all; base += (kThreads / 32) * at_once) {
-    const int row = base + (lane >> shift), t = min(row, all - 1) / heads;
-    const bool is_v = row - t * heads >= p.cache.kv_heads;
-    const int head = row - t * heads - (is_v ? p.cache.kv_heads : 0);
-    const bool live = row < all && e0 < a.head_dim && page_of[t] >= 0;
-    uint32_t v[4] = {};                                // as it is quantised: two elements to a word
-    if (live) {
-      const uint16_t *x = x_rows + (first + t) * a.x_token + (p.q_heads + (is_v ? p.cache.kv_heads : 0) + head) * a.x_head;
+  for (int base = warp * at_once; base < all; base += (kThreads / 32) * at_once, row_head += (kThreads / 32) * at_once) {
+    while (row_head >= heads) { row_head -= heads; ++t; }
+    const bool is_v = row_head >= p.cache.kv_heads;
+    const int head = row_head - (is_v ? p.cache.kv_heads : 0);
+    const int live = t < count && state_of[t] ? octets : 0;
+    uint32_t v[8] = {};                                // as it is quantised: two elements to a word
+    const uint16_t *const x = x_rows + static_cast<int64_t>(first + t) * a.x_token + (p.q_heads + row_head) * a.x_head;
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      if (o >= live) continue;
+      const int e1 = e0 + 8 * o;
       Elements<kFormat, kVec> own[8 / kVec];
 #pragma unroll
-      for (int i = 0; i < 8 / kVec; ++i) own[i].load(x + e0 + i * kVec);
+      for (int i = 0; i < 8 / kVec; ++i) own[i].load(x + e1 + i * kVec);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = kWide ? own[0].w[i & (Elements<kFormat, kVec>::kWords - 1)] : own[2 * i / kVec].w[0] | (own[(2 * i + 1) / kVec].w[0] << 16);
-      const double2 *turns = fine_angles + t * c.pairs;
-      if (!is_v && e0 < 2 * c.pairs) {
-        auto element = [&](int i) { return static_cast<double>(own[i / kVec].get(i % kVec)); };
-        auto rounded = [](double y) { return narrow_bits(static_cast<float>(y), kFormat); };
-        if (a.interleaved) {
+      for (int i = 0; i < 4; ++i) v[4 * o + i] = kWide ? own[0].w[i & (Elements<kFormat, kVec>::kWords - 1)] : own[2 * i / kVec].w[0] | (own[(2 * i + 1) / kVec].w[0] << 16);
+      if (is_v || e1 >= 2 * c.pairs) continue;
+      const float4 *turns = fine_angles + t * c.pairs;
+      auto element = [&](int i) { return own[i / kVec].get(i % kVec); };
+      if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            if (!kWide && e0 + i >= 2 * c.pairs) break;
-            const double2 u = turns[(e0 + i) >> 1];
-            const double b = element(i), w = element(i + 1);
-            v[i >> 1] = rounded(fma(b, u.y, -(w * u.x))) | (rounded(fma(w, u.y, b * u.x)) << 16);
-          }
-        } else {
-          Elements<kFormat, kVec> other[8 / kVec];
-#pragma unroll
-          for (int i = 0; i < 8 / kVec; ++i) {
-            const int e = e0 + i * kVec;
-            if (e < 2 * c.pairs) other[i].load(x + (e < c.pairs ? e + c.pairs : e - c.pairs));
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i;
-            if (!kWide && e >= 2 * c.pairs) break;
-            const double2 u = turns[e < c.pairs ? e : e - c.pairs];
-            const double crossed = static_cast<double>(other[i / kVec].get(i % kVec)) * u.x;
-            const uint32_t y = rounded(fma(element(i), u.y, e < c.pairs ? -crossed : crossed));
-            v[i >> 1] = i & 1 ? (v[i >> 1] & 0xffffu) | (y << 16) : (v[i >> 1] & 0xffff0000u) | y;
-          }
+        for (int i = 0; i < 8; i += 2) {
+          if (!kWide && e1 + i >= 2 * c.pairs) break;
+          const float4 u = turns[(e1 + i) >> 1];
+          const float b = element(i), w = element(i + 1);
+          v[4 * o + (i >> 1)] = narrow_pair<kFormat>(fine_sum(b, u.z, u.w, -w, u.x, u.y), fine_sum(w, u.z, u.w, b, u.x, u.y));
         }
+      } else {
+        Elements<kFormat, kVec> other[8 / kVec];
+#pragma unroll
+        for (int i = 0; i < 8 / kVec; ++i) {
+          const int e = e1 + i * kVec;
+          if (e < 2 * c.pairs) other[i].load(x + (e < c.pairs ? e + c.pairs : e - c.pairs));
+        }
+        // Only rows with narrow accesses have elements that are copied beside others that are turned.
+        auto turned = [&](int i) {
+          const int e = e1 + i;
+          if (!kWide && e >= 2 * c.pairs) return element(i);
+          const float4 u = turns[e < c.pairs ? e : e - c.pairs];
+          const float partner = other[i / kVec].get(i % kVec);
+          return fine_sum(element(i), u.z, u.w, e < c.pairs ? -partner : partner, u.x, u.y);
+        };
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) v[4 * o + (i >> 1)] = narrow_pair<kFormat>(turned(i), turned(i + 1));
       }
     }
     uint32_t pair;
-    const uint32_t word = quantize8<kFormat>(v, live, &pair);
-    if (live) {
+    const uint2 words = quantize16<kFormat>(v, live, &pair);
+    if (live > 0) {
       const QuantizedRows &to = is_v ? rows.v : rows.k;
-      *reinterpret_cast<uint32_t *>(to.codes + page_of[t] * to.codes_page + row_of[t] * to.codes_row + head * to.codes_head + 4 * slot) = word;
-      if ((slot & 7) == 0) to.steps[page_of[t] * to.steps_page + row_of[t] * to.steps_row + head * to.steps_head + (slot >> 3)] = pair;
+      uint32_t *codes = reinterpret_cast<uint32_t *>(to.codes + codes_at[is_v][t] + head * to.codes_head) + 2 * slot;
+      codes[0] = words.x;
+      if (live > 1) codes[1] = words.y;
+      if ((slot & 3) == 0) to.steps[steps_at[is_v][t] + head * to.steps_head + (slot >> 2)] = pair;
     }
   }
 }
