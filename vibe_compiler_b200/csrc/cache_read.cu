@@ -44,23 +44,26 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
       rows_at[1][t] = page * p.cache.v_page + row * p.cache.v_row;
     }
   });
-  constexpr int kOctets = kQuantized ? 2 : 1;          // of elements to an item
-  const int chunks = (p.cache.head_dim + 8 * kOctets - 1) / (8 * kOctets), items = 2 * p.cache.kv_heads * chunks;
+  // Octets of elements to an item: of codes one of each half of the row, so that both are stored by lanes side by side.
+  constexpr int kOctets = kQuantized ? 2 : 1;
+  const int octets = (p.cache.head_dim + 7) / 8, chunks = (octets + kOctets - 1) / kOctets, items = 2 * p.cache.kv_heads * chunks;
 #pragma unroll 1
   for (int item = threadIdx.x; item < items; item += kThreads) {
-    const int row_head = item / chunks, e0 = 8 * kOctets * (item - row_head * chunks);
+    const int row_head = item / chunks, chunk = item - row_head * chunks, e0 = 8 * chunk;
     const bool is_v = row_head >= p.cache.kv_heads;
     const int head = row_head - (is_v ? p.cache.kv_heads : 0);
     const int64_t to_token = is_v ? p.a.v_token : p.a.k_token;
     uint16_t *to = static_cast<uint16_t *>(is_v ? p.a.v : p.a.k) + head * (is_v ? p.a.v_head : p.a.k_head) + e0 + first * to_token;
-    const int width = min(8 * kOctets, p.cache.head_dim - e0);
+    const int width = min(8, p.cache.head_dim - e0);
+    const bool both = kOctets == 2 && chunk + chunks < octets;
     const QuantizedRows &r = is_v ? p.rows.v : p.rows.k;
     const uint8_t *const codes = kQuantized ? r.codes + head * r.codes_head + e0 / 2 : nullptr;
-    const uint32_t *const steps = kQuantized ? r.steps + head * r.steps_head + e0 / kQuantGroup : nullptr;
+    const uint32_t *const steps = kQuantized ? r.steps + head * r.steps_head + chunk / (kQuantGroup / 8) : nullptr;
+    const int next_step = (chunk + chunks) / (kQuantGroup / 8) - chunk / (kQuantGroup / 8);
     const uint16_t *const plain = static_cast<const uint16_t *>(is_v ? p.cache.v : p.cache.k) + head * (is_v ? p.cache.v_head : p.cache.k_head) + e0;
 #pragma unroll 1
     for (int t0 = 0; t0 < count; t0 += kAtOnce) {
-      uint32_t w[kAtOnce][kQuantized ? 3 : 4];
+      uint32_t w[kAtOnce][4];                          // of codes two words and two pairs of steps
       bool live[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
@@ -70,8 +73,11 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
         if constexpr (kQuantized) {
           const uint32_t *const from = reinterpret_cast<const uint32_t *>(codes + rows_at[is_v][t]);
           w[u][0] = from[0];
-          w[u][1] = width > 8 ? from[1] : 0u;
-          w[u][2] = steps[steps_at[is_v][t]];
+          w[u][1] = steps[steps_at[is_v][t]];
+          if (both) {
+            w[u][2] = from[chunks];
+            w[u][3] = steps[steps_at[is_v][t] + next_step];
+          }
         } else {
           const uint16_t *const from = plain + rows_at[is_v][t];
           if constexpr (kWide) {
@@ -88,21 +94,21 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
         if (!live[u]) continue;
 #pragma unroll
         for (int o = 0; o < kOctets; ++o) {
-          if (8 * o >= width) continue;
+          if (o > 0 && !both) continue;
           uint32_t out[4];
           if constexpr (kQuantized) {
-            decode_word<kFormat == WB200_BF16>(w[u][o], __byte_perm(w[u][2], 0u, 0x1010), __byte_perm(w[u][2], 0u, 0x3232), out);
+            decode_word<kFormat == WB200_BF16>(w[u][2 * o], __byte_perm(w[u][2 * o + 1], 0u, 0x1010), __byte_perm(w[u][2 * o + 1], 0u, 0x3232), out);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) out[i] = w[u][i];
           }
-          uint16_t *const dst = to + 8 * o;
+          uint16_t *const dst = to + 8 * chunks * o;
           if constexpr (kWide) {
             *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (8 * o + i < width) dst[i] = static_cast<uint16_t>(out[i >> 1] >> (16 * (i & 1)));
+              if (o > 0 || i < width) dst[i] = static_cast<uint16_t>(out[i >> 1] >> (16 * (i & 1)));
           }
         }
       }
