@@ -642,17 +642,16 @@ class B200TargetModelBackend:
         shape, dtype = (tokens, *cache.shape[2:]), cache.dtype
         if stream is None:
             stream = torch._C._cuda_getCurrentRawStream(device)
-        if out is None:
-            like = batch.key_lengths
-            out = self._empty(like, shape, stream, dtype), self._empty(like, shape, stream, dtype)
+        if out is None:                                    # one allocation for both
+            both = self._empty(batch.key_lengths, (2, *shape), stream, dtype)
+            out, at, row = both.unbind(0), both.data_ptr(), shape[1] * shape[2]
+            fields = at, at + tokens * row * both.element_size(), row, shape[2], row, shape[2]
         else:
-            out = tuple(out)
-            if len(out) != 2:
-                raise ValueError("out must be a pair (k, v)")
-            self._check_rows("out[0]", out[0], shape, dtype)
-            self._check_rows("out[1]", out[1], shape, dtype)
-        k, v = out
-        p = abi.CacheReadParams.from_buffer_copy(_READ_PACK(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], stream))
+            k, v = out = tuple(out)
+            self._check_rows("out[0]", k, shape, dtype)
+            self._check_rows("out[1]", v, shape, dtype)
+            fields = k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2]
+        p = abi.CacheReadParams.from_buffer_copy(_READ_PACK(*fields, stream))
         call = self._lib.wb200_cache_read_quantized if cache.quantized else self._lib.wb200_cache_read
         self._check(call(self._handle, C.byref(cache._desc), C.byref(batch._desc(tokens)), C.byref(p)))
         return out
