@@ -284,6 +284,23 @@ def test_attention_matches_float64(backend, dtype, causal, lengths, news, size, 
         agree(backend, q, cache, hinted, head_dim ** -0.5, causal=causal, zero_fully_masked=max_query == 1)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size,hq,hk,head_dim", [(16, 32, 8, 128), (32, 8, 8, 128), (48, 28, 4, 128), (5, 16, 1, 128), (64, 16, 4, 64), (7, 8, 8, 64), (16, 9, 3, 80)])
+@pytest.mark.parametrize("lengths", [[700, 64, 65, 2000, 0, 1], [33], [9000, 129, 31]])
+def test_few_tokens_take_scores_to_f32(backend, dtype, size, hq, hk, head_dim, lengths):
+    """Without rounded keys: scores to f32's bound, in the log-sum-exp too, and probabilities to f16's (kept in f32 at other head
+    dimensions), whatever the type."""
+    pages = sum(-(-n // size) for n in lengths) + 3
+    cache = make_quantized(pages, size, hk, head_dim, dtype, seed=4)
+    for n in range(1, max(1, 16 * hk // hq) + 1):
+        batch, tokens = make_batch([x + n for x in lengths], [n] * len(lengths), size, pages + len(lengths) * (1 + n // size), 2)
+        batch.page_table.clamp_(max=pages - 1)       # sequences may share pages that are only read
+        q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(n)).to(dtype).cuda()
+        q[0] *= 2.0 ** -12                           # a row of small scores beside others
+        hinted = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=n)
+        agree(backend, q, cache, hinted, head_dim ** -0.5, kernel="rows" if head_dim != 80 else "general")
+
+
 @pytest.mark.parametrize("layout", ["rows", "heads", "joined"])
 @pytest.mark.parametrize("lengths,news", [([300, 1000], [1, 1]), ([300, 1000], [3, 4]), ([300, 1000], [200, 150])])
 def test_layouts_and_strides(backend, layout, lengths, news):

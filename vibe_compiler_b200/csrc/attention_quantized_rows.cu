@@ -29,7 +29,9 @@ constexpr int kWarps = 4;
 constexpr int kBlocks = 2;                      // of 16 keys, a side of the matrix instruction, in a warp's tile
 constexpr int kTileKeys = 16 * kBlocks;
 constexpr int kStepKeys = kWarps * kTileKeys;
-constexpr int kUnitSteps = 5;
+// What a unit costs by itself, in steps of 128 keys: 100 sequences of 100 to 4000 keys, 8 KV heads, with 1 / 2 / 3 / 5 / 8 76 / 69 / 67 /
+// 70 / 73 us, 100 of 20 to 1000 34 / 30 / 29 / 30 / 31.
+constexpr int kUnitSteps = 3;
 constexpr int kLeastSteps = 2;
 constexpr float kMovesBeyond = 8.f;             // log2
 constexpr int kStepExponent = 5;                // of step 2^e when e is chosen; steps of twice that do not move it, so p' < 2^8 2^7
@@ -622,13 +624,16 @@ bool attention_quantized_rows_supports(const AttentionPagedArgs &a, const Quanti
   return (bits & 15u) == 0 && (steps & (step_bytes - 1)) == 0;     // rows begin on 16 bytes, a row's steps on their size
 }
 
-// Clusters where all units' are resident at once and, at the longest the page table can hold, an eighth of a unit's keys through one CTA
-// does not take longer than all keys through the whole GPU and the second launch.
+// Clusters where all units' are resident at once and, at the longest the page table can hold, an eighth of a unit's keys go through one
+// CTA (16 bytes / ns) in 8 us: the second launch costs about 3, and beyond, equal shares for the whole GPU are the shorter. One launch
+// and two, head_dim 128, 16-row pages, per call in a graph: 1 x 8 KV heads, 500 / 2000 / 4000 / 16000 keys 6.6 / 8.0 / 9.9 / 23.4 and
+// 9.6 / 10.6 / 11.7 / 17.0 us; 3 x 4 7.3 / 8.5 / 10.7 / 24.2 and 11.9 / 12.7 / 13.5 / 20.2; 4 x 8 8.2 / 10.0 / 13.1 / 33.3 and
+// 10.6 / 12.9 / 14.7 / 29.4.
 bool attention_quantized_rows_clustered(const AttentionPagedArgs &a, int sm_count) {
   const int64_t units = static_cast<int64_t>(a.batch.sequences) * a.cache.kv_heads;
   if (units * kRowsCluster > sm_count * 2 * 7 / 8) return false;
   const double unit_bytes = (a.cache.head_dim + 8.0 * (a.cache.head_dim / kQuantGroup)) * a.cache.page_size * a.batch.table_width;
-  return unit_bytes / kRowsCluster / 20.0 <= static_cast<double>(units) * unit_bytes / 5500.0 + 4000.0;
+  return unit_bytes / kRowsCluster / 16.0 <= 8000.0;
 }
 
 size_t attention_quantized_rows_workspace(int sm_count) { return rows_record_bytes(sm_count) + static_cast<size_t>(sm_count) * kMostCtas * sizeof(RowsSplit); }
