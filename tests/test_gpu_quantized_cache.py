@@ -467,6 +467,27 @@ def test_one_page_in_many_places(backend):
         agree(backend, torch.randn(n, 8, 128, device="cuda").bfloat16(), cache, batch, 0.1)
 
 
+@pytest.mark.parametrize("hq,hk,head_dim", [(32, 8, 128), (16, 4, 64), (8, 8, 128), (18, 1, 128)])
+@pytest.mark.parametrize("news", [[1] * 11 + [90], [1, 0, 40, 1, 1, 0, 0, 2, 1, 1, 1, 60], [70] + [0] * 11, [0] * 5 + [33, 2] + [0] * 5])
+def test_single_tokens_beside_chunks(backend, news, hq, hk, head_dim):
+    """Batches whose single tokens and chunks go to kernels of their own, by what the host knows: neither writes the other's rows."""
+    lengths = [n + 37 * i for i, n in enumerate(news)]
+    pages = sum(-(-n // 16) for n in lengths) + 3
+    cache = make_quantized(pages, 16, hk, head_dim, torch.bfloat16, seed=6)
+    batch, tokens = make_batch(lengths, news, 16, pages, 2, spare_rows=2)
+    spoil_unused(cache, batch)
+    q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    hinted = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
+    out = agree(backend, q, cache, hinted, head_dim ** -0.5)
+    assert torch.equal(backend.attention_paged(q, cache, hinted, head_dim ** -0.5)[:tokens - 2], out[:tokens - 2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = backend.attention_paged(q, cache, hinted, head_dim ** -0.5)
+    graph.replay()
+    assert torch.equal(again[:tokens - 2], out[:tokens - 2])
+    backend.poll()
+
+
 def test_empty_calls(backend):
     cache = make_quantized(4, 16, 2, 128, torch.bfloat16)
     batch, _ = make_batch([20, 0], [0, 0], 16, 4, 2)

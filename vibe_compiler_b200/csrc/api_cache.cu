@@ -116,6 +116,7 @@ wb200_status make_batch(const wb200_paged_batch *b, const PagedCacheArgs &c, Pag
   a->sequences = static_cast<int>(b->sequences); a->table_width = static_cast<int>(b->table_width);
   a->tokens = static_cast<int>(b->tokens); a->max_query = static_cast<int>(b->max_query);
   a->page_table = b->page_table; a->key_lengths = b->key_lengths; a->query_starts = b->query_starts; a->table_stride = b->table_stride;
+  a->least_count = 0; a->most_count = 0x7fffffff;
   return WB200_OK;
 }
 
@@ -160,7 +161,7 @@ wb200_status make_attention_quantized(wb200_backend *backend, const wb200_quanti
 // is right for any lengths. Where a sequence has at most kRowsAtMost packed rows (one tile of its MMA) the rows kernel streams
 // the keys, which HBM bounds; a row tile of the chunk kernel takes as long for one row as for 128.
 constexpr int kRowsAtMost = 16;
-enum class PagedKernel { general, rows, chunk };
+enum class PagedKernel { general, rows, chunk, dealt };
 // The most packed rows of one sequence.
 int64_t most_rows(const AttentionPagedArgs &a) {
   int64_t longest = a.batch.max_query > 0 ? a.batch.max_query : (a.batch.tokens <= a.batch.sequences ? 1 : a.batch.tokens);
@@ -171,16 +172,31 @@ PagedKernel choose_attention_paged(const AttentionPagedArgs &a) {
   if (!attention_paged_rows_supports(a)) return PagedKernel::general;
   return most_rows(a) > kRowsAtMost && attention_paged_chunk_supports(a) ? PagedKernel::chunk : PagedKernel::rows;
 }
+uint64_t aligned256(uint64_t bytes) { return (bytes + 255) & ~255ull; }
 PagedKernel choose_attention_quantized(const AttentionPagedArgs &a, const QuantizedRowsArgs &rows) {
   if (!attention_quantized_rows_supports(a, rows)) return PagedKernel::general;
   // Two tiles of 16 rows a sequence, which read its keys twice, still are the shorter at head_dim 64: 17 sequences of 5000 keys, 4 KV
   // heads, 32 rows 32 us and 36 us, 48 rows 41 and 36; at head_dim 128, 8 KV heads, 20 rows 81 and 81.
   const int64_t at_most = a.cache.head_dim == 64 ? 2 * kRowsAtMost : kRowsAtMost;
-  return most_rows(a) > at_most && attention_quantized_chunk_supports(a, rows) ? PagedKernel::chunk : PagedKernel::rows;
+  if (most_rows(a) <= at_most || !attention_quantized_chunk_supports(a, rows)) return PagedKernel::rows;
+  // Sequences of one token among chunks, of which there are many where the tokens are few for the longest chunk, go to the rows kernel:
+  // a row tile of the chunk kernel takes 1.7 us for 128 keys whether it holds one token or 32, three times as long as the keys' bytes.
+  const bool mixed = a.batch.max_query > 1 && 2ll * a.batch.tokens <= static_cast<int64_t>(a.batch.sequences) * a.batch.max_query;
+  return mixed && a.q_heads / a.cache.kv_heads <= kRowsAtMost ? PagedKernel::dealt : PagedKernel::chunk;
 }
 uint64_t attention_quantized_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;
-  return kernel == PagedKernel::rows ? attention_quantized_rows_workspace(sm_count) : attention_quantized_chunk_workspace(sm_count);
+  const uint64_t rows = aligned256(attention_quantized_rows_workspace(sm_count)), chunk = attention_quantized_chunk_workspace(sm_count);
+  return kernel == PagedKernel::rows ? rows : kernel == PagedKernel::chunk ? chunk : rows + chunk;
+}
+// The single tokens' part of the workspace in front of the chunks'.
+wb200_status launch_attention_quantized_dealt(AttentionPagedArgs a, const QuantizedRowsArgs &rows, int sm_count, cudaStream_t stream) {
+  AttentionPagedArgs single = a;
+  single.batch.max_query = single.batch.most_count = 1;
+  a.batch.least_count = 2;
+  a.workspace = static_cast<uint8_t *>(a.workspace) + aligned256(attention_quantized_rows_workspace(sm_count));
+  const wb200_status st = launch_attention_quantized_rows(single, rows, sm_count, stream);
+  return st != WB200_OK ? st : launch_attention_quantized_chunk(a, rows, sm_count, stream);
 }
 uint64_t attention_paged_workspace(PagedKernel kernel, int sm_count) {
   if (kernel == PagedKernel::general) return 0;
@@ -377,10 +393,7 @@ wb200_status wb200_attention_paged(wb200_backend *backend, const wb200_paged_cac
 uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
                                                    const wb200_attention_paged_params *p) {
   if (!backend) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
-  if (!cache && !batch && !p) {
-    const uint64_t rows = attention_quantized_rows_workspace(backend->sm_count), chunk = attention_quantized_chunk_workspace(backend->sm_count);
-    return rows > chunk ? rows : chunk;
-  }
+  if (!cache && !batch && !p) return attention_quantized_workspace(PagedKernel::dealt, backend->sm_count);
   if (!cache || !batch || !p) { fail(WB200_ERR_INVALID_ARGUMENT, "null argument"); return 0; }
   AttentionPagedArgs a{};
   QuantizedRowsArgs rows;
@@ -403,9 +416,12 @@ wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quant
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   if (kernel == PagedKernel::general) st = launch_attention_quantized_general(a, rows, stream);
   else if (kernel == PagedKernel::rows) st = launch_attention_quantized_rows(a, rows, backend->sm_count, stream);
-  else st = launch_attention_quantized_chunk(a, rows, backend->sm_count, stream);
-  const bool one = kernel == PagedKernel::general || (kernel == PagedKernel::rows && attention_quantized_rows_clustered(a, backend->sm_count));
-  if (st == WB200_OK) backend->launches += one ? 1 : 2;
+  else if (kernel == PagedKernel::chunk) st = launch_attention_quantized_chunk(a, rows, backend->sm_count, stream);
+  else st = launch_attention_quantized_dealt(a, rows, backend->sm_count, stream);
+  if (st != WB200_OK) return st;
+  if (kernel == PagedKernel::rows || kernel == PagedKernel::dealt) backend->launches += attention_quantized_rows_clustered(a, backend->sm_count) ? 1 : 2;
+  if (kernel == PagedKernel::chunk || kernel == PagedKernel::dealt) backend->launches += 2;
+  if (kernel == PagedKernel::general) backend->launches += 1;
   return st;
 }
 

@@ -18,6 +18,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatchArgs &b,
     if (report) raise_status(refused, kRefusedLength);
     return {0, 0, 0};
   }
+  if (end - begin < b.least_count || end - begin > b.most_count) return {begin, 0, 0};
   return {begin, end - begin, keys};
 }
 // Keys that new token `index` of a sequence sees: key j with j <= keys - count + index under the causal mask.

@@ -321,6 +321,7 @@ struct PagedBatchArgs {
   int sequences, table_width, tokens, max_query;
   const int *page_table, *key_lengths, *query_starts;
   int64_t table_stride;
+  int least_count, most_count;       // sequences of fewer or more new tokens are passed over
 };
 struct RopeArgs {
   int tokens, heads, head_dim, format;
