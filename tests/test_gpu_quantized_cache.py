@@ -301,6 +301,26 @@ def test_few_tokens_take_scores_to_f32(backend, dtype, size, hq, hk, head_dim, l
         agree(backend, q, cache, hinted, head_dim ** -0.5, kernel="rows" if head_dim != 80 else "general")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,head_dim", [(32, 8, 128), (8, 8, 128), (28, 4, 128), (16, 1, 128), (16, 4, 64)])
+def test_means_of_many_values_keep_their_digits(backend, dtype, hq, hk, head_dim):
+    """Values around zero, 30 thousand to a row: the result is 1/100 of a value. In the 2-norm, relative to the result, with u half a
+    step of the type:
+      p'       off by 2^-11 at most, uniformly and apart from one another: 2^-11 / sqrt(3) of (code - 8) step, which is a value's size
+      sums     a product's f32 sums are cut off at 2^-23 of 16 keys' 136 p' at most: 136 step 2^-23 <= 8e-6 (steps up to 0.5), and the
+               result is 1 / sqrt(sum p^2) >= 1/200 of a value: 1.6e-3
+      result   u / sqrt(3)"""
+    cache = make_quantized(500, 64, hk, head_dim, dtype, seed=8)
+    batch, tokens = make_batch([30000, 20000 // 20], [1, 1], 64, 500, 2)
+    q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    got = backend.attention_paged(q, cache, batch, head_dim ** -0.5).double()
+    backend.poll()
+    want = quant.attention(q, cache, batch, head_dim ** -0.5)[0]
+    u = torch.finfo(dtype).eps / 2
+    for row in range(tokens):
+        assert (got[row] - want[row]).norm() <= (2.0 ** -11 / 3 ** 0.5 + 1.6e-3 + u / 3 ** 0.5) * want[row].norm()
+
+
 @pytest.mark.parametrize("layout", ["rows", "heads", "joined"])
 @pytest.mark.parametrize("lengths,news", [([300, 1000], [1, 1]), ([300, 1000], [3, 4]), ([300, 1000], [200, 150])])
 def test_layouts_and_strides(backend, layout, lengths, news):
