@@ -385,6 +385,23 @@ def test_a_key_that_is_not_a_number_reaches_its_own_sequence_only(backend, news)
     assert bool(((got - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("news,hq", [([1, 1], 8), ([1, 1], 16), ([8, 5], 4), ([70, 33], 8)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_value_that_is_not_a_number_stays_in_its_group(backend, dtype, news, hq, value):
+    cache = make_quantized(40, 16, 2, 128, dtype)
+    batch, tokens = make_batch([200, 150], news, 16, 40, 2)
+    q = torch.randn(tokens, hq, 128, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    want, _, bound, _ = quant.attention(q, cache, batch, 0.1)
+    cache.v_steps[int(batch.page_table[1, 0]), 3, 1, 0] = value                # seen by every row of sequence 1, KV head 1
+    got = backend.attention_paged(q, cache, batch, 0.1).double()
+    backend.poll()
+    own = got[news[0]:, hq // 2:, :64]
+    assert bool((~own.isfinite()).all())
+    got[news[0]:, hq // 2:, :64], want[news[0]:, hq // 2:, :64] = 0.0, 0.0
+    assert bool(((got - want).abs() <= bound).all())
+
+
 def test_results_do_not_depend_on_where_the_pages_lie_or_on_the_run(backend):
     size, lengths = 16, [900, 5000, 33, 260]
     cache = make_quantized(420, size, 4, 128, torch.bfloat16)

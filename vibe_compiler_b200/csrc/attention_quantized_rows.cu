@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
   using S = QuantShape<kD>;
   constexpr int kFormat = kBf16 ? WB200_BF16 : WB200_F16;
   constexpr int kMantissa = kBf16 ? 7 : 10, kExponentBias = kBf16 ? 127 : 15;
+  constexpr uint32_t kInfinity = kBf16 ? 0x7f80u : 0x7c00u;
   constexpr int kGroups = S::kGroups, kTiles = kRows == 16 ? 2 : 1;          // eight columns of the products each
   constexpr bool kTwice = kRows == 4;                  // columns 4 to 7 are the same rows, for the second group of V
   constexpr int kWeighed = kTwice ? 1 : kGroups;       // groups that a lane weighs its probabilities for
@@ -417,7 +418,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
       if (__any_sync(0xffffffffu, moves)) {
         // The references move: to the rows' largest scores where those are beyond the bound, all by the change of e.
         const int before = exponent;
-        largest_step = __reduce_max_sync(0xffffffffu, largest_step & 0xffffu);
+        largest_step = 0;                                // of the finite ones: others make their group NaN, and no more
+#pragma unroll
+        for (int k = 0; k < 2 * kBlocks; ++k)
+#pragma unroll
+          for (int gr = 0; gr < kWeighed; ++gr)
+            if ((v_steps[k][gr] & 0xffffu) < kInfinity) largest_step = max(largest_step, v_steps[k][gr] & 0xffffu);
+        largest_step = __reduce_max_sync(0xffffffffu, largest_step);
         if (largest_step > step_limit) {
           const int field = static_cast<int>(largest_step >> kMantissa);
           exponent = min(max(kStepExponent + kExponentBias - max(field, 1), kLeastExponent), kMostExponent);
