@@ -607,7 +607,14 @@ wb200_status wb200_rope_append_quantized(wb200_backend *backend, const wb200_qua
 /* wb200_cache_read: the values low + code * step, rounded to `format`. */
 wb200_status wb200_cache_read_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,
                                         const wb200_cache_read_params *params);
-/* wb200_attention_paged over the values low + code * step. */
+/* wb200_attention_paged over the values low + code * step. Statistics and sums are kept in f32. head_dim 64 and 128, with rows of
+ * codes, queries and output on 16 bytes and a row's steps on their size, take the matrix kernels: up to 16 packed rows (token, head of
+ * the group) of a sequence, 32 at head_dim 64, and single tokens among longer chunks, with scores to f32 and probabilities, weighed by the
+ * steps, rounded to f16 in front of the product with V; longer chunks with K and V rounded to `format` (as wb200_cache_read_quantized
+ * gives them) and probabilities too. Other head dimensions and alignments take a kernel that gives a warp to each row, keeps all in f32
+ * and is 29 to 240 times slower. Steps are not negative. A step or low of V that is not finite reaches its group of 64 elements, of rows
+ * that do not see the key too. The workspace is as for wb200_attention_paged (about 48 MB are enough for any call); its size follows
+ * max_query, which chooses between the kernels. */
 uint64_t wb200_attention_quantized_workspace_bytes(const wb200_backend *backend, const wb200_quantized_cache *cache,
                                                    const wb200_paged_batch *batch, const wb200_attention_paged_params *params);
 wb200_status wb200_attention_quantized(wb200_backend *backend, const wb200_quantized_cache *cache, const wb200_paged_batch *batch,

@@ -21,6 +21,9 @@
 //            few long items fill the GPU alike. Each CTA finds its share from the lengths on the device. A cut near the end of
 //            an item moves to it; others leave f32 records of the item's parts, folded by a second kernel.
 // Results depend on the lengths and the number of SMs only: repeats give the same bits.
+// With codes a step of two row tiles takes 4500 clocks, of one 3050: the decoders share the schedulers with the softmax (their work left
+// out, 3900). All loops together have to stay in the instruction cache: decoders with code of their own for V, which needs fewer
+// instructions in another order of the columns, took 6200 clocks, unrolled twice 8700.
 // Bound: the chain S -> softmax -> P V of a step (see attention_fa.cu), 4 * head_dim flop per visible (row, key) pair. A step of two
 // row tiles takes 3250 clocks, of which its products are 2048. 4096 tokens behind 32768 cached ones, 32/8 heads: 1.9 ms back to
 // back in a graph (1.2 PFLOP/s), 2.2 ms among other work (the clock gives way to the power cap); 8 chunks of 256 tokens at 4096 keys

@@ -121,7 +121,7 @@ class ShardedDecoderLayer:
 
     def forward_paged(self, x: torch.Tensor, cache, batch, rotary=None) -> torch.Tensor:
         """One serving step of this layer: x [tokens, d_model] holds the new tokens of the sequences of `batch`
-        (paged_cache.PagedBatch), whose earlier keys lie in `cache` (paged_cache.PagedCache of this rank's KV heads). The
+        (paged_cache.PagedBatch), whose earlier keys lie in `cache` (paged_cache.PagedCache or QuantizedCache of this rank's KV heads). The
         step's K and V rows are written to their pages, which have to be reserved. `rotary` (paged_cache.RotaryTable):
         default the configuration's theta over the whole head. Rows of tokens that belong to no sequence are undefined."""
         be, cfg = self.backend, self.cfg
