@@ -495,6 +495,18 @@ def test_more_sequences_than_a_block_stages(backend):
     agree(backend, torch.randn(tokens, 8, 128, device="cuda").bfloat16(), cache, few, 0.1)
 
 
+@pytest.mark.parametrize("size", [1, 1000])
+def test_pages_of_one_row_and_of_a_sequence(backend, size):
+    lengths = [300, 41, 1]
+    cache = make_quantized(sum(-(-n // size) for n in lengths) + 2, size, 2, 128, torch.float16)
+    for news in ([1, 1, 1], [2, 4, 1], [70, 41, 1], [300, 0, 0]):
+        batch, tokens = make_batch(lengths, news, size, cache.shape[0], 2)
+        spoil_unused(cache, batch)
+        q = torch.randn(tokens, 8, 128, generator=torch.Generator().manual_seed(3)).half().cuda()
+        for max_query in (0, max(news)):
+            agree(backend, q, cache, PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max_query), 0.1)
+
+
 def test_one_page_in_many_places(backend):
     # a sequence may list a page more than once: 40 thousand keys over three pages
     cache = make_quantized(3, 128, 2, 128, torch.bfloat16)

@@ -393,6 +393,8 @@ wb200_status launch_rope_append_quantized(const RopeArgs &a, const RotaryConstan
   const bool wide = rows_aligned(a.x, a.x_token, a.x_head, 2) && rows_aligned(a.out, a.out_token, a.out_head, 2) && c.pairs % 8 == 0;
   const int step = wide ? 16 : 2;
   p.items = (a.head_dim + step - 1) / step;
+  // Prompts of 15 thousand tokens, 32/8 heads, bf16, with two / four / eight passes (eight elements a lane then): 116 / 108 / 114 us;
+  // now 89, of 49 at the copy rate.
   p.tokens_per_block = tokens_per_block(a, c, p.items, 4, kMaxQuantizeAngles);
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + p.tokens_per_block - 1) / p.tokens_per_block);
   const bool bf16 = a.format == WB200_BF16;
