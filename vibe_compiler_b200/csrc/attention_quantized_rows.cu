@@ -254,9 +254,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
     const int own_group = kTwice ? t >> 1 : 0;         // the first that this lane weighs for
     float minus_reference[kTiles][2], bound[kTiles][2];          // of the exponent, e in it; relative scores beyond the bound move it
     float l_run[kTiles][2], low_sum[kTiles][kWeighed][2], acc[kTiles][kGroups][4][4];
-    float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of the sums over codes; of the lows
+    float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of a row's scores; of the lows, in the units of the sums over codes
     uint32_t q_frag[kTiles][kGroups][2][2][2], q_fix[kTiles][kGroups][2][2];
     int last_key[kTiles][2];                           // that the row sees
+    bool beyond = false;
     int exponent = 0;                                  // e
     uint32_t step_limit = 0;                           // bits of a step; greater ones move e
 #pragma unroll
@@ -281,22 +282,22 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
       };
       float largest = 0.f, sums[kGroups];
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        sums[gr] = 0.f;
+      for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = element(gr, e);
-          largest = fmaxf(largest, fabsf(x));
-          sums[gr] += x;
-        }
-#pragma unroll
-        for (int off = 1; off < 4; off <<= 1) sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], off);
-      }
+        for (int e = 0; e < 16; ++e) largest = fmaxf(largest, fabsf(element(gr, e)));
 #pragma unroll
       for (int off = 1; off < 4; off <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
       // Scaled by a power of two that brings the row's largest to 2^14, and those that meet odd codes, 16 times as large, to a sixteenth.
       // The operands are the same for all warps, who make a part of them each.
       const float power = largest > 0.f && largest < INFINITY ? power_against(largest, 14) : 1.f;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        sums[gr] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[gr] = fmaf(element(gr, e), power, sums[gr]);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], off);
+      }
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
@@ -311,16 +312,17 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
             operands[((((n * kGroups + gr) * 2 + w) * 2 + h) * 2 + 1) * 32 + lane] = *reinterpret_cast<const uint32_t *>(&odd);
           }
         }
-      const float scale = p.scale_log2 * (0x1p24f / power);
+      const float reach = 1.f / power;
+      beyond = beyond || !(p.scale_log2 * 0x1p24f * reach < INFINITY);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        row_scale[n][i] = __shfl_sync(0xffffffffu, scale, 4 * (2 * t + i));
+        row_scale[n][i] = __shfl_sync(0xffffffffu, reach, 4 * (2 * t + i));
         bound[n][i] = -INFINITY;
         minus_reference[n][i] = 0.f;
         l_run[n][i] = 0.f;
         last_key[n][i] = paged_visible(part.sequence, (part.row0 + 8 * n + column_row(2 * t + i)) / p.group, a.causal) - 1;
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) q_sum[n][gr][i] = __shfl_sync(0xffffffffu, sums[gr], 4 * (2 * t + i)) * p.scale_log2;
+        for (int gr = 0; gr < kGroups; ++gr) q_sum[n][gr][i] = __shfl_sync(0xffffffffu, sums[gr], 4 * (2 * t + i));
 #pragma unroll
         for (int gr = 0; gr < kWeighed; ++gr) low_sum[n][gr][i] = 0.f;
       }
@@ -329,6 +331,18 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][gr][j][0] = acc[n][gr][j][1] = acc[n][gr][j][2] = acc[n][gr][j][3] = 0.f;
     }
+    // The sums' unit, 2^-24, goes into the rows' scale. Where that would leave f32 (queries from about 2^118 / scale on, whose scores may
+    // well be finite) it goes into the sums, beside the mask. A scale is not zero, so that what is masked stays at -infinity.
+    beyond = __any_sync(0xffffffffu, beyond);
+    const float sums_scale = beyond ? 0x1p24f : 1.f;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row_scale[n][i] = fmaxf((beyond ? p.scale_log2 : p.scale_log2 * 0x1p24f) * row_scale[n][i], 0x1p-149f);
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) q_sum[n][gr][i] *= 0x1p-24f;
+      }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
@@ -342,7 +356,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
             for (int odd = 0; odd < 2; ++odd) q_frag[n][gr][w][h][odd] = operands[((((n * kGroups + gr) * 2 + w) * 2 + h) * 2 + odd) * 32 + lane];
             q_fix[n][gr][w][h] = q_frag[n][gr][w][h][0] ^ 0x80008000u;
           }
-    const int masked_from = min(part.key_end, paged_visible(part.sequence, part.row0 / p.group, a.causal));   // hidden from some row from here on
+    // Hidden from some row from here on, or all tiles whose sums are scaled.
+    const int masked_from = beyond ? 0 : min(part.key_end, paged_visible(part.sequence, part.row0 / p.group, a.causal));
 
     int stage = 0;                                     // byte offset in the ring
     int key0 = part.first_key;
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint8_t *const k_src = ring + stage, *const v_src = k_src + S::kCodeBytes, *const step_src = v_src + S::kCodeBytes;
-      // S^T: keys g and g + 8 of each block, relative to the reference
+      // S^T: keys g and g + 8 of each block, in the rows' units
       float score[kTiles][2 * kBlocks][2];             // [tile][key][column]
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
@@ -382,13 +397,12 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float x = quant_step(pairs[0], kFormat) * dot[n][0][2 * h + i], y = fmaf(quant_low(pairs[0], kFormat), q_sum[n][0][i], minus_reference[n][i]);
+              float x = quant_low(pairs[0], kFormat) * q_sum[n][0][i];
 #pragma unroll
-              for (int gr = 1; gr < kGroups; ++gr) {
-                x = fmaf(quant_step(pairs[gr], kFormat), dot[n][gr][2 * h + i], x);
-                y = fmaf(quant_low(pairs[gr], kFormat), q_sum[n][gr][i], y);
-              }
-              score[n][2 * b + h][i] = fmaf(x, row_scale[n][i], y);
+              for (int gr = 1; gr < kGroups; ++gr) x = fmaf(quant_low(pairs[gr], kFormat), q_sum[n][gr][i], x);
+#pragma unroll
+              for (int gr = 0; gr < kGroups; ++gr) x = fmaf(quant_step(pairs[gr], kFormat), dot[n][gr][2 * h + i], x);
+              score[n][2 * b + h][i] = x;
             }
         }
       }
@@ -399,8 +413,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
           for (int k = 0; k < 2 * kBlocks; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (key0 + g + 8 * k >= part.key_end || key0 + g + 8 * k > last_key[n][i]) score[n][k][i] = -INFINITY;
+              score[n][k][i] = key0 + g + 8 * k >= part.key_end || key0 + g + 8 * k > last_key[n][i] ? -INFINITY : score[n][k][i] * sums_scale;
       }
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int k = 0; k < 2 * kBlocks; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) score[n][k][i] = fmaf(score[n][k][i], row_scale[n][i], minus_reference[n][i]);
       uint32_t v_steps[2 * kBlocks][kWeighed], largest_step = 0;
 #pragma unroll
       for (int k = 0; k < 2 * kBlocks; ++k) {
