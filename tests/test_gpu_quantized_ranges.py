@@ -45,3 +45,64 @@ def test_queries_of_any_size_whose_scores_are_finite(backend, hq, hk, head_dim, 
     q[0, 1] = 1.0
     batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
     near(backend, q, cache, batch, scale)
+
+
+def vanishing(cache, q_heads, keys):
+    """What the products of probability and step that f16 cannot hold are off by, an element of the result: 2^-25 each at most, in a unit
+    that brings the group's largest step to 2^5 and more, for codes that are 8 away from the middle; a row's sum is 1 and more."""
+    most = cache.v_steps[..., 0].double().amax((0, 1))                          # [kv_heads, groups]
+    return (most * (keys * 2.0 ** -27)).repeat_interleave(64, -1).repeat_interleave(q_heads // cache.shape[2], 0)
+
+
+ROWS = [(8, 2, [1, 1]), (16, 2, [1, 1]), (16, 2, [2, 1])]                       # four, eight and sixteen rows to a tile
+
+
+@pytest.mark.parametrize("dtype,exponent", [(torch.bfloat16, 12), (torch.bfloat16, 20), (torch.bfloat16, 100), (torch.float16, 8)])
+@pytest.mark.parametrize("first_is_small", [True, False])
+@pytest.mark.parametrize("hq,hk,news", ROWS)
+def test_groups_of_a_row_may_differ_in_size(backend, dtype, exponent, first_is_small, hq, hk, news):
+    """The values of one group of 64 elements 2^(2 exponent) times the other's: each to its own bound."""
+    cache = make_quantized(50, 16, hk, 128, dtype)
+    sizes = (2.0 ** -exponent, 2.0 ** exponent) if first_is_small else (2.0 ** exponent, 2.0 ** -exponent)
+    for group, size in enumerate(sizes):
+        cache.v_steps[..., group, :] *= size
+    batch, tokens = make_batch([500, 130], news, 16, 50, 2)
+    q = torch.randn(tokens, hq, 128, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
+    near(backend, q, cache, batch, 128 ** -0.5, vanishes=vanishing(cache, hq, 500))
+
+
+@pytest.mark.parametrize("dtype,exponent", [(torch.bfloat16, 12), (torch.float16, 8)])
+@pytest.mark.parametrize("hq,hk,news", ROWS)
+def test_means_of_many_values_in_groups_of_different_sizes(backend, dtype, exponent, hq, hk, news):
+    """As test_means_of_many_values_keep_their_digits, with its bound for each group."""
+    cache = make_quantized(500, 64, hk, 128, dtype, seed=8)
+    cache.v_steps[..., 0, :] *= 2.0 ** -exponent
+    cache.v_steps[..., 1, :] *= 2.0 ** exponent
+    batch, tokens = make_batch([30000, 1000], news, 64, 500, 2)
+    q = torch.randn(tokens, hq, 128, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
+    got = backend.attention_paged(q, cache, batch, 128 ** -0.5).double()
+    backend.poll()
+    want = quant.attention(q, cache, batch, 128 ** -0.5)[0]
+    u = torch.finfo(dtype).eps / 2
+    for group in (slice(0, 64), slice(64, 128)):
+        for a, b in zip(got[..., group], want[..., group]):
+            assert (a - b).norm() <= (2.0 ** -11 / 3 ** 0.5 + 1.6e-3 + u / 3 ** 0.5) * b.norm()
+
+
+@pytest.mark.parametrize("dtype,sizes", [(torch.bfloat16, (1.0, 2.0 ** 12)), (torch.bfloat16, (2.0 ** 12, 1.0)), (torch.bfloat16, (2.0 ** -100, 2.0 ** 100)),
+                                         (torch.bfloat16, (2.0 ** 100, 2.0 ** -100)), (torch.bfloat16, (2.0 ** 100,)), (torch.bfloat16, (2.0 ** -115,)),
+                                         (torch.float16, (2.0 ** -18,)), (torch.float16, (2.0 ** -20, 2.0 ** 10))])
+@pytest.mark.parametrize("hq,hk,head_dim,news", [(hq, hk, 128, news) for hq, hk, news in ROWS] + [(8, 2, 64, [2, 4])])
+def test_keys_may_differ_in_size(backend, hq, hk, head_dim, news, dtype, sizes):
+    """Pages of values of one size after pages of another."""
+    cache = make_quantized(50, 16, hk, head_dim, dtype)
+    batch, tokens = make_batch([500, 130], news, 16, 50, 2)
+    for s in range(2):
+        pages = batch.page_table[s][batch.page_table[s] >= 0].long()
+        for size, part in zip(sizes, pages.chunk(len(sizes))):
+            cache.v_steps[part] *= size
+    q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
+    near(backend, q, cache, batch, head_dim ** -0.5, vanishes=vanishing(cache, hq, 500))

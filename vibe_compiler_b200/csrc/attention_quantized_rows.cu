@@ -10,11 +10,13 @@
 //            -Q, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g. The products are exact: Q is scaled
 //            to f16 by a power of two of its own a row.
 //   V        O^T = C P^T, sums with the odd codes in them and sums of those alone as rows of one product, subtracted at the end.
-//            step_g is folded into the probabilities, p'_g = p step_g 2^e, rounded to f16 (11 bits, whatever the type), and
+//            step_g is folded into the probabilities, p'_g = p step_g 2^e_g, rounded to f16 (11 bits, whatever the type), and
 //            sum_j p_j (low + 8 step)_g,j runs beside it in f32: a product with a constant takes 8 off every code, so that both sums
 //            are as small as the values are. (A tensor core's f32 sums are cut off, not rounded. Of codes as they are, whose sums only
 //            grow, the values' mean is what is left of two numbers 300 times as large: 17 thousand keys in f16 came out 1.3e-2 off
-//            in the 2-norm, of 2e-4 with codes less 8.) e follows the largest step so far, so p' stays below f16's largest.
+//            in the 2-norm, of 2e-4 with codes less 8.) e_g follows the largest step of the group so far, so p' stays below f16's
+//            largest; p' up to 2^-25, of steps 2^-30 of that one with p = 1, vanish from this sum (one e for both groups took all digits
+//            of the smaller one from 2^24 on).
 //            P, as S^T leaves it, becomes the other operand by movmatrix; rows of K or V are never transposed: two keys' words
 //            interleaved by halves (prmt) are the pairs that the instruction wants.
 //   four rows  of a sequence or fewer, head_dim 128: Q stands in the columns twice, and P^T in the second four carries the second
@@ -42,7 +44,7 @@ constexpr int kUnitSteps = 3;
 constexpr int kLeastSteps = 2;
 constexpr float kMovesBeyond = 8.f;             // log2
 constexpr int kStepExponent = 5;                // of step 2^e when e is chosen; steps of twice that do not move it, so p' < 2^8 2^7
-constexpr int kLeastExponent = -120, kMostExponent = 60;         // of 2^e, so that sums with it stay in f32
+constexpr int kLeastExponent = -120, kMostExponent = 126;        // 2^e and 2^-e are normal numbers of f32
 constexpr uint32_t kBoth = 0x00ff00ffu, kOdd = 0x00f000f0u;
 constexpr uint32_t kMinusBoth = 0x80888088u, kMinusOdd = 0x80808080u;     // -(8 + 16 * 8) 2^-24, -16 * 8 * 2^-24, twice
 
@@ -122,7 +124,6 @@ template <bool kBf16, int kD, int kRows, bool kAligned, bool kClustered>
 __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_quantized_rows_kernel(const __grid_constant__ QuantRowsParams p) {
   using S = QuantShape<kD>;
   constexpr int kFormat = kBf16 ? WB200_BF16 : WB200_F16;
-  constexpr int kMantissa = kBf16 ? 7 : 10, kExponentBias = kBf16 ? 127 : 15;
   constexpr uint32_t kInfinity = kBf16 ? 0x7f80u : 0x7c00u;
   constexpr int kGroups = S::kGroups, kTiles = kRows == 16 ? 2 : 1;          // eight columns of the products each
   constexpr bool kTwice = kRows == 4;                  // columns 4 to 7 are the same rows, for the second group of V
@@ -252,14 +253,19 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
     auto middle = [](uint32_t pair) { return fmaf(8.f, quant_step(pair, kFormat), quant_low(pair, kFormat)); };
     auto column_row = [](int column) { return kTwice ? column & 3 : column; };
     const int own_group = kTwice ? t >> 1 : 0;         // the first that this lane weighs for
-    float minus_reference[kTiles][2], bound[kTiles][2];          // of the exponent, e in it; relative scores beyond the bound move it
+    float minus_reference[kTiles][2], bound[kTiles][2];          // of the exponent; relative scores beyond the bound move it
     float l_run[kTiles][2], low_sum[kTiles][kWeighed][2], acc[kTiles][kGroups][4][4];
     float row_scale[kTiles][2], q_sum[kTiles][kGroups][2];       // of a row's scores; of the lows, in the units of the sums over codes
     uint32_t q_frag[kTiles][kGroups][2][2][2], q_fix[kTiles][kGroups][2][2];
     int last_key[kTiles][2];                           // that the row sees
     bool beyond = false;
-    int exponent = 0;                                  // e
-    uint32_t step_limit = 0;                           // bits of a step; greater ones move e
+    int exponent[kWeighed];                            // e
+    uint32_t step_limit[kWeighed];                     // bits of a step; greater ones move e
+#pragma unroll
+    for (int gr = 0; gr < kWeighed; ++gr) {
+      exponent[gr] = 0;
+      step_limit[gr] = 0;
+    }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       // The row's elements 64 gr + 16 t + .. of this lane's column g.
@@ -421,14 +427,16 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
         for (int k = 0; k < 2 * kBlocks; ++k)
 #pragma unroll
           for (int i = 0; i < 2; ++i) score[n][k][i] = fmaf(score[n][k][i], row_scale[n][i], minus_reference[n][i]);
-      uint32_t v_steps[2 * kBlocks][kWeighed], largest_step = 0;
+      uint32_t v_steps[2 * kBlocks][kWeighed], largest_step[kWeighed] = {};
 #pragma unroll
       for (int k = 0; k < 2 * kBlocks; ++k) {
         load_steps<kWeighed>(step_src + S::kStepBytes + (g + 8 * k) * (4 * kGroups) + 4 * own_group, v_steps[k]);
 #pragma unroll
-        for (int gr = 0; gr < kWeighed; ++gr) largest_step = __vmaxu2(largest_step, v_steps[k][gr]);     // steps are not negative: their bits are in order
+        for (int gr = 0; gr < kWeighed; ++gr) largest_step[gr] = __vmaxu2(largest_step[gr], v_steps[k][gr]);     // steps are not negative: their bits are in order
       }
-      bool moves = (largest_step & 0xffffu) > step_limit;
+      bool moves = false;
+#pragma unroll
+      for (int gr = 0; gr < kWeighed; ++gr) moves = moves || (largest_step[gr] & 0xffffu) > step_limit[gr];
       float row_top[kTiles][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
@@ -440,19 +448,23 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
           moves = moves || row_top[n][i] > bound[n][i];
         }
       if (__any_sync(0xffffffffu, moves)) {
-        // The references move: to the rows' largest scores where those are beyond the bound, all by the change of e.
-        const int before = exponent;
-        largest_step = 0;                                // of the finite ones: others make their group NaN, and no more
+        // e of the groups that have a step beyond the limit, and references, to the rows' largest scores where those are beyond the bound.
+        float change[kWeighed];                          // of 2^e
 #pragma unroll
-        for (int k = 0; k < 2 * kBlocks; ++k)
+        for (int gr = 0; gr < kWeighed; ++gr) {
+          uint32_t most = 0;                             // of the finite ones: others make their group NaN, and no more
 #pragma unroll
-          for (int gr = 0; gr < kWeighed; ++gr)
-            if ((v_steps[k][gr] & 0xffffu) < kInfinity) largest_step = max(largest_step, v_steps[k][gr] & 0xffffu);
-        largest_step = __reduce_max_sync(0xffffffffu, largest_step);
-        if (largest_step > step_limit) {
-          const int field = static_cast<int>(largest_step >> kMantissa);
-          exponent = min(max(kStepExponent + kExponentBias - max(field, 1), kLeastExponent), kMostExponent);
-          step_limit = (static_cast<uint32_t>(field + 2) << kMantissa) - 1;
+          for (int k = 0; k < 2 * kBlocks; ++k)
+            if ((v_steps[k][gr] & 0xffffu) < kInfinity) most = max(most, v_steps[k][gr] & 0xffffu);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));     // lanes of the same groups
+          const int before = exponent[gr];
+          if (most > step_limit[gr]) {
+            const uint32_t field = __float_as_uint(quant_step(most, kFormat)) >> 23;
+            exponent[gr] = min(max(kStepExponent + 127 - static_cast<int>(field), kLeastExponent), kMostExponent);
+            step_limit[gr] = narrow_bits(__uint_as_float(min(field + 2, 255u) << 23), kFormat) - 1;
+          }
+          change[gr] = exp2_fast(static_cast<float>(exponent[gr] - before));     // the first e meets sums of nothing
         }
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
@@ -461,13 +473,12 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
             float top = row_top[n][i];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            float shift = bound[n][i] == -INFINITY ? 0.f : static_cast<float>(before - exponent), alpha = exp2_fast(-shift);
+            float shift = 0.f, alpha = 1.f;
             if (top > bound[n][i]) {
-              shift = top - static_cast<float>(exponent);
+              shift = top;
               alpha = bound[n][i] == -INFINITY ? 0.f : exp2_fast(-shift);
-              bound[n][i] = 0.f;
+              bound[n][i] = kMovesBeyond;
             }
-            if (bound[n][i] != -INFINITY) bound[n][i] = kMovesBeyond + static_cast<float>(exponent);
             minus_reference[n][i] -= shift;
 #pragma unroll
             for (int k = 0; k < 2 * kBlocks; ++k) score[n][k][i] -= shift;
@@ -478,8 +489,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
             for (int gr = 0; gr < kGroups; ++gr)
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                acc[n][gr][j][i] *= alpha;
-                acc[n][gr][j][2 + i] *= alpha;
+                acc[n][gr][j][i] *= alpha * change[kTwice ? 0 : gr];
+                acc[n][gr][j][2 + i] *= alpha * change[kTwice ? 0 : gr];
               }
           }
       }
@@ -503,7 +514,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
           for (int gr = 0; gr < kWeighed; ++gr)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float step = quant_step(v_steps[2 * b + h][gr], kFormat);
+              const float step = quant_step(v_steps[2 * b + h][gr], kFormat) * __uint_as_float(static_cast<uint32_t>(exponent[gr] + 127) << 23);
               const __half2 both = __floats2half2_rn(pr[h][0] * step, pr[h][1] * step);
               p_frag[n][gr][h] = transposed(*reinterpret_cast<const uint32_t *>(&both));
             }
@@ -537,8 +548,6 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
       stage += S::kStageBytes;
       if (stage == S::kRingBytes) stage = 0;
     }
-    // The state without e.
-    const float unscale = exp2_fast(static_cast<float>(-exponent));
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -549,9 +558,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
 #pragma unroll
           for (int gr = 0; gr < kWeighed; ++gr) low_sum[n][gr][i] += __shfl_xor_sync(0xffffffffu, low_sum[n][gr][i], off);
         }
-        l_run[n][i] *= unscale;
-        minus_reference[n][i] = bound[n][i] == -INFINITY ? INFINITY : minus_reference[n][i] - static_cast<float>(exponent);
+        if (bound[n][i] == -INFINITY) minus_reference[n][i] = INFINITY;
       }
+    float unscale[kWeighed];                           // the sums are put together without e
+#pragma unroll
+    for (int gr = 0; gr < kWeighed; ++gr) unscale[gr] = __uint_as_float(static_cast<uint32_t>(127 - exponent[gr]) << 23);
     // The next part's first tiles are on their way while this one's state is put together. (The ring's groups of copies have all
     // been waited for but the empty ones behind the last tile.)
     const Part done = part;
@@ -572,8 +583,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(kRows)) attention_qua
           for (int j = 0; j < 4; ++j) {
             const float both = kTwice && own_group ? acc[n][kGroups - 1][j][i] : acc[n][gr][j][i];
             const float odd = kTwice && own_group ? acc[n][kGroups - 1][j][2 + i] : acc[n][gr][j][2 + i];
-            v[2 * j] = ((both - odd) * 0x1p24f + low_sum[n][gr][i]) * unscale;
-            v[2 * j + 1] = (odd * 0x1p20f + low_sum[n][gr][i]) * unscale;
+            v[2 * j] = fmaf((both - odd) * 0x1p24f, unscale[gr], low_sum[n][gr][i]);
+            v[2 * j + 1] = fmaf(odd * 0x1p20f, unscale[gr], low_sum[n][gr][i]);
           }
           float4 *to = reinterpret_cast<float4 *>(mine_records + row * S::kRecord + (gr + own_group) * kQuantGroup + 8 * g);
           to[0] = make_float4(v[0], v[1], v[2], v[3]);
