@@ -6,7 +6,7 @@ import torch
 from tests import quantized_reference as quant
 from tests.test_gpu_quantized_cache import make_quantized
 from tests.test_gpu_rope import make_batch
-from vibe_compiler_b200.paged_cache import PagedBatch
+from vibe_compiler_b200.paged_cache import PagedBatch, PagedCache
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,17 @@ def test_keys_may_differ_in_size(backend, hq, hk, head_dim, news, dtype, sizes):
     q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
     batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
     near(backend, q, cache, batch, head_dim ** -0.5, vanishes=vanishing(cache, hq, 500))
+
+
+@pytest.mark.parametrize("hq,hk,head_dim,news", [(hq, hk, 128, news) for hq, hk, news in ROWS] + [(8, 2, 64, [2, 4]), (32, 2, 64, [2, 1])])
+def test_runs_of_a_few_sequences_repeat(backend, hq, hk, head_dim, news):
+    """A cluster's CTAs put their warps' states together in the place of the first warp's, which all lanes read before one writes it."""
+    cache = make_quantized(50, 16, hk, head_dim, torch.float16)
+    wide = PagedCache(*(quant.values(codes, steps).half() for codes, steps in (cache._tensors[:2], cache._tensors[2:])))
+    batch, tokens = make_batch([500, 130], news, 16, 50, 2)
+    batch = PagedBatch(batch.page_table, batch.key_lengths, batch.query_starts, max_query=max(news))
+    q = torch.randn(tokens, hq, head_dim, generator=torch.Generator().manual_seed(5)).half().cuda()
+    want = near(backend, q, cache, batch, head_dim ** -0.5), backend.attention_paged(q, wide, batch, head_dim ** -0.5)
+    for _ in range(200):
+        assert torch.equal(backend.attention_paged(q, cache, batch, head_dim ** -0.5), want[0])
+        assert torch.equal(backend.attention_paged(q, wide, batch, head_dim ** -0.5), want[1])

@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attention_paged_rows_kernel(co
         fold_warps<kD, kWarps>(records, r, lane, top, l, sum);
         const int row = r + 8 * h;
         if constexpr (kClustered) {                    // over the first warp's record, which this warp has read
+          __syncwarp();
           sum.store(records + r * S::kRecord, lane);
           if (lane == 0) *reinterpret_cast<float2 *>(records + r * S::kRecord + kD) = make_float2(top, l);
         } else if (whole) {
