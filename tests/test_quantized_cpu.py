@@ -132,3 +132,37 @@ def test_the_format_on_rows_done_by_hand():
     codes, steps = quant.quantized((x / 3).bfloat16())
     step = steps[0, 0, 0].item()
     assert 1 / 3 <= step < 1 / 3 * (1 + 2.0 ** -7) and (quant.values(codes, steps) - (x / 3).bfloat16().double()).abs().max() <= step / 2
+
+
+def test_each_kind_of_cache_has_its_own_scratch():
+    """attention_paged takes what its own kernels need, not the larger of both kinds' scratch."""
+    import types
+    asked = []
+
+    class Library:
+        @staticmethod
+        def wb200_attention_paged_workspace_bytes(*_):
+            return 1000
+
+        @staticmethod
+        def wb200_attention_quantized_workspace_bytes(*_):
+            return 3000
+
+        @staticmethod
+        def wb200_attention_paged(handle, cache, batch, p):
+            asked.append(("plain", p._obj.workspace_bytes))
+            return abi.OK
+
+        @staticmethod
+        def wb200_attention_quantized(handle, cache, batch, p):
+            asked.append(("four bits", p._obj.workspace_bytes))
+            return abi.OK
+    backend = B200TargetModelBackend.__new__(B200TargetModelBackend)
+    backend.device, backend._lib, backend._handle = -1, Library, None               # tensors of the CPU have no device index
+    backend._empty = lambda like, shape, stream, dtype=None: torch.empty(shape, dtype=dtype or like.dtype)
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    rows = types.SimpleNamespace(device_index=-1, _desc=lambda tokens: batch())
+    for quantized, desc in ((True, cache()), (False, abi.PagedCacheDesc()), (True, cache()), (False, abi.PagedCacheDesc())):
+        handle = types.SimpleNamespace(device_index=-1, shape=(4, 16, 2, 64), dtype=torch.bfloat16, quantized=quantized, _desc=desc)
+        backend.attention_paged(q, handle, rows, 0.1, stream=0)
+    assert asked == [("four bits", 3000), ("plain", 1000)] * 2

@@ -162,7 +162,7 @@ class ResultPool:
 
 class B200TargetModelBackend:
     _results = ResultPool()   # shared by the backends of the process
-    _paged_workspace: Optional[int] = None   # bytes that are enough for any attention_paged call
+    _paged_workspace: Optional[tuple] = None   # bytes that are enough for any attention_paged call, over a 16-bit and over a quantized cache
 
     def __init__(self, device: int = 0):
         self._lib = abi.load()
@@ -681,10 +681,11 @@ class B200TargetModelBackend:
             shape[1], bool(causal), bool(zero_fully_masked), C.c_float(scale).value, 0, q.data_ptr(), out.data_ptr(),
             lse.data_ptr() if lse is not None else 0, q_strides[0], q_strides[1], out_strides[0], out_strides[1], 0, 0, stream))
         if self._paged_workspace is None:
-            self._paged_workspace = max(int(query(self._handle, None, None, None)) for query in
-                                        (self._lib.wb200_attention_paged_workspace_bytes, self._lib.wb200_attention_quantized_workspace_bytes))
-        workspace = self._empty(q, self._paged_workspace, stream, torch.uint8)
-        p.workspace, p.workspace_bytes = workspace.data_ptr(), self._paged_workspace
+            self._paged_workspace = tuple(int(query(self._handle, None, None, None)) for query in
+                                          (self._lib.wb200_attention_paged_workspace_bytes, self._lib.wb200_attention_quantized_workspace_bytes))
+        size = self._paged_workspace[cache.quantized]
+        workspace = self._empty(q, size, stream, torch.uint8)
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), size
         call = self._lib.wb200_attention_quantized if cache.quantized else self._lib.wb200_attention_paged
         self._check(call(self._handle, C.byref(cache._desc), C.byref(desc), C.byref(p)))
         return out
