@@ -583,8 +583,8 @@ wb200_status wb200_cache_read(wb200_backend *backend, const wb200_paged_cache *c
  *   low   its least element,  step  (its largest - low) / 15 in f32, rounded up,      both in `format`, and
  *   codes (x - low) / step in f32, to the nearest of 0 .. 15 (ties to even),
  * for the values low + code * step, each within half a step of its element (where low + 15 step would be beyond the format's
- * largest number, step is rounded down). A group that holds an infinity or a NaN (or spans
- * more than f32 does) is NaN as a whole. Element e of a row lies in byte e / 2 of its codes, an even one in the low half;
+ * largest number, step is rounded down, and the largest elements may be 0.117 of a step further off in bf16, 0.0147 in f16). A group
+ * that holds an infinity or a NaN (or spans more than f32 does) is NaN as a whole. Element e of a row lies in byte e / 2 of its codes, an even one in the low half;
  * group g's pair is word g of its steps, step in the low half. head_dim is a multiple of 8 up to 256. Attention and pages_copy
  * read these and nothing else, so a cache may be filled by other means too. Rows of codes begin on 4 bytes; on 16, with
  * head_dim 64 or 128, they take the matrix kernels. Rows of one head that lie one behind the other in a page ([pages, kv_heads,
@@ -609,8 +609,9 @@ wb200_status wb200_cache_read_quantized(wb200_backend *backend, const wb200_quan
                                         const wb200_cache_read_params *params);
 /* wb200_attention_paged over the values low + code * step. Statistics and sums are kept in f32. head_dim 64 and 128, with rows of
  * codes, queries and output on 16 bytes and a row's steps on their size, take the matrix kernels: up to 16 packed rows (token, head of
- * the group) of a sequence, 32 at head_dim 64, and single tokens among longer chunks, with scores to f32 and probabilities, weighed by the
- * steps, rounded to f16 in front of the product with V; longer chunks with K and V rounded to `format` (as wb200_cache_read_quantized
+ * the group) of a sequence, 32 at head_dim 64, and single tokens among longer chunks, with scores to f32 (query elements 2^24 times
+ * smaller than their row's largest are off by up to 2^-35 of it) and probabilities, weighed by the steps, rounded to f16 in front of the
+ * product with V (products up to 2^-30 of the largest step of the same group of 64 elements vanish from it); longer chunks with K and V rounded to `format` (as wb200_cache_read_quantized
  * gives them) and probabilities too. Other head dimensions and alignments take a kernel that gives a warp to each row, keeps all in f32
  * and is 29 to 240 times slower. Steps are not negative. A step or low of V that is not finite reaches its group of 64 elements, of rows
  * that do not see the key too. The workspace is as for wb200_attention_paged (about 48 MB are enough for any call); its size follows

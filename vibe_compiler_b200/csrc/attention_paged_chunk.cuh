@@ -54,8 +54,9 @@ constexpr int kFirstChunks = 3;                 // 32-key chunks of the first pa
 constexpr uint32_t kColS0 = 0, kColO0 = 256;    // S_t at 128 t, O_t at 256 + 128 t
 constexpr int kMaxSequences = 4096;             // staged in shared memory
 // Work, in twelfths of a step of two row tiles (3250 clocks; 4500 with codes to decode): a key tile of two row tiles, of one (1820
-// clocks; 3050), and what an item costs by itself (its Q, the first scores, the write-out: 4700). With codes, of weights 6 to 9 and 14 to
-// 32 these were the shortest over seven mixed batches (40 decoding sequences beside 8 chunks: 8 and 14 438 us, 7 and 24 425).
+// clocks; 3050), and what an item costs by itself (its Q, the first scores, the write-out: 4700). With codes the clocks say 8 twelfths for
+// one row tile and 13 for an item; of weights 6 to 9 and 14 to 32 tried, 7 and 24 were the shortest over seven mixed batches (40 decoding
+// sequences beside 8 chunks: 8 and 14 438 us, 7 and 24 425).
 constexpr int kPairWork = 12, kSingleWork = 7;
 template <bool kQuantized>
 constexpr int kItemWork = kQuantized ? 24 : 18;

@@ -8,7 +8,7 @@
 //            instructions for the eight elements of a word. The powers of two go into Q, and into the result.
 //   K        S^T = C Q^T, keys on the 16-wide side, with the odd codes' share of the even elements' sums taken off by a product with
 //            -Q, a sum for each group of 64 elements: s = sum_g step_g (c.q)_g + low_g (sum q)_g. The products are exact: Q is scaled
-//            to f16 by a power of two of its own a row.
+//            to f16 by a power of two of its own a row (elements 2^24 times smaller than the row's largest lose digits, off by 2^-35 of it).
 //   V        O^T = C P^T, sums with the odd codes in them and sums of those alone as rows of one product, subtracted at the end.
 //            step_g is folded into the probabilities, p'_g = p step_g 2^e_g, rounded to f16 (11 bits, whatever the type), and
 //            sum_j p_j (low + 8 step)_g,j runs beside it in f32: a product with a constant takes 8 off every code, so that both sums
@@ -22,10 +22,11 @@
 //   four rows  of a sequence or fewer, head_dim 128: Q stands in the columns twice, and P^T in the second four carries the second
 //            group's steps, so a lane weighs its probabilities for one group.
 //   maximum  The exponent's reference moves only when a score is beyond 2^8 times it: one vote a tile instead of shuffles.
-// A CTA is four warps; each streams every fourth 16-key tile of the share through a ring of its own (cp.async, rows XOR-swizzled).
-// Bound: HBM would take 396 issue slots for 16 keys; the warps' instructions (260, of which 12 + 16 are products) do, at 0.54 a
-// clock with three warps to a scheduler: 64 sequences of 2000 to 32000 keys, 32/8 heads, f16: 246 us, 4.3 TB/s (the floor is 163).
-// Taken back: e4m3 products for K (three instructions a word, but the assembler widens them to f16 products: 359 us against 221 then);
+// A CTA is four warps; each streams every fourth 32-key tile of the share through a ring of its own (cp.async, rows XOR-swizzled).
+// Bound: 64 sequences of 2000 to 32000 keys, 32/8 heads, f16: 242 us, 4.4 TB/s (the floor is 163). The warps' instructions for 16 keys (306,
+// of which 12 + 16 are products) would fit the 396 issue slots that HBM takes, but are issued at 0.55 a clock: with three warps to a
+// scheduler, as many as the registers allow, results and busy pipes are waited for.
+// Taken back: e4m3 products for K (three instructions a word; 359 us against 221 then);
 // the scores of a tile among the products with V of the one before (168 registers do not hold both: 234); tiles of 16 keys with four
 // CTAs to an SM (271 against 228).
 #include "attention_paged_walk.cuh"

@@ -3,7 +3,7 @@
 //
 // A thread keeps to its elements of the token's K and V heads, sixteen where they are codes, eight of 16 bits, and walks the block's
 // tokens, four loads on their way together.
-// Bound: HBM, the rows read and the rows written: 400 thousand keys of 8 heads, f16, 313 us for 1.9 GB, 6.0 TB/s.
+// Bound: HBM, the rows read and the rows written: 359545 keys of 8 heads, f16, 313 us for 1.9 GB, 6.0 TB/s.
 #include "attention_paged.cuh"
 #include "quantized_rows.cuh"
 

@@ -8,7 +8,8 @@
 // eighth of a turn, is rounded to 24 significant bits of its own for sincospif, so that the small sines of slow pairs are as
 // right as any. The sines and cosines of a token serve all its heads: a block computes them once, into shared memory.
 //
-// Both kernels are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below.
+// The first two are HBM-bound: every element is read once and written once, in 16-byte accesses; measured at launch() below. The one that
+// quantises waits for memory, shared memory and barriers: at launch_rope_append_quantized().
 #include "attention_paged.cuh"
 #include "quantized_rows.cuh"
 
@@ -393,8 +394,8 @@ wb200_status launch_rope_append_quantized(const RopeArgs &a, const RotaryConstan
   const bool wide = rows_aligned(a.x, a.x_token, a.x_head, 2) && rows_aligned(a.out, a.out_token, a.out_head, 2) && c.pairs % 8 == 0;
   const int step = wide ? 16 : 2;
   p.items = (a.head_dim + step - 1) / step;
-  // Prompts of 15 thousand tokens, 32/8 heads, bf16, with two / four / eight passes (eight elements a lane then): 116 / 108 / 114 us;
-  // now 89, of 49 at the copy rate.
+  // Prompts of 12174 tokens, 32/8 heads, bf16, with two / four / eight passes (eight elements a lane then): 116 / 108 / 114 us; now 89,
+  // of 40 for its 263 MB at the copy rate.
   p.tokens_per_block = tokens_per_block(a, c, p.items, 4, kMaxQuantizeAngles);
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.tokens) + p.tokens_per_block - 1) / p.tokens_per_block);
   const bool bf16 = a.format == WB200_BF16;
